@@ -433,6 +433,102 @@ int tgx_co_occurrence(const int32_t* a_ids, const int32_t* c_ids, const uint8_t*
                       const uint8_t* c_mask, int64_t pairs, int32_t k, int32_t* a_cnt,
                       int32_t* c_cnt, float* pair_count, void* stream);
 
+/* ---- Operators of a temporal attention model on prepared batches ----
+ * No counterpart in the reference, whose models (tgengine/models, tgengine/nn) take
+ * these steps in torch.  Values are TGX_F32 or TGX_BF16; sums, statistics and softmax
+ * are held in 32 bits and each output is rounded once.  No atomics: the same inputs
+ * give the same bits. */
+#define TGX_MAX_EMBED_DIM 65536
+#define TGX_MAX_NORM_DIM 16384
+#define TGX_MAX_HEAD_DIM 256
+
+/* out[i] = scale * table[ids[i]] for i < n, rows of dim values; an id outside
+ * [0, rows) (the -1 of a padded neighbour) gives a row of zeros.  table: rows
+ * `stride` values apart; ids int32 (ids_i32 != 0) or int64; out [n, dim]. */
+int tgx_embed(const void* table, int64_t rows, int64_t dim, int64_t stride, int32_t dtype,
+              const void* ids, int32_t ids_i32, int64_t n, float scale, void* out, void* stream);
+/* Its gradient: grad [rows, dim], every row written: scale * the sum of dout[i] over
+ * the i with that id, in an order that the ids alone decide.  workspace:
+ * tgx_embed_grad_workspace_size(n, dim) bytes, 16-byte aligned, no initialisation. */
+size_t tgx_embed_grad_workspace_size(int64_t n, int64_t dim);
+int tgx_embed_grad(const void* dout, const void* ids, int32_t ids_i32, int64_t n, int64_t rows,
+                   int64_t dim, int32_t dtype, float scale, void* grad, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* Layer norm of `rows` rows of dim values (x: `stride` values apart; out [rows, dim]):
+ * (x - mean) * rstd * weight + bias with rstd = 1 / sqrt(var + eps), var the mean of
+ * squares about the mean.  weight and bias [dim] of wdtype, either may be NULL.  mean
+ * and rstd [rows]: both set (the gradient reads them) or both NULL. */
+int tgx_layer_norm(const void* x, int64_t rows, int64_t dim, int64_t stride, int32_t dtype,
+                   const void* weight, const void* bias, int32_t wdtype, float eps, void* out,
+                   float* mean, float* rstd, void* stream);
+/* Its gradient: dx [rows, dim], dw and db [dim] of wdtype; each may be NULL.  dy
+ * [rows, dim].  workspace (needed with dw or db):
+ * tgx_layer_norm_grad_workspace_size(rows, dim) bytes, 16-byte aligned. */
+size_t tgx_layer_norm_grad_workspace_size(int64_t rows, int64_t dim);
+int tgx_layer_norm_grad(const void* x, const void* dy, int64_t rows, int64_t dim, int64_t stride,
+                        int32_t dtype, const void* weight, int32_t wdtype, const float* mean,
+                        const float* rstd, void* dx, void* dw, void* db, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* Attention of lq query tokens to lk states of another sequence, per batch row and
+ * head; query head h reads key/value head h / (heads / kv_heads).  Element (b, i, h, c)
+ * of q is q[b * q_stride[0] + i * q_stride[1] + h * q_stride[2] + c], k and v alike
+ * with kv_heads; a stride may be 0 (a broadcast input).  mask: NULL, or bytes at
+ * mask[b * mask_stride + j], 0 = key j takes no part (its k and v are not used,
+ * whatever they hold).  A row that keeps no key gives zeros and takes no gradient.
+ * out [batch, lq, heads, dim]; lse float [batch, lq, heads], the log of each row's sum
+ * of exp(scale q.k) (-inf without a key): NULL, or kept for the gradient. */
+typedef struct tgx_attention_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  const uint8_t* mask;
+  int64_t batch;
+  int64_t lq;
+  int64_t lk;
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t dim;             /* 1 .. TGX_MAX_HEAD_DIM */
+  int32_t dtype;
+  int64_t q_stride[3];     /* batch, token, head */
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t mask_stride;
+  float scale;
+  int32_t reserved;
+  void* out;
+  float* lse;
+  /* tgx_attention_grad: out and lse as tgx_attention wrote them, grad_out
+   * [batch, lq, heads, dim]; grad_q of q's shape, grad_k and grad_v
+   * [batch, lk, kv_heads, dim], each may be NULL */
+  const void* grad_out;
+  void* grad_q;
+  void* grad_k;
+  void* grad_v;
+  void* workspace;         /* 16-byte aligned, no initialisation; NULL when 0 bytes are needed */
+  size_t workspace_bytes;
+} tgx_attention_args;
+
+/* bytes of workspace that the call of the same arguments needs (0 for arguments that
+ * it refuses) */
+size_t tgx_attention_workspace_size(const tgx_attention_args* args);
+size_t tgx_attention_grad_workspace_size(const tgx_attention_args* args);
+int tgx_attention(const tgx_attention_args* args, void* stream);
+int tgx_attention_grad(const tgx_attention_args* args, void* stream);
+
+/* Clipping by the global norm: norm[0] = sqrt(sum of squares over all `count` tensors),
+ * outs[t] = grads[t] * min(1, max_norm / (norm + 1e-6)).  The arrays are host arrays,
+ * read during the call; tensor t is sizes[t] contiguous values of dtypes[t], its output
+ * of out_dtypes[t] may be the tensor itself (same dtype) and must not overlap another.
+ * A NaN or infinite norm scales as the formula says.  workspace:
+ * tgx_clip_grad_norm_workspace_size(sizes, count) bytes. */
+size_t tgx_clip_grad_norm_workspace_size(const int64_t* sizes, int64_t count);
+int tgx_clip_grad_norm(const void* const* grads, const int32_t* dtypes, void* const* outs,
+                       const int32_t* out_dtypes, const int64_t* sizes, int64_t count,
+                       float max_norm, float* norm, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
 const char* tgx_last_error(void);
 int tgx_abi_version(void);
 

@@ -33,6 +33,9 @@ TGX_MAX_SLOTS = 64
 TGX_MAX_K = 512
 TGX_MAX_GROUP = 8
 TGX_MAX_DT = 512
+TGX_MAX_EMBED_DIM = 65536
+TGX_MAX_NORM_DIM = 16384
+TGX_MAX_HEAD_DIM = 256
 
 c_i32, c_i64, c_vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
 
@@ -89,6 +92,15 @@ TGX_CSR_NONDECREASING = 4
 
 
 # every symbol include/tgx.h declares, with its ctypes signature
+class TgxAttentionArgs(ctypes.Structure):
+    _fields_ = [("q", c_vp), ("k", c_vp), ("v", c_vp), ("mask", c_vp), ("batch", c_i64), ("lq", c_i64),
+                ("lk", c_i64), ("heads", c_i32), ("kv_heads", c_i32), ("dim", c_i32), ("dtype", c_i32),
+                ("q_stride", c_i64 * 3), ("k_stride", c_i64 * 3), ("v_stride", c_i64 * 3),
+                ("mask_stride", c_i64), ("scale", ctypes.c_float), ("reserved", c_i32), ("out", c_vp),
+                ("lse", c_vp), ("grad_out", c_vp), ("grad_q", c_vp), ("grad_k", c_vp), ("grad_v", c_vp),
+                ("workspace", c_vp), ("workspace_bytes", ctypes.c_size_t)]
+
+
 SIGNATURES = {
     "tgx_ring_append": (c_i32, [ctypes.POINTER(TgxRing), c_vp, c_vp, c_vp, c_vp, c_i64, c_i64,
                                 c_vp, ctypes.c_size_t, c_vp, c_vp]),
@@ -125,6 +137,26 @@ SIGNATURES = {
     "tgx_last_error": (ctypes.c_char_p, []),
     "tgx_abi_version": (c_i32, []),
 }
+
+# operators of a temporal attention model
+SIGNATURES.update({
+    "tgx_embed": (c_i32, [c_vp, c_i64, c_i64, c_i64, c_i32, c_vp, c_i32, c_i64, ctypes.c_float, c_vp, c_vp]),
+    "tgx_embed_grad_workspace_size": (ctypes.c_size_t, [c_i64, c_i64]),
+    "tgx_embed_grad": (c_i32, [c_vp, c_vp, c_i32, c_i64, c_i64, c_i64, c_i32, ctypes.c_float, c_vp, c_vp,
+                               ctypes.c_size_t, c_vp]),
+    "tgx_layer_norm": (c_i32, [c_vp, c_i64, c_i64, c_i64, c_i32, c_vp, c_vp, c_i32, ctypes.c_float, c_vp, c_vp,
+                               c_vp, c_vp]),
+    "tgx_layer_norm_grad_workspace_size": (ctypes.c_size_t, [c_i64, c_i64]),
+    "tgx_layer_norm_grad": (c_i32, [c_vp, c_vp, c_i64, c_i64, c_i64, c_i32, c_vp, c_i32, c_vp, c_vp, c_vp, c_vp,
+                                    c_vp, c_vp, ctypes.c_size_t, c_vp]),
+    "tgx_attention_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(TgxAttentionArgs)]),
+    "tgx_attention_grad_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(TgxAttentionArgs)]),
+    "tgx_attention": (c_i32, [ctypes.POINTER(TgxAttentionArgs), c_vp]),
+    "tgx_attention_grad": (c_i32, [ctypes.POINTER(TgxAttentionArgs), c_vp]),
+    "tgx_clip_grad_norm_workspace_size": (ctypes.c_size_t, [c_vp, c_i64]),
+    "tgx_clip_grad_norm": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, ctypes.c_float, c_vp, c_vp,
+                                   ctypes.c_size_t, c_vp]),
+})
 
 _lock = threading.Lock()
 _lib = None

@@ -28,6 +28,8 @@
 
 namespace py = pybind11;
 
+void bind_ops(py::module_& m);  // tgx_ops.cpp: the model-side operators
+
 namespace {
 
 // Event-major launches (co-occurrence) of at most this many queries group only the
@@ -626,4 +628,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ring_plan", &ring_plan, "launch tgx_ring_plan (first half of an append)");
   m.def("ring_commit", &ring_commit, "launch tgx_ring_commit (second half of an append)");
   m.def("ring_discard", &ring_discard, "launch tgx_ring_discard (drop a planned append)");
+  bind_ops(m);
 }
