@@ -9,7 +9,7 @@
 //   dq_i = sum_j ds_ij k_j,  dk_j = sum_i ds_ij q_i      (i over the group's heads too)
 //
 // A masked key's k and v are never used, whatever they hold.
-#include "tgx_ops.h"
+#include "tgx_attention.h"
 
 namespace tgx {
 namespace {
@@ -17,17 +17,6 @@ namespace {
 constexpr int kAttThreads = 256;
 constexpr int kAttWaves = kAttThreads / kWave;
 constexpr int kPer = TGX_MAX_HEAD_DIM / kWave;  // values of a head per lane
-
-struct AttArgs {
-  const void *q, *k, *v, *out, *dout;
-  const uint8_t* mask;
-  void *o, *dq, *dk, *dv;
-  float* lse;
-  int64_t batch, lq, lk, mask_stride;
-  int64_t qs[3], ks[3], vs[3];
-  int32_t heads, kv_heads, dim;
-  float scale;
-};
 
 // one wave per query token and head
 template <typename T>
@@ -212,12 +201,19 @@ AttArgs att_args(const tgx_attention_args* p) {
     a.ks[i] = p->k_stride[i];
     a.vs[i] = p->v_stride[i];
   }
+  a.os[0] = p->lq * p->heads * p->dim;
+  a.os[1] = static_cast<int64_t>(p->heads) * p->dim;
+  a.os[2] = p->dim;
   a.heads = p->heads;
   a.kv_heads = p->kv_heads;
+  a.group = p->heads / p->kv_heads;
   a.dim = p->dim;
   a.scale = p->scale;
   return a;
 }
+
+// few rows to few keys: a row's work is too small for a matrix tile
+bool by_rows(const AttArgs& a) { return a.lq * a.group <= 4 && a.lk <= 512; }
 
 }  // namespace
 }  // namespace tgx
@@ -225,8 +221,9 @@ AttArgs att_args(const tgx_attention_args* p) {
 using namespace tgx;
 
 extern "C" size_t tgx_attention_workspace_size(const tgx_attention_args* args) {
-  (void)args;
-  return 0;
+  if (check_attention("tgx_attention", args, false)) return 0;
+  const AttArgs a = att_args(args);
+  return by_rows(a) || a.batch * a.lq == 0 ? 0 : att_mma_forward_workspace(a, args->dtype);
 }
 
 extern "C" int tgx_attention(const tgx_attention_args* args, void* stream) {
@@ -235,6 +232,12 @@ extern "C" int tgx_attention(const tgx_attention_args* args, void* stream) {
   const AttArgs a = att_args(args);
   const int64_t rows = a.batch * a.lq * a.heads;
   if (rows == 0) return TGX_OK;
+  if (!by_rows(a)) {
+    const size_t need = att_mma_forward_workspace(a, args->dtype);
+    if (need > args->workspace_bytes || (need > 0 && !aligned16(args->workspace)))
+      return fail(TGX_ERR_ARG, "tgx_attention: workspace of %zu bytes, 16-byte aligned, needed", need);
+    return att_mma_forward(a, args->dtype, args->workspace, static_cast<hipStream_t>(stream));
+  }
   return by_type(args->dtype, [&](auto t) {
     using T = decltype(t);
     hipLaunchKernelGGL(att_fwd<T>, dim3(static_cast<unsigned>(ops_cdiv(rows, kAttWaves))), dim3(kAttThreads), 0,
@@ -244,8 +247,9 @@ extern "C" int tgx_attention(const tgx_attention_args* args, void* stream) {
 }
 
 extern "C" size_t tgx_attention_grad_workspace_size(const tgx_attention_args* args) {
-  (void)args;
-  return 0;
+  if (check_attention("tgx_attention_grad", args, false)) return 0;
+  const AttArgs a = att_args(args);
+  return by_rows(a) || a.batch * a.lq == 0 ? 0 : att_mma_backward_workspace(a, args->dtype);
 }
 
 extern "C" int tgx_attention_grad(const tgx_attention_args* args, void* stream) {
@@ -253,6 +257,12 @@ extern "C" int tgx_attention_grad(const tgx_attention_args* args, void* stream) 
   if (rc) return rc;
   const AttArgs a = att_args(args);
   const int64_t rows = a.batch * a.lq * a.heads, keys = a.batch * a.lk * a.kv_heads;
+  if (!by_rows(a) && rows > 0) {
+    const size_t need = att_mma_backward_workspace(a, args->dtype);
+    if (need > args->workspace_bytes || !aligned16(args->workspace))
+      return fail(TGX_ERR_ARG, "tgx_attention_grad: workspace of %zu bytes, 16-byte aligned, needed", need);
+    return att_mma_backward(a, args->dtype, args->workspace, static_cast<hipStream_t>(stream));
+  }
   return by_type(args->dtype, [&](auto t) {
     using T = decltype(t);
     if (rows > 0 && a.dq != nullptr) {
