@@ -19,7 +19,7 @@ INCLUDE = ROOT / "include"
 OUT_DIR = PKG / "_lib"
 LIB = OUT_DIR / "libtgx.so"
 SOURCES = ["tgx_common.hip", "tgx_ring.hip", "tgx_recent.hip", "tgx_csr.hip", "tgx_negpool.hip",
-           "tgx_embed.hip", "tgx_norm.hip", "tgx_attention.hip", "tgx_att_fwd.hip", "tgx_att_bwd.hip",
+           "tgx_embed.hip", "tgx_norm.hip", "tgx_attention.hip", "tgx_att_fwd.hip", "tgx_att_bwd.hip", "tgx_att_rows.hip",
            "tgx_clip.hip"]
 
 ARCH = "gfx950"

@@ -255,11 +255,14 @@ int att_mma_forward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
     }
     return check_launch("att_mma_fwd");
   });
-  if (rc || f.splits == 1) return rc;
+  return rc || f.splits == 1 ? rc : att_join_forward(a, dtype, f.splits, part, s);
+}
+
+int att_join_forward(const AttArgs& a, int dtype, int splits, const float* part, hipStream_t s) {
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
     hipLaunchKernelGGL(att_join<T>, dim3(static_cast<unsigned>(ops_cdiv(a.batch * a.lq * a.heads, 4))), dim3(256), 0, s,
-                       a, f.splits, part);
+                       a, splits, part);
     return check_launch("att_join");
   });
 }

@@ -21,7 +21,15 @@ struct AttArgs {
   float scale;
 };
 
-// tgx_att_fwd.hip, tgx_att_bwd.hip
+// Problems of at most kMostRows rows go to tgx_att_rows.hip, the others to
+// tgx_att_fwd.hip and tgx_att_bwd.hip
+constexpr int kMostRows = 4;
+size_t att_rows_forward_workspace(const AttArgs& a);
+int att_rows_forward(const AttArgs& a, int dtype, void* ws, hipStream_t s);
+size_t att_rows_backward_workspace(const AttArgs& a);
+int att_rows_backward(const AttArgs& a, int dtype, void* ws, hipStream_t s);
+// joins the key ranges' parts, per row and range: maximum, sum, dim outputs
+int att_join_forward(const AttArgs& a, int dtype, int splits, const float* part, hipStream_t s);
 size_t att_mma_forward_workspace(const AttArgs& a, int dtype);
 int att_mma_forward(const AttArgs& a, int dtype, void* ws, hipStream_t s);
 size_t att_mma_backward_workspace(const AttArgs& a, int dtype);

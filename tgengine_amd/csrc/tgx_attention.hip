@@ -14,147 +14,6 @@
 namespace tgx {
 namespace {
 
-constexpr int kAttThreads = 256;
-constexpr int kAttWaves = kAttThreads / kWave;
-constexpr int kPer = TGX_MAX_HEAD_DIM / kWave;  // values of a head per lane
-
-// one wave per query token and head
-template <typename T>
-__global__ __launch_bounds__(kAttThreads) void att_fwd(const AttArgs a) {
-  const int lane = threadIdx.x & (kWave - 1);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kAttWaves + threadIdx.x / kWave;
-  if (row >= a.batch * a.lq * a.heads) return;
-  const int h = static_cast<int>(row % a.heads);
-  const int64_t i = row / a.heads % a.lq, b = row / a.heads / a.lq;
-  const int hk = h / (a.heads / a.kv_heads);
-  const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + i * a.qs[1] + h * a.qs[2];
-  const T* k = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[2];
-  const T* v = static_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[2];
-  float x[kPer], acc[kPer];
-#pragma unroll
-  for (int u = 0; u < kPer; ++u) {
-    x[u] = lane + u * kWave < a.dim ? to_f(q[lane + u * kWave]) : 0.f;
-    acc[u] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  for (int64_t j = 0; j < a.lk; ++j) {
-    if (a.mask != nullptr && !a.mask[b * a.mask_stride + j]) continue;
-    float s = 0.f;
-#pragma unroll
-    for (int u = 0; u < kPer; ++u)
-      if (lane + u * kWave < a.dim) s += x[u] * to_f(k[j * a.ks[1] + lane + u * kWave]);
-    s = group_sum<kWave>(s) * a.scale;
-    const float top = fmaxf(m, s);
-    const float old = top == -INFINITY ? 1.f : expf(m - top), p = top == -INFINITY ? 0.f : expf(s - top);
-    l = l * old + p;
-    m = top;
-#pragma unroll
-    for (int u = 0; u < kPer; ++u)
-      if (lane + u * kWave < a.dim) acc[u] = acc[u] * old + p * to_f(v[j * a.vs[1] + lane + u * kWave]);
-  }
-  T* o = static_cast<T*>(a.o) + row * a.dim;
-#pragma unroll
-  for (int u = 0; u < kPer; ++u)
-    if (lane + u * kWave < a.dim) o[lane + u * kWave] = from_f<T>(l > 0.f ? acc[u] / l : 0.f);
-  if (lane == 0 && a.lse != nullptr) a.lse[row] = l > 0.f ? m + logf(l) : -INFINITY;
-}
-
-// one wave per query token and head: dq
-template <typename T>
-__global__ __launch_bounds__(kAttThreads) void att_bwd_q(const AttArgs a) {
-  const int lane = threadIdx.x & (kWave - 1);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kAttWaves + threadIdx.x / kWave;
-  if (row >= a.batch * a.lq * a.heads) return;
-  const int h = static_cast<int>(row % a.heads);
-  const int64_t i = row / a.heads % a.lq, b = row / a.heads / a.lq;
-  const int hk = h / (a.heads / a.kv_heads);
-  const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + i * a.qs[1] + h * a.qs[2];
-  const T* k = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[2];
-  const T* v = static_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[2];
-  float x[kPer], g[kPer], acc[kPer], delta = 0.f;
-#pragma unroll
-  for (int u = 0; u < kPer; ++u) {
-    const bool in = lane + u * kWave < a.dim;
-    x[u] = in ? to_f(q[lane + u * kWave]) : 0.f;
-    g[u] = in ? to_f(static_cast<const T*>(a.dout)[row * a.dim + lane + u * kWave]) : 0.f;
-    if (in) delta += g[u] * to_f(static_cast<const T*>(a.out)[row * a.dim + lane + u * kWave]);
-    acc[u] = 0.f;
-  }
-  delta = group_sum<kWave>(delta);
-  const float lse = a.lse[row];
-  for (int64_t j = 0; j < a.lk && lse > -INFINITY; ++j) {
-    if (a.mask != nullptr && !a.mask[b * a.mask_stride + j]) continue;
-    float s = 0.f, dp = 0.f, kv[kPer];
-#pragma unroll
-    for (int u = 0; u < kPer; ++u) {
-      const bool in = lane + u * kWave < a.dim;
-      kv[u] = in ? to_f(k[j * a.ks[1] + lane + u * kWave]) : 0.f;
-      s += x[u] * kv[u];
-      if (in) dp += g[u] * to_f(v[j * a.vs[1] + lane + u * kWave]);
-    }
-    s = group_sum<kWave>(s) * a.scale;
-    dp = group_sum<kWave>(dp);
-    const float ds = expf(s - lse) * (dp - delta) * a.scale;
-#pragma unroll
-    for (int u = 0; u < kPer; ++u) acc[u] += ds * kv[u];
-  }
-  T* o = static_cast<T*>(a.dq) + row * a.dim;
-#pragma unroll
-  for (int u = 0; u < kPer; ++u)
-    if (lane + u * kWave < a.dim) o[lane + u * kWave] = from_f<T>(acc[u]);
-}
-
-// one wave per key and key/value head: dk and dv
-template <typename T>
-__global__ __launch_bounds__(kAttThreads) void att_bwd_kv(const AttArgs a) {
-  const int lane = threadIdx.x & (kWave - 1);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kAttWaves + threadIdx.x / kWave;
-  if (row >= a.batch * a.lk * a.kv_heads) return;
-  const int hk = static_cast<int>(row % a.kv_heads);
-  const int64_t j = row / a.kv_heads % a.lk, b = row / a.kv_heads / a.lk;
-  const int group = a.heads / a.kv_heads;
-  float x[kPer], y[kPer], ak[kPer], av[kPer];
-  const bool kept = a.mask == nullptr || a.mask[b * a.mask_stride + j];
-#pragma unroll
-  for (int u = 0; u < kPer; ++u) {
-    const bool in = kept && lane + u * kWave < a.dim;
-    x[u] = in ? to_f(static_cast<const T*>(a.k)[b * a.ks[0] + j * a.ks[1] + hk * a.ks[2] + lane + u * kWave]) : 0.f;
-    y[u] = in ? to_f(static_cast<const T*>(a.v)[b * a.vs[0] + j * a.vs[1] + hk * a.vs[2] + lane + u * kWave]) : 0.f;
-    ak[u] = av[u] = 0.f;
-  }
-  for (int64_t r = 0; kept && r < a.lq * group; ++r) {
-    const int64_t i = r / group;
-    const int h = hk * group + static_cast<int>(r % group);
-    const int64_t at = (b * a.lq + i) * a.heads + h;
-    const float lse = a.lse[at];
-    float qv[kPer], g[kPer], s = 0.f, dp = 0.f, delta = 0.f;
-#pragma unroll
-    for (int u = 0; u < kPer; ++u) {
-      const bool in = lane + u * kWave < a.dim;
-      qv[u] = in ? to_f(static_cast<const T*>(a.q)[b * a.qs[0] + i * a.qs[1] + h * a.qs[2] + lane + u * kWave]) : 0.f;
-      g[u] = in ? to_f(static_cast<const T*>(a.dout)[at * a.dim + lane + u * kWave]) : 0.f;
-      if (in) delta += g[u] * to_f(static_cast<const T*>(a.out)[at * a.dim + lane + u * kWave]);
-      s += qv[u] * x[u];
-      dp += g[u] * y[u];
-    }
-    s = group_sum<kWave>(s) * a.scale;
-    dp = group_sum<kWave>(dp);
-    delta = group_sum<kWave>(delta);
-    const float p = expf(s - lse), ds = p * (dp - delta) * a.scale;
-#pragma unroll
-    for (int u = 0; u < kPer; ++u) {
-      av[u] += p * g[u];
-      ak[u] += ds * qv[u];
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < kPer; ++u) {
-    if (lane + u * kWave >= a.dim) continue;
-    if (a.dk != nullptr) static_cast<T*>(a.dk)[row * a.dim + lane + u * kWave] = from_f<T>(ak[u]);
-    if (a.dv != nullptr) static_cast<T*>(a.dv)[row * a.dim + lane + u * kWave] = from_f<T>(av[u]);
-  }
-}
-
 int check_attention(const char* what, const tgx_attention_args* a, bool grad) {
   if (a == nullptr) return fail(TGX_ERR_ARG, "%s: args is NULL", what);
   if (a->batch < 0 || a->lq < 0 || a->lk < 0 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads != 0 ||
@@ -212,8 +71,10 @@ AttArgs att_args(const tgx_attention_args* p) {
   return a;
 }
 
-// few rows to few keys: a row's work is too small for a matrix tile
-bool by_rows(const AttArgs& a) { return a.lq * a.group <= 4 && a.lk <= 512; }
+bool by_rows(const AttArgs& a, int dtype) {
+  const int64_t rows = a.lq * a.group;
+  return rows <= kMostRows && (rows == 1 || dtype == TGX_F32 || a.lk <= 256);
+}
 
 }  // namespace
 }  // namespace tgx
@@ -223,59 +84,44 @@ using namespace tgx;
 extern "C" size_t tgx_attention_workspace_size(const tgx_attention_args* args) {
   if (check_attention("tgx_attention", args, false)) return 0;
   const AttArgs a = att_args(args);
-  return by_rows(a) || a.batch * a.lq == 0 ? 0 : att_mma_forward_workspace(a, args->dtype);
+  if (a.batch * a.lq == 0) return 0;
+  return by_rows(a, args->dtype) ? att_rows_forward_workspace(a) : att_mma_forward_workspace(a, args->dtype);
 }
 
 extern "C" int tgx_attention(const tgx_attention_args* args, void* stream) {
   const int rc = check_attention("tgx_attention", args, false);
   if (rc) return rc;
   const AttArgs a = att_args(args);
-  const int64_t rows = a.batch * a.lq * a.heads;
-  if (rows == 0) return TGX_OK;
-  if (!by_rows(a)) {
-    const size_t need = att_mma_forward_workspace(a, args->dtype);
-    if (need > args->workspace_bytes || (need > 0 && !aligned16(args->workspace)))
-      return fail(TGX_ERR_ARG, "tgx_attention: workspace of %zu bytes, 16-byte aligned, needed", need);
-    return att_mma_forward(a, args->dtype, args->workspace, static_cast<hipStream_t>(stream));
-  }
-  return by_type(args->dtype, [&](auto t) {
-    using T = decltype(t);
-    hipLaunchKernelGGL(att_fwd<T>, dim3(static_cast<unsigned>(ops_cdiv(rows, kAttWaves))), dim3(kAttThreads), 0,
-                       static_cast<hipStream_t>(stream), a);
-    return check_launch("att_fwd");
-  });
+  if (a.batch * a.lq == 0) return TGX_OK;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const size_t need = by_rows(a, args->dtype) ? att_rows_forward_workspace(a) : att_mma_forward_workspace(a, args->dtype);
+  if (need > args->workspace_bytes || (need > 0 && !aligned16(args->workspace)))
+    return fail(TGX_ERR_ARG, "tgx_attention: workspace of %zu bytes, 16-byte aligned, needed", need);
+  return by_rows(a, args->dtype) ? att_rows_forward(a, args->dtype, args->workspace, s)
+                    : att_mma_forward(a, args->dtype, args->workspace, s);
 }
 
 extern "C" size_t tgx_attention_grad_workspace_size(const tgx_attention_args* args) {
   if (check_attention("tgx_attention_grad", args, false)) return 0;
   const AttArgs a = att_args(args);
-  return by_rows(a) || a.batch * a.lq == 0 ? 0 : att_mma_backward_workspace(a, args->dtype);
+  if (a.batch * a.lq == 0) return 0;
+  return by_rows(a, args->dtype) ? att_rows_backward_workspace(a) : att_mma_backward_workspace(a, args->dtype);
 }
 
 extern "C" int tgx_attention_grad(const tgx_attention_args* args, void* stream) {
   const int rc = check_attention("tgx_attention_grad", args, true);
   if (rc) return rc;
   const AttArgs a = att_args(args);
-  const int64_t rows = a.batch * a.lq * a.heads, keys = a.batch * a.lk * a.kv_heads;
-  if (!by_rows(a) && rows > 0) {
-    const size_t need = att_mma_backward_workspace(a, args->dtype);
-    if (need > args->workspace_bytes || !aligned16(args->workspace))
-      return fail(TGX_ERR_ARG, "tgx_attention_grad: workspace of %zu bytes, 16-byte aligned, needed", need);
-    return att_mma_backward(a, args->dtype, args->workspace, static_cast<hipStream_t>(stream));
-  }
-  return by_type(args->dtype, [&](auto t) {
-    using T = decltype(t);
-    if (rows > 0 && a.dq != nullptr) {
-      hipLaunchKernelGGL(att_bwd_q<T>, dim3(static_cast<unsigned>(ops_cdiv(rows, kAttWaves))), dim3(kAttThreads), 0,
-                         static_cast<hipStream_t>(stream), a);
-      const int e = check_launch("att_bwd_q");
-      if (e) return e;
-    }
-    if (keys > 0 && (a.dk != nullptr || a.dv != nullptr)) {
-      hipLaunchKernelGGL(att_bwd_kv<T>, dim3(static_cast<unsigned>(ops_cdiv(keys, kAttWaves))), dim3(kAttThreads), 0,
-                         static_cast<hipStream_t>(stream), a);
-      return check_launch("att_bwd_kv");
-    }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (a.batch * a.lq == 0) {  // no query: the keys' gradients are zeros
+    const size_t bytes = static_cast<size_t>(a.batch * a.lk * a.kv_heads * a.dim) * elem_bytes(args->dtype);
+    for (void* p : {a.dk, a.dv})
+      if (const int e = fill_zero(p, p != nullptr ? bytes : 0, s)) return e;
     return TGX_OK;
-  });
+  }
+  const size_t need = by_rows(a, args->dtype) ? att_rows_backward_workspace(a) : att_mma_backward_workspace(a, args->dtype);
+  if (need > args->workspace_bytes || (need > 0 && !aligned16(args->workspace)))
+    return fail(TGX_ERR_ARG, "tgx_attention_grad: workspace of %zu bytes, 16-byte aligned, needed", need);
+  return by_rows(a, args->dtype) ? att_rows_backward(a, args->dtype, args->workspace, s)
+                    : att_mma_backward(a, args->dtype, args->workspace, s);
 }

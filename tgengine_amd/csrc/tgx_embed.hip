@@ -53,14 +53,6 @@ __global__ __launch_bounds__(kEmbThreads) void embed_keys(const I* __restrict__ 
   keys[i] = static_cast<uint32_t>(r < 0 ? rows : r);
 }
 
-__global__ __launch_bounds__(kEmbThreads) void embed_zero(uint4* __restrict__ p, int64_t n16, uint8_t* __restrict__ tail,
-                                                          int ntail) {
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kEmbThreads;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kEmbThreads + threadIdx.x;
-  for (int64_t i = t; i < n16; i += step) p[i] = make_uint4(0, 0, 0, 0);
-  if (t < ntail) tail[t] = 0;
-}
-
 // A tile is kTile consecutive sorted tokens.  A run of equal keys inside one tile is
 // summed and written out; of a run that reaches into other tiles each tile leaves its
 // part in 32 bits: part[2 t] for a run that the tile did not begin, part[2 t + 1] for
@@ -204,19 +196,7 @@ extern "C" int tgx_embed_grad(const void* dout, const void* ids, int32_t ids_i32
   const EmbedWs w(n, dim);
   if (n > 0 && (workspace == nullptr || workspace_bytes < w.bytes || !aligned16(workspace)))
     return fail(TGX_ERR_ARG, "tgx_embed_grad: workspace of %zu bytes, 16-byte aligned, needed", w.bytes);
-  const size_t all = static_cast<size_t>(rows) * dim * elem_bytes(dtype);
-  const size_t head = std::min(all, static_cast<size_t>(-addr(grad) & 15));
-  if (head > 0) {  // an address between 16-byte steps
-    hipLaunchKernelGGL(embed_zero, dim3(1), dim3(kEmbThreads), 0, s, nullptr, 0, static_cast<uint8_t*>(grad),
-                       static_cast<int>(head));
-    if ((rc = check_launch("embed_zero"))) return rc;
-  }
-  uint8_t* body = static_cast<uint8_t*>(grad) + head;
-  const int64_t n16 = static_cast<int64_t>((all - head) / 16);
-  hipLaunchKernelGGL(embed_zero, dim3(static_cast<unsigned>(std::clamp<int64_t>(ops_cdiv(n16, kEmbThreads), 1, 8192))),
-                     dim3(kEmbThreads), 0, s, reinterpret_cast<uint4*>(body), n16, body + n16 * 16,
-                     static_cast<int>((all - head) % 16));
-  if ((rc = check_launch("embed_zero"))) return rc;
+  if ((rc = fill_zero(grad, static_cast<size_t>(rows) * dim * elem_bytes(dtype), s))) return rc;
   if (n == 0) return TGX_OK;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   uint32_t* k[2];
