@@ -53,57 +53,142 @@ __global__ __launch_bounds__(kEmbThreads) void embed_keys(const I* __restrict__ 
   keys[i] = static_cast<uint32_t>(r < 0 ? rows : r);
 }
 
-// A tile is kTile consecutive sorted tokens.  A run of equal keys inside one tile is
-// summed and written out; of a run that reaches into other tiles each tile leaves its
-// part in 32 bits: part[2 t] for a run that the tile did not begin, part[2 t + 1] for
-// one that begins in it and goes on after it.
-constexpr int kTile = 64;
+// A tile is `tile` consecutive sorted tokens, taken by LT lanes (one pack of V columns
+// each, further columns in turns); the workgroup's tiles lie beside each other.  A run
+// of equal keys inside one tile is summed and written out; of a run that reaches into
+// other tiles each tile leaves its part in 32 bits: part[2 t] for a run that the tile
+// did not begin, part[2 t + 1] for one that begins in it and goes on after it.  A row's
+// last pack overlaps the one before: both lanes come to the same sums there.
+constexpr int kMostTile = 64;
+constexpr int kAhead = 8;  // rows of one lane that are read at a time
 
-template <typename T>
+template <typename T, int V, int LT>
 __global__ __launch_bounds__(kEmbThreads) void embed_sum(const uint32_t* __restrict__ keys,
                                                          const uint32_t* __restrict__ tokens, int64_t n, int64_t rows,
-                                                         int dim, const T* __restrict__ dout, float scale,
+                                                         int tile, int dim, const T* __restrict__ dout, float scale,
                                                          T* __restrict__ grad, float* __restrict__ part) {
-  const int64_t lo = static_cast<int64_t>(blockIdx.x) * kTile;
-  const int64_t hi = lo + kTile < n ? lo + kTile : n;
-  const uint32_t prev = lo > 0 ? keys[lo - 1] : 0xffffffffu;
-  const uint32_t next = hi < n ? keys[hi] : 0xffffffffu;
-  for (int c = threadIdx.x; c < dim; c += kEmbThreads) {
-    float acc = 0.f;
-    for (int64_t i = lo; i < hi; ++i) {
-      const uint32_t key = keys[i];
-      if (key >= rows) break;  // ids outside the table come last
-      acc += to_f(dout[static_cast<int64_t>(tokens[i]) * dim + c]);
-      const uint32_t after = i + 1 < hi ? keys[i + 1] : next;
-      if (i + 1 < hi && after == key) continue;
-      // the run's end, or the tile's
-      const bool from_before = key == prev && keys[lo] == key;
-      const bool goes_on = i + 1 == hi && after == key;
-      if (from_before) part[(2 * static_cast<int64_t>(blockIdx.x)) * dim + c] = acc;
-      else if (goes_on) part[(2 * static_cast<int64_t>(blockIdx.x) + 1) * dim + c] = acc;
-      else grad[static_cast<int64_t>(key) * dim + c] = from_f<T>(acc * scale);
-      acc = 0.f;
+  constexpr int TILES = kEmbThreads / LT;
+  __shared__ uint32_t skey[TILES * kMostTile + 2], stok[TILES * kMostTile];
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * TILES * tile;
+  // skey[i + 1]: key of the block's token i; 0xffffffff before the first and after the last
+  for (int i = threadIdx.x; i < TILES * tile + 2; i += kEmbThreads) {
+    const int64_t j = first + i - 1;
+    skey[i] = j >= 0 && j < n ? keys[j] : 0xffffffffu;
+    if (i < TILES * tile) stok[i] = j + 1 < n ? tokens[j + 1] : 0u;
+  }
+  __syncthreads();
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * TILES + threadIdx.x / LT;
+  const uint32_t* key = skey + 1 + threadIdx.x / LT * tile;
+  const uint32_t* tok = stok + threadIdx.x / LT * tile;
+  // ids outside the table come last
+  int count = 0;
+  for (int step = kMostTile; step > 0; step >>= 1)
+    if (count + step <= tile && key[count + step - 1] < rows) count += step;
+  const bool from_before = count > 0 && key[0] == key[-1];
+  for (int c = (threadIdx.x % LT) * V; c < dim; c += LT * V) {
+    const int col = min(c, dim - V);
+    float acc[V];
+#pragma unroll
+    for (int u = 0; u < V; ++u) acc[u] = 0.f;
+    bool head = from_before;
+    for (int i0 = 0; i0 < count; i0 += kAhead) {
+      Pack<T, V> x[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        x[i] = load_pack<T, V>(dout + static_cast<int64_t>(tok[min(i0 + i, count - 1)]) * dim + col);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (i0 + i >= count) break;
+#pragma unroll
+        for (int u = 0; u < V; ++u) acc[u] += to_f(x[i].v[u]);
+        const uint32_t k = key[i0 + i];
+        const bool last = i0 + i + 1 == tile;
+        if (key[i0 + i + 1] == k && !last) continue;
+        // the run's end, or the tile's
+        if (head || (last && key[i0 + i + 1] == k)) {
+          Pack<float, V> y;
+#pragma unroll
+          for (int u = 0; u < V; ++u) y.v[u] = acc[u];
+          store_pack<float, V>(part + (2 * t + (head ? 0 : 1)) * dim + col, y);
+        } else {
+          Pack<T, V> y;
+#pragma unroll
+          for (int u = 0; u < V; ++u) y.v[u] = from_f<T>(acc[u] * scale);
+          store_pack<T, V>(grad + static_cast<int64_t>(k) * dim + col, y);
+        }
+        head = false;
+#pragma unroll
+        for (int u = 0; u < V; ++u) acc[u] = 0.f;
+      }
     }
   }
 }
 
-// one workgroup per tile in which a run begins that later tiles go on with: its parts in tile order
-template <typename T>
+// One workgroup per tile in which a run begins that later tiles go on with: its parts,
+// every TILES-th of them summed by one group of lanes, then the groups' sums in order.
+// A hub's run crosses thousands of tiles; its end is searched 64 tiles a step.
+template <typename T, int V, int LT>
 __global__ __launch_bounds__(kEmbThreads) void embed_join(const uint32_t* __restrict__ keys, int64_t n, int64_t rows,
-                                                          int dim, const float* __restrict__ part, float scale,
-                                                          T* __restrict__ grad) {
+                                                          int tile, int dim, const float* __restrict__ part,
+                                                          float scale, T* __restrict__ grad) {
+  constexpr int TILES = kEmbThreads / LT;
+  __shared__ float lds[TILES > 1 ? kEmbThreads * V : 1];
   const int64_t t = blockIdx.x;
-  const int64_t hi = (t + 1) * kTile;
+  const int64_t hi = (t + 1) * tile;
   if (hi >= n) return;
   const uint32_t key = keys[hi - 1];
   if (key >= rows || keys[hi] != key) return;
-  if (t > 0 && keys[t * kTile] == key && keys[t * kTile - 1] == key) return;  // begun before this tile
-  for (int c = threadIdx.x; c < dim; c += kEmbThreads) {
-    float acc = part[(2 * t + 1) * dim + c];
-    for (int64_t u = t + 1; u * kTile < n && keys[u * kTile] == key; ++u) acc += part[2 * u * dim + c];
-    grad[static_cast<int64_t>(key) * dim + c] = from_f<T>(acc * scale);
+  if (t > 0 && keys[t * tile] == key && keys[t * tile - 1] == key) return;  // begun before this tile
+  // tiles t + 1 .. end - 1 begin with the key
+  int64_t lo = t + 1, end = (n + tile - 1) / tile;  // lo does, end does not
+  while (end - lo > 1) {
+    const int64_t step = (end - lo + kWave - 1) / kWave;
+    const int64_t at = lo + (threadIdx.x & (kWave - 1)) * step;
+    const uint64_t with = __ballot(at < end && keys[min(at, end - 1) * tile] == key);
+    const int last = 63 - __builtin_clzll(with);  // lane 0's is
+    end = min(end, lo + (last + 1) * step);
+    lo += last * step;
+  }
+  const int group = threadIdx.x / LT;
+  for (int c0 = 0; c0 < dim; c0 += LT * V) {  // workgroup-uniform
+    const int c = c0 + (threadIdx.x % LT) * V, col = min(c, dim - V);
+    float acc[V];
+#pragma unroll
+    for (int u = 0; u < V; ++u) acc[u] = 0.f;
+    if (c < dim) {
+      if (group == 0) {
+        const Pack<float, V> x = load_pack<float, V>(part + (2 * t + 1) * dim + col);
+#pragma unroll
+        for (int u = 0; u < V; ++u) acc[u] = x.v[u];
+      }
+#pragma unroll 8
+      for (int64_t y = t + 1 + group; y < end; y += TILES) {
+        const Pack<float, V> x = load_pack<float, V>(part + 2 * y * dim + col);
+#pragma unroll
+        for (int u = 0; u < V; ++u) acc[u] += x.v[u];
+      }
+    }
+    if constexpr (TILES > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < V; ++u) lds[u * kEmbThreads + threadIdx.x] = acc[u];
+      __syncthreads();
+      if (group == 0)
+#pragma unroll
+        for (int u = 0; u < V; ++u)
+          for (int g = 1; g < TILES; ++g) acc[u] += lds[u * kEmbThreads + g * LT + threadIdx.x];
+    }
+    if (group == 0 && c < dim) {
+      Pack<T, V> y;
+#pragma unroll
+      for (int u = 0; u < V; ++u) y.v[u] = from_f<T>(acc[u] * scale);
+      store_pack<T, V>(grad + static_cast<int64_t>(key) * dim + col, y);
+    }
   }
 }
+
+// tokens per tile: short ones spread few tokens over the device, long ones leave fewer parts
+int tile_of(int64_t n) { return n <= (1 << 15) ? 16 : n <= (1 << 17) ? 32 : kMostTile; }
 
 int check_embed(const char* what, const void* a, const void* b, int64_t rows, int64_t dim, int32_t dtype,
                 const void* ids, int64_t n) {
@@ -143,7 +228,7 @@ struct EmbedWs {
     sums = o;
     o += radix.sums_bytes;
     part = o;
-    o += ops_align(static_cast<size_t>(ops_cdiv(n, kTile)) * 2 * static_cast<size_t>(dim) * 4);
+    o += ops_align(static_cast<size_t>(ops_cdiv(n, tile_of(n))) * 2 * static_cast<size_t>(dim) * 4);
     bytes = o;
   }
 };
@@ -200,10 +285,10 @@ extern "C" int tgx_embed_grad(const void* dout, const void* ids, int32_t ids_i32
   if (n == 0) return TGX_OK;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   uint32_t* k[2];
-  uint32_t* v[2];
+  uint32_t* v_[2];
   for (int j = 0; j < 2; ++j) {
     k[j] = reinterpret_cast<uint32_t*>(ws + w.keys[j]);
-    v[j] = reinterpret_cast<uint32_t*>(ws + w.tokens[j]);
+    v_[j] = reinterpret_cast<uint32_t*>(ws + w.tokens[j]);
   }
   const unsigned blocks = static_cast<unsigned>(ops_cdiv(n, kEmbThreads));
   if (ids_i32)
@@ -214,19 +299,32 @@ extern "C" int tgx_embed_grad(const void* dout, const void* ids, int32_t ids_i32
                        rows, k[0]);
   if ((rc = check_launch("embed_keys"))) return rc;
   int cur = 0;
-  if ((rc = radix_sort<uint32_t>(k, v, cur, n, key_bits(rows), w.radix, reinterpret_cast<uint32_t*>(ws + w.count),
+  if ((rc = radix_sort<uint32_t>(k, v_, cur, n, key_bits(rows), w.radix, reinterpret_cast<uint32_t*>(ws + w.count),
                                  reinterpret_cast<uint32_t*>(ws + w.sums), s, true)))
     return rc;
   float* part = reinterpret_cast<float*>(ws + w.part);
-  const unsigned tiles = static_cast<unsigned>(ops_cdiv(n, kTile));
+  const int tile = tile_of(n);
+  const int64_t tiles = ops_cdiv(n, tile);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL(embed_sum<T>, dim3(tiles), dim3(kEmbThreads), 0, s, k[cur], v[cur], n, rows,
-                       static_cast<int>(dim), static_cast<const T*>(dout), scale, static_cast<T*>(grad), part);
-    int e = check_launch("embed_sum");
-    if (e) return e;
-    hipLaunchKernelGGL(embed_join<T>, dim3(tiles), dim3(kEmbThreads), 0, s, k[cur], n, rows, static_cast<int>(dim),
-                       part, scale, static_cast<T*>(grad));
-    return check_launch("embed_join");
+    auto launch = [&](auto v, auto lt) {
+      constexpr int V = decltype(v)::value, LT = decltype(lt)::value;
+      hipLaunchKernelGGL((embed_sum<T, V, LT>), dim3(static_cast<unsigned>(ops_cdiv(tiles, kEmbThreads / LT))),
+                         dim3(kEmbThreads), 0, s, k[cur], v_[cur], n, rows, tile, static_cast<int>(dim),
+                         static_cast<const T*>(dout), scale, static_cast<T*>(grad), part);
+      const int e = check_launch("embed_sum");
+      if (e) return e;
+      hipLaunchKernelGGL((embed_join<T, V, LT>), dim3(static_cast<unsigned>(tiles)), dim3(kEmbThreads), 0, s, k[cur], n,
+                         rows, tile, static_cast<int>(dim), part, scale, static_cast<T*>(grad));
+      return check_launch("embed_join");
+    };
+#define TGX_LANES(V, LT) launch(std::integral_constant<int, V>{}, std::integral_constant<int, LT>{})
+    constexpr int W = kWide<T>;
+    if (dim < W) return TGX_LANES(1, 8);
+    if (dim <= 8 * W) return TGX_LANES(W, 8);
+    if (dim <= 16 * W) return TGX_LANES(W, 16);
+    if (dim <= 32 * W) return TGX_LANES(W, 32);
+    return TGX_LANES(W, 64);
+#undef TGX_LANES
   });
 }
