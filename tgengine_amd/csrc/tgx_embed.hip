@@ -20,37 +20,193 @@ __device__ __forceinline__ int64_t row_of(const I* __restrict__ ids, int64_t i, 
   return r >= 0 && r < rows ? r : -1;
 }
 
-// one thread per pack of V values, token-major
-template <typename T, int V, typename I>
+// LT lanes take a token's row, a pack of V values each (further packs in turns), and
+// kRowsAhead tokens at a time: their ids, then their rows, are in flight together.
+constexpr int kRowsAhead = 4;
+
+template <typename T, int V, int LT, typename I>
 __global__ __launch_bounds__(kEmbThreads) void embed_rows(const T* __restrict__ table, int64_t rows, int64_t stride,
-                                                          const I* __restrict__ ids, int64_t n, int dim, int packs,
-                                                          float scale, T* __restrict__ out) {
-  const int64_t total = n * packs;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kEmbThreads;
-  for (int64_t e = static_cast<int64_t>(blockIdx.x) * kEmbThreads + threadIdx.x; e < total; e += step) {
-    const int64_t i = e / packs;
-    const int c = min(static_cast<int>(e - i * packs) * V, dim - V);
-    const int64_t r = row_of(ids, i, rows);
-    Pack<T, V> x;
+                                                          const I* __restrict__ ids, int64_t n, int dim, float scale,
+                                                          T* __restrict__ out) {
+  constexpr int GROUPS = kEmbThreads / LT;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * GROUPS * kRowsAhead;
+  for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * GROUPS * kRowsAhead + threadIdx.x / LT; i0 < n; i0 += step) {
+    int64_t r[kRowsAhead];
 #pragma unroll
-    for (int u = 0; u < V; ++u) x.v[u] = from_f<T>(0.f);
-    if (r >= 0) {
-      x = load_pack<T, V>(table + r * stride + c);
+    for (int a = 0; a < kRowsAhead; ++a) r[a] = i0 + a * GROUPS < n ? row_of(ids, i0 + a * GROUPS, rows) : -1;
+    for (int c = (threadIdx.x % LT) * V; c < dim; c += LT * V) {
+      const int col = min(c, dim - V);
+      Pack<T, V> x[kRowsAhead];
 #pragma unroll
-      for (int u = 0; u < V; ++u) x.v[u] = from_f<T>(to_f(x.v[u]) * scale);
+      for (int a = 0; a < kRowsAhead; ++a) {
+#pragma unroll
+        for (int u = 0; u < V; ++u) x[a].v[u] = from_f<T>(0.f);
+        if (r[a] >= 0) x[a] = load_pack<T, V>(table + r[a] * stride + col);
+      }
+#pragma unroll
+      for (int a = 0; a < kRowsAhead; ++a) {
+        if (i0 + a * GROUPS >= n) break;
+        if (r[a] >= 0)
+#pragma unroll
+          for (int u = 0; u < V; ++u) x[a].v[u] = from_f<T>(to_f(x[a].v[u]) * scale);
+        store_pack<T, V>(out + (i0 + a * GROUPS) * dim + col, x[a]);
+      }
     }
-    store_pack<T, V>(out + i * dim + c, x);
   }
 }
 
-// sort keys: the row, or `rows` for an id outside the table
+// calls f(V, LT) with the pack and the lanes that rows of `dim` values take
+template <typename T, typename F>
+int by_row(int64_t dim, F&& f) {
+#define TGX_LANES(V, LT) f(std::integral_constant<int, V>{}, std::integral_constant<int, LT>{})
+  constexpr int W = kWide<T>;
+  if (dim < W) return TGX_LANES(1, 8);
+  if (dim <= 8 * W) return TGX_LANES(W, 8);
+  if (dim <= 16 * W) return TGX_LANES(W, 16);
+  if (dim <= 32 * W) return TGX_LANES(W, 32);
+  return TGX_LANES(W, 64);
+#undef TGX_LANES
+}
+
+// The sort's keys are the rows, and `rows` for an id outside the table.
+
+// Up to kSmallTokens tokens: workgroup 0 sorts them alone, each thread holding ITEMS keys
+// (a wave's lie beside each other) and LDS one array of them; the other workgroups write
+// the gradient's zeros meanwhile.  A pass ranks the keys of each wave by ballots, counts
+// digits per wave, and moves keys, then tokens, through the LDS array: one launch in
+// place of six.
+constexpr int kSmallThreads = 1024;
+constexpr int kSmallWaves = kSmallThreads / kWave;
+constexpr int kSmallItems = 8;  // 24 keys a thread do not fit the registers: 19,200 tokens took 601 us
+constexpr int kSmallBits = 9;  // of a pass
+constexpr int64_t kSmallTokens = int64_t(kSmallThreads) * kSmallItems;
+
+constexpr size_t small_lds(int items) {
+  return static_cast<size_t>(kSmallThreads) * items * 4 + kSmallWaves * (size_t(2) << kSmallBits);
+}
+
+template <int ITEMS, typename I>
+__global__ __launch_bounds__(kSmallThreads) void embed_small_sort(const I* __restrict__ ids, int n, int64_t rows,
+                                                                  int bits, uint32_t* __restrict__ keys,
+                                                                  uint32_t* __restrict__ tokens,
+                                                                  uint8_t* __restrict__ zero, int head, int64_t n16,
+                                                                  int tail) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ uint32_t wsum[kSmallWaves];
+  if (blockIdx.x > 0) {
+    const int64_t t = static_cast<int64_t>(blockIdx.x - 1) * kSmallThreads + threadIdx.x;
+    zero_bytes(zero, head, n16, tail, t, static_cast<int64_t>(gridDim.x - 1) * kSmallThreads);
+    return;
+  }
+  uint32_t* buf = reinterpret_cast<uint32_t*>(smem);
+  uint16_t* count = reinterpret_cast<uint16_t*>(smem + static_cast<size_t>(kSmallThreads) * ITEMS * 4);
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const uint64_t below_mask = (uint64_t(1) << lane) - 1;
+  const int i0 = wave * (kWave * ITEMS) + lane;
+  uint32_t k[ITEMS], v[ITEMS], rank[ITEMS];
+#pragma unroll
+  for (int r = 0; r < ITEMS; ++r) {
+    const int i = i0 + r * kWave;
+    const int64_t row = i < n ? row_of(ids, i, rows) : -1;
+    k[r] = static_cast<uint32_t>(row < 0 ? rows : row);
+    v[r] = static_cast<uint32_t>(i);
+  }
+  int passes = (bits + kSmallBits - 1) / kSmallBits;
+  for (int shift = 0; shift < bits; --passes) {  // workgroup-uniform
+    const int dbits = (bits - shift + passes - 1) / passes, bins = 1 << dbits;
+    uint16_t* mine = count + (wave << dbits);
+    for (int d = lane; d < bins; d += kWave) mine[d] = 0;
+    sort_wave_sync();
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {
+      const bool valid = i0 + r * kWave < n;
+      const int d = digit_of(k[r], shift, bins);
+      uint64_t peers = __ballot(valid);
+      for (int bit = 0; bit < dbits; ++bit) {
+        const bool on = d >> bit & 1;
+        const uint64_t m = __ballot(on);
+        peers &= on ? m : ~m;
+      }
+      const uint32_t before = valid ? mine[d] : 0u;
+      sort_wave_sync();  // every lane has read its counter
+      const uint32_t below = static_cast<uint32_t>(__popcll(peers & below_mask));
+      if (valid && below == 0) mine[d] = static_cast<uint16_t>(before + __popcll(peers));
+      sort_wave_sync();
+      rank[r] = before + below;
+    }
+    __syncthreads();
+    uint32_t sum = 0, all;
+    if (static_cast<int>(threadIdx.x) < bins)
+      for (int w = 0; w < kSmallWaves; ++w) sum += count[(w << dbits) + threadIdx.x];
+    uint32_t at = block_exclusive<kSmallThreads>(sum, wsum, all);
+    if (static_cast<int>(threadIdx.x) < bins)
+      for (int w = 0; w < kSmallWaves; ++w) {
+        const uint32_t c = count[(w << dbits) + threadIdx.x];
+        count[(w << dbits) + threadIdx.x] = static_cast<uint16_t>(at);
+        at += c;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r)
+      if (i0 + r * kWave < n) {
+        rank[r] += mine[digit_of(k[r], shift, bins)];
+        buf[rank[r]] = k[r];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r)
+      if (i0 + r * kWave < n) k[r] = buf[i0 + r * kWave];
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r)
+      if (i0 + r * kWave < n) buf[rank[r]] = v[r];
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r)
+      if (i0 + r * kWave < n) v[r] = buf[i0 + r * kWave];
+    __syncthreads();
+    shift += dbits;
+  }
+#pragma unroll
+  for (int r = 0; r < ITEMS; ++r)
+    if (i0 + r * kWave < n) {
+      keys[i0 + r * kWave] = k[r];
+      tokens[i0 + r * kWave] = v[r];
+    }
+}
+
+// More tokens: the first `ranges` workgroups write the keys and count the first pass's
+// digits as radix_hist does, the others write the gradient's zeros.
 template <typename I>
-__global__ __launch_bounds__(kEmbThreads) void embed_keys(const I* __restrict__ ids, int64_t n, int64_t rows,
-                                                          uint32_t* __restrict__ keys) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kEmbThreads + threadIdx.x;
-  if (i >= n) return;
-  const int64_t r = row_of(ids, i, rows);
-  keys[i] = static_cast<uint32_t>(r < 0 ? rows : r);
+__global__ __launch_bounds__(kSortThreads) void embed_keys(const I* __restrict__ ids, int64_t n, int64_t range,
+                                                           int64_t rows, int bins, int ranges,
+                                                           uint32_t* __restrict__ keys, uint32_t* __restrict__ count,
+                                                           uint8_t* __restrict__ zero, int head, int64_t n16,
+                                                           int tail) {
+  __shared__ uint32_t h[kMaxBins * kHistCopies];
+  if (static_cast<int>(blockIdx.x) >= ranges) {
+    const int64_t t = static_cast<int64_t>(blockIdx.x - ranges) * kSortThreads + threadIdx.x;
+    zero_bytes(zero, head, n16, tail, t, static_cast<int64_t>(gridDim.x - ranges) * kSortThreads);
+    return;
+  }
+  for (int i = threadIdx.x; i < bins * kHistCopies; i += kSortThreads) h[i] = 0;
+  __syncthreads();
+  const int64_t lo = blockIdx.x * range, hi = lo + range < n ? lo + range : n;
+  uint32_t* mine = h + (threadIdx.x & (kHistCopies - 1));
+#pragma unroll 4
+  for (int64_t i = lo + threadIdx.x; i < hi; i += kSortThreads) {
+    const int64_t r = row_of(ids, i, rows);
+    const uint32_t k = static_cast<uint32_t>(r < 0 ? rows : r);
+    keys[i] = k;
+    atomicAdd(&mine[digit_of(k, 0, bins) * kHistCopies], 1u);
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < bins; d += kSortThreads) {
+    uint32_t c = 0;
+#pragma unroll
+    for (int u = 0; u < kHistCopies; ++u) c += h[d * kHistCopies + u];
+    count[static_cast<int64_t>(d) * ranges + blockIdx.x] = c;
+  }
 }
 
 // A tile is `tile` consecutive sorted tokens, taken by LT lanes (one pack of V columns
@@ -60,7 +216,7 @@ __global__ __launch_bounds__(kEmbThreads) void embed_keys(const I* __restrict__ 
 // did not begin, part[2 t + 1] for one that begins in it and goes on after it.  A row's
 // last pack overlaps the one before: both lanes come to the same sums there.
 constexpr int kMostTile = 64;
-constexpr int kAhead = 8;  // rows of one lane that are read at a time
+constexpr int kAhead = 16;  // rows of one lane that are read at a time
 
 template <typename T, int V, int LT>
 __global__ __launch_bounds__(kEmbThreads) void embed_sum(const uint32_t* __restrict__ keys,
@@ -127,12 +283,14 @@ __global__ __launch_bounds__(kEmbThreads) void embed_sum(const uint32_t* __restr
 // One workgroup per tile in which a run begins that later tiles go on with: its parts,
 // every TILES-th of them summed by one group of lanes, then the groups' sums in order.
 // A hub's run crosses thousands of tiles; its end is searched 64 tiles a step.
+constexpr int kJoinThreads = 512;
+
 template <typename T, int V, int LT>
-__global__ __launch_bounds__(kEmbThreads) void embed_join(const uint32_t* __restrict__ keys, int64_t n, int64_t rows,
+__global__ __launch_bounds__(kJoinThreads) void embed_join(const uint32_t* __restrict__ keys, int64_t n, int64_t rows,
                                                           int tile, int dim, const float* __restrict__ part,
                                                           float scale, T* __restrict__ grad) {
-  constexpr int TILES = kEmbThreads / LT;
-  __shared__ float lds[TILES > 1 ? kEmbThreads * V : 1];
+  constexpr int TILES = kJoinThreads / LT;
+  __shared__ float lds[TILES > 1 ? kJoinThreads * V : 1];
   const int64_t t = blockIdx.x;
   const int64_t hi = (t + 1) * tile;
   if (hi >= n) return;
@@ -171,12 +329,12 @@ __global__ __launch_bounds__(kEmbThreads) void embed_join(const uint32_t* __rest
     if constexpr (TILES > 1) {
       __syncthreads();
 #pragma unroll
-      for (int u = 0; u < V; ++u) lds[u * kEmbThreads + threadIdx.x] = acc[u];
+      for (int u = 0; u < V; ++u) lds[u * kJoinThreads + threadIdx.x] = acc[u];
       __syncthreads();
       if (group == 0)
 #pragma unroll
         for (int u = 0; u < V; ++u)
-          for (int g = 1; g < TILES; ++g) acc[u] += lds[u * kEmbThreads + g * LT + threadIdx.x];
+          for (int g = 1; g < TILES; ++g) acc[u] += lds[u * kJoinThreads + g * LT + threadIdx.x];
     }
     if (group == 0 && c < dim) {
       Pack<T, V> y;
@@ -233,6 +391,69 @@ struct EmbedWs {
   }
 };
 
+// Ranges whose counts each workgroup of the sort's scatter adds up itself: a launch less
+// for every pass
+constexpr int kRawRanges = 32;
+
+// the tokens of `ids` in the stable order of their rows: keys in k[cur], tokens in
+// v[cur]; the gradient's zeros are written on the way
+template <typename I>
+int sort_tokens(const I* ids, int64_t n, int64_t rows, const EmbedWs& w, const ZeroSpan& z, uint8_t* ws,
+                uint32_t* k[2], uint32_t* v[2], int& cur, hipStream_t s) {
+  const int bits = key_bits(rows);
+  if (n <= kSmallTokens) {
+    const unsigned blocks = 1 + static_cast<unsigned>(std::clamp<int64_t>(ops_cdiv(z.n16, 4 * kSmallThreads), 1, 512));
+    auto go = [&](auto items) {
+      constexpr int ITEMS = decltype(items)::value;
+      static const hipError_t allowed =
+          hipFuncSetAttribute(reinterpret_cast<const void*>(&embed_small_sort<ITEMS, I>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(small_lds(ITEMS)));
+      (void)allowed;  // a launch that needs it says so
+      hipLaunchKernelGGL((embed_small_sort<ITEMS, I>), dim3(blocks), dim3(kSmallThreads), small_lds(ITEMS), s, ids,
+                         static_cast<int>(n), rows, bits, k[0], v[0], z.p, z.head, z.n16, z.tail);
+      return check_launch("embed_small_sort");
+    };
+    cur = 0;
+    if (n <= 2 * kSmallThreads) return go(std::integral_constant<int, 2>{});
+    return go(std::integral_constant<int, kSmallItems>{});
+  }
+  uint32_t* count = reinterpret_cast<uint32_t*>(ws + w.count);
+  uint32_t* sums = reinterpret_cast<uint32_t*>(ws + w.sums);
+  const int passes = static_cast<int>(cdiv(bits, kMaxDigitBits)), dbits = static_cast<int>(cdiv(bits, passes));
+  const int ranges = static_cast<int>(w.radix.nblocks);
+  const unsigned blocks = static_cast<unsigned>(ranges + std::clamp<int64_t>(ops_cdiv(z.n16, 4 * kSortThreads), 1, 2048));
+  hipLaunchKernelGGL(embed_keys<I>, dim3(blocks), dim3(kSortThreads), 0, s, ids, n, w.radix.range, rows, 1 << dbits,
+                     ranges, k[0], count, z.p, z.head, z.n16, z.tail);
+  int rc = check_launch("embed_keys");
+  if (rc) return rc;
+  cur = 0;
+  for (int shift = 0, left = passes; rc == TGX_OK && shift < bits; --left) {
+    const int d = static_cast<int>(cdiv(bits - shift, left));
+    const uint32_t* vin = shift == 0 ? nullptr : v[cur];  // the tokens in order at first
+    if (shift > 0 || ranges > kRawRanges) {
+      if (shift == 0) {
+        hipLaunchKernelGGL(radix_rows, dim3(1u << d), dim3(kThreads), 0, s, count, ranges, sums);
+        if ((rc = check_launch("radix_rows"))) return rc;
+        rc = w.radix.items == 4
+                 ? radix_scatter_launch<uint32_t, 4>(k[0], vin, k[1], v[1], n, 0, d, w.radix, count, sums, s)
+                 : radix_scatter_launch<uint32_t, 8>(k[0], vin, k[1], v[1], n, 0, d, w.radix, count, sums, s);
+      } else if (ranges > kRawRanges) {
+        rc = radix_pass<uint32_t>(k[cur], vin, k[1 - cur], v[1 - cur], n, shift, d, w.radix, count, sums, s);
+      } else {
+        hipLaunchKernelGGL(radix_hist<uint32_t>, dim3(ranges), dim3(kSortThreads), (size_t(4) << d) * kHistCopies, s,
+                           k[cur], n, w.radix.range, shift, 1 << d, count);
+        if ((rc = check_launch("radix_hist"))) return rc;
+      }
+    }
+    if (ranges <= kRawRanges)
+      rc = radix_scatter_launch<uint32_t, 4, true>(k[cur], vin, k[1 - cur], v[1 - cur], n, shift, d, w.radix, count,
+                                                   sums, s);
+    cur = 1 - cur;
+    shift += d;
+  }
+  return rc;
+}
+
 }  // namespace
 }  // namespace tgx
 
@@ -247,21 +468,18 @@ extern "C" int tgx_embed(const void* table, int64_t rows, int64_t dim, int64_t s
   if (n == 0) return TGX_OK;
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    auto launch = [&](auto i, auto v) {
-      using I = decltype(i);
-      constexpr int V = decltype(v)::value;
-      const int packs = static_cast<int>(ops_cdiv(dim, V));
-      const int64_t blocks = std::min<int64_t>(ops_cdiv(n * packs, kEmbThreads), 1 << 20);
-      hipLaunchKernelGGL((embed_rows<T, V, I>), dim3(static_cast<unsigned>(blocks)), dim3(kEmbThreads), 0,
-                         static_cast<hipStream_t>(stream), static_cast<const T*>(table), rows, stride,
-                         static_cast<const I*>(ids), n, static_cast<int>(dim), packs, scale, static_cast<T*>(out));
-      return check_launch("embed_rows");
-    };
-    auto wide = [&](auto i) {
-      if (dim >= kWide<T>) return launch(i, std::integral_constant<int, kWide<T>>{});
-      return launch(i, std::integral_constant<int, 1>{});
-    };
-    return ids_i32 ? wide(int32_t{}) : wide(int64_t{});
+    return by_row<T>(dim, [&](auto v, auto lt) {
+      constexpr int V = decltype(v)::value, LT = decltype(lt)::value;
+      const int64_t blocks = std::min<int64_t>(ops_cdiv(n, kEmbThreads / LT * kRowsAhead), 1 << 20);
+      auto launch = [&](auto i) {
+        using I = decltype(i);
+        hipLaunchKernelGGL((embed_rows<T, V, LT, I>), dim3(static_cast<unsigned>(blocks)), dim3(kEmbThreads), 0,
+                           static_cast<hipStream_t>(stream), static_cast<const T*>(table), rows, stride,
+                           static_cast<const I*>(ids), n, static_cast<int>(dim), scale, static_cast<T*>(out));
+        return check_launch("embed_rows");
+      };
+      return ids_i32 ? launch(int32_t{}) : launch(int64_t{});
+    });
   });
 }
 
@@ -281,8 +499,8 @@ extern "C" int tgx_embed_grad(const void* dout, const void* ids, int32_t ids_i32
   const EmbedWs w(n, dim);
   if (n > 0 && (workspace == nullptr || workspace_bytes < w.bytes || !aligned16(workspace)))
     return fail(TGX_ERR_ARG, "tgx_embed_grad: workspace of %zu bytes, 16-byte aligned, needed", w.bytes);
-  if ((rc = fill_zero(grad, static_cast<size_t>(rows) * dim * elem_bytes(dtype), s))) return rc;
-  if (n == 0) return TGX_OK;
+  const ZeroSpan z(grad, static_cast<size_t>(rows) * dim * elem_bytes(dtype));
+  if (n == 0) return fill_zero(grad, z.bytes, s);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   uint32_t* k[2];
   uint32_t* v_[2];
@@ -290,18 +508,10 @@ extern "C" int tgx_embed_grad(const void* dout, const void* ids, int32_t ids_i32
     k[j] = reinterpret_cast<uint32_t*>(ws + w.keys[j]);
     v_[j] = reinterpret_cast<uint32_t*>(ws + w.tokens[j]);
   }
-  const unsigned blocks = static_cast<unsigned>(ops_cdiv(n, kEmbThreads));
-  if (ids_i32)
-    hipLaunchKernelGGL(embed_keys<int32_t>, dim3(blocks), dim3(kEmbThreads), 0, s, static_cast<const int32_t*>(ids), n,
-                       rows, k[0]);
-  else
-    hipLaunchKernelGGL(embed_keys<int64_t>, dim3(blocks), dim3(kEmbThreads), 0, s, static_cast<const int64_t*>(ids), n,
-                       rows, k[0]);
-  if ((rc = check_launch("embed_keys"))) return rc;
   int cur = 0;
-  if ((rc = radix_sort<uint32_t>(k, v_, cur, n, key_bits(rows), w.radix, reinterpret_cast<uint32_t*>(ws + w.count),
-                                 reinterpret_cast<uint32_t*>(ws + w.sums), s, true)))
-    return rc;
+  rc = ids_i32 ? sort_tokens(static_cast<const int32_t*>(ids), n, rows, w, z, ws, k, v_, cur, s)
+               : sort_tokens(static_cast<const int64_t*>(ids), n, rows, w, z, ws, k, v_, cur, s);
+  if (rc) return rc;
   float* part = reinterpret_cast<float*>(ws + w.part);
   const int tile = tile_of(n);
   const int64_t tiles = ops_cdiv(n, tile);
@@ -314,17 +524,10 @@ extern "C" int tgx_embed_grad(const void* dout, const void* ids, int32_t ids_i32
                          static_cast<const T*>(dout), scale, static_cast<T*>(grad), part);
       const int e = check_launch("embed_sum");
       if (e) return e;
-      hipLaunchKernelGGL((embed_join<T, V, LT>), dim3(static_cast<unsigned>(tiles)), dim3(kEmbThreads), 0, s, k[cur], n,
+      hipLaunchKernelGGL((embed_join<T, V, LT>), dim3(static_cast<unsigned>(tiles)), dim3(kJoinThreads), 0, s, k[cur], n,
                          rows, tile, static_cast<int>(dim), part, scale, static_cast<T*>(grad));
       return check_launch("embed_join");
     };
-#define TGX_LANES(V, LT) launch(std::integral_constant<int, V>{}, std::integral_constant<int, LT>{})
-    constexpr int W = kWide<T>;
-    if (dim < W) return TGX_LANES(1, 8);
-    if (dim <= 8 * W) return TGX_LANES(W, 8);
-    if (dim <= 16 * W) return TGX_LANES(W, 16);
-    if (dim <= 32 * W) return TGX_LANES(W, 32);
-    return TGX_LANES(W, 64);
-#undef TGX_LANES
+    return by_row<T>(dim, launch);
   });
 }

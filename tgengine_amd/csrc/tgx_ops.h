@@ -54,24 +54,39 @@ __device__ __forceinline__ float group_sum(float x) {  // over groups of L <= 64
   return x;
 }
 
-// the bytes before and after the 16-byte steps of an array are written one by one
-__global__ __launch_bounds__(256) void zero_kernel(uint8_t* __restrict__ p, int head, int64_t n16, int tail) {
-  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+// thread t of `step` writes its share of an array's zeros: 16 bytes at a time, the bytes
+// before and after the 16-byte steps one by one
+__device__ __forceinline__ void zero_bytes(uint8_t* __restrict__ p, int head, int64_t n16, int tail, int64_t t,
+                                           int64_t step) {
   uint4* body = reinterpret_cast<uint4*>(p + head);
   for (int64_t i = t; i < n16; i += step) body[i] = make_uint4(0, 0, 0, 0);
   if (t < head) p[t] = 0;
   if (t < tail) p[head + n16 * 16 + t] = 0;
 }
 
+struct ZeroSpan {
+  uint8_t* p;
+  size_t bytes;
+  int head, tail;
+  int64_t n16;
+  ZeroSpan(void* to, size_t n) : p(static_cast<uint8_t*>(to)), bytes(n) {
+    head = static_cast<int>(std::min(bytes, static_cast<size_t>(-addr(p) & 15)));
+    n16 = static_cast<int64_t>((bytes - head) / 16);
+    tail = static_cast<int>((bytes - head) % 16);
+  }
+};
+
+__global__ __launch_bounds__(256) void zero_kernel(uint8_t* __restrict__ p, int head, int64_t n16, int tail) {
+  zero_bytes(p, head, n16, tail, static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x,
+             static_cast<int64_t>(gridDim.x) * 256);
+}
+
 // a kernel, not a memset: callers may capture the call in a graph
 inline int fill_zero(void* p, size_t bytes, hipStream_t s) {
   if (bytes == 0) return TGX_OK;
-  const size_t head = std::min(bytes, static_cast<size_t>(-addr(p) & 15));
-  const int64_t n16 = static_cast<int64_t>((bytes - head) / 16);
-  const int64_t blocks = std::clamp<int64_t>(ops_cdiv(n16, 256), 1, 8192);
-  hipLaunchKernelGGL(zero_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, static_cast<uint8_t*>(p),
-                     static_cast<int>(head), n16, static_cast<int>((bytes - head) % 16));
+  const ZeroSpan z(p, bytes);
+  const int64_t blocks = std::clamp<int64_t>(ops_cdiv(z.n16, 256), 1, 8192);
+  hipLaunchKernelGGL(zero_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, z.p, z.head, z.n16, z.tail);
   return check_launch("zero_kernel");
 }
 

@@ -11,6 +11,8 @@
 //             queue at eight counters instead of one;
 //   rows    : one workgroup per digit scans its row of counts, so count[d][b] is
 //             range b's place among digit d's keys, and total[d] their number;
+//             A sort of few ranges may leave this launch out: its scatter (RAW)
+//             sums the rows of counts itself;
 //   scatter : a workgroup scans the totals and then takes its range tile by
 //             tile.  Each wavefront ranks its consecutive part of the tile on its
 //             own, 64 keys at a time: lanes with equal digits find each other
@@ -143,7 +145,7 @@ constexpr size_t scatter_lds(size_t key_bytes, int items, int bins) {
   return static_cast<size_t>(kSortThreads) * items * key_bytes + static_cast<size_t>(bins) * (2 * kSortWaves + 8);
 }
 
-template <typename K, int ITEMS>
+template <typename K, int ITEMS, bool RAW>
 __global__ __launch_bounds__(kSortThreads) __attribute__((amdgpu_waves_per_eu(4))) void radix_scatter(const K* __restrict__ kin,
                                                               const uint32_t* __restrict__ vin, K* __restrict__ kout,
                                                               uint32_t* __restrict__ vout, int64_t n, int64_t range,
@@ -164,15 +166,31 @@ __global__ __launch_bounds__(kSortThreads) __attribute__((amdgpu_waves_per_eu(4)
   const uint64_t lt = (uint64_t(1) << lane) - 1;
   const int d0 = static_cast<int>(threadIdx.x) * 2;  // this thread's digits in the prefix steps: d0, d0 + 1
   {
-    uint32_t t0 = 0, t1 = 0, all;
+    uint32_t t0 = 0, t1 = 0, p0 = 0, p1 = 0, all;
     if (d0 < bins) {
-      t0 = total[d0];
-      t1 = total[d0 + 1];
+      const uint32_t* row = count + static_cast<int64_t>(d0) * gridDim.x;
+      if constexpr (RAW) {
+#pragma unroll 8
+        for (uint32_t b = 0; b < gridDim.x; ++b) {
+          const uint32_t x = row[b], y = row[gridDim.x + b];
+          if (b < blockIdx.x) {
+            p0 += x;
+            p1 += y;
+          }
+          t0 += x;
+          t1 += y;
+        }
+      } else {
+        t0 = total[d0];
+        t1 = total[d0 + 1];
+        p0 = row[blockIdx.x];
+        p1 = row[gridDim.x + blockIdx.x];
+      }
     }
     const uint32_t at = block_exclusive<kSortThreads>(t0 + t1, wsum, all);
     if (d0 < bins) {
-      gpos[d0] = at + count[static_cast<int64_t>(d0) * gridDim.x + blockIdx.x];
-      gpos[d0 + 1] = at + t0 + count[static_cast<int64_t>(d0 + 1) * gridDim.x + blockIdx.x];
+      gpos[d0] = at + p0;
+      gpos[d0 + 1] = at + t0 + p1;
     }
   }
   uint16_t* mycnt = wcnt + wv * bins;
@@ -307,10 +325,10 @@ RadixScratch radix_scratch(int64_t n) {
   return r;
 }
 
-template <typename K, int ITEMS>
+template <typename K, int ITEMS, bool RAW = false>
 int radix_scatter_launch(const K* kin, const uint32_t* vin, K* kout, uint32_t* vout, int64_t n, int shift, int dbits,
                          const RadixScratch& w, const uint32_t* count, const uint32_t* total, hipStream_t stream) {
-  hipLaunchKernelGGL((radix_scatter<K, ITEMS>), dim3(static_cast<unsigned>(w.nblocks)), dim3(kSortThreads),
+  hipLaunchKernelGGL((radix_scatter<K, ITEMS, RAW>), dim3(static_cast<unsigned>(w.nblocks)), dim3(kSortThreads),
                      scatter_lds(sizeof(K), ITEMS, 1 << dbits), stream, kin, vin, kout, vout, n, w.range, shift, dbits,
                      count, total);
   return check_launch("radix_scatter");
