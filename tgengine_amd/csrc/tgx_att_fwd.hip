@@ -3,7 +3,7 @@
 // A wave owns 32 rows of a problem and keeps their queries as fragments.  A tile of
 // keys gives S^T = K Q^T (keys down a lane's registers, one row a lane), so that the
 // running maximum and sum of the softmax are a lane's own but for one exchange between
-// the wave's halves, and P^T, still in the same registers, is the second operand of
+// the wave's halves now and then, and P^T, still in the same registers, is the second operand of
 // O^T += V^T P^T.  Scores are in units of log 2.  Probabilities are rounded to the
 // inputs' type for that product, as the matrix units take them; sums stay in 32 bits.
 #include "tgx_attention.h"
@@ -19,11 +19,11 @@ constexpr int kKeys = (sizeof(T) == 2 || WK == 2) ? 64 : 32;
 // over half of each tile's keys and are joined at the end.  With splits > 1 the keys are
 // cut in as many ranges of `span` keys and each leaves its maximum, sum and unscaled
 // output in `part` for att_join.
-template <typename T, int DP, int WQ, int WK>
+template <typename T, bool TINY, int DP, int WQ, int WK>
 __global__ __launch_bounds__(64 * WQ * WK, DP > 128 ? 1 : 2) void att_mma_fwd(const AttArgs a, int mtiles, int splits,
                                                                              int64_t span, float* __restrict__ part) {
   constexpr int NT = 64 * WQ * WK, KT = kKeys<T, WK>, SUB = KT / 32 / WK, V = kWide<T>;
-  constexpr int KS = DP + 16 / static_cast<int>(sizeof(T)), VS = DP + 16 / static_cast<int>(sizeof(T));
+  constexpr int KS = DP + 16 / static_cast<int>(sizeof(T)), VS = DP + (sizeof(T) == 2 ? 16 : 4);
   __shared__ __align__(16) T smem[KT * (KS + VS)];
   T* sk = smem;
   T* sv = smem + KT * KS;
@@ -42,72 +42,82 @@ __global__ __launch_bounds__(64 * WQ * WK, DP > 128 ? 1 : 2) void att_mma_fwd(co
   const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[2];
   const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[2];
   u32x4 qf[DP / kStep<T>];
-  row_frags<T, DP>(qf, r < rows ? static_cast<const T*>(a.q) + b * a.qs[0] + tok * a.qs[1] + head * a.qs[2] : nullptr,
+  row_frags<T, TINY, DP>(qf, r < rows ? static_cast<const T*>(a.q) + b * a.qs[0] + tok * a.qs[1] + head * a.qs[2] : nullptr,
                    a.dim);
-  const float c = a.scale * kLog2e;
+  // Scores are in units of 1 / c: the sign of the scale goes to the queries, so that the
+  // largest score is the largest product, and a scale of zero makes them zero.
+  const float c = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
+  if (!(a.scale > 0.f))
+#pragma unroll
+    for (int e = 0; e < DP / kStep<T>; ++e)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        qf[e][u] = a.scale == 0.f ? 0u : qf[e][u] ^ (sizeof(T) == 2 ? 0x80008000u : 0x80000000u);
   f32x16 o[DP / 32];
 #pragma unroll
   for (int t = 0; t < DP / 32; ++t) o[t] = f32x16{};
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, from = 0.f, l = 0.f;  // from: m, or 0 as long as no key was kept
 
   const int64_t lo = sp * span, hi = lo + span < a.lk ? lo + span : a.lk;
   Keys<KT> keys(a.mask == nullptr ? nullptr : a.mask + b * a.mask_stride, lo, hi);
   int64_t key;
   uint64_t bits;
   bool more = keys.next(key, bits);
-  Stage<T, KT, DP, NT, KS> st;
+  Stage<T, TINY, KT, DP, NT, KS> sk_(a.dim);
+  Stage<T, TINY, KT, DP, NT, VS> sv_(a.dim);
   if (more) {
-    st.load(a.dim, [&](int row) { return bits >> row & 1 ? kp + (key + row) * a.ks[1] : nullptr; });
-    st.store(sk, a.dim);
+    sk_.load(kp + key * a.ks[1], a.ks[1], bits, a.dim);
+    sk_.store(sk, a.dim);
   }
   __syncthreads();
   while (more) {  // workgroup-uniform
-    st.load(a.dim, [&](int row) { return bits >> row & 1 ? vp + (key + row) * a.vs[1] : nullptr; });
+    sv_.load(vp + key * a.vs[1], a.vs[1], bits, a.dim);
     f32x16 s[SUB];
-    float top = m;
+    float top = -INFINITY;
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
       const int row0 = (wk * SUB + u) * 32;
       s[u] = f32x16{};
 #pragma unroll
       for (int e = 0; e < DP / kStep<T>; ++e)
-        if (e * kStep<T> < a.dim)
-          s[u] = mma<T>(s[u], *reinterpret_cast<const u32x4*>(sk + (row0 + (lane & 31)) * KS + e * kStep<T> + h * V),
-                        qf[e]);
-      const uint32_t kept = static_cast<uint32_t>(bits >> row0) >> (4 * h);
+        s[u] = mma<T>(s[u], *reinterpret_cast<const u32x4*>(sk + (row0 + (lane & 31)) * KS + e * kStep<T> + h * V),
+                      qf[e]);
+      if (static_cast<uint32_t>(bits >> row0) != ~0u) {
+        const uint32_t kept = static_cast<uint32_t>(bits >> row0) >> (4 * h);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[u][i] = kept >> mma_row(i, 0) & 1 ? s[u][i] * c : -INFINITY;
-        top = fmaxf(top, s[u][i]);
+        for (int i = 0; i < 16; ++i) s[u][i] = kept >> mma_row(i, 0) & 1 ? s[u][i] : -INFINITY;
       }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
     }
-    top = fmaxf(top, __shfl_xor(top, 32, kWave));
-    const float at = top == -INFINITY ? 0.f : top;
-    if (__any(top > m)) {
-      const float old = exp2_(m - at);
+    // The running maximum moves only when it is passed by more than 8: probabilities of up
+    // to 2^8 cost no accuracy, and most tiles neither exchange maxima nor scale the sums.
+    if (__any(top * c > m + 8.f)) {
+      const float now = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, kWave)) * c);
+      const float old = now == -INFINITY ? 1.f : exp2_(m - now);
       l *= old;
 #pragma unroll
       for (int t = 0; t < DP / 32; ++t) o[t] *= old;
-      m = top;
+      m = now;
+      from = now == -INFINITY ? 0.f : now;
     }
     u32x4 pf[SUB][16 / V];
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[u][i] = exp2_(s[u][i] - at);
+        s[u][i] = exp2_(fmaf(s[u][i], c, -from));
         l += s[u][i];
       }
 #pragma unroll
       for (int f = 0; f < 16 / V; ++f) pf[u][f] = to_frag<T>(s[u], f);
     }
-    st.store(sv, a.dim);
+    sv_.store(sv, a.dim);
     more = keys.next(key, bits);
-    if (more) st.load(a.dim, [&](int row) { return bits >> row & 1 ? kp + (key + row) * a.ks[1] : nullptr; });
+    if (more) sk_.load(kp + key * a.ks[1], a.ks[1], bits, a.dim);
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) {
-      if (t * 32 >= a.dim) break;
 #pragma unroll
       for (int u = 0; u < SUB; ++u)
 #pragma unroll
@@ -115,7 +125,7 @@ __global__ __launch_bounds__(64 * WQ * WK, DP > 128 ? 1 : 2) void att_mma_fwd(co
           o[t] = mma<T>(o[t], transposed(sv, VS, (wk * SUB + u) * 32, f, t * 32), pf[u][f]);
     }
     if (more) {
-      st.store(sk, a.dim);
+      sk_.store(sk, a.dim);
       __syncthreads();
     }
   }
@@ -241,17 +251,18 @@ int att_mma_forward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
   const FwdShape f(a, dtype);
   float* part = static_cast<float*>(ws);
   const int64_t blocks = a.batch * a.kv_heads * f.mtiles * f.splits;
-  int rc = by_head(dtype, a.dim, [&](auto t, auto dp) {
+  int rc = by_head(dtype, a.dim, [&](auto t, auto dp, auto tiny) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
+    constexpr bool TINY = decltype(tiny)::value;
     const dim3 grid(static_cast<unsigned>(blocks));
     if (f.wk == 2) {
       if constexpr (sizeof(T) == 2 || DP <= 128)
-        hipLaunchKernelGGL((att_mma_fwd<T, DP, 1, 2>), grid, dim3(128), 0, s, a, f.mtiles, f.splits, f.span, part);
+        hipLaunchKernelGGL((att_mma_fwd<T, TINY, DP, 1, 2>), grid, dim3(128), 0, s, a, f.mtiles, f.splits, f.span, part);
     } else if (f.wq == 2) {
-      hipLaunchKernelGGL((att_mma_fwd<T, DP, 2, 1>), grid, dim3(128), 0, s, a, f.mtiles, f.splits, f.span, part);
+      hipLaunchKernelGGL((att_mma_fwd<T, TINY, DP, 2, 1>), grid, dim3(128), 0, s, a, f.mtiles, f.splits, f.span, part);
     } else {
-      hipLaunchKernelGGL((att_mma_fwd<T, DP, 4, 1>), grid, dim3(256), 0, s, a, f.mtiles, f.splits, f.span, part);
+      hipLaunchKernelGGL((att_mma_fwd<T, TINY, DP, 4, 1>), grid, dim3(256), 0, s, a, f.mtiles, f.splits, f.span, part);
     }
     return check_launch("att_mma_fwd");
   });

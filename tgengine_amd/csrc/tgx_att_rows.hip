@@ -32,7 +32,7 @@ struct Lanes {
   __device__ __forceinline__ void values(float (&f)[C * V], const u32x4 (&x)[C]) const {
 #pragma unroll
     for (int j = 0; j < C; ++j) {
-      const Pack<T, V> p = __builtin_bit_cast(Pack<T, V>, finish<T>(x[j], col(j), dim));
+      const Pack<T, V> p = __builtin_bit_cast(Pack<T, V>, dim < V ? x[j] : finish<T>(x[j], col(j), dim));
 #pragma unroll
       for (int u = 0; u < V; ++u) f[j * V + u] = to_f(p.v[u]);
     }

@@ -41,6 +41,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -75,10 +77,15 @@ __device__ __forceinline__ constexpr int mma_row(int i, int h) { return 8 * (i /
 // over their rows: no lane gives a value to another.
 template <typename T>
 __device__ __forceinline__ u32x4 to_frag(const f32x16& x, int f) {
-  Pack<T, kWide<T>> p;
+  u32x4 y;
 #pragma unroll
-  for (int u = 0; u < kWide<T>; ++u) p.v[u] = from_f<T>(x[f * kWide<T> + u]);
-  return __builtin_bit_cast(u32x4, p);
+  for (int u = 0; u < 4; ++u) {
+    if constexpr (sizeof(T) == 2)  // two values at a time: one conversion
+      y[u] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x[f * 8 + 2 * u], x[f * 8 + 2 * u + 1]}), bf16x2));
+    else
+      y[u] = __float_as_uint(x[f * 4 + u]);
+  }
+  return y;
 }
 
 // The first operand that goes with it: 32 columns from `col` on of rows of an LDS tile,
@@ -109,72 +116,109 @@ __device__ __forceinline__ u32x4 load16(const T* p) {
 }
 
 // V values of a row of `dim` from column c on as they are in memory: the row's last V
-// values where fewer than V are left (finish() moves them), one by one where the row has
-// fewer than V
-template <typename T>
+// values where fewer than V are left (finish() moves them).  TINY: rows of fewer than V
+// values, read one by one.
+template <typename T, bool TINY>
 __device__ __forceinline__ u32x4 row_part(const T* row, int c, int dim) {
   constexpr int V = kWide<T>;
-  u32x4 x = {0, 0, 0, 0};
-  if (dim >= V) {
-    x = load16(row + min(c, dim - V));
-  } else {
-    Pack<T, V> p = __builtin_bit_cast(Pack<T, V>, x);
+  if constexpr (TINY) {
+    Pack<T, V> p = {};
     for (int u = 0; u < V; ++u)
       if (c + u < dim) p.v[u] = row[c + u];
-    x = __builtin_bit_cast(u32x4, p);
+    return __builtin_bit_cast(u32x4, p);
+  } else {
+    return load16(row + min(c, dim - V));
   }
-  return x;
+}
+template <typename T>
+__device__ __forceinline__ u32x4 row_part(const T* row, int c, int dim) {
+  return dim < kWide<T> ? row_part<T, true>(row, c, dim) : row_part<T, false>(row, c, dim);
 }
 
-// row_part's values in their places, zeros after the row's end
+// row_part's values in their places, zeros after the row's end (rows of at least V values)
 template <typename T>
 __device__ __forceinline__ u32x4 finish(u32x4 x, int c, int dim) {
   constexpr int V = kWide<T>;
   const int over = c + V - dim;
-  if (over <= 0 || dim < V) return x;
-  if (over >= V) return u32x4{0, 0, 0, 0};
+  if (over <= 0 || over >= V) return x;  // whole, or zeros already
   const unsigned __int128 w = __builtin_bit_cast(unsigned __int128, x) >> (over * 8 * static_cast<int>(sizeof(T)));
   return __builtin_bit_cast(u32x4, w);
 }
 
+// both at once
+template <typename T>
+__device__ __forceinline__ u32x4 row_values(const T* row, int c, int dim) {
+  return dim < kWide<T> ? row_part<T, true>(row, c, dim) : finish<T>(row_part<T, false>(row, c, dim), c, dim);
+}
+
+constexpr int pow2_at_least(int x) {
+  int p = 1;
+  while (p < x) p *= 2;
+  return p;
+}
+
 // NT threads move ROWS rows of up to DP values into an LDS tile of rows STRIDE apart:
-// load() issues the reads, store() waits for them and writes.  at(row) gives a row's
-// address, or nullptr for zeros.
-template <typename T, int ROWS, int DP, int NT, int STRIDE>
+// load() issues the reads, store() waits for them and writes.  A thread keeps one column
+// of all its rows, so that a row costs it one address step; lanes past the last column
+// stay idle.
+template <typename T, bool TINY, int ROWS, int DP, int NT, int STRIDE>
 struct Stage {
-  static constexpr int V = kWide<T>, PER = DP / V, N = (ROWS * PER + NT - 1) / NT;
+  static constexpr int V = kWide<T>, LANES = pow2_at_least(DP / V), STEP = NT / LANES,
+                       N = (ROWS + STEP - 1) / STEP;
+  static_assert(N * STEP == ROWS || N == 1, "whole steps");
   u32x4 x[N];
+  int col, row0;
+  bool in;
+  __device__ explicit Stage(int dim) : col(threadIdx.x % LANES * V), row0(threadIdx.x / LANES) {
+    in = col < dim && row0 < ROWS;
+  }
+  // rows base, base + stride, ...: those whose bit is set, zeros for the others
+  __device__ __forceinline__ void load(const T* base, int64_t stride, uint64_t bits, int dim) {
+    const T* p = base + row0 * stride;
+    const uint64_t mine = in ? bits >> row0 : 0;
+#pragma unroll
+    for (int n = 0; n < N; ++n, p += STEP * stride) {
+      x[n] = u32x4{0, 0, 0, 0};
+      if (mine >> (n * STEP) & 1) x[n] = row_part<T, TINY>(p, col, dim);
+    }
+  }
+  // the rows that p(n) gives the addresses of, nullptr for zeros
   template <typename At>
-  __device__ __forceinline__ void load(int dim, At&& at) {
+  __device__ __forceinline__ void load(int dim, At&& p) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int e = threadIdx.x + n * NT, row = e / PER, c = e % PER * V;
       x[n] = u32x4{0, 0, 0, 0};
-      if (ROWS * PER % NT != 0 && e >= ROWS * PER) continue;
-      const T* p = at(row);
-      if (p != nullptr && c < dim) x[n] = row_part(p, c, dim);
+      const T* row = p(n);
+      if (in && row != nullptr) x[n] = row_part<T, TINY>(row, col, dim);
     }
   }
   __device__ __forceinline__ void store(T* tile, int dim) const {
+    if (LANES * V > DP && col >= DP) return;
+    if (STEP > ROWS && row0 >= ROWS) return;
+    T* p = tile + row0 * STRIDE + col;
+    if (TINY || dim % V == 0) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int e = threadIdx.x + n * NT, row = e / PER, c = e % PER * V;
-      if (ROWS * PER % NT != 0 && e >= ROWS * PER) continue;
-      *reinterpret_cast<u32x4*>(tile + row * STRIDE + c) = finish<T>(x[n], c, dim);
+      for (int n = 0; n < N; ++n) *reinterpret_cast<u32x4*>(p + n * STEP * STRIDE) = x[n];
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n) *reinterpret_cast<u32x4*>(p + n * STEP * STRIDE) = finish<T>(x[n], col, dim);
     }
   }
 };
 
 // The fragments of one row a lane (row l % 32), from global memory; nullptr gives zeros
-template <typename T, int DP>
+template <typename T, bool TINY, int DP>
 __device__ __forceinline__ void row_frags(u32x4 (&x)[DP / kStep<T>], const T* row, int dim) {
   const int h = (threadIdx.x & (kWave - 1)) / 32;
 #pragma unroll
   for (int s = 0; s < DP / kStep<T>; ++s) {
     const int c = s * kStep<T> + h * kWide<T>;
     x[s] = u32x4{0, 0, 0, 0};
-    if (row != nullptr && c < dim) x[s] = finish<T>(row_part(row, c, dim), c, dim);
+    if (row != nullptr && c < dim) x[s] = row_part<T, TINY>(row, c, dim);
   }
+  if (!TINY && dim % kWide<T> != 0)
+#pragma unroll
+    for (int s = 0; s < DP / kStep<T>; ++s) x[s] = finish<T>(x[s], s * kStep<T> + h * kWide<T>, dim);
 }
 
 // bit j: byte j of x is not zero
@@ -257,16 +301,18 @@ __device__ __forceinline__ int64_t by_die(int64_t id, int64_t total) {
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Calls f(T{}, DP) with the head size padded to whole 32-column tiles
+// Calls f(T{}, DP, TINY) with the head size padded to whole 32-column tiles
 template <typename F>
 int by_head(int dtype, int dim, F&& f) {
   return by_type(dtype, [&](auto t) {
-    if (dim <= 32) return f(t, std::integral_constant<int, 32>{});
-    if (dim <= 64) return f(t, std::integral_constant<int, 64>{});
-    if (dim <= 96) return f(t, std::integral_constant<int, 96>{});
-    if (dim <= 128) return f(t, std::integral_constant<int, 128>{});
-    if (dim <= 192) return f(t, std::integral_constant<int, 192>{});
-    return f(t, std::integral_constant<int, 256>{});
+    constexpr std::false_type no{};
+    if (dim < kWide<decltype(t)>) return f(t, std::integral_constant<int, 32>{}, std::true_type{});
+    if (dim <= 32) return f(t, std::integral_constant<int, 32>{}, no);
+    if (dim <= 64) return f(t, std::integral_constant<int, 64>{}, no);
+    if (dim <= 96) return f(t, std::integral_constant<int, 96>{}, no);
+    if (dim <= 128) return f(t, std::integral_constant<int, 128>{}, no);
+    if (dim <= 192) return f(t, std::integral_constant<int, 192>{}, no);
+    return f(t, std::integral_constant<int, 256>{}, no);
   });
 }
 
