@@ -1,8 +1,8 @@
 // Attention backward on the matrix units.
 //
-// Three launches: delta_i = do_i . o_i and the log sum of every row; dk and dv, where a wave owns 32
-// keys and walks over the problem's rows; dq, where a wave owns 32 rows and walks over
-// the keys.  Scores are computed anew in both from the saved log sums (7 products of
+// Three launches: delta_i = do_i . o_i and the log sum of every row; dk and dv, where a wave owns a
+// tile of keys and walks over the problem's rows; dq, where a wave owns a tile of rows and
+// walks over the keys.  Scores are computed anew in both from the saved log sums (7 products of
 // M x Lk x D, the sums of each output in one place and in one order, no atomics).
 //
 // As in the forward pass every score tile stays in the registers it was computed in: a
@@ -43,66 +43,61 @@ __global__ __launch_bounds__(256) void att_stats(const T* __restrict__ out, cons
   stats[to] = make_float2(x == -INFINITY ? INFINITY : x * kLog2e, s);
 }
 
-// 32 columns of a product with 4 values of a row in a lane, to rows of `dim` values
-template <typename T, int DP>
-__device__ __forceinline__ void store_columns(T* row, const f32x16 (&x)[DP / 32], float by, int dim) {
-  const int h = (threadIdx.x & (kWave - 1)) / 32;
-#pragma unroll
-  for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int d = t * 32 + mma_row(4 * j, h);
-      Pack<T, 4> y;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) y.v[u] = from_f<T>(x[t][4 * j + u] * by);
-      if (d + 4 <= dim) {
-        store_pack<T, 4>(row + d, y);
-      } else {
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (d + u < dim) row[d + u] = y.v[u];
-      }
-    }
-}
-
-// dk and dv (WHAT: 1 = dv, 2 = dk, 3 = both) of 32 W keys.  S = Q K^T and dP = dO V^T
-// have the rows down a lane's registers and one key a lane; dV^T += dO^T P and
-// dK^T += Q^T dS follow.
-template <typename T, bool TINY, int DP, int W, int WHAT>
-__global__ __launch_bounds__(64 * W, DP > 64 ? 1 : 2) void att_mma_kv(const AttArgs a, int ktiles,
-                                                                      const float2* __restrict__ stats) {
-  constexpr int NT = 64 * W, V = kWide<T>, ST = DP + 16 / static_cast<int>(sizeof(T)), R = 32;
-  constexpr bool DV = (WHAT & 1) != 0, DK = (WHAT & 2) != 0;
-  __shared__ __align__(16) T sq[R * ST], sg[R * ST];
+// dk and dv of kTile W keys.  S = Q K^T and dP = dO V^T have the rows down a lane's
+// registers and one key a lane; dV^T += dO^T P and dK^T += Q^T dS follow.
+template <typename T, bool TINY, int DP, int W>
+__global__ __launch_bounds__(64 * W, DP > 128 || (W == 2 && DP > 64) ? 1 : 2) void att_mma_kv(const AttArgs a, int ktiles,
+                                                                                       const float2* __restrict__ stats) {
+  using Tile = LdsTile<T, DP, Reads::kBoth>;
+  using Own = LdsTile<T, DP, Reads::kRows>;
+  constexpr int NT = 64 * W, TS = kTile<T>, R = 32, OT = DP / TS, ST = DP / kStep;
+  // a wave holds its keys and values as fragments; wide bf16 heads, whose sums alone take
+  // 256 registers, leave them in LDS
+  constexpr bool HELD = sizeof(T) == 4 || DP <= 128;
+  __shared__ __align__(16) T sq[R * Tile::ROW], sg[R * Tile::ROW];
+  __shared__ __align__(16) T sk[HELD ? 8 : TS * W * Own::ROW], sv[HELD ? 8 : TS * W * Own::ROW];
   __shared__ __align__(16) float slse[R], sdelta[R];
-  const int lane = threadIdx.x & (kWave - 1), h = lane / 32, wave = threadIdx.x / kWave;
+  const int group = lane_group<T>(), wave = threadIdx.x / kWave;
   const int64_t w = by_die(blockIdx.x, gridDim.x);
-  const int64_t j = w % ktiles * (32 * W) + wave * 32 + (lane & 31);
+  const int64_t j = w % ktiles * (TS * W) + wave * TS + lane_row<T>();
   const int64_t p = w / ktiles;
   const int hk = static_cast<int>(p % a.kv_heads);
   const int64_t b = p / a.kv_heads;
   const bool kept = j < a.lk && (a.mask == nullptr || a.mask[b * a.mask_stride + j] != 0);
   const int64_t at = (b * a.lk + j) * a.kv_heads + hk;
-  f32x16 dk[DK ? DP / 32 : 1], dv[DV ? DP / 32 : 1];
+  Acc<T> dk[OT], dv[OT];
 #pragma unroll
-  for (int t = 0; t < DP / 32; ++t) {
-    if constexpr (DK) dk[t] = f32x16{};
-    if constexpr (DV) dv[t] = f32x16{};
-  }
+  for (int t = 0; t < OT; ++t) dk[t] = dv[t] = Acc<T>{};
   if (__syncthreads_or(kept)) {
-    const bool all = __all(kept);
-    u32x4 kf[DP / kStep<T>], vf[DK ? DP / kStep<T> : 1];
-    row_frags<T, TINY, DP>(kf, kept ? static_cast<const T*>(a.k) + b * a.ks[0] + j * a.ks[1] + hk * a.ks[2] : nullptr, a.dim);
-    if constexpr (DK)
-      row_frags<T, TINY, DP>(vf, kept ? static_cast<const T*>(a.v) + b * a.vs[0] + j * a.vs[1] + hk * a.vs[2] : nullptr,
-                       a.dim);
+    const bool all = __all(kept), busy = __any(kept);
+    const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[2];
+    const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[2];
+    u32x4 kf[HELD ? ST : 1], vf[HELD ? ST : 1];
+    if constexpr (HELD) {
+      row_frags<T, TINY, DP>(kf, kept ? kp + j * a.ks[1] : nullptr, a.dim);
+      row_frags<T, TINY, DP>(vf, kept ? vp + j * a.vs[1] : nullptr, a.dim);
+    } else {
+      static_assert(HELD || TS * W == 64, "a bit of a word for each key");
+      // every wave's lanes hold the same 32 keys twice: a wave's ballot has its keys' bits
+      __shared__ uint32_t bits[W];
+      const uint64_t mine = __ballot(kept);
+      if ((threadIdx.x & (kWave - 1)) == 0) bits[wave] = static_cast<uint32_t>(mine);
+      __syncthreads();
+      const uint64_t both = static_cast<uint64_t>(bits[1]) << 32 | bits[0];
+      const int64_t first = j - (wave * TS + lane_row<T>());
+      Stage<T, TINY, TS * W, DP, NT> kv(a.dim);
+      kv.load(kp + first * a.ks[1], a.ks[1], both, a.dim);
+      kv.template store<Own::ROW>(sk, a.dim);
+      kv.load(vp + first * a.vs[1], a.vs[1], both, a.dim);
+      kv.template store<Own::ROW>(sv, a.dim);
+    }
     const float c = a.scale * kLog2e;
     const int64_t rows = a.lq * a.group;
     const T* qp = static_cast<const T*>(a.q) + b * a.qs[0] + static_cast<int64_t>(hk) * a.group * a.qs[2];
     const T* gp = static_cast<const T*>(a.dout) + b * a.os[0] + static_cast<int64_t>(hk) * a.group * a.os[2];
     stats += p * rows;
-    Stage<T, TINY, R, DP, NT, ST> q(a.dim), g(a.dim);
-    constexpr int N = Stage<T, TINY, R, DP, NT, ST>::N, STEP = Stage<T, TINY, R, DP, NT, ST>::STEP;
+    Stage<T, TINY, R, DP, NT> q(a.dim), g(a.dim);
+    constexpr int N = Stage<T, TINY, R, DP, NT>::N, STEP = Stage<T, TINY, R, DP, NT>::STEP;
     // each of the thread's rows: its head of the group and its offsets, moved on by R rows
     // a tile without a division
     int hg[N];
@@ -132,136 +127,188 @@ __global__ __launch_bounds__(64 * W, DP > 64 ? 1 : 2) void att_mma_kv(const AttA
         }
       }
     };
+    __builtin_amdgcn_s_waitcnt(kNoLoads);  // the fragments are here: the loop does not wait for them again
     fetch(0);
     for (int64_t first = 0; first < rows; first += R) {
       __syncthreads();
-      q.store(sq, a.dim);
-      g.store(sg, a.dim);
+      q.template store<Tile::ROW>(sq, a.dim);
+      g.template store<Tile::ROW>(sg, a.dim);
       if (threadIdx.x < R) {
         slse[threadIdx.x] = st.x;
         sdelta[threadIdx.x] = st.y;
       }
       __syncthreads();
       if (first + R < rows) fetch(first + R);
-      f32x16 s = f32x16{}, dp = f32x16{};
+      if (sizeof(T) == 4 && !busy) continue;
 #pragma unroll
-      for (int e = 0; e < DP / kStep<T>; ++e) {
-        s = mma<T>(s, *reinterpret_cast<const u32x4*>(sq + (lane & 31) * ST + e * kStep<T> + h * V), kf[e]);
-        if constexpr (DK)
-          dp = mma<T>(dp, *reinterpret_cast<const u32x4*>(sg + (lane & 31) * ST + e * kStep<T> + h * V), vf[e]);
-      }
+      for (int u = 0; u < R / TS; ++u) {
+        if (R > TS && first + u * TS >= rows) break;
+        // One step after the other: left to itself the compiler reads all operands ahead
+        // and runs out of registers.  The other wave of the SIMD fills the gaps.
+        Acc<T> s = Acc<T>{}, dp = Acc<T>{};
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int r = mma_row(i, h);
-        s[i] = exp2_(fmaf(s[i], c, -slse[r]));
-        if (!all) s[i] = kept ? s[i] : 0.f;
-        if constexpr (DK) dp[i] = s[i] * (dp[i] - sdelta[r]);
-      }
+        for (int e = 0; e < ST; ++e) {
+          s = mma<T>(s, Tile::frag(sq, u * TS, e), HELD ? kf[HELD ? e : 0] : Own::frag(sk, wave * TS, e));
+          if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int f = 0; f < 16 / V; ++f) {
-        const u32x4 pf = to_frag<T>(s, f);
-        u32x4 df;
-        if constexpr (DK) df = to_frag<T>(dp, f);
+        for (int i = 0; i < kRegs<T>; ++i) {
+          s[i] = exp2_(fmaf(s[i], c, -slse[u * TS + mma_row<T>(i, group)]));
+          if (!all) s[i] = kept ? s[i] : 0.f;
+        }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int t = 0; t < DP / 32; ++t) {
-          if constexpr (DV) dv[t] = mma<T>(dv[t], transposed(sg, ST, 0, f, t * 32), pf);
-          if constexpr (DK) dk[t] = mma<T>(dk[t], transposed(sq, ST, 0, f, t * 32), df);
+        for (int f = 0; f < kFrags<T>; ++f) {
+          const u32x4 pf = to_frag<T>(s, f);
+#pragma unroll
+          for (int t = 0; t < OT; ++t) dv[t] = mma<T>(dv[t], Tile::transposed(sg, u * TS, f, t), pf);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int e = 0; e < ST; ++e) {
+          dp = mma<T>(dp, Tile::frag(sg, u * TS, e), HELD ? vf[HELD ? e : 0] : Own::frag(sv, wave * TS, e));
+          if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < kRegs<T>; ++i) dp[i] = s[i] * (dp[i] - sdelta[u * TS + mma_row<T>(i, group)]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int f = 0; f < kFrags<T>; ++f) {
+          const u32x4 df = to_frag<T>(dp, f);
+#pragma unroll
+          for (int t = 0; t < OT; ++t) dk[t] = mma<T>(dk[t], Tile::transposed(sq, u * TS, f, t), df);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
   }
   if (j >= a.lk) return;
-  if constexpr (DK)
-    if (a.dk != nullptr) store_columns<T, DP>(static_cast<T*>(a.dk) + at * a.dim, dk, a.scale, a.dim);
-  if constexpr (DV)
-    if (a.dv != nullptr) store_columns<T, DP>(static_cast<T*>(a.dv) + at * a.dim, dv, 1.f, a.dim);
+  if (a.dk != nullptr) store_columns<T, DP>(static_cast<T*>(a.dk) + at * a.dim, dk, a.scale, a.dim);
+  if (a.dv != nullptr) store_columns<T, DP>(static_cast<T*>(a.dv) + at * a.dim, dv, 1.f, a.dim);
 }
 
-// dq of 32 W rows.  S^T = K Q^T and dP^T = V dO^T have the keys down a lane's registers
-// and one row a lane; dQ^T += K^T dS^T follows.
+// dq of kTile W rows.  S^T = K Q^T and dP^T = V dO^T have the keys down a lane's registers
+// and one row a lane; dQ^T += K^T dS^T follows.  With splits > 1 each range of `span` keys
+// leaves its sum in `part`.
 template <typename T, bool TINY, int DP, int W>
-__global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void att_mma_q(const AttArgs a, int mtiles,
-                                                                     const float2* __restrict__ stats) {
-  constexpr int NT = 64 * W, V = kWide<T>, ST = DP + 16 / static_cast<int>(sizeof(T)), KT = 32;
-  __shared__ __align__(16) T sk[KT * ST], sv[KT * ST];
-  const int lane = threadIdx.x & (kWave - 1), h = lane / 32, wave = threadIdx.x / kWave;
-  const int64_t w = by_die(blockIdx.x, gridDim.x);
-  const int64_t r = w % mtiles * (32 * W) + wave * 32 + (lane & 31);
+__global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void att_mma_q(const AttArgs a, int mtiles, int splits,
+                                                                     int64_t span, const float2* __restrict__ stats,
+                                                                     float* __restrict__ part) {
+  using KTile = LdsTile<T, DP, Reads::kBoth>;
+  using VTile = LdsTile<T, DP, Reads::kRows>;
+  constexpr int NT = 64 * W, TS = kTile<T>, KT = 32, OT = DP / TS, ST = DP / kStep;
+  __shared__ __align__(16) T sk[KT * KTile::ROW], sv[KT * VTile::ROW];
+  const int group = lane_group<T>(), wave = threadIdx.x / kWave;
+  int64_t w = by_die(blockIdx.x, gridDim.x);
+  const int sp = static_cast<int>(w % splits);
+  w /= splits;
+  const int64_t r0 = w % mtiles * (TS * W) + wave * TS, r = r0 + lane_row<T>();
   const int64_t p = w / mtiles;
   const int hk = static_cast<int>(p % a.kv_heads);
   const int64_t b = p / a.kv_heads;
   const int64_t rows = a.lq * a.group, tok = r < rows ? r / a.group : 0;
+  const bool busy = r0 < rows;  // a wave past the last row only helps to move keys and values
   const int head = hk * a.group + static_cast<int>(r - tok * a.group);
   const int64_t row = (b * a.lq + tok) * a.heads + head;
   const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[2];
   const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[2];
-  u32x4 qf[DP / kStep<T>], gf[DP / kStep<T>];
-  row_frags<T, TINY, DP>(qf, r < rows ? static_cast<const T*>(a.q) + b * a.qs[0] + tok * a.qs[1] + head * a.qs[2] : nullptr,
-                   a.dim);
+  u32x4 qf[ST], gf[ST];
+  row_frags<T, TINY, DP>(
+      qf, r < rows ? static_cast<const T*>(a.q) + b * a.qs[0] + tok * a.qs[1] + head * a.qs[2] : nullptr, a.dim);
   row_frags<T, TINY, DP>(gf, r < rows ? static_cast<const T*>(a.dout) + row * a.dim : nullptr, a.dim);
   const float2 st = r < rows ? stats[p * rows + r] : make_float2(INFINITY, 0.f);
   const float c = a.scale * kLog2e;
-  f32x16 dq[DP / 32];
+  Acc<T> dq[OT];
 #pragma unroll
-  for (int t = 0; t < DP / 32; ++t) dq[t] = f32x16{};
+  for (int t = 0; t < OT; ++t) dq[t] = Acc<T>{};
 
-  Keys<KT> keys(a.mask == nullptr ? nullptr : a.mask + b * a.mask_stride, 0, a.lk);
+  const int64_t lo = sp * span, hi = lo + span < a.lk ? lo + span : a.lk;
+  Keys<KT> keys(a.mask == nullptr ? nullptr : a.mask + b * a.mask_stride, lo, hi);
   int64_t key;
   uint64_t bits;
   bool more = keys.next(key, bits);
-  Stage<T, TINY, KT, DP, NT, ST> k(a.dim), v(a.dim);
+  Stage<T, TINY, KT, DP, NT> k(a.dim), v(a.dim);
   auto fetch = [&]() {
     k.load(kp + key * a.ks[1], a.ks[1], bits, a.dim);
     v.load(vp + key * a.vs[1], a.vs[1], bits, a.dim);
   };
+  __builtin_amdgcn_s_waitcnt(kNoLoads);  // the fragments are here: the loop does not wait for them again
   if (more) fetch();
   while (more) {  // workgroup-uniform
     __syncthreads();
-    k.store(sk, a.dim);
-    v.store(sv, a.dim);
+    k.template store<KTile::ROW>(sk, a.dim);
+    v.template store<VTile::ROW>(sv, a.dim);
     __syncthreads();
-    const uint32_t now = static_cast<uint32_t>(bits), kept = now >> (4 * h);
+    const uint32_t now = static_cast<uint32_t>(bits);
     more = keys.next(key, bits);
     if (more) fetch();
-    f32x16 s = f32x16{}, dp = f32x16{};
+    if (!busy) continue;
+    constexpr uint32_t ALL = TS == 32 ? ~0u : 0xffffu;
 #pragma unroll
-    for (int e = 0; e < DP / kStep<T>; ++e) {
-      s = mma<T>(s, *reinterpret_cast<const u32x4*>(sk + (lane & 31) * ST + e * kStep<T> + h * V), qf[e]);
-      dp = mma<T>(dp, *reinterpret_cast<const u32x4*>(sv + (lane & 31) * ST + e * kStep<T> + h * V), gf[e]);
-    }
+    for (int u = 0; u < KT / TS; ++u) {
+      const uint32_t here = now >> (u * TS) & ALL;
+      if (here == 0) continue;
+      Acc<T> s = Acc<T>{}, dp = Acc<T>{};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      dp[i] = exp2_(fmaf(s[i], c, -st.x)) * (dp[i] - st.y);
-      if (now != ~0u) dp[i] = kept >> mma_row(i, 0) & 1 ? dp[i] : 0.f;
-    }
+      for (int e = 0; e < ST; ++e) {
+        s = mma<T>(s, KTile::frag(sk, u * TS, e), qf[e]);
+        dp = mma<T>(dp, VTile::frag(sv, u * TS, e), gf[e]);
+      }
 #pragma unroll
-    for (int f = 0; f < 16 / V; ++f) {
-      const u32x4 df = to_frag<T>(dp, f);
+      for (int i = 0; i < kRegs<T>; ++i) {
+        dp[i] = exp2_(fmaf(s[i], c, -st.x)) * (dp[i] - st.y);
+        if (here != ALL) dp[i] = here >> (4 * group) >> mma_row<T>(i, 0) & 1 ? dp[i] : 0.f;
+      }
 #pragma unroll
-      for (int t = 0; t < DP / 32; ++t) {
-        dq[t] = mma<T>(dq[t], transposed(sk, ST, 0, f, t * 32), df);
+      for (int f = 0; f < kFrags<T>; ++f) {
+        const u32x4 df = to_frag<T>(dp, f);
+#pragma unroll
+        for (int t = 0; t < OT; ++t) dq[t] = mma<T>(dq[t], KTile::transposed(sk, u * TS, f, t), df);
       }
     }
   }
   if (r >= rows) return;
-  store_columns<T, DP>(static_cast<T*>(a.dq) + row * a.dim, dq, a.scale, a.dim);
+  if (splits > 1) store_parts<T, DP>(part + (row * splits + sp) * a.dim, dq, a.dim);
+  else store_columns<T, DP>(static_cast<T*>(a.dq) + row * a.dim, dq, a.scale, a.dim);
 }
 
-int waves_for(int64_t n) { return n <= 64 ? 2 : 4; }
+// dq's row tiles, and the ranges the keys are cut in where those alone leave compute units
+// without work
+struct QShape {
+  int w, mtiles, splits;
+  int64_t span;
+  QShape(const AttArgs& a, int dtype) {
+    const int64_t rows = a.lq * a.group;
+    const int tile = dtype == TGX_BF16 ? 32 : 16;
+    w = a.dim > 128 ? 4 : (rows <= 64 ? 64 : 128) / tile;  // wide heads: as many registers as there are
+    mtiles = static_cast<int>(ops_cdiv(rows, tile * w));
+    const int64_t blocks = a.batch * a.kv_heads * mtiles;
+    const int64_t tiles = ops_cdiv(std::max<int64_t>(a.lk, 1), 64);
+    const int64_t want = blocks >= 512 ? 1 : ops_cdiv(1024, blocks);
+    const int64_t per = ops_cdiv(tiles, std::min(std::min(want, ops_cdiv(tiles, 8)), int64_t(256)));
+    span = per * 64;
+    splits = a.dq != nullptr ? static_cast<int>(ops_cdiv(tiles, per)) : 1;
+  }
+};
+
+size_t stats_bytes(const AttArgs& a) { return ops_align(static_cast<size_t>(a.batch * a.lq * a.heads) * sizeof(float2)); }
 
 }  // namespace
 
 size_t att_mma_backward_workspace(const AttArgs& a, int dtype) {
-  (void)dtype;
-  return ops_align(static_cast<size_t>(a.batch * a.lq * a.heads) * sizeof(float2));
+  const QShape f(a, dtype);
+  return stats_bytes(a) + (f.splits > 1 ? static_cast<size_t>(a.batch * a.lq * a.heads) * f.splits * a.dim * 4 : 0);
 }
 
 int att_mma_backward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
   const int64_t rows = a.batch * a.lq * a.heads;
   float2* stats = static_cast<float2*>(ws);
+  float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + stats_bytes(a));
   return by_head(dtype, a.dim, [&](auto t, auto dp, auto tiny) {
     using T = decltype(t);
-    constexpr int DP = decltype(dp)::value;
+    constexpr int DP = decltype(dp)::value, TS = kTile<T>;
     constexpr bool TINY = decltype(tiny)::value;
     hipLaunchKernelGGL(att_stats<T>, dim3(static_cast<unsigned>(ops_cdiv(rows, 256 / kDeltaLanes))), dim3(256), 0, s,
                        static_cast<const T*>(a.out), static_cast<const T*>(a.dout), a.lse, rows, a.lq, a.heads, a.group,
@@ -269,38 +316,30 @@ int att_mma_backward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
     int rc = check_launch("att_stats");
     if (rc) return rc;
     if (a.lk > 0 && (a.dk != nullptr || a.dv != nullptr)) {
-      auto go = [&](auto w, auto what) {
-        constexpr int W = decltype(w)::value, WHAT = decltype(what)::value;
-        const int ktiles = static_cast<int>(ops_cdiv(a.lk, 32 * W));
-        hipLaunchKernelGGL((att_mma_kv<T, TINY, DP, W, WHAT>), dim3(static_cast<unsigned>(a.batch * a.kv_heads * ktiles)),
+      auto go = [&](auto w) {
+        constexpr int W = decltype(w)::value;
+        const int ktiles = static_cast<int>(ops_cdiv(a.lk, TS * W));
+        hipLaunchKernelGGL((att_mma_kv<T, TINY, DP, W>), dim3(static_cast<unsigned>(a.batch * a.kv_heads * ktiles)),
                            dim3(64 * W), 0, s, a, ktiles, stats);
         return check_launch("att_mma_kv");
       };
-      auto by_waves = [&](auto what) {
-        if (waves_for(a.lk) == 2) return go(std::integral_constant<int, 2>{}, what);
-        return go(std::integral_constant<int, 4>{}, what);
-      };
-      // both sums and both operands of one wave exceed the registers for wide f32 heads
-      if constexpr (sizeof(T) == 2 || DP <= 128) {
-        rc = by_waves(std::integral_constant<int, 3>{});
-      } else {
-        if (a.dv != nullptr) rc = by_waves(std::integral_constant<int, 1>{});
-        if (rc == TGX_OK && a.dk != nullptr) rc = by_waves(std::integral_constant<int, 2>{});
-      }
+      // wide heads: 64 keys a workgroup, as many registers a wave as there are
+      if constexpr (DP > 128) rc = go(std::integral_constant<int, 64 / TS>{});
+      else rc = a.lk <= 64 ? go(std::integral_constant<int, 64 / TS>{}) : go(std::integral_constant<int, 8>{});
       if (rc) return rc;
     }
-    if (a.dq != nullptr) {
-      auto go = [&](auto w) {
-        constexpr int W = decltype(w)::value;
-        const int mtiles = static_cast<int>(ops_cdiv(a.lq * a.group, 32 * W));
-        hipLaunchKernelGGL((att_mma_q<T, TINY, DP, W>), dim3(static_cast<unsigned>(a.batch * a.kv_heads * mtiles)),
-                           dim3(64 * W), 0, s, a, mtiles, stats);
-        return check_launch("att_mma_q");
-      };
-      if (waves_for(a.lq * a.group) == 2) return go(std::integral_constant<int, 2>{});
-      return go(std::integral_constant<int, 4>{});
-    }
-    return TGX_OK;
+    if (a.dq == nullptr) return TGX_OK;
+    const QShape f(a, dtype);
+    auto go = [&](auto w) {
+      constexpr int W = decltype(w)::value;
+      hipLaunchKernelGGL((att_mma_q<T, TINY, DP, W>),
+                         dim3(static_cast<unsigned>(a.batch * a.kv_heads * f.mtiles * f.splits)), dim3(64 * W), 0, s, a,
+                         f.mtiles, f.splits, f.span, stats, part);
+      return check_launch("att_mma_q");
+    };
+    if constexpr (DP > 128) rc = go(std::integral_constant<int, 4>{});
+    else rc = f.w * TS == 64 ? go(std::integral_constant<int, 64 / TS>{}) : go(std::integral_constant<int, 128 / TS>{});
+    return rc || f.splits == 1 ? rc : att_join_sums(a.dq, rows, a.dim, dtype, a.scale, f.splits, part, s);
   });
 }
 

@@ -94,7 +94,7 @@ struct RowUnit {
 
 template <typename T, int LP, int C, int M>
 __global__ __launch_bounds__(kRowThreads) void att_rows_fwd(const AttArgs a, int wpp, int splits, int64_t span,
-                                                            float* __restrict__ part) {
+                                                            const AttParts part) {
   constexpr int V = kWide<T>, N = C * V, G = kWave / LP, U = M == 1 ? 4 : 2;
   __shared__ float join[kRowWaves][M][LP * N + 2];
   const int lane = threadIdx.x & (kWave - 1), grp = lane / LP, wave = threadIdx.x / kWave;
@@ -224,14 +224,11 @@ __global__ __launch_bounds__(kRowThreads) void att_rows_fwd(const AttArgs a, int
     const int i = r / a.group, head = w.hk * a.group + r % a.group;
     const int64_t row = (w.b * a.lq + i) * a.heads + head;
     if (splits > 1) {
-      float* out = part + (row * splits + w.sp) * (a.dim + 2);
-      if (at.gl == 0) {
-        out[0] = m[r];
-        out[1] = l[r];
-      }
+      float* out = part.o + (row * splits + w.sp) * a.dim;
+      if (at.gl == 0) part.ml[row * splits + w.sp] = make_float2(m[r], l[r]);
 #pragma unroll
       for (int x = 0; x < N; ++x)
-        if (at.col(x / V) + x % V < a.dim) out[2 + at.col(x / V) + x % V] = acc[r][x];
+        if (at.col(x / V) + x % V < a.dim) out[at.col(x / V) + x % V] = acc[r][x];
       continue;
     }
     const float inv = l[r] > 0.f ? 1.f / l[r] : 0.f;
@@ -346,20 +343,6 @@ __global__ __launch_bounds__(kRowThreads) void att_rows_bwd(const AttArgs a, int
   }
 }
 
-// dq of one row per wave: the key ranges' parts in their order
-template <typename T>
-__global__ __launch_bounds__(kRowThreads) void att_rows_join(T* __restrict__ dq, int64_t rows, int dim, int splits,
-                                                             const float* __restrict__ part) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowWaves + threadIdx.x / kWave;
-  if (row >= rows) return;
-  for (int d = threadIdx.x & (kWave - 1); d < dim; d += kWave) {
-    float s = 0.f;
-#pragma unroll 8
-    for (int y = 0; y < splits; ++y) s += part[(row * splits + y) * dim + d];
-    dq[row * dim + d] = from_f<T>(s);
-  }
-}
-
 // Waves per problem and key ranges: one wave a problem where the problems fill the
 // device, four where they do not, and then ranges of at least 512 keys.
 struct RowShape {
@@ -403,13 +386,12 @@ int by_lanes(int dtype, int dim, int64_t rows, F&& f) {
 }  // namespace
 
 size_t att_rows_forward_workspace(const AttArgs& a) {
-  const RowShape f(a);
-  return f.splits > 1 ? static_cast<size_t>(a.batch * a.lq * a.heads) * f.splits * (a.dim + 2) * 4 : 0;
+  return AttParts::bytes(a.batch * a.lq * a.heads, RowShape(a).splits, a.dim);
 }
 
 int att_rows_forward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
   const RowShape f(a);
-  float* part = static_cast<float*>(ws);
+  const AttParts part(ws, a.batch * a.lq * a.heads, f.splits);
   const int rc = by_lanes(dtype, a.dim, a.lq * a.group, [&](auto t, auto lp, auto c, auto m) {
     hipLaunchKernelGGL((att_rows_fwd<decltype(t), decltype(lp)::value, decltype(c)::value, decltype(m)::value>),
                        dim3(static_cast<unsigned>(f.blocks)), dim3(kRowThreads), 0, s, a, f.wpp, f.splits, f.span, part);
@@ -432,13 +414,7 @@ int att_rows_backward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
     return check_launch("att_rows_bwd");
   });
   if (rc || f.splits == 1 || a.dq == nullptr) return rc;
-  const int64_t rows = a.batch * a.lq * a.heads;
-  return by_type(dtype, [&](auto t) {
-    using T = decltype(t);
-    hipLaunchKernelGGL(att_rows_join<T>, dim3(static_cast<unsigned>(ops_cdiv(rows, kRowWaves))), dim3(kRowThreads), 0, s,
-                       static_cast<T*>(a.dq), rows, a.dim, f.splits, part);
-    return check_launch("att_rows_join");
-  });
+  return att_join_sums(a.dq, a.batch * a.lq * a.heads, a.dim, dtype, 1.f, f.splits, part, s);
 }
 
 }  // namespace tgx

@@ -28,8 +28,20 @@ size_t att_rows_forward_workspace(const AttArgs& a);
 int att_rows_forward(const AttArgs& a, int dtype, void* ws, hipStream_t s);
 size_t att_rows_backward_workspace(const AttArgs& a);
 int att_rows_backward(const AttArgs& a, int dtype, void* ws, hipStream_t s);
-// joins the key ranges' parts, per row and range: maximum, sum, dim outputs
-int att_join_forward(const AttArgs& a, int dtype, int splits, const float* part, hipStream_t s);
+// Parts of key ranges: per row and range, its maximum and sum in ml, its outputs in o.
+// att_join_forward joins them into a.o and a.lse, att_join_sums adds up the ranges' o.
+struct AttParts {
+  float2* ml;
+  float* o;
+  AttParts(void* ws, int64_t rows, int splits)
+      : ml(static_cast<float2*>(ws)), o(reinterpret_cast<float*>(ml + (rows * splits + 1) / 2 * 2)) {}
+  static size_t bytes(int64_t rows, int splits, int dim) {
+    return splits > 1 ? static_cast<size_t>((rows * splits + 1) / 2 * 2) * 8 + static_cast<size_t>(rows) * splits * dim * 4
+                      : 0;
+  }
+};
+int att_join_forward(const AttArgs& a, int dtype, int splits, const AttParts& part, hipStream_t s);
+int att_join_sums(void* out, int64_t rows, int dim, int dtype, float by, int splits, const float* part, hipStream_t s);
 size_t att_mma_forward_workspace(const AttArgs& a, int dtype);
 int att_mma_forward(const AttArgs& a, int dtype, void* ws, hipStream_t s);
 size_t att_mma_backward_workspace(const AttArgs& a, int dtype);
@@ -40,6 +52,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -48,67 +61,114 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
-// A fragment is 16 bytes a lane of a 32-row operand of the 32 x 32 matrix instructions:
-// lane l holds row l % 32, and its half h = l / 32 the values [h V, h V + V) of a step
-// of kStep = 2 V values along the summed axis.  For f32 that is four instructions of two
-// values each (the halves' values stand in for two neighbours: the order of a sum's
-// terms is free as long as both operands agree on it).
+// The matrix instructions: bf16 takes the 32 x 32 tile, whose operands cost half the LDS
+// reads of the 16 x 16 one; f32, eight times slower for the same bytes, the 16 x 16 one,
+// which pads sequences of 1 + 32 or 1 + 64 tokens less.
+//   kTile  : rows and columns of a tile
+//   kRegs  : a lane's values of a product
+//   kFrags : fragments that the kTile rows of a product make as the next one's operand
 template <typename T>
-constexpr int kStep = 2 * kWide<T>;
+constexpr int kTile = sizeof(T) == 2 ? 32 : 16;
+template <typename T>
+constexpr int kRegs = kTile<T> * kTile<T> / kWave;
+template <typename T>
+constexpr int kFrags = kRegs<T> / kWide<T>;
+template <typename T>
+using Acc = std::conditional_t<sizeof(T) == 2, f32x16, f32x4>;
+
+// A fragment is 16 bytes a lane of a kTile-row operand: lane l holds row l % kTile, and
+// its group l / kTile the values [group V, group V + V) of a step of 16 along the summed
+// axis.  For f32 that is four instructions, each with one value of every group (they
+// stand in for four neighbours: the order of a sum's terms is free as long as both
+// operands agree on it).
+constexpr int kStep = 16;
 
 template <typename T>
-__device__ __forceinline__ f32x16 mma(f32x16 c, u32x4 a, u32x4 b) {
+__device__ __forceinline__ int lane_row() { return threadIdx.x & (kTile<T> - 1); }
+template <typename T>
+__device__ __forceinline__ int lane_group() { return (threadIdx.x & (kWave - 1)) / kTile<T>; }
+
+template <typename T>
+__device__ __forceinline__ Acc<T> mma(Acc<T> c, u32x4 a, u32x4 b) {
   if constexpr (sizeof(T) == 2) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
                                                    0);
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0,
-                                               0);
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
     return c;
   }
 }
 
-// A product's 16 values a lane belong to column l % 32 and rows 8 (i / 4) + 4 h + i % 4.
-__device__ __forceinline__ constexpr int mma_row(int i, int h) { return 8 * (i / 4) + 4 * h + i % 4; }
+// Value i of a lane of a product belongs to column lane_row and to this row
+template <typename T>
+__device__ __forceinline__ constexpr int mma_row(int i, int group) {
+  return sizeof(T) == 2 ? 8 * (i / 4) + 4 * group + i % 4 : 4 * group + i;
+}
 
-// Fragment f (of 16 / V) of such values as the second operand of a product that sums
+// Fragment f (of kFrags) of such values as the second operand of a product that sums
 // over their rows: no lane gives a value to another.
 template <typename T>
-__device__ __forceinline__ u32x4 to_frag(const f32x16& x, int f) {
+__device__ __forceinline__ u32x4 to_frag(const Acc<T>& x, int f) {
   u32x4 y;
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
     if constexpr (sizeof(T) == 2)  // two values at a time: one conversion
       y[u] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x[f * 8 + 2 * u], x[f * 8 + 2 * u + 1]}), bf16x2));
     else
-      y[u] = __float_as_uint(x[f * 4 + u]);
+      y[u] = __float_as_uint(x[u]);
   }
   return y;
 }
 
-// The first operand that goes with it: 32 columns from `col` on of rows of an LDS tile,
-// transposed, in the rows' order of to_frag.  In bf16 by the transposing LDS read: a
-// group of 16 lanes reads 4 rows of 16 values and each lane gets a column of 4.
-template <typename T>
-__device__ __forceinline__ u32x4 transposed(const T* tile, int stride, int row0, int f, int col) {
-  const int lane = threadIdx.x & (kWave - 1), h = lane / 32;
-  if constexpr (sizeof(T) == 2) {
-    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    const int i = lane & 15;
-    const T* p = tile + (row0 + 16 * f + 4 * h + i / 4) * stride + col + (lane & 16) + (i & 3) * 4;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * stride));
-    return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-  } else {
-    u32x4 x;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      x[e] = __builtin_bit_cast(uint32_t, tile[(row0 + 8 * f + 4 * h + e) * stride + col + (lane & 31)]);
-    return x;
+// An LDS tile of rows of DP values, longer by what keeps its reads off each other's banks
+// (64 of 4 bytes).  A fragment reads 16 bytes of each of 16 rows at a time: rows an odd
+// multiple of 16 bytes apart are free of conflicts.  The transposed reads of bf16 take 64
+// bytes of each of 4 rows at a time: rows 64 bytes apart (mod 256).  A tile read both ways
+// takes rows 80 bytes apart, or 176: fragments are free, a transposed read meets one
+// conflict.  (Chunks that trade places by row would meet none, but their addresses cost the
+// backward pass more registers and instructions than the conflicts: 633 us for dk and dv of
+// 1,000 x 8,000 tokens against 470 with rows of 16 bytes more.)  f32 rows 16 bytes longer
+// serve both.
+enum class Reads { kRows, kColumns, kBoth };
+
+template <typename T, int DP, Reads HOW>
+struct LdsTile {
+  static constexpr int next(int bytes, int x, int y) {  // the next length that is x or y mod 256
+    while (bytes % 256 != x && bytes % 256 != y) bytes += 16;
+    return bytes;
   }
-}
+  static constexpr int ROW =  // values
+      sizeof(T) == 4            ? DP + 4
+      : HOW == Reads::kRows     ? DP + (DP / 8 % 2 == 0 ? 8 : 0)
+      : HOW == Reads::kColumns  ? next(DP * 2, 64, 192) / 2
+                                : next(DP * 2, 80, 176) / 2;
+  // fragment e of rows row0 .. (a multiple of kTile): a lane's 16 bytes
+  __device__ static __forceinline__ u32x4 frag(const T* tile, int row0, int e) {
+    return *reinterpret_cast<const u32x4*>(tile + (row0 + lane_row<T>()) * ROW + e * kStep +
+                                           lane_group<T>() * kWide<T>);
+  }
+  // The first operand that goes with to_frag's: kTile columns from kTile t on of rows
+  // row0 .., transposed, in the rows' order of to_frag.  In bf16 by the transposing LDS
+  // read: 16 lanes read 4 rows of 16 values and each lane gets a column of 4.
+  __device__ static __forceinline__ u32x4 transposed(const T* tile, int row0, int f, int t) {
+    const int lane = threadIdx.x & (kWave - 1), group = lane_group<T>();
+    if constexpr (sizeof(T) == 2) {
+      typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+      const int i = lane & 15;
+      const T* p = tile + (row0 + 16 * f + 4 * group + i / 4) * ROW + t * 32 + (lane & 16) + (i & 3) * 4;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * ROW));
+      return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      u32x4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = __float_as_uint(tile[(row0 + 4 * group + e) * ROW + t * 16 + lane_row<T>()]);
+      return x;
+    }
+  }
+};
 
 template <typename T>
 __device__ __forceinline__ u32x4 load16(const T* p) {
@@ -157,11 +217,10 @@ constexpr int pow2_at_least(int x) {
   return p;
 }
 
-// NT threads move ROWS rows of up to DP values into an LDS tile of rows STRIDE apart:
-// load() issues the reads, store() waits for them and writes.  A thread keeps one column
+// NT threads move ROWS rows of up to DP values into an LDS tile: load() issues the reads, store() waits for them and writes.  A thread keeps one column
 // of all its rows, so that a row costs it one address step; lanes past the last column
 // stay idle.
-template <typename T, bool TINY, int ROWS, int DP, int NT, int STRIDE>
+template <typename T, bool TINY, int ROWS, int DP, int NT>
 struct Stage {
   static constexpr int V = kWide<T>, LANES = pow2_at_least(DP / V), STEP = NT / LANES,
                        N = (ROWS + STEP - 1) / STEP;
@@ -192,33 +251,76 @@ struct Stage {
       if (in && row != nullptr) x[n] = row_part<T, TINY>(row, col, dim);
     }
   }
+  template <int ROW>  // values from row to row of the tile
   __device__ __forceinline__ void store(T* tile, int dim) const {
     if (LANES * V > DP && col >= DP) return;
     if (STEP > ROWS && row0 >= ROWS) return;
-    T* p = tile + row0 * STRIDE + col;
     if (TINY || dim % V == 0) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) *reinterpret_cast<u32x4*>(p + n * STEP * STRIDE) = x[n];
+      for (int n = 0; n < N; ++n) *reinterpret_cast<u32x4*>(tile + (row0 + n * STEP) * ROW + col) = x[n];
     } else {
 #pragma unroll
-      for (int n = 0; n < N; ++n) *reinterpret_cast<u32x4*>(p + n * STEP * STRIDE) = finish<T>(x[n], col, dim);
+      for (int n = 0; n < N; ++n)
+        *reinterpret_cast<u32x4*>(tile + (row0 + n * STEP) * ROW + col) = finish<T>(x[n], col, dim);
     }
   }
 };
 
-// The fragments of one row a lane (row l % 32), from global memory; nullptr gives zeros
+// The fragments of one row a lane (lane_row), from global memory; nullptr gives zeros
 template <typename T, bool TINY, int DP>
-__device__ __forceinline__ void row_frags(u32x4 (&x)[DP / kStep<T>], const T* row, int dim) {
-  const int h = (threadIdx.x & (kWave - 1)) / 32;
+__device__ __forceinline__ void row_frags(u32x4 (&x)[DP / kStep], const T* row, int dim) {
+  const int at = lane_group<T>() * kWide<T>;
 #pragma unroll
-  for (int s = 0; s < DP / kStep<T>; ++s) {
-    const int c = s * kStep<T> + h * kWide<T>;
+  for (int s = 0; s < DP / kStep; ++s) {
     x[s] = u32x4{0, 0, 0, 0};
-    if (row != nullptr && c < dim) x[s] = row_part<T, TINY>(row, c, dim);
+    if (row != nullptr && s * kStep + at < dim) x[s] = row_part<T, TINY>(row, s * kStep + at, dim);
   }
   if (!TINY && dim % kWide<T> != 0)
 #pragma unroll
-    for (int s = 0; s < DP / kStep<T>; ++s) x[s] = finish<T>(x[s], s * kStep<T> + h * kWide<T>, dim);
+    for (int s = 0; s < DP / kStep; ++s) x[s] = finish<T>(x[s], s * kStep + at, dim);
+}
+
+// A product with the head's columns down a lane's registers and one row a lane, to rows
+// of `dim` values: 4 neighbours at a time
+template <typename T, int DP>
+__device__ __forceinline__ void store_columns(T* row, const Acc<T> (&x)[DP / kTile<T>], float by, int dim) {
+#pragma unroll
+  for (int t = 0; t < DP / kTile<T>; ++t)
+#pragma unroll
+    for (int j = 0; j < kRegs<T> / 4; ++j) {
+      const int d = t * kTile<T> + mma_row<T>(4 * j, lane_group<T>());
+      Pack<T, 4> y;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) y.v[u] = from_f<T>(x[t][4 * j + u] * by);
+      if (d + 4 <= dim) {
+        store_pack<T, 4>(row + d, y);
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (d + u < dim) row[d + u] = y.v[u];
+      }
+    }
+}
+
+// the same in 32 bits, for the parts of ranges
+template <typename T, int DP>
+__device__ __forceinline__ void store_parts(float* row, const Acc<T> (&x)[DP / kTile<T>], int dim) {
+#pragma unroll
+  for (int t = 0; t < DP / kTile<T>; ++t)
+#pragma unroll
+    for (int j = 0; j < kRegs<T> / 4; ++j) {
+      const int d = t * kTile<T> + mma_row<T>(4 * j, lane_group<T>());
+      Pack<float, 4> y;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) y.v[u] = x[t][4 * j + u];
+      if (d + 4 <= dim) {
+        store_pack<float, 4>(row + d, y);
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (d + u < dim) row[d + u] = y.v[u];
+      }
+    }
 }
 
 // bit j: byte j of x is not zero
@@ -299,21 +401,31 @@ __device__ __forceinline__ int64_t by_die(int64_t id, int64_t total) {
   return die * q + min(die, r) + id / 8;
 }
 
+constexpr int kNoLoads = 0x0f70;  // s_waitcnt: no vector load outstanding
+
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Calls f(T{}, DP, TINY) with the head size padded to whole 32-column tiles
+// Calls f(T{}, DP, TINY) with the head size padded to whole tiles: for f32 mostly to the
+// next 16, for bf16 to the next 32
 template <typename F>
 int by_head(int dtype, int dim, F&& f) {
+#define TGX_HEAD(DP) f(t, std::integral_constant<int, DP>{}, std::false_type{})
   return by_type(dtype, [&](auto t) {
-    constexpr std::false_type no{};
+    constexpr bool F32 = sizeof(t) == 4;
     if (dim < kWide<decltype(t)>) return f(t, std::integral_constant<int, 32>{}, std::true_type{});
-    if (dim <= 32) return f(t, std::integral_constant<int, 32>{}, no);
-    if (dim <= 64) return f(t, std::integral_constant<int, 64>{}, no);
-    if (dim <= 96) return f(t, std::integral_constant<int, 96>{}, no);
-    if (dim <= 128) return f(t, std::integral_constant<int, 128>{}, no);
-    if (dim <= 192) return f(t, std::integral_constant<int, 192>{}, no);
-    return f(t, std::integral_constant<int, 256>{}, no);
+    if (dim <= 32) return TGX_HEAD(32);
+    if (dim <= 64) return TGX_HEAD(64);
+    if (dim <= 96) return TGX_HEAD(96);
+    if constexpr (F32)
+      if (dim <= 112) return TGX_HEAD(112);
+    if (dim <= 128) return TGX_HEAD(128);
+    if constexpr (F32)
+      if (dim <= 176) return TGX_HEAD(176);
+    if constexpr (!F32)
+      if (dim <= 192) return TGX_HEAD(192);
+    return TGX_HEAD(256);
   });
+#undef TGX_HEAD
 }
 
 }  // namespace
