@@ -43,23 +43,49 @@ __global__ __launch_bounds__(256) void att_stats(const T* __restrict__ out, cons
   stats[to] = make_float2(x == -INFINITY ? INFINITY : x * kLog2e, s);
 }
 
-// dk and dv of kTile W keys.  S = Q K^T and dP = dO V^T have the rows down a lane's
+// Keeps the steps of bf16's dk and dv apart: left to itself the compiler reads all operands
+// ahead and runs out of registers (605 us for 1,000 x 8,000 tokens, 422 so; the other wave
+// of the SIMD fills the gaps).  f32 has the registers.
+template <typename T>
+__device__ __forceinline__ void one_by_one() {
+  if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
+}
+
+// dk and dv, kTile keys a wave.  S = Q K^T and dP = dO V^T have the rows down a lane's
 // registers and one key a lane; dV^T += dO^T P and dK^T += Q^T dS follow.
-template <typename T, bool TINY, int DP, int W>
-__global__ __launch_bounds__(64 * W, DP > 128 || (W == 2 && DP > 64) ? 1 : 2) void att_mma_kv(const AttArgs a, int ktiles,
-                                                                                       const float2* __restrict__ stats) {
+//
+// The rows' tiles stand in LDS twice, so that one is filled while the other is read and a
+// tile takes one barrier.
+//
+// LEAST to kv_most() waves a workgroup.  bf16 heads of 65 to 128 values come two ways: 8
+// waves, which leaves each the registers for one row of staging and two waves a SIMD, or 2
+// to 4 with all registers, where there are few keys.
+template <typename T, int DP>
+constexpr bool kTwoWays = sizeof(T) == 2 && DP > 64 && DP <= 128;
+template <typename T, int DP>
+constexpr int kKvLeast = sizeof(T) == 2 ? 2 : 4;
+template <typename T>
+constexpr int kv_most(int dp, int least) {
+  if (dp > 128) return sizeof(T) == 2 ? 2 : 4;  // wide heads: as many registers as there are
+  return sizeof(T) == 2 && dp > 64 && least < 8 ? 4 : 8;
+}
+
+template <typename T, bool TINY, int DP, int LEAST>
+__global__ __launch_bounds__(64 * kv_most<T>(DP, LEAST), DP > 128 || (sizeof(T) == 2 && DP > 64 && LEAST < 8) ? 1 : 2)
+void att_mma_kv(const AttArgs a, int ktiles, const float2* __restrict__ stats) {
   using Tile = LdsTile<T, DP, Reads::kBoth>;
   using Own = LdsTile<T, DP, Reads::kRows>;
-  constexpr int NT = 64 * W, TS = kTile<T>, R = 32, OT = DP / TS, ST = DP / kStep;
+  constexpr int TS = kTile<T>, R = TS, OT = DP / TS, ST = DP / kStep, W = LEAST;
+  constexpr bool FIXED = LEAST == kv_most<T>(DP, LEAST);
   // a wave holds its keys and values as fragments; wide bf16 heads, whose sums alone take
   // 256 registers, leave them in LDS
   constexpr bool HELD = sizeof(T) == 4 || DP <= 128;
-  __shared__ __align__(16) T sq[R * Tile::ROW], sg[R * Tile::ROW];
+  __shared__ __align__(16) T sq[2][R * Tile::ROW], sg[2][R * Tile::ROW];
   __shared__ __align__(16) T sk[HELD ? 8 : TS * W * Own::ROW], sv[HELD ? 8 : TS * W * Own::ROW];
-  __shared__ __align__(16) float slse[R], sdelta[R];
+  __shared__ __align__(16) float slse[2][R], sdelta[2][R];
   const int group = lane_group<T>(), wave = threadIdx.x / kWave;
   const int64_t w = by_die(blockIdx.x, gridDim.x);
-  const int64_t j = w % ktiles * (TS * W) + wave * TS + lane_row<T>();
+  const int64_t j = w % ktiles * (TS * (blockDim.x / kWave)) + wave * TS + lane_row<T>();
   const int64_t p = w / ktiles;
   const int hk = static_cast<int>(p % a.kv_heads);
   const int64_t b = p / a.kv_heads;
@@ -85,7 +111,7 @@ __global__ __launch_bounds__(64 * W, DP > 128 || (W == 2 && DP > 64) ? 1 : 2) vo
       __syncthreads();
       const uint64_t both = static_cast<uint64_t>(bits[1]) << 32 | bits[0];
       const int64_t first = j - (wave * TS + lane_row<T>());
-      Stage<T, TINY, TS * W, DP, NT> kv(a.dim);
+      Stage<T, TINY, TS * W, DP, W, true> kv(a.dim);
       kv.load(kp + first * a.ks[1], a.ks[1], both, a.dim);
       kv.template store<Own::ROW>(sk, a.dim);
       kv.load(vp + first * a.vs[1], a.vs[1], both, a.dim);
@@ -96,15 +122,15 @@ __global__ __launch_bounds__(64 * W, DP > 128 || (W == 2 && DP > 64) ? 1 : 2) vo
     const T* qp = static_cast<const T*>(a.q) + b * a.qs[0] + static_cast<int64_t>(hk) * a.group * a.qs[2];
     const T* gp = static_cast<const T*>(a.dout) + b * a.os[0] + static_cast<int64_t>(hk) * a.group * a.os[2];
     stats += p * rows;
-    Stage<T, TINY, R, DP, NT> q(a.dim), g(a.dim);
-    constexpr int N = Stage<T, TINY, R, DP, NT>::N, STEP = Stage<T, TINY, R, DP, NT>::STEP;
+    Stage<T, TINY, R, DP, W, FIXED> q(a.dim), g(a.dim);
+    constexpr int N = Stage<T, TINY, R, DP, W, FIXED>::N;
     // each of the thread's rows: its head of the group and its offsets, moved on by R rows
     // a tile without a division
     int hg[N];
     int64_t qo[N], go[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int row = q.row0 + n * STEP, tok = row / a.group;
+      const int row = q.row(n), tok = row / a.group;
       hg[n] = row - tok * a.group;
       qo[n] = tok * a.qs[1] + hg[n] * a.qs[2];
       go[n] = tok * a.os[1] + hg[n] * a.os[2];
@@ -112,8 +138,8 @@ __global__ __launch_bounds__(64 * W, DP > 128 || (W == 2 && DP > 64) ? 1 : 2) vo
     const int dt = R / a.group, dh = R % a.group;
     float2 st = make_float2(INFINITY, 0.f);
     auto fetch = [&](int64_t first) {
-      q.load(a.dim, [&](int n) { return first + q.row0 + n * STEP < rows ? qp + qo[n] : nullptr; });
-      g.load(a.dim, [&](int n) { return first + q.row0 + n * STEP < rows ? gp + go[n] : nullptr; });
+      q.load(a.dim, [&](int n) { return (q.whole(n) || q.row(n) < R) && first + q.row(n) < rows ? qp + qo[n] : nullptr; });
+      g.load(a.dim, [&](int n) { return (q.whole(n) || q.row(n) < R) && first + q.row(n) < rows ? gp + go[n] : nullptr; });
       if (threadIdx.x < R) st = first + threadIdx.x < rows ? stats[first + threadIdx.x] : make_float2(INFINITY, 0.f);
 #pragma unroll
       for (int n = 0; n < N; ++n) {
@@ -128,59 +154,61 @@ __global__ __launch_bounds__(64 * W, DP > 128 || (W == 2 && DP > 64) ? 1 : 2) vo
       }
     };
     __builtin_amdgcn_s_waitcnt(kNoLoads);  // the fragments are here: the loop does not wait for them again
-    fetch(0);
-    for (int64_t first = 0; first < rows; first += R) {
-      __syncthreads();
-      q.template store<Tile::ROW>(sq, a.dim);
-      g.template store<Tile::ROW>(sg, a.dim);
+    auto put = [&](int to) {
+      q.template store<Tile::ROW>(sq[to], a.dim);
+      g.template store<Tile::ROW>(sg[to], a.dim);
       if (threadIdx.x < R) {
-        slse[threadIdx.x] = st.x;
-        sdelta[threadIdx.x] = st.y;
+        slse[to][threadIdx.x] = st.x;
+        sdelta[to][threadIdx.x] = st.y;
       }
+    };
+    fetch(0);
+    put(0);
+    if (R < rows) fetch(R);
+    int cur = 0;
+    for (int64_t first = 0; first < rows; first += R, cur ^= 1) {
       __syncthreads();
-      if (first + R < rows) fetch(first + R);
-      if (sizeof(T) == 4 && !busy) continue;
-#pragma unroll
-      for (int u = 0; u < R / TS; ++u) {
-        if (R > TS && first + u * TS >= rows) break;
-        // One step after the other: left to itself the compiler reads all operands ahead
-        // and runs out of registers.  The other wave of the SIMD fills the gaps.
+      if (sizeof(T) == 2 || busy) {
         Acc<T> s = Acc<T>{}, dp = Acc<T>{};
 #pragma unroll
         for (int e = 0; e < ST; ++e) {
-          s = mma<T>(s, Tile::frag(sq, u * TS, e), HELD ? kf[HELD ? e : 0] : Own::frag(sk, wave * TS, e));
-          if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+          s = mma<T>(s, Tile::frag(sq[cur], 0, e), HELD ? kf[HELD ? e : 0] : Own::frag(sk, wave * TS, e));
+          if (e % 4 == 3) one_by_one<T>();
         }
-        __builtin_amdgcn_sched_barrier(0);
+        one_by_one<T>();
 #pragma unroll
         for (int i = 0; i < kRegs<T>; ++i) {
-          s[i] = exp2_(fmaf(s[i], c, -slse[u * TS + mma_row<T>(i, group)]));
+          s[i] = exp2_(fmaf(s[i], c, -slse[cur][mma_row<T>(i, group)]));
           if (!all) s[i] = kept ? s[i] : 0.f;
         }
-        __builtin_amdgcn_sched_barrier(0);
+        one_by_one<T>();
 #pragma unroll
         for (int f = 0; f < kFrags<T>; ++f) {
           const u32x4 pf = to_frag<T>(s, f);
 #pragma unroll
-          for (int t = 0; t < OT; ++t) dv[t] = mma<T>(dv[t], Tile::transposed(sg, u * TS, f, t), pf);
-          __builtin_amdgcn_sched_barrier(0);
+          for (int t = 0; t < OT; ++t) dv[t] = mma<T>(dv[t], Tile::transposed(sg[cur], 0, f, t), pf);
+          one_by_one<T>();
         }
 #pragma unroll
         for (int e = 0; e < ST; ++e) {
-          dp = mma<T>(dp, Tile::frag(sg, u * TS, e), HELD ? vf[HELD ? e : 0] : Own::frag(sv, wave * TS, e));
-          if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+          dp = mma<T>(dp, Tile::frag(sg[cur], 0, e), HELD ? vf[HELD ? e : 0] : Own::frag(sv, wave * TS, e));
+          if (e % 4 == 3) one_by_one<T>();
         }
-        __builtin_amdgcn_sched_barrier(0);
+        one_by_one<T>();
 #pragma unroll
-        for (int i = 0; i < kRegs<T>; ++i) dp[i] = s[i] * (dp[i] - sdelta[u * TS + mma_row<T>(i, group)]);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < kRegs<T>; ++i) dp[i] = s[i] * (dp[i] - sdelta[cur][mma_row<T>(i, group)]);
+        one_by_one<T>();
 #pragma unroll
         for (int f = 0; f < kFrags<T>; ++f) {
           const u32x4 df = to_frag<T>(dp, f);
 #pragma unroll
-          for (int t = 0; t < OT; ++t) dk[t] = mma<T>(dk[t], Tile::transposed(sq, u * TS, f, t), df);
-          __builtin_amdgcn_sched_barrier(0);
+          for (int t = 0; t < OT; ++t) dk[t] = mma<T>(dk[t], Tile::transposed(sq[cur], 0, f, t), df);
+          one_by_one<T>();
         }
+      }
+      if (first + R < rows) {
+        put(cur ^ 1);
+        if (first + 2 * R < rows) fetch(first + 2 * R);
       }
     }
   }
@@ -189,22 +217,23 @@ __global__ __launch_bounds__(64 * W, DP > 128 || (W == 2 && DP > 64) ? 1 : 2) vo
   if (a.dv != nullptr) store_columns<T, DP>(static_cast<T*>(a.dv) + at * a.dim, dv, 1.f, a.dim);
 }
 
-// dq of kTile W rows.  S^T = K Q^T and dP^T = V dO^T have the keys down a lane's registers
+// dq, kTile rows a wave.  S^T = K Q^T and dP^T = V dO^T have the keys down a lane's registers
 // and one row a lane; dQ^T += K^T dS^T follows.  With splits > 1 each range of `span` keys
 // leaves its sum in `part`.
+// W waves, or 4 to 8 for W = 0
 template <typename T, bool TINY, int DP, int W>
-__global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void att_mma_q(const AttArgs a, int mtiles, int splits,
+__global__ __launch_bounds__(W == 0 ? 512 : 64 * W, DP > 128 ? 1 : 2) void att_mma_q(const AttArgs a, int mtiles, int splits,
                                                                      int64_t span, const float2* __restrict__ stats,
                                                                      float* __restrict__ part) {
   using KTile = LdsTile<T, DP, Reads::kBoth>;
   using VTile = LdsTile<T, DP, Reads::kRows>;
-  constexpr int NT = 64 * W, TS = kTile<T>, KT = 32, OT = DP / TS, ST = DP / kStep;
+  constexpr int TS = kTile<T>, KT = 32, OT = DP / TS, ST = DP / kStep;
   __shared__ __align__(16) T sk[KT * KTile::ROW], sv[KT * VTile::ROW];
   const int group = lane_group<T>(), wave = threadIdx.x / kWave;
   int64_t w = by_die(blockIdx.x, gridDim.x);
   const int sp = static_cast<int>(w % splits);
   w /= splits;
-  const int64_t r0 = w % mtiles * (TS * W) + wave * TS, r = r0 + lane_row<T>();
+  const int64_t r0 = w % mtiles * (TS * (W == 0 ? blockDim.x / kWave : W)) + wave * TS, r = r0 + lane_row<T>();
   const int64_t p = w / mtiles;
   const int hk = static_cast<int>(p % a.kv_heads);
   const int64_t b = p / a.kv_heads;
@@ -229,7 +258,7 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void att_mma_q(const AttA
   int64_t key;
   uint64_t bits;
   bool more = keys.next(key, bits);
-  Stage<T, TINY, KT, DP, NT> k(a.dim), v(a.dim);
+  Stage<T, TINY, KT, DP, (W == 0 ? 4 : W), (W > 0)> k(a.dim), v(a.dim);
   auto fetch = [&]() {
     k.load(kp + key * a.ks[1], a.ks[1], bits, a.dim);
     v.load(vp + key * a.vs[1], a.vs[1], bits, a.dim);
@@ -282,7 +311,7 @@ struct QShape {
   QShape(const AttArgs& a, int dtype) {
     const int64_t rows = a.lq * a.group;
     const int tile = dtype == TGX_BF16 ? 32 : 16;
-    w = a.dim > 128 ? 4 : (rows <= 64 ? 64 : 128) / tile;  // wide heads: as many registers as there are
+    w = a.dim > 128 ? 4 : tile == 32 ? (rows <= 64 ? 2 : 4) : waves_for(ops_cdiv(rows, tile), 4, 8);
     mtiles = static_cast<int>(ops_cdiv(rows, tile * w));
     const int64_t blocks = a.batch * a.kv_heads * mtiles;
     const int64_t tiles = ops_cdiv(std::max<int64_t>(a.lk, 1), 64);
@@ -316,29 +345,31 @@ int att_mma_backward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
     int rc = check_launch("att_stats");
     if (rc) return rc;
     if (a.lk > 0 && (a.dk != nullptr || a.dv != nullptr)) {
-      auto go = [&](auto w) {
-        constexpr int W = decltype(w)::value;
-        const int ktiles = static_cast<int>(ops_cdiv(a.lk, TS * W));
-        hipLaunchKernelGGL((att_mma_kv<T, TINY, DP, W>), dim3(static_cast<unsigned>(a.batch * a.kv_heads * ktiles)),
-                           dim3(64 * W), 0, s, a, ktiles, stats);
+      auto go = [&](auto least) {
+        constexpr int LEAST = decltype(least)::value;
+        const int w = waves_for(ops_cdiv(a.lk, TS), LEAST, kv_most<T>(DP, LEAST));
+        const int ktiles = static_cast<int>(ops_cdiv(a.lk, TS * w));
+        hipLaunchKernelGGL((att_mma_kv<T, TINY, DP, LEAST>), dim3(static_cast<unsigned>(a.batch * a.kv_heads * ktiles)),
+                           dim3(64 * w), 0, s, a, ktiles, stats);
         return check_launch("att_mma_kv");
       };
-      // wide heads: 64 keys a workgroup, as many registers a wave as there are
-      if constexpr (DP > 128) rc = go(std::integral_constant<int, 64 / TS>{});
-      else rc = a.lk <= 64 ? go(std::integral_constant<int, 64 / TS>{}) : go(std::integral_constant<int, 8>{});
+      if constexpr (kTwoWays<T, DP>)
+        rc = a.lk > 160 ? go(std::integral_constant<int, 8>{}) : go(std::integral_constant<int, 2>{});
+      else
+        rc = go(std::integral_constant<int, kKvLeast<T, DP>>{});
       if (rc) return rc;
     }
     if (a.dq == nullptr) return TGX_OK;
     const QShape f(a, dtype);
     auto go = [&](auto w) {
-      constexpr int W = decltype(w)::value;
-      hipLaunchKernelGGL((att_mma_q<T, TINY, DP, W>),
-                         dim3(static_cast<unsigned>(a.batch * a.kv_heads * f.mtiles * f.splits)), dim3(64 * W), 0, s, a,
-                         f.mtiles, f.splits, f.span, stats, part);
+      hipLaunchKernelGGL((att_mma_q<T, TINY, DP, decltype(w)::value>),
+                         dim3(static_cast<unsigned>(a.batch * a.kv_heads * f.mtiles * f.splits)), dim3(64 * f.w), 0, s,
+                         a, f.mtiles, f.splits, f.span, stats, part);
       return check_launch("att_mma_q");
     };
     if constexpr (DP > 128) rc = go(std::integral_constant<int, 4>{});
-    else rc = f.w * TS == 64 ? go(std::integral_constant<int, 64 / TS>{}) : go(std::integral_constant<int, 128 / TS>{});
+    else if constexpr (sizeof(T) == 4) rc = go(std::integral_constant<int, 0>{});
+    else rc = f.w == 2 ? go(std::integral_constant<int, 2>{}) : go(std::integral_constant<int, 4>{});
     return rc || f.splits == 1 ? rc : att_join_sums(a.dq, rows, a.dim, dtype, a.scale, f.splits, part, s);
   });
 }

@@ -11,27 +11,28 @@
 namespace tgx {
 namespace {
 
-// WQ waves share the rows of a workgroup, kTile each; WK > 1: WK waves take the same rows,
-// one tile of each KT = 64 keys each, and are joined at the end.  With splits > 1 the keys
+// The waves of a workgroup take kTile rows each: WQ of them, or 4 to 8 for WQ = 0 (f32,
+// whose 16-row tiles fit odd lengths better); WK > 1: WK
+// waves take the same rows, one tile of each KT = 64 keys each, and are joined at the end.  With splits > 1 the keys
 // are cut in as many ranges of `span` keys and each leaves its maximum, sum and unscaled
 // output in `part` for att_join.
 template <typename T, bool TINY, int DP, int WQ, int WK>
-__global__ __launch_bounds__(64 * WQ * WK, DP > 128 ? 1 : 2) void att_mma_fwd(const AttArgs a, int mtiles, int splits,
+__global__ __launch_bounds__(WQ == 0 ? 512 : 64 * WQ * WK, DP > 128 ? 1 : WQ == 0 && DP <= 112 ? 4 : 2) void att_mma_fwd(const AttArgs a, int mtiles, int splits,
                                                                              int64_t span, const AttParts part) {
   using KTile = LdsTile<T, DP, Reads::kRows>;
   using VTile = LdsTile<T, DP, Reads::kColumns>;
-  constexpr int NT = 64 * WQ * WK, TS = kTile<T>, KT = sizeof(T) == 2 || WK > 1 ? 64 : 32, SUB = KT / TS / WK,
+  constexpr int TS = kTile<T>, KT = sizeof(T) == 2 || WK > 1 ? 64 : 32, SUB = KT / TS / WK,
                 OT = DP / TS, ST = DP / kStep;
-  static_assert(WK == 1 || (WQ == 1 && SUB == 1), "one tile of keys a wave");
+  static_assert(WK == 1 || SUB == 1, "one tile of keys a wave");
   __shared__ __align__(16) T smem[KT * (KTile::ROW + VTile::ROW)];
   T* sk = smem;
   T* sv = smem + KT * KTile::ROW;
   const int lane = threadIdx.x & (kWave - 1), group = lane_group<T>(), wave = threadIdx.x / kWave;
-  const int wq = wave / WK, wk = wave % WK;
+  const int wq = WK > 1 ? 0 : wave, wk = WK > 1 ? wave : 0, waves = WQ == 0 ? blockDim.x / kWave : WQ;
   int64_t w = by_die(blockIdx.x, gridDim.x);
   const int sp = static_cast<int>(w % splits);
   w /= splits;
-  const int64_t r0 = w % mtiles * (TS * WQ) + wq * TS;
+  const int64_t r0 = w % mtiles * (TS * waves) + wq * TS;
   const int64_t p = w / mtiles;
   const int hk = static_cast<int>(p % a.kv_heads);
   const int64_t b = p / a.kv_heads;
@@ -63,7 +64,7 @@ __global__ __launch_bounds__(64 * WQ * WK, DP > 128 ? 1 : 2) void att_mma_fwd(co
   int64_t key;
   uint64_t bits;
   bool more = keys.next(key, bits);
-  Stage<T, TINY, KT, DP, NT> st(a.dim);
+  Stage<T, TINY, KT, DP, (WQ == 0 ? 4 : WQ * WK), (WQ > 0)> st(a.dim);
   if (more) {
     st.load(kp + key * a.ks[1], a.ks[1], bits, a.dim);
     st.template store<KTile::ROW>(sk, a.dim);
@@ -253,7 +254,7 @@ struct FwdShape {
     const int64_t rows = a.lq * a.group;
     const int tile = dtype == TGX_BF16 ? 32 : 16;
     wk = rows <= tile ? 64 / tile : 1;
-    wq = rows <= tile ? 1 : (rows <= 64 ? 64 : 128) / tile;
+    wq = wk > 1 ? 1 : tile == 32 ? (rows <= 64 ? 2 : 4) : waves_for(ops_cdiv(rows, tile), 4, 8);
     mtiles = static_cast<int>(ops_cdiv(rows, tile * wq));
     const int64_t blocks = a.batch * a.kv_heads * mtiles;
     const int64_t tiles = ops_cdiv(std::max<int64_t>(a.lk, 1), 64);
@@ -279,12 +280,15 @@ int att_mma_forward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
     constexpr int DP = decltype(dp)::value, TS = kTile<T>;
     constexpr bool TINY = decltype(tiny)::value;
     const dim3 grid(static_cast<unsigned>(blocks)), block(64 * f.wq * f.wk);
-    if (f.wk > 1)
-      hipLaunchKernelGGL((att_mma_fwd<T, TINY, DP, 1, 64 / TS>), grid, block, 0, s, a, f.mtiles, f.splits, f.span, part);
-    else if (f.wq * TS == 64)
-      hipLaunchKernelGGL((att_mma_fwd<T, TINY, DP, 64 / TS, 1>), grid, block, 0, s, a, f.mtiles, f.splits, f.span, part);
-    else
-      hipLaunchKernelGGL((att_mma_fwd<T, TINY, DP, 128 / TS, 1>), grid, block, 0, s, a, f.mtiles, f.splits, f.span, part);
+    auto go = [&](auto wq, auto wk) {
+      hipLaunchKernelGGL((att_mma_fwd<T, TINY, DP, decltype(wq)::value, decltype(wk)::value>), grid, block, 0, s, a,
+                         f.mtiles, f.splits, f.span, part);
+    };
+    constexpr std::integral_constant<int, 1> one{};
+    if (f.wk > 1) go(one, std::integral_constant<int, 64 / TS>{});
+    else if constexpr (sizeof(T) == 4) go(std::integral_constant<int, 0>{}, one);
+    else if (f.wq == 2) go(std::integral_constant<int, 2>{}, one);
+    else go(std::integral_constant<int, 4>{}, one);
     return check_launch("att_mma_fwd");
   });
   return rc || f.splits == 1 ? rc : att_join_forward(a, dtype, f.splits, part, s);

@@ -217,28 +217,32 @@ constexpr int pow2_at_least(int x) {
   return p;
 }
 
-// NT threads move ROWS rows of up to DP values into an LDS tile: load() issues the reads, store() waits for them and writes.  A thread keeps one column
-// of all its rows, so that a row costs it one address step; lanes past the last column
-// stay idle.
-template <typename T, bool TINY, int ROWS, int DP, int NT>
+// The workgroup's waves, MINW of them (or more, if not FIXED), move ROWS rows of up to DP
+// values into an LDS tile: load() issues the reads, store() waits for them and writes.  A thread keeps
+// one column of all its rows, so that a row costs it one address step; lanes past the last
+// column stay idle.
+template <typename T, bool TINY, int ROWS, int DP, int MINW, bool FIXED>
 struct Stage {
-  static constexpr int V = kWide<T>, LANES = pow2_at_least(DP / V), STEP = NT / LANES,
-                       N = (ROWS + STEP - 1) / STEP;
-  static_assert(N * STEP == ROWS || N == 1, "whole steps");
+  static constexpr int V = kWide<T>, LANES = pow2_at_least(DP / V), N = (ROWS * LANES + 64 * MINW - 1) / (64 * MINW);
   u32x4 x[N];
-  int col, row0;
+  int col, row0, steps;
   bool in;
-  __device__ explicit Stage(int dim) : col(threadIdx.x % LANES * V), row0(threadIdx.x / LANES) {
-    in = col < dim && row0 < ROWS;
+  __device__ explicit Stage(int dim)
+      : col(threadIdx.x % LANES * V), row0(threadIdx.x / LANES), steps(blockDim.x / LANES), in(col < dim) {}
+  __device__ __forceinline__ int step() const { return FIXED ? 64 * MINW / LANES : steps; }
+  __device__ __forceinline__ int row(int n) const { return row0 + n * step(); }
+  __device__ __forceinline__ bool whole(int n) const {  // row n of every thread is a row of the tile
+    return FIXED && (n + 1) * (64 * MINW / LANES) <= ROWS;
   }
   // rows base, base + stride, ...: those whose bit is set, zeros for the others
   __device__ __forceinline__ void load(const T* base, int64_t stride, uint64_t bits, int dim) {
     const T* p = base + row0 * stride;
-    const uint64_t mine = in ? bits >> row0 : 0;
+    const int64_t by = step() * stride;
+    const uint64_t mine = in && row0 < ROWS ? bits >> row0 : 0;
 #pragma unroll
-    for (int n = 0; n < N; ++n, p += STEP * stride) {
+    for (int n = 0; n < N; ++n, p += by) {
       x[n] = u32x4{0, 0, 0, 0};
-      if (mine >> (n * STEP) & 1) x[n] = row_part<T, TINY>(p, col, dim);
+      if ((whole(n) || row(n) < ROWS) && (mine >> (n * step()) & 1)) x[n] = row_part<T, TINY>(p, col, dim);
     }
   }
   // the rows that p(n) gives the addresses of, nullptr for zeros
@@ -247,22 +251,18 @@ struct Stage {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       x[n] = u32x4{0, 0, 0, 0};
-      const T* row = p(n);
-      if (in && row != nullptr) x[n] = row_part<T, TINY>(row, col, dim);
+      const T* at = p(n);
+      if (in && at != nullptr) x[n] = row_part<T, TINY>(at, col, dim);
     }
   }
   template <int ROW>  // values from row to row of the tile
   __device__ __forceinline__ void store(T* tile, int dim) const {
     if (LANES * V > DP && col >= DP) return;
-    if (STEP > ROWS && row0 >= ROWS) return;
-    if (TINY || dim % V == 0) {
+    const bool asis = TINY || dim % V == 0;
 #pragma unroll
-      for (int n = 0; n < N; ++n) *reinterpret_cast<u32x4*>(tile + (row0 + n * STEP) * ROW + col) = x[n];
-    } else {
-#pragma unroll
-      for (int n = 0; n < N; ++n)
-        *reinterpret_cast<u32x4*>(tile + (row0 + n * STEP) * ROW + col) = finish<T>(x[n], col, dim);
-    }
+    for (int n = 0; n < N; ++n)
+      if (whole(n) || row(n) < ROWS)
+        *reinterpret_cast<u32x4*>(tile + row(n) * ROW + col) = asis ? x[n] : finish<T>(x[n], col, dim);
   }
 };
 
@@ -399,6 +399,13 @@ struct Keys {
 __device__ __forceinline__ int64_t by_die(int64_t id, int64_t total) {
   const int64_t q = total / 8, r = total % 8, die = id % 8;
   return die * q + min(die, r) + id / 8;
+}
+
+// Waves of a workgroup for n tiles of rows (or keys): as few workgroups as `most` waves
+// each allow, and then as few waves, but `least`
+inline int waves_for(int64_t n, int least, int most) {
+  const int64_t groups = std::max<int64_t>(ops_cdiv(n, most), 1);
+  return static_cast<int>(std::max<int64_t>(ops_cdiv(n, groups), least));
 }
 
 constexpr int kNoLoads = 0x0f70;  // s_waitcnt: no vector load outstanding
