@@ -43,62 +43,86 @@ struct Place {
   }
 };
 
+// Rows that a group of lanes takes at a time: with one pack a lane, several rows are in
+// flight, share the weights and hide each other's sums.  Lanes that take a whole row side
+// by side touch fewer cache lines than few lanes with more packs each where rows do not
+// begin on a line (786,432 x 172 bf16 rows, forward: 8 lanes of 3 packs 137 us, 32 lanes of
+// one 159, and with four rows 120; backward 206, 202, and with two rows 175).
+constexpr int fwd_rows(int c) { return c == 1 ? 4 : c == 2 ? 2 : 1; }
+constexpr int bwd_rows(int c) { return c == 1 ? 2 : 1; }
+
 template <typename T, typename W, int V, int L, int C>
 __global__ __launch_bounds__(kNormThreads) void norm_fwd(const T* __restrict__ x, int64_t rows, int dim, int64_t stride,
                                                          const W* __restrict__ weight, const W* __restrict__ bias,
                                                          float eps, T* __restrict__ out, float* __restrict__ mean,
                                                          float* __restrict__ rstd) {
+  constexpr int U = fwd_rows(C), G = kNormThreads / L;
   __shared__ float lds[kNormThreads / kWave];
   const Place<V, L> at(dim);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kNormThreads / L) + threadIdx.x / L;
-  const bool live = row < rows;
-  const T* xr = x + (live ? row : 0) * stride;
-  float f[C][V];
-  float s = 0.f;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (G * U) + threadIdx.x / L;
+  Pack<T, V> p[U][C];
 #pragma unroll
-  for (int j = 0; j < C; ++j) {
-    const Pack<T, V> p = load_pack<T, V>(xr + at.at(j));
-    const int skip = at.skip(j);
+  for (int a = 0; a < U; ++a)
 #pragma unroll
-    for (int u = 0; u < V; ++u) {
-      f[j][u] = to_f(p.v[u]);
-      s += u >= skip ? f[j][u] : 0.f;
+    for (int j = 0; j < C; ++j) p[a][j] = load_pack<T, V>(x + min(row0 + a * G, rows - 1) * stride + at.at(j));
+  float m[U], r[U];
+#pragma unroll
+  for (int a = 0; a < U; ++a) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      const int skip = at.skip(j);
+#pragma unroll
+      for (int u = 0; u < V; ++u) s += u >= skip ? to_f(p[a][j].v[u]) : 0.f;
     }
+    m[a] = s;
   }
-  const float m = row_sum<L>(s, lds) / static_cast<float>(dim);
-  float q = 0.f;
 #pragma unroll
-  for (int j = 0; j < C; ++j) {
-    const int skip = at.skip(j);
+  for (int a = 0; a < U; ++a) m[a] = row_sum<L>(m[a], lds) / static_cast<float>(dim);
 #pragma unroll
-    for (int u = 0; u < V; ++u) {
-      f[j][u] -= m;
-      q += u >= skip ? f[j][u] * f[j][u] : 0.f;
+  for (int a = 0; a < U; ++a) {
+    float q = 0.f;
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      const int skip = at.skip(j);
+#pragma unroll
+      for (int u = 0; u < V; ++u) {
+        const float f = to_f(p[a][j].v[u]) - m[a];
+        q += u >= skip ? f * f : 0.f;
+      }
     }
+    r[a] = q;
   }
-  const float r = 1.f / sqrtf(row_sum<L>(q, lds) / static_cast<float>(dim) + eps);
-  if (!live) return;
+#pragma unroll
+  for (int a = 0; a < U; ++a) r[a] = 1.f / sqrtf(row_sum<L>(r[a], lds) / static_cast<float>(dim) + eps);
 #pragma unroll
   for (int j = 0; j < C; ++j) {
     if (at.skip(j) == V) continue;
     const int c = at.at(j);
-    Pack<T, V> p;
     Pack<W, V> w, b;
     if (weight != nullptr) w = load_pack<W, V>(weight + c);
     if (bias != nullptr) b = load_pack<W, V>(bias + c);
 #pragma unroll
-    for (int u = 0; u < V; ++u) {
-      float y = f[j][u] * r;
-      if (weight != nullptr) y *= to_f(w.v[u]);
-      if (bias != nullptr) y += to_f(b.v[u]);
-      p.v[u] = from_f<T>(y);
+    for (int a = 0; a < U; ++a) {
+      if (row0 + a * G >= rows) break;
+      Pack<T, V> o;
+#pragma unroll
+      for (int u = 0; u < V; ++u) {
+        float y = (to_f(p[a][j].v[u]) - m[a]) * r[a];
+        if (weight != nullptr) y *= to_f(w.v[u]);
+        if (bias != nullptr) y += to_f(b.v[u]);
+        o.v[u] = from_f<T>(y);
+      }
+      store_pack<T, V>(out + (row0 + a * G) * dim + c, o);
     }
-    store_pack<T, V>(out + row * dim + c, p);
   }
-  if (at.lane == 0 && mean != nullptr) {
-    mean[row] = m;
-    rstd[row] = r;
-  }
+  if (at.lane == 0 && mean != nullptr)
+#pragma unroll
+    for (int a = 0; a < U; ++a) {
+      if (row0 + a * G >= rows) break;
+      mean[row0 + a * G] = m[a];
+      rstd[row0 + a * G] = r[a];
+    }
 }
 
 // A workgroup takes every gridDim.x-th group of rows.  Its lanes own fixed columns, so
@@ -118,48 +142,68 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd(const T* __restrict__ x
   for (int j = 0; j < C; ++j)
 #pragma unroll
     for (int u = 0; u < V; ++u) aw[j][u] = ab[j][u] = 0.f;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * R;
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * R; base < rows; base += step) {  // workgroup-uniform
-    const int64_t row = base + threadIdx.x / L;
-    const bool live = row < rows;
-    const int64_t rr = live ? row : 0;
-    const float m = mean[rr], r = rstd[rr];
-    Pack<T, V> px[C], pg[C];
+  constexpr int U = bwd_rows(C);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * R * U;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * R * U; base < rows; base += step) {  // workgroup-uniform
+    const int64_t row0 = base + threadIdx.x / L;
+    Pack<T, V> px[U][C], pg[U][C];
+    float m[U], r[U], s1[U], s2[U];
 #pragma unroll
-    for (int j = 0; j < C; ++j) {
-      px[j] = load_pack<T, V>(x + rr * stride + at.at(j));
-      pg[j] = load_pack<T, V>(dy + rr * dim + at.at(j));
+    for (int a = 0; a < U; ++a) {
+      const int64_t row = min(row0 + a * R, rows - 1);
+      m[a] = mean[row];
+      r[a] = rstd[row];
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        px[a][j] = load_pack<T, V>(x + row * stride + at.at(j));
+        pg[a][j] = load_pack<T, V>(dy + row * dim + at.at(j));
+      }
     }
-    float s1 = 0.f, s2 = 0.f;
-    float h[C][V], g[C][V];
+    Pack<W, V> w[C];
 #pragma unroll
-    for (int j = 0; j < C; ++j) {
-      const int skip = live ? at.skip(j) : V;
-      Pack<W, V> w;
-      if (weight != nullptr) w = load_pack<W, V>(weight + at.at(j));
+    for (int j = 0; j < C; ++j)
+      if (weight != nullptr) w[j] = load_pack<W, V>(weight + at.at(j));
 #pragma unroll
-      for (int u = 0; u < V; ++u) {
-        h[j][u] = (to_f(px[j].v[u]) - m) * r;
-        const float d = to_f(pg[j].v[u]);
-        g[j][u] = weight != nullptr ? d * to_f(w.v[u]) : d;
-        if (u >= skip) {
-          s1 += g[j][u];
-          s2 += g[j][u] * h[j][u];
-          aw[j][u] += d * h[j][u];
-          ab[j][u] += d;
+    for (int a = 0; a < U; ++a) {
+      s1[a] = s2[a] = 0.f;
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        const int skip = row0 + a * R < rows ? at.skip(j) : V;
+#pragma unroll
+        for (int u = 0; u < V; ++u) {
+          const float h = (to_f(px[a][j].v[u]) - m[a]) * r[a], d = to_f(pg[a][j].v[u]);
+          const float g = weight != nullptr ? d * to_f(w[j].v[u]) : d;
+          if (u >= skip) {
+            s1[a] += g;
+            s2[a] = fmaf(g, h, s2[a]);
+            aw[j][u] = fmaf(d, h, aw[j][u]);
+            ab[j][u] += d;
+          }
         }
       }
     }
-    s1 = row_sum<L>(s1, lds) / static_cast<float>(dim);
-    s2 = row_sum<L>(s2, lds) / static_cast<float>(dim);
-    if (dx == nullptr || !live) continue;
 #pragma unroll
-    for (int j = 0; j < C; ++j) {
-      if (at.skip(j) == V) continue;
-      Pack<T, V> p;
+    for (int a = 0; a < U; ++a) {
+      s1[a] = row_sum<L>(s1[a], lds) / static_cast<float>(dim);
+      s2[a] = row_sum<L>(s2[a], lds) / static_cast<float>(dim);
+    }
+    if (dx == nullptr) continue;
 #pragma unroll
-      for (int u = 0; u < V; ++u) p.v[u] = from_f<T>(r * (g[j][u] - s1 - h[j][u] * s2));
-      store_pack<T, V>(dx + row * dim + at.at(j), p);
+    for (int a = 0; a < U; ++a) {
+      const int64_t row = row0 + a * R;
+      if (row >= rows) break;
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        if (at.skip(j) == V) continue;
+        Pack<T, V> o;
+#pragma unroll
+        for (int u = 0; u < V; ++u) {
+          const float h = (to_f(px[a][j].v[u]) - m[a]) * r[a], d = to_f(pg[a][j].v[u]);
+          const float g = weight != nullptr ? d * to_f(w[j].v[u]) : d;
+          o.v[u] = from_f<T>(r[a] * (g - s1[a] - h * s2[a]));
+        }
+        store_pack<T, V>(dx + row * dim + at.at(j), o);
+      }
     }
   }
   if (part == nullptr) return;
@@ -224,9 +268,12 @@ __global__ __launch_bounds__(kJoinThreads) void norm_join(const float* __restric
   }
 }
 
-// Calls f(V, L, C) with the lanes and packs a row of `dim` values takes: as few lanes as
-// hold it in up to four packs each, so that a wave works on several short rows.
-template <typename T, typename F>
+// Calls f(V, L, C) with the lanes and packs a row of `dim` values takes: one pack a lane up
+// to 64 lanes, then more, then the whole workgroup.
+// The backward pass of f32 rows of 33 to 64 packs takes 16 lanes of 3 or 4: 393,216 x 172
+// take 169 us so and 193 with 64 lanes (bf16 rows of 512, whose sums take twice the
+// registers, 206 and 165).
+template <typename T, bool GRAD, typename F>
 int by_shape(int64_t dim, F&& f) {
 #define TGX_SHAPE(V, L, C) \
   f(std::integral_constant<int, V>{}, std::integral_constant<int, L>{}, std::integral_constant<int, C>{})
@@ -234,11 +281,14 @@ int by_shape(int64_t dim, F&& f) {
   if (dim < V) return TGX_SHAPE(1, 8, 1);
   const int64_t packs = ops_cdiv(dim, V);
   if (packs <= 8) return TGX_SHAPE(V, 8, 1);
-  if (packs <= 16) return TGX_SHAPE(V, 8, 2);
-  if (packs <= 24) return TGX_SHAPE(V, 8, 3);
-  if (packs <= 32) return TGX_SHAPE(V, 8, 4);
-  if (packs <= 48) return TGX_SHAPE(V, 16, 3);
-  if (packs <= 64) return TGX_SHAPE(V, 16, 4);
+  if (packs <= 16) return TGX_SHAPE(V, 16, 1);
+  if (packs <= 32) return TGX_SHAPE(V, 32, 1);
+  if constexpr (GRAD && sizeof(T) == 4) {
+    if (packs <= 48) return TGX_SHAPE(V, 16, 3);
+    if (packs <= 64) return TGX_SHAPE(V, 16, 4);
+  } else {
+    if (packs <= 64) return TGX_SHAPE(V, 64, 1);
+  }
   if (packs <= 128) return TGX_SHAPE(V, 64, 2);
   if (packs <= 256) return TGX_SHAPE(V, 64, 4);
   if (packs <= 512) return TGX_SHAPE(V, 256, 2);
@@ -290,9 +340,9 @@ extern "C" int tgx_layer_norm(const void* x, int64_t rows, int64_t dim, int64_t 
     using T = decltype(t);
     return by_type(wdtype, [&](auto wt) {
       using W = decltype(wt);
-      return by_shape<T>(dim, [&](auto v, auto l, auto c) {
+      return by_shape<T, false>(dim, [&](auto v, auto l, auto c) {
         constexpr int V = decltype(v)::value, L = decltype(l)::value, C = decltype(c)::value;
-        const unsigned blocks = static_cast<unsigned>(ops_cdiv(rows, kNormThreads / L));
+        const unsigned blocks = static_cast<unsigned>(ops_cdiv(rows, kNormThreads / L * fwd_rows(C)));
         hipLaunchKernelGGL((norm_fwd<T, W, V, L, C>), dim3(blocks), dim3(kNormThreads), 0,
                            static_cast<hipStream_t>(stream), static_cast<const T*>(x), rows, static_cast<int>(dim),
                            stride, static_cast<const W*>(weight), static_cast<const W*>(bias), eps,
@@ -328,7 +378,7 @@ extern "C" int tgx_layer_norm_grad(const void* x, const void* dy, int64_t rows, 
       using T = decltype(t);
       return by_type(wdtype, [&](auto wt) {
         using W = decltype(wt);
-        return by_shape<T>(dim, [&](auto v, auto l, auto c) {
+        return by_shape<T, true>(dim, [&](auto v, auto l, auto c) {
           constexpr int V = decltype(v)::value, L = decltype(l)::value, C = decltype(c)::value;
           hipLaunchKernelGGL((norm_bwd<T, W, V, L, C>), dim3(static_cast<unsigned>(blocks)), dim3(kNormThreads), 0, s,
                              static_cast<const T*>(x), static_cast<const T*>(dy), rows, static_cast<int>(dim), stride,
