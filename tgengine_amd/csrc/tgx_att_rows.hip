@@ -15,41 +15,68 @@ namespace {
 constexpr int kRowThreads = 256;
 constexpr int kRowWaves = kRowThreads / kWave;
 
-// A lane's C packs of rows of `dim` values: pack j covers columns [col(j), col(j) + V)
-template <typename T, int LP, int C>
+// A lane's C packs of rows of `dim` values, the j-th from column col(j) on.  The row's last
+// pack, which is some lane's last, ends with the row and may overlap the one before: both
+// lanes then come to the same values there, and a dot product takes them from one (own()).
+// TINY: rows of fewer than V values, read and written one by one.
+template <typename T, bool TINY, int LP, int C>
 struct Lanes {
-  static constexpr int V = kWide<T>;
-  int gl, dim;
-  __device__ explicit Lanes(int dim_) : gl(threadIdx.x & (LP - 1)), dim(dim_) {}
-  __device__ int col(int j) const { return (j * LP + gl) * V; }
-  __device__ __forceinline__ void read(u32x4 (&x)[C], const T* row) const {  // as in memory
+  static constexpr int V = kWide<T>, N = C * V;
+  int gl, dim, last;  // last: column of the last pack
+  bool on;            // the last pack is within the row
+  __device__ explicit Lanes(int dim_) : gl(threadIdx.x & (LP - 1)), dim(dim_) {
+    last = ((C - 1) * LP + gl) * V;
+    on = last < dim;
+    if (!TINY) last = min(last, dim - V);
+  }
+  __device__ __forceinline__ int col(int j) const { return j == C - 1 ? last : (j * LP + gl) * V; }
+  __device__ __forceinline__ bool has(int j) const { return j < C - 1 || on; }
+  __device__ __forceinline__ void read(u32x4 (&x)[C], const T* row) const {
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       x[j] = u32x4{0, 0, 0, 0};
-      if (row != nullptr && col(j) < dim) x[j] = row_part(row, col(j), dim);
+      if (row == nullptr || !has(j)) continue;
+      if constexpr (TINY) x[j] = row_part<T, true>(row, col(j), dim);
+      else x[j] = load16(row + col(j));
     }
   }
-  __device__ __forceinline__ void values(float (&f)[C * V], const u32x4 (&x)[C]) const {
+  __device__ __forceinline__ static void values(float (&f)[N], const u32x4 (&x)[C]) {
 #pragma unroll
     for (int j = 0; j < C; ++j) {
-      const Pack<T, V> p = __builtin_bit_cast(Pack<T, V>, dim < V ? x[j] : finish<T>(x[j], col(j), dim));
+      const Pack<T, V> p = __builtin_bit_cast(Pack<T, V>, x[j]);
 #pragma unroll
       for (int u = 0; u < V; ++u) f[j * V + u] = to_f(p.v[u]);
     }
   }
-  __device__ __forceinline__ void load(float (&f)[C * V], const T* row) const {
+  __device__ __forceinline__ void load(float (&f)[N], const T* row) const {
     u32x4 x[C];
     read(x, row);
     values(f, x);
   }
-  __device__ __forceinline__ void store(T* row, const float (&f)[C * V]) const {
+  // the last pack without what the lane before has too
+  __device__ __forceinline__ void own(float (&z)[V], const float (&f)[N]) const {
+    const int twice = TINY ? 0 : ((C - 1) * LP + gl) * V - last;
+#pragma unroll
+    for (int u = 0; u < V; ++u) z[u] = u >= twice ? f[(C - 1) * V + u] : 0.f;
+  }
+  __device__ __forceinline__ static float dot(const float (&q)[N], const float (&z)[V], const float (&f)[N]) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < N - V; ++i) s = fmaf(q[i], f[i], s);
+#pragma unroll
+    for (int u = 0; u < V; ++u) s = fmaf(z[u], f[N - V + u], s);
+    return group_sum<LP>(s);
+  }
+  template <typename U>
+  __device__ __forceinline__ void store(U* row, const float (&f)[N]) const {
 #pragma unroll
     for (int j = 0; j < C; ++j) {
-      Pack<T, V> p;
+      if (!has(j)) continue;
+      Pack<U, V> p;
 #pragma unroll
-      for (int u = 0; u < V; ++u) p.v[u] = from_f<T>(f[j * V + u]);
-      if (col(j) + V <= dim) {
-        store_pack<T, V>(row + col(j), p);
+      for (int u = 0; u < V; ++u) p.v[u] = from_f<U>(f[j * V + u]);
+      if constexpr (!TINY) {
+        store_pack<U, V>(row + col(j), p);
       } else {
 #pragma unroll
         for (int u = 0; u < V; ++u)
@@ -58,14 +85,6 @@ struct Lanes {
     }
   }
 };
-
-template <int N>
-__device__ __forceinline__ float dot(const float (&x)[N], const float (&y)[N]) {
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) s += x[i] * y[i];
-  return s;
-}
 
 // What a wave works on: problem (b, hk), keys [lo, hi) in tiles of 64 from lo + 64 part on,
 // every wpp-th
@@ -92,23 +111,24 @@ struct RowUnit {
   }
 };
 
-template <typename T, int LP, int C, int M>
-__global__ __launch_bounds__(kRowThreads) void att_rows_fwd(const AttArgs a, int wpp, int splits, int64_t span,
+template <typename T, bool TINY, int LP, int C, int M>
+__global__ __launch_bounds__(kRowThreads, M == 1 && C < 4 ? 3 : 2) void att_rows_fwd(const AttArgs a, int wpp, int splits, int64_t span,
                                                             const AttParts part) {
   constexpr int V = kWide<T>, N = C * V, G = kWave / LP, U = M == 1 ? 4 : 2;
   __shared__ float join[kRowWaves][M][LP * N + 2];
   const int lane = threadIdx.x & (kWave - 1), grp = lane / LP, wave = threadIdx.x / kWave;
   const RowUnit w(a, wpp, splits, span);
   if (!w.live) return;  // wpp = 1 only: no barrier follows
-  const Lanes<T, LP, C> at(a.dim);
+  const Lanes<T, TINY, LP, C> at(a.dim);
   const int rows = static_cast<int>(a.lq) * a.group;
   const T* kp = static_cast<const T*>(a.k) + w.b * a.ks[0] + w.hk * a.ks[2];
   const T* vp = static_cast<const T*>(a.v) + w.b * a.vs[0] + w.hk * a.vs[2];
-  float q[M][N], acc[M][N], m[M], l[M];
+  float q[M][N], qo[M][V], acc[M][N], m[M], l[M];
 #pragma unroll
   for (int r = 0; r < M; ++r) {
     const int i = r / a.group, head = w.hk * a.group + r % a.group;
     at.load(q[r], r < rows ? static_cast<const T*>(a.q) + w.b * a.qs[0] + i * a.qs[1] + head * a.qs[2] : nullptr);
+    at.own(qo[r], q[r]);
 #pragma unroll
     for (int x = 0; x < N; ++x) acc[r][x] = 0.f;
     m[r] = -INFINITY;
@@ -117,6 +137,7 @@ __global__ __launch_bounds__(kRowThreads) void att_rows_fwd(const AttArgs a, int
   const float c = a.scale * kLog2e;
   for (int64_t t = w.lo + w.part * 64; t < w.hi; t += wpp * 64) {  // wave-uniform
     const uint64_t bits = w.kept(a, t);
+#pragma unroll 1
     for (int k0 = 0; k0 < 64; k0 += G * U) {
       const uint64_t here = G * U == 64 ? bits : bits >> k0 & ((uint64_t(1) << (G * U % 64)) - 1);
       if (here == 0) continue;
@@ -138,7 +159,7 @@ __global__ __launch_bounds__(kRowThreads) void att_rows_fwd(const AttArgs a, int
         at.values(f, kx[u]);
 #pragma unroll
         for (int r = 0; r < M; ++r) {
-          const float x = group_sum<LP>(dot(q[r], f)) * c;
+          const float x = at.dot(q[r], qo[r], f) * c;
           s[r][u] = here >> (u * G + grp) & 1 ? x : -INFINITY;
         }
       }
@@ -226,9 +247,7 @@ __global__ __launch_bounds__(kRowThreads) void att_rows_fwd(const AttArgs a, int
     if (splits > 1) {
       float* out = part.o + (row * splits + w.sp) * a.dim;
       if (at.gl == 0) part.ml[row * splits + w.sp] = make_float2(m[r], l[r]);
-#pragma unroll
-      for (int x = 0; x < N; ++x)
-        if (at.col(x / V) + x % V < a.dim) out[at.col(x / V) + x % V] = acc[r][x];
+      at.store(out, acc[r]);
       continue;
     }
     const float inv = l[r] > 0.f ? 1.f / l[r] : 0.f;
@@ -239,20 +258,20 @@ __global__ __launch_bounds__(kRowThreads) void att_rows_fwd(const AttArgs a, int
   }
 }
 
-template <typename T, int LP, int C, int M>
-__global__ __launch_bounds__(kRowThreads) void att_rows_bwd(const AttArgs a, int wpp, int splits, int64_t span,
+template <typename T, bool TINY, int LP, int C, int M>
+__global__ __launch_bounds__(kRowThreads, M == 1 ? (C < 4 ? 3 : 2) : (C < 4 ? 2 : 1)) void att_rows_bwd(const AttArgs a, int wpp, int splits, int64_t span,
                                                             float* __restrict__ part) {
-  constexpr int V = kWide<T>, N = C * V, G = kWave / LP, U = M == 1 && C <= 3 ? 4 : 2;
+  constexpr int V = kWide<T>, N = C * V, G = kWave / LP, U = M == 1 ? 2 : 1;
   __shared__ float join[kRowWaves][M][LP * N];
   const int lane = threadIdx.x & (kWave - 1), grp = lane / LP, wave = threadIdx.x / kWave;
   const RowUnit w(a, wpp, splits, span);
   if (!w.live) return;  // wpp = 1 only: no barrier follows
-  const Lanes<T, LP, C> at(a.dim);
+  const Lanes<T, TINY, LP, C> at(a.dim);
   const int rows = static_cast<int>(a.lq) * a.group;
   const T* kp = static_cast<const T*>(a.k) + w.b * a.ks[0] + w.hk * a.ks[2];
   const T* vp = static_cast<const T*>(a.v) + w.b * a.vs[0] + w.hk * a.vs[2];
   const int64_t key0 = w.b * a.lk * a.kv_heads + w.hk;
-  float q[M][N], g[M][N], dq[M][N], lse[M], delta[M];
+  float q[M][N], g[M][N], qo[M][V], go[M][V], dq[M][N], lse[M], delta[M];
 #pragma unroll
   for (int r = 0; r < M; ++r) {
     const bool in = r < rows;
@@ -262,7 +281,9 @@ __global__ __launch_bounds__(kRowThreads) void att_rows_bwd(const AttArgs a, int
     at.load(q[r], in ? static_cast<const T*>(a.q) + w.b * a.qs[0] + i * a.qs[1] + head * a.qs[2] : nullptr);
     at.load(g[r], in ? static_cast<const T*>(a.dout) + row * a.dim : nullptr);
     at.load(o, in ? static_cast<const T*>(a.out) + row * a.dim : nullptr);
-    delta[r] = group_sum<LP>(dot(g[r], o));
+    at.own(qo[r], q[r]);
+    at.own(go[r], g[r]);
+    delta[r] = at.dot(g[r], go[r], o);
     lse[r] = in ? a.lse[row] * kLog2e : INFINITY;
     if (lse[r] == -INFINITY) lse[r] = INFINITY;  // no key kept: p = 0
 #pragma unroll
@@ -271,6 +292,7 @@ __global__ __launch_bounds__(kRowThreads) void att_rows_bwd(const AttArgs a, int
   const float c = a.scale * kLog2e;
   for (int64_t t = w.lo + w.part * 64; t < w.hi; t += wpp * 64) {  // wave-uniform
     const uint64_t bits = w.kept(a, t);
+#pragma unroll 1
     for (int k0 = 0; k0 < 64 && t + k0 < w.hi; k0 += G * U) {
       u32x4 kx[U][C], vx[U][C];
 #pragma unroll
@@ -289,7 +311,7 @@ __global__ __launch_bounds__(kRowThreads) void att_rows_bwd(const AttArgs a, int
         for (int x = 0; x < N; ++x) dk[x] = dv[x] = 0.f;
 #pragma unroll
         for (int r = 0; r < M; ++r) {
-          const float s = group_sum<LP>(dot(q[r], f)) * c, dp = group_sum<LP>(dot(g[r], y));
+          const float s = at.dot(q[r], qo[r], f) * c, dp = at.dot(g[r], go[r], y);
           const float p = bits >> j & 1 ? exp2_(s - lse[r]) : 0.f;
           const float ds = p * (dp - delta[r]) * a.scale;
 #pragma unroll
@@ -337,9 +359,7 @@ __global__ __launch_bounds__(kRowThreads) void att_rows_bwd(const AttArgs a, int
       at.store(static_cast<T*>(a.dq) + row * a.dim, dq[r]);
       continue;
     }
-#pragma unroll
-    for (int x = 0; x < N; ++x)
-      if (at.col(x / V) + x % V < a.dim) part[(row * splits + w.sp) * a.dim + at.col(x / V) + x % V] = dq[r][x];
+    at.store(part + (row * splits + w.sp) * a.dim, dq[r]);
   }
 }
 
@@ -359,26 +379,29 @@ struct RowShape {
   }
 };
 
-// calls f(T{}, LP, C, M) with the lanes and packs that a head of `dim` values takes
+// calls f(T{}, TINY, LP, C, M) with the lanes and packs that a head of `dim` values takes
 template <typename F>
 int by_lanes(int dtype, int dim, int64_t rows, F&& f) {
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    auto with = [&](auto lp, auto c) {
-      if (rows == 1) return f(t, lp, c, std::integral_constant<int, 1>{});
-      return f(t, lp, c, std::integral_constant<int, kMostRows>{});
+    auto with = [&](auto lp, auto c, auto tiny) {
+      if (rows == 1) return f(t, tiny, lp, c, std::integral_constant<int, 1>{});
+      return f(t, tiny, lp, c, std::integral_constant<int, kMostRows>{});
     };
     const int packs = static_cast<int>(ops_cdiv(dim, kWide<T>));
-#define TGX_LANES(LP, C) with(std::integral_constant<int, LP>{}, std::integral_constant<int, C>{})
+#define TGX_LANES(LP, C) with(std::integral_constant<int, LP>{}, std::integral_constant<int, C>{}, std::false_type{})
+    if (dim < kWide<T>) return with(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{}, std::true_type{});
     if (packs <= 8) return TGX_LANES(8, 1);
-    if (packs <= 16) return TGX_LANES(8, 2);
-    if (packs <= 24) return TGX_LANES(8, 3);
-    if (sizeof(T) == 2 || packs <= 32) return TGX_LANES(8, 4);
     if constexpr (sizeof(T) == 4) {
+      if (packs <= 16) return TGX_LANES(8, 2);
+      if (packs <= 24) return TGX_LANES(8, 3);
+      if (packs <= 32) return TGX_LANES(8, 4);
       if (packs <= 48) return TGX_LANES(16, 3);
       return TGX_LANES(16, 4);
+    } else {  // a pack is eight values: more lanes with fewer of them
+      if (packs <= 16) return rows == 1 ? TGX_LANES(8, 2) : TGX_LANES(16, 1);
+      return TGX_LANES(16, 2);
     }
-    return TGX_OK;
 #undef TGX_LANES
   });
 }
@@ -392,8 +415,9 @@ size_t att_rows_forward_workspace(const AttArgs& a) {
 int att_rows_forward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
   const RowShape f(a);
   const AttParts part(ws, a.batch * a.lq * a.heads, f.splits);
-  const int rc = by_lanes(dtype, a.dim, a.lq * a.group, [&](auto t, auto lp, auto c, auto m) {
-    hipLaunchKernelGGL((att_rows_fwd<decltype(t), decltype(lp)::value, decltype(c)::value, decltype(m)::value>),
+  const int rc = by_lanes(dtype, a.dim, a.lq * a.group, [&](auto t, auto tiny, auto lp, auto c, auto m) {
+    hipLaunchKernelGGL((att_rows_fwd<decltype(t), decltype(tiny)::value, decltype(lp)::value, decltype(c)::value,
+                                     decltype(m)::value>),
                        dim3(static_cast<unsigned>(f.blocks)), dim3(kRowThreads), 0, s, a, f.wpp, f.splits, f.span, part);
     return check_launch("att_rows_fwd");
   });
@@ -408,8 +432,9 @@ size_t att_rows_backward_workspace(const AttArgs& a) {
 int att_rows_backward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
   const RowShape f(a);
   float* part = static_cast<float*>(ws);
-  const int rc = by_lanes(dtype, a.dim, a.lq * a.group, [&](auto t, auto lp, auto c, auto m) {
-    hipLaunchKernelGGL((att_rows_bwd<decltype(t), decltype(lp)::value, decltype(c)::value, decltype(m)::value>),
+  const int rc = by_lanes(dtype, a.dim, a.lq * a.group, [&](auto t, auto tiny, auto lp, auto c, auto m) {
+    hipLaunchKernelGGL((att_rows_bwd<decltype(t), decltype(tiny)::value, decltype(lp)::value, decltype(c)::value,
+                                     decltype(m)::value>),
                        dim3(static_cast<unsigned>(f.blocks)), dim3(kRowThreads), 0, s, a, f.wpp, f.splits, f.span, part);
     return check_launch("att_rows_bwd");
   });

@@ -71,9 +71,16 @@ AttArgs att_args(const tgx_attention_args* p) {
   return a;
 }
 
-bool by_rows(const AttArgs& a, int dtype) {
+// Whether a call takes the kernels of tgx_att_rows.hip.  A backward pass of at most 4 rows
+// a problem does (2,000 x 2 problems of 4 rows and 64 keys, dim 128: 80 us in bf16 and 133
+// in f32, against 158 and 249 of the matrix units), and a forward pass of one row (f32, 64
+// keys: 42 us against 71; 10,000 keys, 8 x 2 problems: 37 against 50).  More rows take a
+// vector kernel several times as many instructions and the matrix units none: above 64 keys
+// they go there (500 x 2 problems of 4 rows and 256 keys, bf16: 37 us here, 26 there; at 20
+// keys, 2,000 x 2 problems: 20 here, 30 there).
+bool by_rows(const AttArgs& a, bool grad) {
   const int64_t rows = a.lq * a.group;
-  return rows <= kMostRows && (rows == 1 || dtype == TGX_F32 || a.lk <= 256);
+  return rows <= kMostRows && (grad || rows == 1 || a.lk <= 64);
 }
 
 }  // namespace
@@ -85,7 +92,7 @@ extern "C" size_t tgx_attention_workspace_size(const tgx_attention_args* args) {
   if (check_attention("tgx_attention", args, false)) return 0;
   const AttArgs a = att_args(args);
   if (a.batch * a.lq == 0) return 0;
-  return by_rows(a, args->dtype) ? att_rows_forward_workspace(a) : att_mma_forward_workspace(a, args->dtype);
+  return by_rows(a, false) ? att_rows_forward_workspace(a) : att_mma_forward_workspace(a, args->dtype);
 }
 
 extern "C" int tgx_attention(const tgx_attention_args* args, void* stream) {
@@ -94,10 +101,10 @@ extern "C" int tgx_attention(const tgx_attention_args* args, void* stream) {
   const AttArgs a = att_args(args);
   if (a.batch * a.lq == 0) return TGX_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const size_t need = by_rows(a, args->dtype) ? att_rows_forward_workspace(a) : att_mma_forward_workspace(a, args->dtype);
+  const size_t need = by_rows(a, false) ? att_rows_forward_workspace(a) : att_mma_forward_workspace(a, args->dtype);
   if (need > args->workspace_bytes || (need > 0 && !aligned16(args->workspace)))
     return fail(TGX_ERR_ARG, "tgx_attention: workspace of %zu bytes, 16-byte aligned, needed", need);
-  return by_rows(a, args->dtype) ? att_rows_forward(a, args->dtype, args->workspace, s)
+  return by_rows(a, false) ? att_rows_forward(a, args->dtype, args->workspace, s)
                     : att_mma_forward(a, args->dtype, args->workspace, s);
 }
 
@@ -105,7 +112,7 @@ extern "C" size_t tgx_attention_grad_workspace_size(const tgx_attention_args* ar
   if (check_attention("tgx_attention_grad", args, false)) return 0;
   const AttArgs a = att_args(args);
   if (a.batch * a.lq == 0) return 0;
-  return by_rows(a, args->dtype) ? att_rows_backward_workspace(a) : att_mma_backward_workspace(a, args->dtype);
+  return by_rows(a, true) ? att_rows_backward_workspace(a) : att_mma_backward_workspace(a, args->dtype);
 }
 
 extern "C" int tgx_attention_grad(const tgx_attention_args* args, void* stream) {
@@ -119,9 +126,9 @@ extern "C" int tgx_attention_grad(const tgx_attention_args* args, void* stream) 
       if (const int e = fill_zero(p, p != nullptr ? bytes : 0, s)) return e;
     return TGX_OK;
   }
-  const size_t need = by_rows(a, args->dtype) ? att_rows_backward_workspace(a) : att_mma_backward_workspace(a, args->dtype);
+  const size_t need = by_rows(a, true) ? att_rows_backward_workspace(a) : att_mma_backward_workspace(a, args->dtype);
   if (need > args->workspace_bytes || (need > 0 && !aligned16(args->workspace)))
     return fail(TGX_ERR_ARG, "tgx_attention_grad: workspace of %zu bytes, 16-byte aligned, needed", need);
-  return by_rows(a, args->dtype) ? att_rows_backward(a, args->dtype, args->workspace, s)
+  return by_rows(a, true) ? att_rows_backward(a, args->dtype, args->workspace, s)
                     : att_mma_backward(a, args->dtype, args->workspace, s);
 }

@@ -106,9 +106,11 @@ __global__ __launch_bounds__(kClipThreads) void clip_scale(const ClipList l, int
   if (blockIdx.x >= l.first[l.count]) return;  // a launch of no parts still writes the norm
   float by = max_norm / (total + 1e-6f);
   by = by > 1.f ? 1.f : by;  // NaN stays
-  const int t = tensor_of(l, blockIdx.x);
+  // from the last part to the first: what the sums read last is still in the caches
+  const uint32_t at = l.first[l.count] - 1 - blockIdx.x;
+  const int t = tensor_of(l, at);
   if (by == 1.f && l.in[t] == l.out[t]) return;  // nothing changes
-  const int64_t lo = (blockIdx.x - l.first[t]) * per;
+  const int64_t lo = (at - l.first[t]) * per;
   const int64_t hi = lo + per < l.size[t] ? lo + per : l.size[t];
   if (l.in_bf16[t]) {
     if (l.out_bf16[t]) scaled(static_cast<const bf16*>(l.in[t]), static_cast<bf16*>(l.out[t]), lo, hi, by);

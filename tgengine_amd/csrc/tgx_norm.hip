@@ -270,9 +270,9 @@ __global__ __launch_bounds__(kJoinThreads) void norm_join(const float* __restric
 
 // Calls f(V, L, C) with the lanes and packs a row of `dim` values takes: one pack a lane up
 // to 64 lanes, then more, then the whole workgroup.
-// The backward pass of f32 rows of 33 to 64 packs takes 16 lanes of 3 or 4: 393,216 x 172
-// take 169 us so and 193 with 64 lanes (bf16 rows of 512, whose sums take twice the
-// registers, 206 and 165).
+// The backward pass of f32 rows of 33 to 64 packs takes 16 lanes of 3 or 4: 264,192 x 256
+// take 163 us so and 169 with 64 lanes, 393,216 x 172 189 and 193 (bf16 rows of 512, whose
+// sums take twice the registers, 206 and 165).
 template <typename T, bool GRAD, typename F>
 int by_shape(int64_t dim, F&& f) {
 #define TGX_SHAPE(V, L, C) \

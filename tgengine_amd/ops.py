@@ -70,7 +70,8 @@ def clip_grad_norm_(grads: Union[Tensor, Iterable[Tensor]], max_norm: float,
     """
     if isinstance(grads, Tensor):
         grads = [grads]
-    grads = [g.grad if isinstance(g, torch.nn.Parameter) else g for g in grads]
+    # a Parameter's isinstance check runs Python code: plain tensors skip it
+    grads = [g if type(g) is Tensor or not isinstance(g, torch.nn.Parameter) else g.grad for g in grads]
     if out is None:
         grads = [g for g in grads if g is not None]
         if not grads:
