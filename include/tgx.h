@@ -499,7 +499,9 @@ typedef struct tgx_attention_args {
   int32_t reserved;
   void* out;
   float* lse;
-  /* tgx_attention_grad: out and lse as tgx_attention wrote them, grad_out
+  void* out_rest;          /* TGX_BF16: NULL, or [batch, lq, heads, dim] for what rounding took
+                              from out, which the gradient's inner products then add again */
+  /* tgx_attention_grad: out, lse and out_rest as tgx_attention wrote them, grad_out
    * [batch, lq, heads, dim]; grad_q of q's shape, grad_k and grad_v
    * [batch, lk, kv_heads, dim], each may be NULL */
   const void* grad_out;

@@ -97,7 +97,7 @@ class TgxAttentionArgs(ctypes.Structure):
                 ("lk", c_i64), ("heads", c_i32), ("kv_heads", c_i32), ("dim", c_i32), ("dtype", c_i32),
                 ("q_stride", c_i64 * 3), ("k_stride", c_i64 * 3), ("v_stride", c_i64 * 3),
                 ("mask_stride", c_i64), ("scale", ctypes.c_float), ("reserved", c_i32), ("out", c_vp),
-                ("lse", c_vp), ("grad_out", c_vp), ("grad_q", c_vp), ("grad_k", c_vp), ("grad_v", c_vp),
+                ("lse", c_vp), ("out_rest", c_vp), ("grad_out", c_vp), ("grad_q", c_vp), ("grad_k", c_vp), ("grad_v", c_vp),
                 ("workspace", c_vp), ("workspace_bytes", ctypes.c_size_t)]
 
 

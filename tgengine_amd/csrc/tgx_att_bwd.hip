@@ -17,10 +17,17 @@ namespace {
 
 constexpr int kDeltaLanes = 16;
 
+// keys of a row of kept scores: whole 16-byte pieces
+__host__ __device__ __forceinline__ int64_t scores_row(int64_t lk) { return (lk + 3) / 4 * 4; }
+
 // Per row, in the order of problems and their rows: its log sum in units of log 2 (+inf
-// for a row that keeps no key: its probabilities are then zeros) and delta
+// for a row that keeps no key: its probabilities are then zeros) and delta, from the output
+// as it was before rounding where its rest was kept: delta's error reaches every score of
+// the row alike, and with ds rounded too dq was up to 1.52 times as far off as its own
+// rounding
 template <typename T>
-__global__ __launch_bounds__(256) void att_stats(const T* __restrict__ out, const T* __restrict__ dout,
+__global__ __launch_bounds__(256) void att_stats(const T* __restrict__ out, const T* __restrict__ rest,
+                                                 const T* __restrict__ dout,
                                                  const float* __restrict__ lse, int64_t rows, int64_t lq, int heads,
                                                  int group, int dim, float2* __restrict__ stats) {
   constexpr int V = kWide<T>;
@@ -33,6 +40,11 @@ __global__ __launch_bounds__(256) void att_stats(const T* __restrict__ out, cons
     const Pack<T, V> y = __builtin_bit_cast(Pack<T, V>, row_values(dout + at, c, dim));
 #pragma unroll
     for (int u = 0; u < V; ++u) s += to_f(x.v[u]) * to_f(y.v[u]);
+    if (sizeof(T) == 2 && rest != nullptr) {
+      const Pack<T, V> z = __builtin_bit_cast(Pack<T, V>, row_values(rest + at, c, dim));
+#pragma unroll
+      for (int u = 0; u < V; ++u) s += to_f(z.v[u]) * to_f(y.v[u]);
+    }
   }
   s = group_sum<kDeltaLanes>(s);
   if (lane != 0 || row >= rows) return;
@@ -57,6 +69,8 @@ __device__ __forceinline__ void one_by_one() {
 // The rows' tiles stand in LDS twice, so that one is filled while the other is read and a
 // tile takes one barrier.
 //
+// KEEP (f32): ds goes to `scores`, rows of scores_row() keys, for att_scores_q.
+//
 // LEAST to kv_most() waves a workgroup.  bf16 heads of 65 to 128 values come two ways: 8
 // waves, which leaves each the registers for one row of staging and two waves a SIMD, or 2
 // to 4 with all registers, where there are few keys.
@@ -70,9 +84,9 @@ constexpr int kv_most(int dp, int least) {
   return sizeof(T) == 2 && dp > 64 && least < 8 ? 4 : 8;
 }
 
-template <typename T, bool TINY, int DP, int LEAST>
+template <typename T, bool TINY, int DP, int LEAST, bool KEEP>
 __global__ __launch_bounds__(64 * kv_most<T>(DP, LEAST), DP > 128 || (sizeof(T) == 2 && DP > 64 && LEAST < 8) ? 1 : 2)
-void att_mma_kv(const AttArgs a, int ktiles, const float2* __restrict__ stats) {
+void att_mma_kv(const AttArgs a, int ktiles, const float2* __restrict__ stats, float* __restrict__ scores) {
   using Tile = LdsTile<T, DP, Reads::kBoth>;
   using Own = LdsTile<T, DP, Reads::kRows>;
   constexpr int TS = kTile<T>, R = TS, OT = DP / TS, ST = DP / kStep, W = LEAST;
@@ -197,6 +211,13 @@ void att_mma_kv(const AttArgs a, int ktiles, const float2* __restrict__ stats) {
         one_by_one<T>();
 #pragma unroll
         for (int i = 0; i < kRegs<T>; ++i) dp[i] = s[i] * (dp[i] - sdelta[cur][mma_row<T>(i, group)]);
+        if constexpr (KEEP) {
+          float* to = scores + (p * rows + first) * scores_row(a.lk) + j;
+          if (j < scores_row(a.lk))
+#pragma unroll
+            for (int i = 0; i < kRegs<T>; ++i)
+              if (first + mma_row<T>(i, group) < rows) to[mma_row<T>(i, group) * scores_row(a.lk)] = dp[i];
+        }
         one_by_one<T>();
 #pragma unroll
         for (int f = 0; f < kFrags<T>; ++f) {
@@ -220,6 +241,71 @@ void att_mma_kv(const AttArgs a, int ktiles, const float2* __restrict__ stats) {
 // dq, kTile rows a wave.  S^T = K Q^T and dP^T = V dO^T have the keys down a lane's registers
 // and one row a lane; dQ^T += K^T dS^T follows.  With splits > 1 each range of `span` keys
 // leaves its sum in `part`.
+// f32's dq from the ds that att_mma_kv kept: one product where att_mma_q takes three, for
+// the writing and reading of the scores.  16 rows a wave, 4 to 8 waves; a wave reads its
+// rows' scores as fragments.
+template <bool TINY, int DP>
+__global__ __launch_bounds__(512, 2) void att_scores_q(const AttArgs a, int mtiles, const float* __restrict__ scores) {
+  using T = float;
+  using KTile = LdsTile<T, DP, Reads::kColumns>;
+  constexpr int TS = kTile<T>, KT = 32, OT = DP / TS;
+  __shared__ __align__(16) T sk[2][KT * KTile::ROW];
+  const int group = lane_group<T>(), wave = threadIdx.x / kWave;
+  const int64_t w = by_die(blockIdx.x, gridDim.x);
+  const int64_t r0 = w % mtiles * (TS * (blockDim.x / kWave)) + wave * TS, r = r0 + lane_row<T>();
+  const int64_t p = w / mtiles;
+  const int hk = static_cast<int>(p % a.kv_heads);
+  const int64_t b = p / a.kv_heads;
+  const int64_t rows = a.lq * a.group, ks = scores_row(a.lk);
+  const bool busy = r0 < rows;  // a wave past the last row only helps to move keys
+  const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[2];
+  scores += (p * rows + (r < rows ? r : 0)) * ks + 4 * group;
+  Acc<T> dq[OT];
+#pragma unroll
+  for (int t = 0; t < OT; ++t) dq[t] = Acc<T>{};
+  Keys<KT> keys(a.mask == nullptr ? nullptr : a.mask + b * a.mask_stride, 0, a.lk);
+  int64_t key;
+  uint64_t bits;
+  bool more = keys.next(key, bits);
+  Stage<T, TINY, KT, DP, 4, false> k(a.dim);
+  u32x4 next[KT / TS] = {};
+  auto fetch = [&]() {
+    k.load(kp + key * a.ks[1], a.ks[1], bits, a.dim);
+#pragma unroll
+    for (int u = 0; u < KT / TS; ++u) {
+      next[u] = u32x4{0, 0, 0, 0};
+      // tiles that keep no key were not written
+      if (r < rows && (bits >> (u * TS) & 0xffff) != 0 && key + u * TS + 4 * group < ks)
+        next[u] = load16(scores + key + u * TS);
+    }
+  };
+  if (more) {
+    fetch();
+    k.template store<KTile::ROW>(sk[0], a.dim);
+  }
+  for (int cur = 0; more; cur ^= 1) {  // workgroup-uniform
+    u32x4 ds[KT / TS];
+#pragma unroll
+    for (int u = 0; u < KT / TS; ++u) ds[u] = next[u];
+    const uint32_t now = static_cast<uint32_t>(bits);
+    __syncthreads();
+    more = keys.next(key, bits);
+    if (more) fetch();
+    if (busy) {
+#pragma unroll
+      for (int u = 0; u < KT / TS; ++u)
+        if ((now >> (u * TS) & 0xffff) != 0)
+#pragma unroll
+          for (int t = 0; t < OT; ++t) dq[t] = mma<T>(dq[t], KTile::transposed(sk[cur], u * TS, 0, t), ds[u]);
+    }
+    if (more) k.template store<KTile::ROW>(sk[cur ^ 1], a.dim);
+  }
+  if (r >= rows) return;
+  const int64_t tok = r / a.group;
+  const int head = hk * a.group + static_cast<int>(r - tok * a.group);
+  store_columns<T, DP>(static_cast<T*>(a.dq) + ((b * a.lq + tok) * a.heads + head) * a.dim, dq, a.scale, a.dim);
+}
+
 // W waves, or 4 to 8 for W = 0
 template <typename T, bool TINY, int DP, int W>
 __global__ __launch_bounds__(W == 0 ? 512 : 64 * W, DP > 128 ? 1 : 2) void att_mma_q(const AttArgs a, int mtiles, int splits,
@@ -326,7 +412,18 @@ size_t stats_bytes(const AttArgs& a) { return ops_align(static_cast<size_t>(a.ba
 
 }  // namespace
 
+// f32 keeps ds for dq where that is at most this much: its matrix units, not HBM, bound
+// the backward pass (400 x (65 x 65) tokens, 2 heads of 100: dq 74 us by three products)
+constexpr int64_t kMostScores = int64_t(1) << 29;
+
+size_t scores_bytes(const AttArgs& a, int dtype) {
+  if (dtype != TGX_F32 || a.dq == nullptr || (a.dk == nullptr && a.dv == nullptr) || a.lk == 0) return 0;
+  const int64_t rows = a.batch * a.lq * a.heads;
+  return rows <= kMostScores / 4 / scores_row(a.lk) ? static_cast<size_t>(rows * scores_row(a.lk)) * 4 : 0;
+}
+
 size_t att_mma_backward_workspace(const AttArgs& a, int dtype) {
+  if (const size_t kept = scores_bytes(a, dtype)) return stats_bytes(a) + kept;
   const QShape f(a, dtype);
   return stats_bytes(a) + (f.splits > 1 ? static_cast<size_t>(a.batch * a.lq * a.heads) * f.splits * a.dim * 4 : 0);
 }
@@ -335,13 +432,14 @@ int att_mma_backward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
   const int64_t rows = a.batch * a.lq * a.heads;
   float2* stats = static_cast<float2*>(ws);
   float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + stats_bytes(a));
+  const bool keep = scores_bytes(a, dtype) > 0;  // the same workspace holds them in the parts' place
   return by_head(dtype, a.dim, [&](auto t, auto dp, auto tiny) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value, TS = kTile<T>;
     constexpr bool TINY = decltype(tiny)::value;
     hipLaunchKernelGGL(att_stats<T>, dim3(static_cast<unsigned>(ops_cdiv(rows, 256 / kDeltaLanes))), dim3(256), 0, s,
-                       static_cast<const T*>(a.out), static_cast<const T*>(a.dout), a.lse, rows, a.lq, a.heads, a.group,
-                       a.dim, stats);
+                       static_cast<const T*>(a.out), static_cast<const T*>(a.rest), static_cast<const T*>(a.dout), a.lse, rows,
+                       a.lq, a.heads, a.group, a.dim, stats);
     int rc = check_launch("att_stats");
     if (rc) return rc;
     if (a.lk > 0 && (a.dk != nullptr || a.dv != nullptr)) {
@@ -349,8 +447,12 @@ int att_mma_backward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
         constexpr int LEAST = decltype(least)::value;
         const int w = waves_for(ops_cdiv(a.lk, TS), LEAST, kv_most<T>(DP, LEAST));
         const int ktiles = static_cast<int>(ops_cdiv(a.lk, TS * w));
-        hipLaunchKernelGGL((att_mma_kv<T, TINY, DP, LEAST>), dim3(static_cast<unsigned>(a.batch * a.kv_heads * ktiles)),
-                           dim3(64 * w), 0, s, a, ktiles, stats);
+        const dim3 grid(static_cast<unsigned>(a.batch * a.kv_heads * ktiles));
+        if (sizeof(T) == 4 && keep)
+          hipLaunchKernelGGL((att_mma_kv<T, TINY, DP, LEAST, sizeof(T) == 4>), grid, dim3(64 * w), 0, s, a, ktiles,
+                             stats, part);
+        else
+          hipLaunchKernelGGL((att_mma_kv<T, TINY, DP, LEAST, false>), grid, dim3(64 * w), 0, s, a, ktiles, stats, part);
         return check_launch("att_mma_kv");
       };
       if constexpr (kTwoWays<T, DP>)
@@ -360,6 +462,15 @@ int att_mma_backward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
       if (rc) return rc;
     }
     if (a.dq == nullptr) return TGX_OK;
+    if constexpr (sizeof(T) == 4) {
+      if (keep) {
+        const int w = waves_for(ops_cdiv(a.lq * a.group, TS), 4, 8);
+        const int mtiles = static_cast<int>(ops_cdiv(a.lq * a.group, TS * w));
+        hipLaunchKernelGGL((att_scores_q<TINY, DP>), dim3(static_cast<unsigned>(a.batch * a.kv_heads * mtiles)),
+                           dim3(64 * w), 0, s, a, mtiles, part);
+        return check_launch("att_scores_q");
+      }
+    }
     const QShape f(a, dtype);
     auto go = [&](auto w) {
       hipLaunchKernelGGL((att_mma_q<T, TINY, DP, decltype(w)::value>),

@@ -175,14 +175,22 @@ __global__ __launch_bounds__(WQ == 0 ? 512 : 64 * WQ * WK, DP > 128 ? 1 : WQ == 
     return;
   }
   if (group == 0 && a.lse != nullptr) a.lse[row] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
-  store_columns<T, DP>(static_cast<T*>(a.o) + row * a.dim, o, l > 0.f ? 1.f / l : 0.f, a.dim);
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  store_columns<T, DP>(static_cast<T*>(a.o) + row * a.dim, o, inv, a.dim);
+  if (sizeof(T) == 2 && a.rest != nullptr) {
+#pragma unroll
+    for (int t = 0; t < OT; ++t)
+#pragma unroll
+      for (int i = 0; i < kRegs<T>; ++i) o[t][i] = lost<T>(o[t][i] * inv);
+    store_columns<T, DP>(static_cast<T*>(a.rest) + row * a.dim, o, 1.f, a.dim);
+  }
 }
 
 // One wave per row, LT lanes per range of 4 values each and 64 / LT ranges at a time.
 // SUMS: the ranges' outputs added up; else each weighed by exp(its maximum - the largest)
 // and divided by the sum.
 template <typename T, int LT, bool SUMS>
-__global__ __launch_bounds__(256) void att_join(T* __restrict__ out, float* __restrict__ lse, int64_t rows, int dim,
+__global__ __launch_bounds__(256) void att_join(T* __restrict__ out, T* __restrict__ rest, float* __restrict__ lse, int64_t rows, int dim,
                                                 float by, int splits, const AttParts part) {
   constexpr int G = kWave / LT;
   const int lane = threadIdx.x & (kWave - 1), grp = lane / LT;
@@ -226,21 +234,24 @@ __global__ __launch_bounds__(256) void att_join(T* __restrict__ out, float* __re
     if (grp == 0)
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        if (u < n) out[row * dim + c + u] = from_f<T>(acc[u] * by);
+        if (u < n) {
+          out[row * dim + c + u] = from_f<T>(acc[u] * by);
+          if (!SUMS && rest != nullptr) rest[row * dim + c + u] = from_f<T>(lost<T>(acc[u] * by));
+        }
   }
 }
 
 template <bool SUMS>
-int join_launch(void* out, float* lse, int64_t rows, int dim, int dtype, float by, int splits, const AttParts& part,
+int join_launch(void* out, void* rest, float* lse, int64_t rows, int dim, int dtype, float by, int splits, const AttParts& part,
                 hipStream_t s) {
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
     const dim3 grid(static_cast<unsigned>(ops_cdiv(rows, 4)));
-    T* o = static_cast<T*>(out);
-    if (dim <= 64) hipLaunchKernelGGL((att_join<T, 16, SUMS>), grid, dim3(256), 0, s, o, lse, rows, dim, by, splits, part);
+    T *o = static_cast<T*>(out), *r = static_cast<T*>(rest);
+    if (dim <= 64) hipLaunchKernelGGL((att_join<T, 16, SUMS>), grid, dim3(256), 0, s, o, r, lse, rows, dim, by, splits, part);
     else if (dim <= 128)
-      hipLaunchKernelGGL((att_join<T, 32, SUMS>), grid, dim3(256), 0, s, o, lse, rows, dim, by, splits, part);
-    else hipLaunchKernelGGL((att_join<T, 64, SUMS>), grid, dim3(256), 0, s, o, lse, rows, dim, by, splits, part);
+      hipLaunchKernelGGL((att_join<T, 32, SUMS>), grid, dim3(256), 0, s, o, r, lse, rows, dim, by, splits, part);
+    else hipLaunchKernelGGL((att_join<T, 64, SUMS>), grid, dim3(256), 0, s, o, r, lse, rows, dim, by, splits, part);
     return check_launch("att_join");
   });
 }
@@ -295,13 +306,13 @@ int att_mma_forward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
 }
 
 int att_join_forward(const AttArgs& a, int dtype, int splits, const AttParts& part, hipStream_t s) {
-  return join_launch<false>(a.o, a.lse, a.batch * a.lq * a.heads, a.dim, dtype, 1.f, splits, part, s);
+  return join_launch<false>(a.o, a.rest, a.lse, a.batch * a.lq * a.heads, a.dim, dtype, 1.f, splits, part, s);
 }
 
 int att_join_sums(void* out, int64_t rows, int dim, int dtype, float by, int splits, const float* part, hipStream_t s) {
   AttParts p(nullptr, 0, 1);
   p.o = const_cast<float*>(part);
-  return join_launch<true>(out, nullptr, rows, dim, dtype, by, splits, p, s);
+  return join_launch<true>(out, nullptr, nullptr, rows, dim, dtype, by, splits, p, s);
 }
 
 }  // namespace tgx

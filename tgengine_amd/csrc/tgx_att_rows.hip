@@ -254,6 +254,12 @@ __global__ __launch_bounds__(kRowThreads, M == 1 && C < 4 ? 3 : 2) void att_rows
 #pragma unroll
     for (int x = 0; x < N; ++x) acc[r][x] *= inv;
     at.store(static_cast<T*>(a.o) + row * a.dim, acc[r]);
+    if (sizeof(T) == 2 && a.rest != nullptr) {
+      float z[N];
+#pragma unroll
+      for (int x = 0; x < N; ++x) z[x] = lost<T>(acc[r][x]);
+      at.store(static_cast<T*>(a.rest) + row * a.dim, z);
+    }
     if (at.gl == 0 && a.lse != nullptr) a.lse[row] = l[r] > 0.f ? (m[r] + log2f(l[r])) * kLn2 : -INFINITY;
   }
 }
@@ -284,6 +290,10 @@ __global__ __launch_bounds__(kRowThreads, M == 1 ? (C < 4 ? 3 : 2) : (C < 4 ? 2 
     at.own(qo[r], q[r]);
     at.own(go[r], g[r]);
     delta[r] = at.dot(g[r], go[r], o);
+    if (sizeof(T) == 2 && a.rest != nullptr) {
+      at.load(o, in ? static_cast<const T*>(a.rest) + row * a.dim : nullptr);
+      delta[r] += at.dot(g[r], go[r], o);
+    }
     lse[r] = in ? a.lse[row] * kLog2e : INFINITY;
     if (lse[r] == -INFINITY) lse[r] = INFINITY;  // no key kept: p = 0
 #pragma unroll

@@ -13,7 +13,7 @@ namespace tgx {
 struct AttArgs {
   const void *q, *k, *v, *out, *dout;
   const uint8_t* mask;
-  void *o, *dq, *dk, *dv;
+  void *o, *rest, *dq, *dk, *dv;  // rest: what rounding took from o (bf16), or nullptr
   float* lse;
   int64_t batch, lq, lk, mask_stride;
   int64_t qs[3], ks[3], vs[3], os[3];  // os: of out, dout and dq
@@ -301,6 +301,10 @@ __device__ __forceinline__ void store_columns(T* row, const Acc<T> (&x)[DP / kTi
       }
     }
 }
+
+// what rounding to T takes from x
+template <typename T>
+__device__ __forceinline__ float lost(float x) { return x - to_f(from_f<T>(x)); }
 
 // the same in 32 bits, for the parts of ranges
 template <typename T, int DP>

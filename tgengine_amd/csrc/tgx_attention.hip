@@ -46,6 +46,7 @@ AttArgs att_args(const tgx_attention_args* p) {
   a.mask = p->mask;
   a.out = p->out;
   a.o = p->out;
+  a.rest = p->dtype == TGX_BF16 ? p->out_rest : nullptr;
   a.dout = p->grad_out;
   a.dq = p->grad_q;
   a.dk = p->grad_k;

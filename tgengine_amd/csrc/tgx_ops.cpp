@@ -275,12 +275,14 @@ tgx_attention_args attention_args(const Tensor& q, const Tensor& k, const Tensor
   return a;
 }
 
-Tensor attention_out(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& mask, double scale, Tensor* lse) {
+Tensor attention_out(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& mask, double scale, Tensor* lse,
+                     Tensor* rest) {
   Tensor out = at::empty(q.sizes(), q.options());
   tgx_attention_args a = attention_args(q, k, v, mask, scale);
   if (lse != nullptr) *lse = at::empty({a.batch, a.lq, a.heads}, q.options().dtype(at::kFloat));
   a.out = out.data_ptr();
   a.lse = lse != nullptr ? lse->data_ptr<float>() : nullptr;
+  a.out_rest = rest != nullptr ? ptr(*rest) : nullptr;
   const Tensor ws = workspace(tgx_attention_workspace_size(&a), q);
   a.workspace = ptr(ws);
   a.workspace_bytes = ws.defined() ? ws.numel() : 0;
@@ -294,9 +296,10 @@ class Attention : public torch::autograd::Function<Attention> {
                         const OptTensor& mask_in, double scale) {
     const c10::OptionalDeviceGuard guard(q.device());
     const Tensor mask = mask_in.value_or(Tensor());
-    Tensor lse;
-    Tensor out = attention_out(q, k, v, mask, scale, &lse);
-    ctx->save_for_backward({q, k, v, mask, out, lse});
+    Tensor lse, rest;
+    if (q.scalar_type() == at::kBFloat16) rest = at::empty(q.sizes(), q.options());
+    Tensor out = attention_out(q, k, v, mask, scale, &lse, &rest);
+    ctx->save_for_backward({q, k, v, mask, out, lse, rest});
     ctx->saved_data["scale"] = scale;
     return out;
   }
@@ -310,6 +313,7 @@ class Attention : public torch::autograd::Function<Attention> {
     tgx_attention_args a = attention_args(q, k, v, saved[3], ctx->saved_data["scale"].toDouble());
     a.out = saved[4].data_ptr();
     a.lse = saved[5].data_ptr<float>();
+    a.out_rest = ptr(saved[6]);
     a.grad_out = g.data_ptr();
     Tensor d[3];
     for (int i = 0; i < 3; ++i)
@@ -334,7 +338,7 @@ Tensor cross_attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_i
   const double scale = scale_in.has_value() ? *scale_in : 1.0 / std::sqrt(static_cast<double>(q.size(3)));
   if (keeps_grad({&q, &k, &v})) return Attention::apply(q, k, v, mask.defined() ? OptTensor(mask) : c10::nullopt, scale);
   const c10::OptionalDeviceGuard guard(q.device());
-  return attention_out(q, k, v, mask, scale, nullptr);
+  return attention_out(q, k, v, mask, scale, nullptr, nullptr);
 }
 
 // ------------------------------------------------------------------ clipping
