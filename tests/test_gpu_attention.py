@@ -299,3 +299,19 @@ def test_refusals():
     leaf = q.detach().requires_grad_()
     with pytest.raises(RuntimeError, match="once only"):
         torch.autograd.grad(A(leaf, k, v).sum(), leaf, create_graph=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("b,lq,lk,h,kv,d,mask", [(1, 300, 500, 4, 2, 64, "holes"), (3, 40, 70, 2, 2, 100, "recent"),
+                                                 (1, 2000, 60, 2, 1, 112, "holes"), (1, 90, 2600, 3, 3, 176, "prefix")])
+def test_gradients_one_at_a_time(b, lq, lk, h, kv, d, mask, dtype):
+    """Each gradient asked for alone, within the bounds of the whole backward pass: few
+    workgroups, whose rows and keys are cut in ranges, and f32 without kept scores."""
+    q, k, v, g = _inputs(b, lq, lk, h, kv, d, dtype, seed=3)
+    m = _mask(mask, b, lk, seed=4)
+    ref = _exact(q, k, v, g, m, d ** -0.5)
+    for name in "qkv":
+        x = {n: t.detach().requires_grad_(n == name) for n, t in (("q", q), ("k", k), ("v", v))}
+        (got,) = torch.autograd.grad(ops.cross_attention(x["q"], x["k"], x["v"], mask=m), x[name], g)
+        y, e = ref["d" + name]
+        assert bool(((got.double() - y).abs() <= e).all()), name

@@ -23,8 +23,8 @@ __host__ __device__ __forceinline__ int64_t scores_row(int64_t lk) { return (lk 
 // Per row, in the order of problems and their rows: its log sum in units of log 2 (+inf
 // for a row that keeps no key: its probabilities are then zeros) and delta, from the output
 // as it was before rounding where its rest was kept: delta's error reaches every score of
-// the row alike, and with ds rounded too dq was up to 1.52 times as far off as its own
-// rounding
+// the row alike.  Without it dq was over 1.5 times as far off as one rounding of it is, with
+// it 1.42 to 1.45 times, which rounded probabilities and a rounded result account for
 template <typename T>
 __global__ __launch_bounds__(256) void att_stats(const T* __restrict__ out, const T* __restrict__ rest,
                                                  const T* __restrict__ dout,
@@ -69,6 +69,8 @@ __device__ __forceinline__ void one_by_one() {
 // The rows' tiles stand in LDS twice, so that one is filled while the other is read and a
 // tile takes one barrier.
 //
+// With splits > 1 the rows are cut in ranges of `span` and each leaves its sums in `part`,
+// dk's before dv's.
 // KEEP (f32): ds goes to `scores`, rows of scores_row() keys, for att_scores_q.
 //
 // LEAST to kv_most() waves a workgroup.  bf16 heads of 65 to 128 values come two ways: 8
@@ -86,7 +88,8 @@ constexpr int kv_most(int dp, int least) {
 
 template <typename T, bool TINY, int DP, int LEAST, bool KEEP>
 __global__ __launch_bounds__(64 * kv_most<T>(DP, LEAST), DP > 128 || (sizeof(T) == 2 && DP > 64 && LEAST < 8) ? 1 : 2)
-void att_mma_kv(const AttArgs a, int ktiles, const float2* __restrict__ stats, float* __restrict__ scores) {
+void att_mma_kv(const AttArgs a, int ktiles, int splits, int64_t span, const float2* __restrict__ stats,
+                float* __restrict__ scores, float* __restrict__ part) {
   using Tile = LdsTile<T, DP, Reads::kBoth>;
   using Own = LdsTile<T, DP, Reads::kRows>;
   constexpr int TS = kTile<T>, R = TS, OT = DP / TS, ST = DP / kStep, W = LEAST;
@@ -98,7 +101,9 @@ void att_mma_kv(const AttArgs a, int ktiles, const float2* __restrict__ stats, f
   __shared__ __align__(16) T sk[HELD ? 8 : TS * W * Own::ROW], sv[HELD ? 8 : TS * W * Own::ROW];
   __shared__ __align__(16) float slse[2][R], sdelta[2][R];
   const int group = lane_group<T>(), wave = threadIdx.x / kWave;
-  const int64_t w = by_die(blockIdx.x, gridDim.x);
+  int64_t w = by_die(blockIdx.x, gridDim.x);
+  const int sp = static_cast<int>(w % splits);
+  w /= splits;
   const int64_t j = w % ktiles * (TS * (blockDim.x / kWave)) + wave * TS + lane_row<T>();
   const int64_t p = w / ktiles;
   const int hk = static_cast<int>(p % a.kv_heads);
@@ -132,10 +137,10 @@ void att_mma_kv(const AttArgs a, int ktiles, const float2* __restrict__ stats, f
       kv.template store<Own::ROW>(sv, a.dim);
     }
     const float c = a.scale * kLog2e;
-    const int64_t rows = a.lq * a.group;
+    const int64_t all_rows = a.lq * a.group, lo = sp * span, rows = lo + span < all_rows ? lo + span : all_rows;
     const T* qp = static_cast<const T*>(a.q) + b * a.qs[0] + static_cast<int64_t>(hk) * a.group * a.qs[2];
     const T* gp = static_cast<const T*>(a.dout) + b * a.os[0] + static_cast<int64_t>(hk) * a.group * a.os[2];
-    stats += p * rows;
+    stats += p * all_rows;
     Stage<T, TINY, R, DP, W, FIXED> q(a.dim), g(a.dim);
     constexpr int N = Stage<T, TINY, R, DP, W, FIXED>::N;
     // each of the thread's rows: its head of the group and its offsets, moved on by R rows
@@ -144,8 +149,8 @@ void att_mma_kv(const AttArgs a, int ktiles, const float2* __restrict__ stats, f
     int64_t qo[N], go[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int row = q.row(n), tok = row / a.group;
-      hg[n] = row - tok * a.group;
+      const int64_t row = lo + q.row(n), tok = row / a.group;
+      hg[n] = static_cast<int>(row - tok * a.group);
       qo[n] = tok * a.qs[1] + hg[n] * a.qs[2];
       go[n] = tok * a.os[1] + hg[n] * a.os[2];
     }
@@ -176,11 +181,11 @@ void att_mma_kv(const AttArgs a, int ktiles, const float2* __restrict__ stats, f
         sdelta[to][threadIdx.x] = st.y;
       }
     };
-    fetch(0);
+    fetch(lo);
     put(0);
-    if (R < rows) fetch(R);
+    if (lo + R < rows) fetch(lo + R);
     int cur = 0;
-    for (int64_t first = 0; first < rows; first += R, cur ^= 1) {
+    for (int64_t first = lo; first < rows; first += R, cur ^= 1) {
       __syncthreads();
       if (sizeof(T) == 2 || busy) {
         Acc<T> s = Acc<T>{}, dp = Acc<T>{};
@@ -212,7 +217,7 @@ void att_mma_kv(const AttArgs a, int ktiles, const float2* __restrict__ stats, f
 #pragma unroll
         for (int i = 0; i < kRegs<T>; ++i) dp[i] = s[i] * (dp[i] - sdelta[cur][mma_row<T>(i, group)]);
         if constexpr (KEEP) {
-          float* to = scores + (p * rows + first) * scores_row(a.lk) + j;
+          float* to = scores + (p * all_rows + first) * scores_row(a.lk) + j;
           if (j < scores_row(a.lk))
 #pragma unroll
             for (int i = 0; i < kRegs<T>; ++i)
@@ -234,6 +239,12 @@ void att_mma_kv(const AttArgs a, int ktiles, const float2* __restrict__ stats, f
     }
   }
   if (j >= a.lk) return;
+  if (splits > 1) {
+    float* to = part + (at * splits + sp) * a.dim;
+    if (a.dk != nullptr) store_parts<T, DP>(to, dk, a.dim);
+    if (a.dv != nullptr) store_parts<T, DP>(to + a.batch * a.lk * a.kv_heads * splits * a.dim, dv, a.dim);
+    return;
+  }
   if (a.dk != nullptr) store_columns<T, DP>(static_cast<T*>(a.dk) + at * a.dim, dk, a.scale, a.dim);
   if (a.dv != nullptr) store_columns<T, DP>(static_cast<T*>(a.dv) + at * a.dim, dv, 1.f, a.dim);
 }
@@ -408,9 +419,26 @@ struct QShape {
   }
 };
 
-size_t stats_bytes(const AttArgs& a) { return ops_align(static_cast<size_t>(a.batch * a.lq * a.heads) * sizeof(float2)); }
+// dk's and dv's key tiles, and the ranges the rows are cut in where those alone leave
+// compute units without work
+struct KvShape {
+  int least, w, ktiles, splits;
+  int64_t span, sums;  // sums: values of dk's parts, and of dv's
+  KvShape(const AttArgs& a, int dtype) {
+    const bool bf = dtype == TGX_BF16;
+    least = !bf ? 4 : a.dim > 64 && a.dim <= 128 && a.lk > 160 ? 8 : 2;
+    w = waves_for(ops_cdiv(a.lk, bf ? 32 : 16), least, bf ? kv_most<bf16>(a.dim, least) : kv_most<float>(a.dim, least));
+    ktiles = static_cast<int>(ops_cdiv(a.lk, (bf ? 32 : 16) * w));
+    const int64_t blocks = std::max<int64_t>(a.batch * a.kv_heads * ktiles, 1), tiles = ops_cdiv(a.lq * a.group, 32);
+    const int64_t want = blocks >= 256 ? 1 : ops_cdiv(512, blocks);
+    const int64_t per = ops_cdiv(tiles, std::min(std::min(want, ops_cdiv(tiles, 8)), int64_t(64)));
+    span = per * 32;
+    splits = a.dk != nullptr || a.dv != nullptr ? static_cast<int>(ops_cdiv(tiles, per)) : 1;
+    sums = splits > 1 ? a.batch * a.lk * a.kv_heads * splits * a.dim : 0;
+  }
+};
 
-}  // namespace
+size_t stats_bytes(const AttArgs& a) { return ops_align(static_cast<size_t>(a.batch * a.lq * a.heads) * sizeof(float2)); }
 
 // f32 keeps ds for dq where that is at most this much: its matrix units, not HBM, bound
 // the backward pass (400 x (65 x 65) tokens, 2 heads of 100: dq 74 us by three products)
@@ -422,16 +450,24 @@ size_t scores_bytes(const AttArgs& a, int dtype) {
   return rows <= kMostScores / 4 / scores_row(a.lk) ? static_cast<size_t>(rows * scores_row(a.lk)) * 4 : 0;
 }
 
-size_t att_mma_backward_workspace(const AttArgs& a, int dtype) {
-  if (const size_t kept = scores_bytes(a, dtype)) return stats_bytes(a) + kept;
+// what dq's kernel leaves between its launches: kept scores, or the parts of its ranges
+size_t q_bytes(const AttArgs& a, int dtype) {
+  if (const size_t kept = scores_bytes(a, dtype)) return ops_align(kept);
   const QShape f(a, dtype);
-  return stats_bytes(a) + (f.splits > 1 ? static_cast<size_t>(a.batch * a.lq * a.heads) * f.splits * a.dim * 4 : 0);
+  return f.splits > 1 ? ops_align(static_cast<size_t>(a.batch * a.lq * a.heads) * f.splits * a.dim * 4) : 0;
+}
+
+}  // namespace
+
+size_t att_mma_backward_workspace(const AttArgs& a, int dtype) {
+  return stats_bytes(a) + q_bytes(a, dtype) + static_cast<size_t>(KvShape(a, dtype).sums) * 8;
 }
 
 int att_mma_backward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
   const int64_t rows = a.batch * a.lq * a.heads;
   float2* stats = static_cast<float2*>(ws);
   float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + stats_bytes(a));
+  float* kv_part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + stats_bytes(a) + q_bytes(a, dtype));
   const bool keep = scores_bytes(a, dtype) > 0;  // the same workspace holds them in the parts' place
   return by_head(dtype, a.dim, [&](auto t, auto dp, auto tiny) {
     using T = decltype(t);
@@ -443,22 +479,27 @@ int att_mma_backward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
     int rc = check_launch("att_stats");
     if (rc) return rc;
     if (a.lk > 0 && (a.dk != nullptr || a.dv != nullptr)) {
+      const KvShape f(a, dtype);
       auto go = [&](auto least) {
         constexpr int LEAST = decltype(least)::value;
-        const int w = waves_for(ops_cdiv(a.lk, TS), LEAST, kv_most<T>(DP, LEAST));
-        const int ktiles = static_cast<int>(ops_cdiv(a.lk, TS * w));
-        const dim3 grid(static_cast<unsigned>(a.batch * a.kv_heads * ktiles));
+        const dim3 grid(static_cast<unsigned>(a.batch * a.kv_heads * f.ktiles * f.splits));
         if (sizeof(T) == 4 && keep)
-          hipLaunchKernelGGL((att_mma_kv<T, TINY, DP, LEAST, sizeof(T) == 4>), grid, dim3(64 * w), 0, s, a, ktiles,
-                             stats, part);
+          hipLaunchKernelGGL((att_mma_kv<T, TINY, DP, LEAST, sizeof(T) == 4>), grid, dim3(64 * f.w), 0, s, a, f.ktiles,
+                             f.splits, f.span, stats, part, kv_part);
         else
-          hipLaunchKernelGGL((att_mma_kv<T, TINY, DP, LEAST, false>), grid, dim3(64 * w), 0, s, a, ktiles, stats, part);
+          hipLaunchKernelGGL((att_mma_kv<T, TINY, DP, LEAST, false>), grid, dim3(64 * f.w), 0, s, a, f.ktiles, f.splits,
+                             f.span, stats, part, kv_part);
         return check_launch("att_mma_kv");
       };
       if constexpr (kTwoWays<T, DP>)
-        rc = a.lk > 160 ? go(std::integral_constant<int, 8>{}) : go(std::integral_constant<int, 2>{});
+        rc = f.least == 8 ? go(std::integral_constant<int, 8>{}) : go(std::integral_constant<int, 2>{});
       else
         rc = go(std::integral_constant<int, kKvLeast<T, DP>>{});
+      const int64_t keys = a.batch * a.lk * a.kv_heads;
+      if (!rc && f.splits > 1 && a.dk != nullptr)
+        rc = att_join_sums(a.dk, keys, a.dim, dtype, a.scale, f.splits, kv_part, s);
+      if (!rc && f.splits > 1 && a.dv != nullptr)
+        rc = att_join_sums(a.dv, keys, a.dim, dtype, 1.f, f.splits, kv_part + f.sums, s);
       if (rc) return rc;
     }
     if (a.dq == nullptr) return TGX_OK;

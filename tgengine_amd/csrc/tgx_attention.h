@@ -190,10 +190,6 @@ __device__ __forceinline__ u32x4 row_part(const T* row, int c, int dim) {
     return load16(row + min(c, dim - V));
   }
 }
-template <typename T>
-__device__ __forceinline__ u32x4 row_part(const T* row, int c, int dim) {
-  return dim < kWide<T> ? row_part<T, true>(row, c, dim) : row_part<T, false>(row, c, dim);
-}
 
 // row_part's values in their places, zeros after the row's end (rows of at least V values)
 template <typename T>
