@@ -75,7 +75,9 @@ __device__ __forceinline__ void one_by_one() {
 //
 // LEAST to kv_most() waves a workgroup.  bf16 heads of 65 to 128 values come two ways: 8
 // waves, which leaves each the registers for one row of staging and two waves a SIMD, or 2
-// to 4 with all registers, where there are few keys.
+// to 4 with all registers for up to 64 keys, which 8 waves would mostly idle through (200 x
+// 100 rows, 4/2 heads: of 128 with 64 keys 94 us by 8 waves and 71 so, with 100 103 and 102,
+// with 144 110 and 152; of 80 with 64 60 and 52, with 90 64 and 75).
 template <typename T, int DP>
 constexpr bool kTwoWays = sizeof(T) == 2 && DP > 64 && DP <= 128;
 template <typename T, int DP>
@@ -404,13 +406,13 @@ __global__ __launch_bounds__(W == 0 ? 512 : 64 * W, DP > 128 ? 1 : 2) void att_m
 // without work
 struct QShape {
   int w, mtiles, splits;
-  int64_t span;
+  int64_t span, blocks;  // blocks: of one range
   QShape(const AttArgs& a, int dtype) {
     const int64_t rows = a.lq * a.group;
     const int tile = dtype == TGX_BF16 ? 32 : 16;
     w = a.dim > 128 ? 4 : tile == 32 ? (rows <= 64 ? 2 : 4) : waves_for(ops_cdiv(rows, tile), 4, 8);
     mtiles = static_cast<int>(ops_cdiv(rows, tile * w));
-    const int64_t blocks = a.batch * a.kv_heads * mtiles;
+    blocks = a.batch * a.kv_heads * mtiles;
     const int64_t tiles = ops_cdiv(std::max<int64_t>(a.lk, 1), 64);
     const int64_t want = blocks >= 512 ? 1 : ops_cdiv(1024, blocks);
     const int64_t per = ops_cdiv(tiles, std::min(std::min(want, ops_cdiv(tiles, 8)), int64_t(256)));
@@ -419,18 +421,20 @@ struct QShape {
   }
 };
 
-// dk's and dv's key tiles, and the ranges the rows are cut in where those alone leave
-// compute units without work
+// dk's and dv's key tiles, and the ranges the rows are cut in where those alone leave half
+// of the compute units without work: at most 256 workgroups, since every range writes
+// its sums of all keys (1 x (2,000 x 2,000 tokens), 2/1 heads of 128, bf16: 87 us, 389 uncut;
+// 2 x (300 x 6,000), 8/4 heads of 128: 123 us, 185 in three ranges)
 struct KvShape {
   int least, w, ktiles, splits;
   int64_t span, sums;  // sums: values of dk's parts, and of dv's
   KvShape(const AttArgs& a, int dtype) {
     const bool bf = dtype == TGX_BF16;
-    least = !bf ? 4 : a.dim > 64 && a.dim <= 128 && a.lk > 160 ? 8 : 2;
+    least = !bf ? 4 : a.dim > 64 && a.dim <= 128 && a.lk > 64 ? 8 : 2;
     w = waves_for(ops_cdiv(a.lk, bf ? 32 : 16), least, bf ? kv_most<bf16>(a.dim, least) : kv_most<float>(a.dim, least));
     ktiles = static_cast<int>(ops_cdiv(a.lk, (bf ? 32 : 16) * w));
     const int64_t blocks = std::max<int64_t>(a.batch * a.kv_heads * ktiles, 1), tiles = ops_cdiv(a.lq * a.group, 32);
-    const int64_t want = blocks >= 256 ? 1 : ops_cdiv(512, blocks);
+    const int64_t want = std::max<int64_t>(256 / blocks, 1);
     const int64_t per = ops_cdiv(tiles, std::min(std::min(want, ops_cdiv(tiles, 8)), int64_t(64)));
     span = per * 32;
     splits = a.dk != nullptr || a.dv != nullptr ? static_cast<int>(ops_cdiv(tiles, per)) : 1;
@@ -440,12 +444,16 @@ struct KvShape {
 
 size_t stats_bytes(const AttArgs& a) { return ops_align(static_cast<size_t>(a.batch * a.lq * a.heads) * sizeof(float2)); }
 
-// f32 keeps ds for dq where that is at most this much: its matrix units, not HBM, bound
-// the backward pass (400 x (65 x 65) tokens, 2 heads of 100: dq 74 us by three products)
+// f32 keeps ds for dq where that is at most this much, because its matrix units, not HBM,
+// bound the backward pass (400 x (65 x 65) tokens, 2 heads of 100: 142 us, 189 with three
+// products for dq; 8 x (1,000 x 2,000), 4 heads of 100: 743 and 929).  att_scores_q walks over
+// all keys in one workgroup, so few rows with long keys do without (1 x (300 x 6,000), 8/4
+// heads of 128: 308 us, 630 with kept scores).
 constexpr int64_t kMostScores = int64_t(1) << 29;
 
 size_t scores_bytes(const AttArgs& a, int dtype) {
   if (dtype != TGX_F32 || a.dq == nullptr || (a.dk == nullptr && a.dv == nullptr) || a.lk == 0) return 0;
+  if (a.lk > 1024 && QShape(a, dtype).blocks < 128) return 0;
   const int64_t rows = a.batch * a.lq * a.heads;
   return rows <= kMostScores / 4 / scores_row(a.lk) ? static_cast<size_t>(rows * scores_row(a.lk)) * 4 : 0;
 }
