@@ -1,9 +1,9 @@
 // Attention backward on the matrix units.
 //
-// Three launches: delta_i = do_i . o_i and the log sum of every row; dk and dv, where a wave owns a
-// tile of keys and walks over the problem's rows; dq, where a wave owns a tile of rows and
-// walks over the keys.  Scores are computed anew in both from the saved log sums (7 products of
-// M x Lk x D, the sums of each output in one place and in one order, no atomics).
+// Three launches: delta_i = do_i . o_i and the log sum of every row; dk and dv, where a wave
+// owns a tile of keys and walks over the problem's rows; dq, where a wave owns a tile of rows
+// and walks over the keys.  Scores are computed anew in both from the saved log sums (7
+// products of M x Lk x D, the sums of each output in one place and in one order, no atomics).
 //
 // As in the forward pass every score tile stays in the registers it was computed in: a
 // wave's columns are what it owns (keys for dk and dv, rows for dq), a lane's 16 values
@@ -24,7 +24,8 @@ __host__ __device__ __forceinline__ int64_t scores_row(int64_t lk) { return (lk 
 // for a row that keeps no key: its probabilities are then zeros) and delta, from the output
 // as it was before rounding where its rest was kept: delta's error reaches every score of
 // the row alike.  Without it dq was over 1.5 times as far off as one rounding of it is, with
-// it 1.42 to 1.45 times, which rounded probabilities and a rounded result account for
+// it 1.42 to 1.45 times, which rounded probabilities and a rounded result account for.
+// kDeltaLanes lanes a row; HBM bounds it (52,000 f32 rows of 100: 42 MB in 11 us, 3.7 TB/s)
 template <typename T>
 __global__ __launch_bounds__(256) void att_stats(const T* __restrict__ out, const T* __restrict__ rest,
                                                  const T* __restrict__ dout,
@@ -72,6 +73,11 @@ __device__ __forceinline__ void one_by_one() {
 // With splits > 1 the rows are cut in ranges of `span` and each leaves its sums in `part`,
 // dk's before dv's.
 // KEEP (f32): ds goes to `scores`, rows of scores_row() keys, for att_scores_q.
+//
+// Bounded by the LDS reads, each operand of four products, and the exchange with the softmax
+// for bf16: 2 x (1,000 x 8,000 tokens), 16/4 heads of 128, 92% kept, 400 us, 601 TFLOP/s;
+// by the matrix units for f32: 400 x (65 x 65), 2 heads of 100, 95 us, 48 TFLOP/s with the
+// padding to 80 x 80 x 112 and 29 without.
 //
 // LEAST to kv_most() waves a workgroup.  bf16 heads of 65 to 128 values come two ways: 8
 // waves, which leaves each the registers for one row of staging and two waves a SIMD, or 2
@@ -251,12 +257,10 @@ void att_mma_kv(const AttArgs a, int ktiles, int splits, int64_t span, const flo
   if (a.dv != nullptr) store_columns<T, DP>(static_cast<T*>(a.dv) + at * a.dim, dv, 1.f, a.dim);
 }
 
-// dq, kTile rows a wave.  S^T = K Q^T and dP^T = V dO^T have the keys down a lane's registers
-// and one row a lane; dQ^T += K^T dS^T follows.  With splits > 1 each range of `span` keys
-// leaves its sum in `part`.
 // f32's dq from the ds that att_mma_kv kept: one product where att_mma_q takes three, for
 // the writing and reading of the scores.  16 rows a wave, 4 to 8 waves; a wave reads its
-// rows' scores as fragments.
+// rows' scores as fragments.  400 x (65 x 65) tokens, 2 heads of 100: 29 us; by three
+// products 74.
 template <bool TINY, int DP>
 __global__ __launch_bounds__(512, 2) void att_scores_q(const AttArgs a, int mtiles, const float* __restrict__ scores) {
   using T = float;
@@ -319,7 +323,10 @@ __global__ __launch_bounds__(512, 2) void att_scores_q(const AttArgs a, int mtil
   store_columns<T, DP>(static_cast<T*>(a.dq) + ((b * a.lq + tok) * a.heads + head) * a.dim, dq, a.scale, a.dim);
 }
 
-// W waves, or 4 to 8 for W = 0
+// dq, kTile rows a wave.  S^T = K Q^T and dP^T = V dO^T have the keys down a lane's registers
+// and one row a lane; dQ^T += K^T dS^T follows.  With splits > 1 each range of `span` keys
+// leaves its sum in `part`.  W waves, or 4 to 8 for W = 0.  Bounded as att_mma_kv is: 2 x
+// (1,000 x 8,000 tokens), 16/4 heads of 128, bf16, 92% kept, 256 us, 705 TFLOP/s.
 template <typename T, bool TINY, int DP, int W>
 __global__ __launch_bounds__(W == 0 ? 512 : 64 * W, DP > 128 ? 1 : 2) void att_mma_q(const AttArgs a, int mtiles, int splits,
                                                                      int64_t span, const float2* __restrict__ stats,
@@ -403,7 +410,9 @@ __global__ __launch_bounds__(W == 0 ? 512 : 64 * W, DP > 128 ? 1 : 2) void att_m
 }
 
 // dq's row tiles, and the ranges the keys are cut in where those alone leave compute units
-// without work
+// without work: 1,024 workgroups (2 x (300 x 6,000 tokens), 8/4 heads of 128, bf16, with dk
+// and dv: 115 us, 126 with 256 workgroups and 368 uncut), of 4 waves where heads of more than
+// 128 values take all registers
 struct QShape {
   int w, mtiles, splits;
   int64_t span, blocks;  // blocks: of one range

@@ -5,17 +5,27 @@
 // running maximum and sum of the softmax are a lane's own but for an exchange between
 // the lanes of a row now and then, and P^T, still in the same registers, is the second operand of
 // O^T += V^T P^T.  Scores are in units of log 2.  Probabilities are rounded to the
-// inputs' type for that product, as the matrix units take them; sums stay in 32 bits.
+// inputs' type for that product, as the matrix units take them; sums stay in 32 bits.  (With
+// bf16 that rounding and the output's own make sqrt 2 of one rounding's error: 0.0024 where
+// the output's alone is 0.0017.  A second product for what rounding took would double the
+// cost of P V.)
+//
+// What bounds it: for bf16 the softmax between the products and the LDS reads that feed
+// them (2 x (1,000 x 8,000 tokens), 16/4 heads of 128, 92% kept: 190 us, 631 TFLOP/s of the
+// 1,225 that a matrix product of 8,192 reaches); for f32 the matrix units, eight times slower
+// (400 x (65 x 65), 2 heads of 100: 51 us for 75 MB and 1.4 GFLOP, whose 16-row tiles pad
+// 65 to 80 and 100 to 112); for single tokens the reads of keys and values (5 x 30,001 keys
+// of 8 heads of 128, bf16, 73% kept: 99 us for 447 MB, 4.5 TB/s).
 #include "tgx_attention.h"
 
 namespace tgx {
 namespace {
 
 // The waves of a workgroup take kTile rows each: WQ of them, or 4 to 8 for WQ = 0 (f32,
-// whose 16-row tiles fit odd lengths better); WK > 1: WK
-// waves take the same rows, one tile of each KT = 64 keys each, and are joined at the end.  With splits > 1 the keys
-// are cut in as many ranges of `span` keys and each leaves its maximum, sum and unscaled
-// output in `part` for att_join.
+// whose 16-row tiles fit odd lengths better); WK > 1: WK waves take the same rows, one tile
+// of each KT = 64 keys each, and are joined at the end.  With splits > 1 the keys are cut in
+// as many ranges of `span` keys and each leaves its maximum, sum and unscaled output in
+// `part` for att_join.
 template <typename T, bool TINY, int DP, int WQ, int WK>
 __global__ __launch_bounds__(WQ == 0 ? 512 : 64 * WQ * WK, DP > 128 ? 1 : WQ == 0 && DP <= 112 ? 4 : 2) void att_mma_fwd(const AttArgs a, int mtiles, int splits,
                                                                              int64_t span, const AttParts part) {
@@ -188,7 +198,8 @@ __global__ __launch_bounds__(WQ == 0 ? 512 : 64 * WQ * WK, DP > 128 ? 1 : WQ == 
 
 // One wave per row, LT lanes per range of 4 values each and 64 / LT ranges at a time.
 // SUMS: the ranges' outputs added up; else each weighed by exp(its maximum - the largest)
-// and divided by the sum.
+// and divided by the sum.  Reads bound it: 160 rows of 128 in 26 ranges 9 us, 32,000 rows in
+// 2 to 4 ranges 13 to 17 us.
 template <typename T, int LT, bool SUMS>
 __global__ __launch_bounds__(256) void att_join(T* __restrict__ out, T* __restrict__ rest, float* __restrict__ lse, int64_t rows, int dim,
                                                 float by, int splits, const AttParts part) {

@@ -7,6 +7,9 @@
 // of LP lanes keeps a running maximum, sum and output of its own; groups, then the
 // `wpp` waves of a problem, are joined once at the end.  The backward pass reads the
 // keys once too: dk and dv of a key are complete as soon as its scores are.
+//
+// HBM bounds both: 24,576 rows with 32 keys, 2 f32 heads of 86, 80% kept: forward 198 us for
+// 0.90 GB, 4.5 TB/s; backward 388 us for 2.0 GB, 5.2 TB/s.
 #include "tgx_attention.h"
 
 namespace tgx {
@@ -374,7 +377,10 @@ __global__ __launch_bounds__(kRowThreads, M == 1 ? (C < 4 ? 3 : 2) : (C < 4 ? 2 
 }
 
 // Waves per problem and key ranges: one wave a problem where the problems fill the
-// device, four where they do not, and then ranges of at least 512 keys.
+// device, four where they do not, and then ranges of at least 512 keys (f32, 2 heads of 64:
+// 300 rows with 200 keys forward 13 us, 16 with one wave each, backward 23 and 26; from
+// 1,000 rows on the two are even.  bf16, 4 rows with 4,000 keys forward 14 us, 39 in one
+// range, backward 21 and 66).
 struct RowShape {
   int wpp, splits;
   int64_t span, blocks;

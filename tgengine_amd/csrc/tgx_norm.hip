@@ -48,6 +48,10 @@ struct Place {
 // by side touch fewer cache lines than few lanes with more packs each where rows do not
 // begin on a line (786,432 x 172 bf16 rows, forward: 8 lanes of 3 packs 137 us, 32 lanes of
 // one 159, and with four rows 120; backward 206, 202, and with two rows 175).
+//
+// HBM bounds it: those 541 MB take the forward pass 128 us, 4.3 TB/s where a copy without
+// gaps in its lines reaches 6.2; 240 x 172 f32 rows take 4.4 us, a chain of one read, two
+// sums over the lanes and one write.
 constexpr int fwd_rows(int c) { return c == 1 ? 4 : c == 2 ? 2 : 1; }
 constexpr int bwd_rows(int c) { return c == 1 ? 2 : 1; }
 
@@ -128,6 +132,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd(const T* __restrict__ x
 // A workgroup takes every gridDim.x-th group of rows.  Its lanes own fixed columns, so
 // the sums over rows for dw and db stay in registers until the end, are joined over the
 // workgroup's rows in LDS in a fixed order and left in part[block][2][dim].
+// HBM bounds it: 786,432 x 172 bf16 rows (818 MB) 171 us, 4.8 TB/s, and norm_join 7.5 us.
 template <typename T, typename W, int V, int L, int C>
 __global__ __launch_bounds__(kNormThreads) void norm_bwd(const T* __restrict__ x, const T* __restrict__ dy, int64_t rows,
                                                          int dim, int64_t stride, const W* __restrict__ weight,
