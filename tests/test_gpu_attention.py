@@ -315,3 +315,20 @@ def test_gradients_one_at_a_time(b, lq, lk, h, kv, d, mask, dtype):
         (got,) = torch.autograd.grad(ops.cross_attention(x["q"], x["k"], x["v"], mask=m), x[name], g)
         y, e = ref["d" + name]
         assert bool(((got.double() - y).abs() <= e).all()), name
+
+
+@pytest.mark.parametrize("lk", [1, 2, 6, 40, 64, 65, 128])
+@pytest.mark.parametrize("lq,group,d", [(33, 1, 64), (40, 2, 40), (7, 1, 32)])
+def test_few_keys_round_the_output_only(lk, lq, group, d):
+    """bf16 with few keys: probabilities keep 16 bits (what their rounding to 2^-8 took is
+    rounded to 2^-8 of itself), so that the output is off by its own rounding, 2^-8, and by
+    2^-16 of the sum of p |v|.  A score's 32-bit sum of d <= 64 products whose magnitudes
+    add up to less than 24 is off by less than 64 x 2^-24 x 24 < 2^-13, which moves its
+    probability, and the sum of all, by as much: 2^-11 of the sum of p |v| covers both."""
+    q, k, v, _ = _inputs(5, lq, lk, 2 * group, 2, d, "bf16", seed=lk)
+    m = _mask("holes", 5, lk, seed=lk)
+    zero = torch.zeros_like(q)
+    y = _exact(q, k, v, zero, m, d ** -0.5)["out"][0]
+    spread = _exact(q, k, v.abs(), zero, m, d ** -0.5)["out"][0]
+    got = ops.cross_attention(q, k, v, mask=m)
+    assert bool(((got.double() - y).abs() <= 2.0 ** -8 * y.abs() + 2.0 ** -11 * spread).all())

@@ -326,7 +326,7 @@ __global__ __launch_bounds__(512, 2) void att_scores_q(const AttArgs a, int mtil
 // dq, kTile rows a wave.  S^T = K Q^T and dP^T = V dO^T have the keys down a lane's registers
 // and one row a lane; dQ^T += K^T dS^T follows.  With splits > 1 each range of `span` keys
 // leaves its sum in `part`.  W waves, or 4 to 8 for W = 0.  Bounded as att_mma_kv is: 2 x
-// (1,000 x 8,000 tokens), 16/4 heads of 128, bf16, 92% kept, 256 us, 705 TFLOP/s.
+// (1,000 x 8,000 tokens), 16/4 heads of 128, bf16, 92% kept, 250 us, 721 TFLOP/s.
 template <typename T, bool TINY, int DP, int W>
 __global__ __launch_bounds__(W == 0 ? 512 : 64 * W, DP > 128 ? 1 : 2) void att_mma_q(const AttArgs a, int mtiles, int splits,
                                                                      int64_t span, const float2* __restrict__ stats,
