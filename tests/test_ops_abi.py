@@ -102,3 +102,11 @@ def test_no_cpu_path():
             call()
     with pytest.raises(ValueError, match="no gradients"):
         ops.clip_grad_norm_([torch.nn.Parameter(x)], 1.0)
+
+
+def test_grids_that_one_launch_does_not_take():
+    L = _lib.lib()
+    for lq in (1, 40):  # few rows a problem, and a tile of them
+        a = _att(batch=1 << 28, lq=lq, heads=2, kv_heads=2)
+        assert L.tgx_attention(a, None) == 3 and "one launch" in _err()
+    assert L.tgx_embed_grad(8, 8, 1, 1 << 29, 5, 4, 0, 1.0, 8, 8, 1 << 50, None) == 3 and "2^29" in _err()

@@ -486,6 +486,13 @@ int att_mma_backward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
   float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + stats_bytes(a));
   float* kv_part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + stats_bytes(a) + q_bytes(a, dtype));
   const bool keep = scores_bytes(a, dtype) > 0;  // the same workspace holds them in the parts' place
+  const KvShape kv(a, dtype);
+  const QShape q(a, dtype);
+  const int64_t problems = a.batch * a.kv_heads;
+  int fits = check_grid("tgx_attention_grad", ops_cdiv(rows, 256 / kDeltaLanes), 256);
+  if (!fits) fits = check_grid("tgx_attention_grad", problems * kv.ktiles * kv.splits, 512);
+  if (!fits) fits = check_grid("tgx_attention_grad", problems * q.mtiles * q.splits, 512);
+  if (fits) return fits;
   return by_head(dtype, a.dim, [&](auto t, auto dp, auto tiny) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value, TS = kTile<T>;

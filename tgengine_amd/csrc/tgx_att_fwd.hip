@@ -323,7 +323,9 @@ int att_mma_forward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
   const FwdShape f(a, dtype);
   const AttParts part(ws, a.batch * a.lq * a.heads, f.splits);
   const int64_t blocks = a.batch * a.kv_heads * f.mtiles * f.splits;
-  int rc = by_head(dtype, a.dim, [&](auto t, auto dp, auto tiny) {
+  int rc = check_grid("tgx_attention", blocks, 64 * f.wq * f.wk);
+  if (rc) return rc;
+  rc = by_head(dtype, a.dim, [&](auto t, auto dp, auto tiny) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value, TS = kTile<T>;
     constexpr bool TINY = decltype(tiny)::value;

@@ -431,7 +431,9 @@ size_t att_rows_forward_workspace(const AttArgs& a) {
 int att_rows_forward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
   const RowShape f(a);
   const AttParts part(ws, a.batch * a.lq * a.heads, f.splits);
-  const int rc = by_lanes(dtype, a.dim, a.lq * a.group, [&](auto t, auto tiny, auto lp, auto c, auto m) {
+  int rc = check_grid("tgx_attention", f.blocks, kRowThreads);
+  if (rc) return rc;
+  rc = by_lanes(dtype, a.dim, a.lq * a.group, [&](auto t, auto tiny, auto lp, auto c, auto m) {
     hipLaunchKernelGGL((att_rows_fwd<decltype(t), decltype(tiny)::value, decltype(lp)::value, decltype(c)::value,
                                      decltype(m)::value>),
                        dim3(static_cast<unsigned>(f.blocks)), dim3(kRowThreads), 0, s, a, f.wpp, f.splits, f.span, part);
@@ -448,7 +450,9 @@ size_t att_rows_backward_workspace(const AttArgs& a) {
 int att_rows_backward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
   const RowShape f(a);
   float* part = static_cast<float*>(ws);
-  const int rc = by_lanes(dtype, a.dim, a.lq * a.group, [&](auto t, auto tiny, auto lp, auto c, auto m) {
+  int rc = check_grid("tgx_attention_grad", f.blocks, kRowThreads);
+  if (rc) return rc;
+  rc = by_lanes(dtype, a.dim, a.lq * a.group, [&](auto t, auto tiny, auto lp, auto c, auto m) {
     hipLaunchKernelGGL((att_rows_bwd<decltype(t), decltype(tiny)::value, decltype(lp)::value, decltype(c)::value,
                                      decltype(m)::value>),
                        dim3(static_cast<unsigned>(f.blocks)), dim3(kRowThreads), 0, s, a, f.wpp, f.splits, f.span, part);

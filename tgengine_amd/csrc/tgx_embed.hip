@@ -503,6 +503,8 @@ extern "C" int tgx_embed_grad(const void* dout, const void* ids, int32_t ids_i32
                               void* stream) {
   int rc = check_embed("tgx_embed_grad", grad, dout, rows, dim, dtype, ids, n);
   if (rc) return rc;
+  if (n >= int64_t(1) << 29)  // embed_join takes 512 threads for every tile of 64
+    return fail(TGX_ERR_LIMIT, "tgx_embed_grad: n=%lld (below 2^29)", static_cast<long long>(n));
   if (rows == 0) return TGX_OK;
   if (grad == nullptr) return fail(TGX_ERR_ARG, "tgx_embed_grad: grad must not be NULL");
   hipStream_t s = static_cast<hipStream_t>(stream);
