@@ -4,42 +4,36 @@
 // keys gives S^T = K Q^T (keys down a lane's registers, one row a lane), so that the
 // running maximum and sum of the softmax are a lane's own but for an exchange between
 // the lanes of a row now and then, and P^T, still in the same registers, is the second operand of
-// O^T += V^T P^T.  Scores are in units of log 2.  Probabilities are rounded to the
-// inputs' type for that product, as the matrix units take them; sums stay in 32 bits.  (With
-// bf16 and many keys that rounding and the output's own make sqrt 2 of one rounding's error:
-// 0.0024 where the output's alone is 0.0017.  A second product for what rounding took doubles
-// the cost of P V, so only few keys have it.)
+// O^T += V^T P^T.  Scores are in units of log 2.  bf16's matrix units take probabilities of
+// bf16: a second product adds what rounding them took (itself rounded to bf16, 2^-16 of a
+// probability), so that an output is off by its own rounding only.  Without it the two
+// roundings' errors together were 1.41 times the output's own, however many keys there were.
+// It uses the same reads of V: 2 x (1,000 x 8,000 tokens), 16/4 heads of 128, take 237 us
+// with it and 185 without, 200 x (200 x 200), 4 heads of 64, 61 and 55, single tokens to
+// 30,001 keys 96 either way.
 //
 // What bounds it: for bf16 the softmax between the products and the LDS reads that feed
-// them (2 x (1,000 x 8,000 tokens), 16/4 heads of 128, 92% kept: 177 us, 679 TFLOP/s of the
-// 1,225 that a matrix product of 8,192 reaches); for f32 the matrix units, eight times slower
+// them (that first call, 92% kept: 510 TFLOP/s of the 1,225 that a matrix product of 8,192
+// reaches, 760 with the second product counted); for f32 the matrix units, eight times slower
 // (400 x (65 x 65), 2 heads of 100: 51 us for 75 MB and 1.4 GFLOP, whose 16-row tiles pad
 // 65 to 80 and 100 to 112); for single tokens the reads of keys and values (5 x 30,001 keys
-// of 8 heads of 128, bf16, 73% kept: 99 us for 447 MB, 4.5 TB/s).
+// of 8 heads of 128, bf16, 73% kept: 97 us for 447 MB, 4.6 TB/s).
 #include "tgx_attention.h"
 
 namespace tgx {
 namespace {
-
-constexpr int64_t kFineKeys = 128;
 
 // The waves of a workgroup take kTile rows each: WQ of them, or 4 to 8 for WQ = 0 (f32,
 // whose 16-row tiles fit odd lengths better); WK > 1: WK waves take the same rows, one tile
 // of each KT = 64 keys each, and are joined at the end.  With splits > 1 the keys are cut in
 // as many ranges of `span` keys and each leaves its maximum, sum and unscaled output in
 // `part` for att_join.
-//
-// FINE: what rounding took from the probabilities goes through a second product, for bf16
-// with at most kFineKeys keys.  Few kept keys do not average those errors away, and the
-// gradient's inner products of output and its gradient would hand them to every score: with
-// 1 or 2 of 6 keys kept dq and dk were over 1.5 times as far off as one rounding of them, and
-// are 1.42 times so.  It takes 1,000 x (100 x 128 tokens), 4/2 heads of 128, from 108 to 117 us,
-// 2,000 x (20 x 20), 2 heads of 64, from 20.5 to 21.5.
-template <typename T, bool TINY, int DP, int WQ, int WK, bool FINE>
+template <typename T, bool TINY, int DP, int WQ, int WK>
 __global__ __launch_bounds__(WQ == 0 ? 512 : 64 * WQ * WK, DP > 128 ? 1 : WQ == 0 && DP <= 112 ? 4 : 2) void att_mma_fwd(const AttArgs a, int mtiles, int splits,
                                                                              int64_t span, const AttParts part) {
   using KTile = LdsTile<T, DP, Reads::kRows>;
   using VTile = LdsTile<T, DP, Reads::kColumns>;
+  constexpr bool FINE = sizeof(T) == 2;  // the second product
   constexpr int TS = kTile<T>, KT = sizeof(T) == 2 || WK > 1 ? 64 : 32, SUB = KT / TS / WK,
                 OT = DP / TS, ST = DP / kStep;
   static_assert(WK == 1 || SUB == 1, "one tile of keys a wave");
@@ -137,9 +131,7 @@ __global__ __launch_bounds__(WQ == 0 ? 512 : 64 * WQ * WK, DP > 128 ? 1 : WQ == 
         for (int f = 0; f < kFrags<T>; ++f) pf[u][f] = to_frag<T>(s[u], f);
         if constexpr (FINE) {
 #pragma unroll
-          for (int i = 0; i < kRegs<T>; ++i) s[u][i] = lost<T>(s[u][i]);
-#pragma unroll
-          for (int f = 0; f < kFrags<T>; ++f) rest[u][f] = to_frag<T>(s[u], f);
+          for (int f = 0; f < kFrags<T>; ++f) rest[u][f] = lost_frag<T>(s[u], f);
         }
       }
     }
@@ -330,14 +322,9 @@ int att_mma_forward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
     constexpr int DP = decltype(dp)::value, TS = kTile<T>;
     constexpr bool TINY = decltype(tiny)::value;
     const dim3 grid(static_cast<unsigned>(blocks)), block(64 * f.wq * f.wk);
-    auto launch = [&](auto wq, auto wk, auto fine) {
-      hipLaunchKernelGGL((att_mma_fwd<T, TINY, DP, decltype(wq)::value, decltype(wk)::value, decltype(fine)::value>), grid,
-                         block, 0, s, a, f.mtiles, f.splits, f.span, part);
-    };
     auto go = [&](auto wq, auto wk) {
-      if constexpr (sizeof(T) == 2)
-        if (a.lk <= kFineKeys) return launch(wq, wk, std::true_type{});
-      launch(wq, wk, std::false_type{});
+      hipLaunchKernelGGL((att_mma_fwd<T, TINY, DP, decltype(wq)::value, decltype(wk)::value>), grid, block, 0, s, a, f.mtiles,
+                         f.splits, f.span, part);
     };
     constexpr std::integral_constant<int, 1> one{};
     if (f.wk > 1) go(one, std::integral_constant<int, 64 / TS>{});

@@ -122,6 +122,21 @@ __device__ __forceinline__ u32x4 to_frag(const Acc<T>& x, int f) {
   return y;
 }
 
+// what rounding to T takes from x
+template <typename T>
+__device__ __forceinline__ float lost(float x) { return x - to_f(from_f<T>(x)); }
+
+// to_frag of what rounding to bf16 takes from the values
+template <typename T>
+__device__ __forceinline__ u32x4 lost_frag(const Acc<T>& x, int f) {
+  u32x4 y;
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    y[u] = __builtin_bit_cast(uint32_t, __builtin_convertvector(
+                                            (f32x2{lost<T>(x[f * 8 + 2 * u]), lost<T>(x[f * 8 + 2 * u + 1])}), bf16x2));
+  return y;
+}
+
 // An LDS tile of rows of DP values, longer by what keeps its reads off each other's banks
 // (64 of 4 bytes).  A fragment reads 16 bytes of each of 16 rows at a time: rows an odd
 // multiple of 16 bytes apart are free of conflicts.  The transposed reads of bf16 take 64
@@ -297,10 +312,6 @@ __device__ __forceinline__ void store_columns(T* row, const Acc<T> (&x)[DP / kTi
       }
     }
 }
-
-// what rounding to T takes from x
-template <typename T>
-__device__ __forceinline__ float lost(float x) { return x - to_f(from_f<T>(x)); }
 
 // the same in 32 bits, for the parts of ranges
 template <typename T, int DP>
