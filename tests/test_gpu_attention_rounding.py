@@ -1,9 +1,9 @@
-"""bf16 cross_attention rounds its outputs once, however many keys there are and however
-many of them the mask keeps.
+"""bf16 cross_attention rounds outputs and gradients once, however many keys there are and
+however many of them the mask keeps.
 
-Matrix products take probabilities in two parts, bf16 and what rounding to it took: r = 2^-8
-of what r took, so s = 2^-16 of the value is left out.  The output adds its own rounding,
-r.  Scores, sums and exponentials are of 32 bits, u = 2^-24: a score is off by at most
+Matrix products take probabilities and score gradients in two parts, bf16 and what rounding
+to it took, and the gradient takes the output likewise: r = 2^-8 of what r took, so s = 2^-16
+of the value is left out.  Results add their own rounding, r.  Scores, sums and exponentials are of 32 bits, u = 2^-24: a score is off by at most
 E = (D + 4) u scale max |q|.|k|, a probability by 2 E + (Lk + 16) u relatively."""
 import pytest
 import torch
@@ -53,7 +53,26 @@ def _exact(q, k, v, g, mask):
     E = (d + 4) * U * scale * ((Q.abs() @ K.abs().mT) * keep).amax(-1, keepdim=True)
     rel = 2 * E + (lk + 16) * U
     eP = P * (rel + S)
-    return {"out": (cols(O), cols(eP @ V.abs() + O.abs() * (R + U)))}
+    out = {"out": (cols(O), cols(eP @ V.abs() + O.abs() * (R + U)))}
+    if g is None:
+        return out
+    G = rows(g)
+    delta = (G * O).sum(-1, keepdim=True)
+    dP = torch.where(keep, G @ V.mT, 0.0)
+    dS = P * (dP - delta) * scale
+    dot = (d + 4) * U  # a product's or delta's own sum of d terms
+    eS = P * scale * ((dP.abs() + delta.abs()) * rel + dot * (G.abs() @ V.abs().mT)
+                      + (S + rel + dot) * (G.abs() * (P @ V.abs())).sum(-1, keepdim=True)) + dS.abs() * S
+    n = (lq * (h // kv) + 8) * U
+
+    def shared(x):
+        return x.reshape(b, kv, h // kv, lk, d).sum(2).permute(0, 2, 1, 3)
+
+    dq, dk, dv = cols(dS @ K), shared(dS.mT @ Q), shared(P.mT @ G)
+    out["dq"] = dq, cols(eS @ K.abs() + (lk + 8) * U * (dS.abs() @ K.abs())) + dq.abs() * R
+    out["dk"] = dk, shared(eS.mT @ Q.abs() + n * (dS.abs().mT @ Q.abs())) + dk.abs() * R
+    out["dv"] = dv, shared(eP.mT @ G.abs() + n * (P.mT @ G.abs())) + dv.abs() * R
+    return out
 
 
 def _check(got, ref):
@@ -70,7 +89,19 @@ SHAPES = [(33, 1, 64), (40, 2, 40), (7, 1, 100), (1, 8, 128), (130, 1, 96), (20,
 def test_output(lq, group, d, lk, most):
     q, k, v, g = _inputs(3, lq, lk, 2 * group, 2, d, lk + most)
     mask = _few(3, lk, most, lk)
-    _check({"out": ops.cross_attention(q, k, v, mask=mask)}, _exact(q, k, v, g, mask))
+    _check({"out": ops.cross_attention(q, k, v, mask=mask)}, _exact(q, k, v, None, mask))
+
+
+@pytest.mark.parametrize("lk,most", [(6, 2), (64, 0), (129, 2), (300, 8), (1000, 1), (5000, 3), (300, 0), (1100, 0)])
+@pytest.mark.parametrize("lq,group,d", SHAPES)
+def test_gradients(lq, group, d, lk, most):
+    q, k, v, g = _inputs(3, lq, lk, 2 * group, 2, d, lk + most)
+    mask = _few(3, lk, most, lk)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    o = ops.cross_attention(*leaves, mask=mask)
+    got = dict(zip(("out", "dq", "dk", "dv"), (o, *torch.autograd.grad(o, leaves, g))))
+    with torch.no_grad():
+        _check(got, _exact(q, k, v, g, mask))
 
 
 def test_padding_changes_nothing():

@@ -8,8 +8,8 @@
 // As in the forward pass every score tile stays in the registers it was computed in: a
 // wave's columns are what it owns (keys for dk and dv, rows for dq), a lane's 16 values
 // run along the axis that the next product sums over, and that product's first operand
-// comes transposed out of LDS.  p and ds are rounded to the inputs' type for those
-// products, sums stay in 32 bits.
+// comes transposed out of LDS.  Sums stay in 32 bits, and bf16's products take p and ds in two
+// parts, so that a gradient is off by its own rounding only (mma_fine).
 #include "tgx_attention.h"
 
 namespace tgx {
@@ -23,8 +23,7 @@ __host__ __device__ __forceinline__ int64_t scores_row(int64_t lk) { return (lk 
 // Per row, in the order of problems and their rows: its log sum in units of log 2 (+inf
 // for a row that keeps no key: its probabilities are then zeros) and delta, from the output
 // as it was before rounding where its rest was kept: delta's error reaches every score of
-// the row alike.  Without it dq was over 1.5 times as far off as one rounding of it is, with
-// it 1.42 to 1.45 times, which rounded probabilities and a rounded result account for.
+// the row alike.
 // kDeltaLanes lanes a row; HBM bounds it (52,000 f32 rows of 100: 42 MB in 11 us, 3.7 TB/s)
 template <typename T>
 __global__ __launch_bounds__(256) void att_stats(const T* __restrict__ out, const T* __restrict__ rest,
@@ -56,9 +55,27 @@ __global__ __launch_bounds__(256) void att_stats(const T* __restrict__ out, cons
   stats[to] = make_float2(x == -INFINITY ? INFINITY : x * kLog2e, s);
 }
 
+// sums += fragment f of x times the tile's rows from row0 on.  bf16 takes what rounding x to
+// bf16 loses through a second product with the same operand out of LDS (2^-16 of x is left
+// out): without it dq, dk and dv were 1.41 to 1.45 times as far off as one rounding of them.
+// 2 x (1,000 x 8,000 tokens), 16/4 heads of 128, 92% kept: dk and dv 494 us with it and 406
+// without, dq 314 and 257; 400 x (65 x 65), 2 heads of 100: 72 and 64, 28 and 27.
+template <typename T, int DP, typename TILE>
+__device__ __forceinline__ void mma_fine(Acc<T> (&sums)[DP / kTile<T>], const T* tile, int row0, const Acc<T>& x, int f) {
+  const u32x4 xf = to_frag<T>(x, f);
+  u32x4 rest;
+  if constexpr (sizeof(T) == 2) rest = lost_frag<T>(x, f);
+#pragma unroll
+  for (int t = 0; t < DP / kTile<T>; ++t) {
+    const u32x4 y = TILE::transposed(tile, row0, f, t);
+    sums[t] = mma<T>(sums[t], y, xf);
+    if constexpr (sizeof(T) == 2) sums[t] = mma<T>(sums[t], y, rest);
+  }
+}
+
 // Keeps the steps of bf16's dk and dv apart: left to itself the compiler reads all operands
-// ahead and runs out of registers (605 us for 1,000 x 8,000 tokens, 422 so; the other wave
-// of the SIMD fills the gaps).  f32 has the registers.
+// ahead and runs out of registers (605 us for 1,000 x 8,000 tokens, 422 so, both with one
+// product each; the other wave of the SIMD fills the gaps).  f32 has the registers.
 template <typename T>
 __device__ __forceinline__ void one_by_one() {
   if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
@@ -74,16 +91,17 @@ __device__ __forceinline__ void one_by_one() {
 // dk's before dv's.
 // KEEP (f32): ds goes to `scores`, rows of scores_row() keys, for att_scores_q.
 //
-// Bounded by the LDS reads, each operand of four products, and the exchange with the softmax
-// for bf16: 2 x (1,000 x 8,000 tokens), 16/4 heads of 128, 92% kept, 400 us, 601 TFLOP/s;
+// Bounded by the matrix units and the LDS reads that feed them, behind the steps that registers
+// keep apart, for bf16: 2 x (1,000 x 8,000 tokens), 16/4 heads of 128, 92% kept, 494 us, 488
+// TFLOP/s of four products and 732 of the six;
 // by the matrix units for f32: 400 x (65 x 65), 2 heads of 100, 95 us, 48 TFLOP/s with the
 // padding to 80 x 80 x 112 and 29 without.
 //
 // LEAST to kv_most() waves a workgroup.  bf16 heads of 65 to 128 values come two ways: 8
 // waves, which leaves each the registers for one row of staging and two waves a SIMD, or 2
 // to 4 with all registers for up to 64 keys, which 8 waves would mostly idle through (200 x
-// 100 rows, 4/2 heads: of 128 with 64 keys 94 us by 8 waves and 71 so, with 100 103 and 102,
-// with 144 110 and 152; of 80 with 64 60 and 52, with 90 64 and 75).
+// 100 rows, 4/2 heads: of 128 with 64 keys 62 us by 8 waves and 36 so, with 100 66 and 64,
+// with 144 72 and 120; of 80 with 64 42 and 27, with 90 43 and 48).
 template <typename T, int DP>
 constexpr bool kTwoWays = sizeof(T) == 2 && DP > 64 && DP <= 128;
 template <typename T, int DP>
@@ -211,9 +229,7 @@ void att_mma_kv(const AttArgs a, int ktiles, int splits, int64_t span, const flo
         one_by_one<T>();
 #pragma unroll
         for (int f = 0; f < kFrags<T>; ++f) {
-          const u32x4 pf = to_frag<T>(s, f);
-#pragma unroll
-          for (int t = 0; t < OT; ++t) dv[t] = mma<T>(dv[t], Tile::transposed(sg[cur], 0, f, t), pf);
+          mma_fine<T, DP, Tile>(dv, sg[cur], 0, s, f);
           one_by_one<T>();
         }
 #pragma unroll
@@ -234,9 +250,7 @@ void att_mma_kv(const AttArgs a, int ktiles, int splits, int64_t span, const flo
         one_by_one<T>();
 #pragma unroll
         for (int f = 0; f < kFrags<T>; ++f) {
-          const u32x4 df = to_frag<T>(dp, f);
-#pragma unroll
-          for (int t = 0; t < OT; ++t) dk[t] = mma<T>(dk[t], Tile::transposed(sq[cur], 0, f, t), df);
+          mma_fine<T, DP, Tile>(dk, sq[cur], 0, dp, f);
           one_by_one<T>();
         }
       }
@@ -326,7 +340,8 @@ __global__ __launch_bounds__(512, 2) void att_scores_q(const AttArgs a, int mtil
 // dq, kTile rows a wave.  S^T = K Q^T and dP^T = V dO^T have the keys down a lane's registers
 // and one row a lane; dQ^T += K^T dS^T follows.  With splits > 1 each range of `span` keys
 // leaves its sum in `part`.  W waves, or 4 to 8 for W = 0.  Bounded as att_mma_kv is: 2 x
-// (1,000 x 8,000 tokens), 16/4 heads of 128, bf16, 92% kept, 250 us, 721 TFLOP/s.
+// (1,000 x 8,000 tokens), 16/4 heads of 128, bf16, 92% kept, 314 us, 576 TFLOP/s of three
+// products and 768 of the four.
 template <typename T, bool TINY, int DP, int W>
 __global__ __launch_bounds__(W == 0 ? 512 : 64 * W, DP > 128 ? 1 : 2) void att_mma_q(const AttArgs a, int mtiles, int splits,
                                                                      int64_t span, const float2* __restrict__ stats,
@@ -397,11 +412,7 @@ __global__ __launch_bounds__(W == 0 ? 512 : 64 * W, DP > 128 ? 1 : 2) void att_m
         if (here != ALL) dp[i] = here >> (4 * group) >> mma_row<T>(i, 0) & 1 ? dp[i] : 0.f;
       }
 #pragma unroll
-      for (int f = 0; f < kFrags<T>; ++f) {
-        const u32x4 df = to_frag<T>(dp, f);
-#pragma unroll
-        for (int t = 0; t < OT; ++t) dq[t] = mma<T>(dq[t], KTile::transposed(sk, u * TS, f, t), df);
-      }
+      for (int f = 0; f < kFrags<T>; ++f) mma_fine<T, DP, KTile>(dq, sk, u * TS, dp, f);
     }
   }
   if (r >= rows) return;
@@ -411,7 +422,7 @@ __global__ __launch_bounds__(W == 0 ? 512 : 64 * W, DP > 128 ? 1 : 2) void att_m
 
 // dq's row tiles, and the ranges the keys are cut in where those alone leave compute units
 // without work: 1,024 workgroups (2 x (300 x 6,000 tokens), 8/4 heads of 128, bf16, with dk
-// and dv: 115 us, 126 with 256 workgroups and 368 uncut), of 4 waves where heads of more than
+// and dv: 136 us, 151 with 256 workgroups and 342 uncut), of 4 waves where heads of more than
 // 128 values take all registers
 struct QShape {
   int w, mtiles, splits;
@@ -432,8 +443,8 @@ struct QShape {
 
 // dk's and dv's key tiles, and the ranges the rows are cut in where those alone leave half
 // of the compute units without work: at most 256 workgroups, since every range writes
-// its sums of all keys (1 x (2,000 x 2,000 tokens), 2/1 heads of 128, bf16: 87 us, 389 uncut;
-// 2 x (300 x 6,000), 8/4 heads of 128: 123 us, 185 in three ranges)
+// its sums of all keys (1 x (2,000 x 2,000 tokens), 2/1 heads of 128, bf16: 91 us, 436 uncut;
+// 2 x (300 x 6,000), 8/4 heads of 128: 136 us, 175 in three ranges)
 struct KvShape {
   int least, w, ktiles, splits;
   int64_t span, sums;  // sums: values of dk's parts, and of dv's

@@ -280,13 +280,13 @@ int join_launch(void* out, void* rest, float* lse, int64_t rows, int dim, int dt
 
 // Row tiles, and the ranges the keys are cut in where the row tiles alone would leave most
 // of the 256 compute units without work: 512 workgroups, the most that the registers let run
-// at a time (2 x (300 x 6,000 tokens), 8/4 heads of 128, bf16: 40 us, 51 with 1,024 and 171
+// at a time (2 x (300 x 6,000 tokens), 8/4 heads of 128, bf16: 43 us, 54 with 1,024 and 206
 // uncut; f32 192, 210 and 977), or 1,024 of the smaller ones that share a row tile (5 x
-// 30,001 keys, 32/8 heads of 128, bf16: 105 us, 108 with 512, 127 with 2,048).
+// 30,001 keys, 32/8 heads of 128, bf16, all kept: 118 us, 124 with 512, 135 with 2,048).
 //
 // A problem of one row tile gives every tile of keys to WK waves (f32, 4 x 10,000 keys,
-// 32/8 heads of 128: 68 us, 94 with a tile of rows each; bf16 38 and 35 there, but 25 and 31
-// for 2,000 x 70 keys, 8/2 heads of 64).
+// 32/8 heads of 128: 68 us, 94 with a tile of rows each; bf16 38 and 39 there, 27 and 34 for
+// 2,000 x 70 keys, 8/2 heads of 64).
 struct FwdShape {
   int wq, wk, mtiles, splits;
   int64_t span;

@@ -73,12 +73,12 @@ AttArgs att_args(const tgx_attention_args* p) {
 }
 
 // Whether a call takes the kernels of tgx_att_rows.hip.  A backward pass of at most 4 rows
-// a problem does (2,000 x 2 problems of 4 rows and 64 keys, dim 128: 80 us in bf16 and 133
-// in f32, against 158 and 249 of the matrix units), and a forward pass of one row (f32, 64
+// a problem does (2,000 x 2 problems of 4 rows and 64 keys, dim 128: 84 us in bf16 and 133
+// in f32, against 174 and 249 of the matrix units), and a forward pass of one row (f32, 64
 // keys: 42 us against 71; 10,000 keys, 8 x 2 problems: 37 against 50).  More rows take a
 // vector kernel several times as many instructions and the matrix units none: above 64 keys
-// they go there (500 x 2 problems of 4 rows and 256 keys, bf16: 37 us here, 26 there; at 20
-// keys, 2,000 x 2 problems: 20 here, 30 there).
+// they go there (500 x 2 problems of 4 rows and 256 keys, bf16: 39 us here, 28 there; at 20
+// keys, 2,000 x 2 problems: 21 here, 42 there).
 bool by_rows(const AttArgs& a, bool grad) {
   const int64_t rows = a.lq * a.group;
   return rows <= kMostRows && (grad || rows == 1 || a.lk <= 64);
