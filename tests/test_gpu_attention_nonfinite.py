@@ -1,0 +1,68 @@
+"""cross_attention where inputs are NaN or infinite: they reach what the formulas lead them to and nothing else."""
+import pytest
+import torch
+
+from tgengine_amd import ops
+
+pytestmark = pytest.mark.gpu
+NAN, INF = float("nan"), float("inf")
+# (lq, lk, d) with 2 heads a key/value head: few rows, cut keys, matrix units, f32 kept scores and without, wide heads
+SHAPES = [(1, 40, 50), (2, 900, 64), (1, 3000, 172), (70, 90, 100), (65, 300, 128), (40, 3000, 64), (20, 70, 200)]
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+def _inputs(lq, lk, d, dtype, seed=0):
+    """q, k, v, g and a mask with holes; batch row 2 keeps no key."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = [torch.randn(*s, generator=g, device="cuda").to(TYPES[dtype])
+         for s in ((4, lq, 4, d), (4, lk, 2, d), (4, lk, 2, d), (4, lq, 4, d))]
+    mask = torch.rand(4, lk, generator=g, device="cuda") < 0.5
+    mask[:, lk // 3] = True
+    mask[2] = False
+    return *x, mask
+
+
+def _run(q, k, v, g, mask):
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    o = ops.cross_attention(*leaves, mask=mask)
+    return dict(zip(("out", "dq", "dk", "dv"), (o.detach(), *torch.autograd.grad(o, leaves, g))))
+
+
+def _same_but(got, want, nan):
+    """``got`` is NaN where ``nan`` says (a mask for each output), and elsewhere has ``want``'s bits."""
+    for name, x in got.items():
+        at = nan.get(name, torch.zeros((), device="cuda", dtype=torch.bool)).expand(x.shape)
+        assert bool(x[at].isnan().all()), name
+        assert torch.equal(x[~at], want[name][~at]), name
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lq,lk,d", SHAPES)
+def test_rows_without_keys_hold_anything(lq, lk, d, dtype):
+    """Queries and gradients of a batch row whose mask is empty change nothing."""
+    q, k, v, g, mask = _inputs(lq, lk, d, dtype)
+    want = _run(q, k, v, g, mask)
+    for x in (NAN, INF, -INF):
+        for which in ("q", "g", "qg"):
+            q1, g1 = q.clone(), g.clone()
+            if "q" in which:
+                q1[2] = x
+            if "g" in which:
+                g1[2] = x
+            got = _run(q1, k, v, g1, mask)
+            _same_but(got, want, {})
+            assert not any(got[n][2].any() for n in got)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lq,lk,d", SHAPES)
+def test_masked_keys_take_no_gradient(lq, lk, d, dtype):
+    """A gradient of NaN in one row reaches the kept keys of its batch row and head, and no masked key."""
+    q, k, v, g, mask = _inputs(lq, lk, d, dtype)
+    want = _run(q, k, v, g, mask)
+    g[1, lq - 1, 0] = NAN
+    row = torch.zeros(4, lq, 4, 1, device="cuda", dtype=torch.bool)
+    row[1, lq - 1, 0] = True
+    keys = torch.zeros(4, lk, 2, 1, device="cuda", dtype=torch.bool)
+    keys[1, :, 0, 0] = mask[1]
+    _same_but(_run(q, k, v, g, mask), want, {"dq": row, "dk": keys, "dv": keys})

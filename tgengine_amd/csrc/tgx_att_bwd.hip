@@ -140,7 +140,7 @@ void att_mma_kv(const AttArgs a, int ktiles, int splits, int64_t span, const flo
 #pragma unroll
   for (int t = 0; t < OT; ++t) dk[t] = dv[t] = Acc<T>{};
   if (__syncthreads_or(kept)) {
-    const bool all = __all(kept), busy = __any(kept);
+    const bool busy = __any(kept);
     const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[2];
     const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[2];
     u32x4 kf[HELD ? ST : 1], vf[HELD ? ST : 1];
@@ -222,10 +222,7 @@ void att_mma_kv(const AttArgs a, int ktiles, int splits, int64_t span, const flo
         }
         one_by_one<T>();
 #pragma unroll
-        for (int i = 0; i < kRegs<T>; ++i) {
-          s[i] = exp2_(fmaf(s[i], c, -slse[cur][mma_row<T>(i, group)]));
-          if (!all) s[i] = kept ? s[i] : 0.f;
-        }
+        for (int i = 0; i < kRegs<T>; ++i) s[i] = exp2_(fmaf(s[i], c, -slse[cur][mma_row<T>(i, group)]));
         one_by_one<T>();
 #pragma unroll
         for (int f = 0; f < kFrags<T>; ++f) {
@@ -245,7 +242,8 @@ void att_mma_kv(const AttArgs a, int ktiles, int splits, int64_t span, const flo
           if (j < scores_row(a.lk))
 #pragma unroll
             for (int i = 0; i < kRegs<T>; ++i)
-              if (first + mma_row<T>(i, group) < rows) to[mma_row<T>(i, group) * scores_row(a.lk)] = dp[i];
+              if (first + mma_row<T>(i, group) < rows)
+                to[mma_row<T>(i, group) * scores_row(a.lk)] = kept ? dp[i] : 0.f;
         }
         one_by_one<T>();
 #pragma unroll
@@ -261,6 +259,11 @@ void att_mma_kv(const AttArgs a, int ktiles, int splits, int64_t span, const flo
     }
   }
   if (j >= a.lk) return;
+  // A masked key's sums were taken along: a product's columns are its lanes' own, and what
+  // the rows hold (a gradient of NaN, say) must not reach it
+  if (!kept)
+#pragma unroll
+    for (int t = 0; t < OT; ++t) dk[t] = dv[t] = Acc<T>{};
   if (splits > 1) {
     float* to = part + (at * splits + sp) * a.dim;
     if (a.dk != nullptr) store_parts<T, DP>(to, dk, a.dim);

@@ -317,6 +317,7 @@ __global__ __launch_bounds__(kRowThreads, M == 1 ? (C < 4 ? 3 : 2) : (C < 4 ? 2 
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int j = k0 + u * G + grp;
+        const bool on = bits >> j & 1;
         float f[N], y[N], dk[N], dv[N];
         at.values(f, kx[u]);
         at.values(y, vx[u]);
@@ -325,8 +326,8 @@ __global__ __launch_bounds__(kRowThreads, M == 1 ? (C < 4 ? 3 : 2) : (C < 4 ? 2 
 #pragma unroll
         for (int r = 0; r < M; ++r) {
           const float s = at.dot(q[r], qo[r], f) * c, dp = at.dot(g[r], go[r], y);
-          const float p = bits >> j & 1 ? exp2_(s - lse[r]) : 0.f;
-          const float ds = p * (dp - delta[r]) * a.scale;
+          const float p = exp2_(s - lse[r]);
+          const float ds = on ? p * (dp - delta[r]) * a.scale : 0.f;
 #pragma unroll
           for (int x = 0; x < N; ++x) {
             dq[r][x] = fmaf(ds, f[x], dq[r][x]);
@@ -334,6 +335,9 @@ __global__ __launch_bounds__(kRowThreads, M == 1 ? (C < 4 ? 3 : 2) : (C < 4 ? 2 
             dv[x] = fmaf(p, g[r][x], dv[x]);
           }
         }
+        if (!on)  // whatever the rows hold (a gradient of NaN, say), a masked key takes none of it
+#pragma unroll
+          for (int x = 0; x < N; ++x) dk[x] = dv[x] = 0.f;
         if (t + j < w.hi) {
           const int64_t to = (key0 + (t + j) * a.kv_heads) * a.dim;
           if (a.dk != nullptr) at.store(static_cast<T*>(a.dk) + to, dk);
