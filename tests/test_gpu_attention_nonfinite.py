@@ -66,3 +66,49 @@ def test_masked_keys_take_no_gradient(lq, lk, d, dtype):
     keys = torch.zeros(4, lk, 2, 1, device="cuda", dtype=torch.bool)
     keys[1, :, 0, 0] = mask[1]
     _same_but(_run(q, k, v, g, mask), want, {"dq": row, "dk": keys, "dv": keys})
+
+
+def _spread(q, mask, lq, lk, rows):
+    """What a score of NaN in ``rows`` of batch row 1 and head 0 reaches."""
+    row = torch.zeros(4, lq, 4, 1, device="cuda", dtype=torch.bool)
+    row[1, rows, 0] = True
+    keys = torch.zeros(4, lk, 2, 1, device="cuda", dtype=torch.bool)
+    keys[1, :, 0, 0] = mask[1]
+    return {"out": row, "dq": row, "dk": keys, "dv": keys}
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lq,lk,d", SHAPES)
+def test_scores_of_nan(lq, lk, d, dtype):
+    """A NaN query makes all its probabilities NaN, so out and dq of its row and dk and dv of
+    every kept key of its head; a NaN key does so for every row of its head."""
+    q, k, v, g, mask = _inputs(lq, lk, d, dtype)
+    want = _run(q, k, v, g, mask)
+    q1 = q.clone()
+    q1[1, lq - 1, 0, d // 2] = NAN
+    _same_but(_run(q1, k, v, g, mask), want, _spread(q, mask, lq, lk, lq - 1))
+    k1 = k.clone()
+    k1[1, lk // 3, 0, 0] = NAN
+    nan = _spread(q, mask, lq, lk, slice(None))
+    for name in ("out", "dq"):
+        nan[name][1, :, 1] = True  # the head's second query head
+    _same_but(_run(q, k1, v, g, mask), want, nan)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lq,lk,d", SHAPES)
+def test_scores_of_infinity(lq, lk, d, dtype):
+    """A score of +inf: exp(inf - inf) is NaN, and so is the row's sum."""
+    q, k, v, g, mask = _inputs(lq, lk, d, dtype)
+    k[1, lk // 3, 0, 0] = 2.0
+    want = _run(q, k, v, g, mask)
+    q[1, lq - 1, 0] = 0.0
+    q[1, lq - 1, 0, 0] = INF
+    k1 = k.clone()
+    k1[1, mask[1], 0, 0] = k1[1, mask[1], 0, 0].abs() + 1.0  # all of the row's scores are +inf or masked
+    for keys in (k, k1):
+        got = _run(q, keys, v, g, mask)
+        assert got["out"][1, lq - 1, 0].isnan().all() and got["dq"][1, lq - 1, 0].isnan().all()
+        assert got["dv"][1, mask[1], 0].isnan().all() and not got["dv"][1, ~mask[1]].any()
+        for n in got:
+            assert torch.equal(got[n][[0, 2, 3]], want[n][[0, 2, 3]]), n

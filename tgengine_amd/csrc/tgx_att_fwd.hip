@@ -195,8 +195,8 @@ __global__ __launch_bounds__(WQ == 0 ? 512 : 64 * WQ * WK, DP > 128 ? 1 : WQ == 
     store_parts<T, DP>(part.o + (row * splits + sp) * a.dim, o, a.dim);
     return;
   }
-  if (group == 0 && a.lse != nullptr) a.lse[row] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  if (group == 0 && a.lse != nullptr) a.lse[row] = log_sum(m, l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   store_columns<T, DP>(static_cast<T*>(a.o) + row * a.dim, o, inv, a.dim);
   if (sizeof(T) == 2 && a.rest != nullptr) {
 #pragma unroll
@@ -227,8 +227,8 @@ __global__ __launch_bounds__(256) void att_join(T* __restrict__ out, T* __restri
     if (m == -INFINITY) m = 0.f;  // no range kept a key: all sums are 0
     for (int y = lane; y < splits; y += kWave) l += ml[y].y * exp2_(ml[y].x - m);
     l = group_sum<kWave>(l);
-    by = l > 0.f ? 1.f / l : 0.f;
-    if (lane == 0 && lse != nullptr) lse[row] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+    by = l == 0.f ? 0.f : 1.f / l;
+    if (lane == 0 && lse != nullptr) lse[row] = log_sum(m, l);
   }
   const float* o = part.o + row * splits * dim;
   for (int c = (lane % LT) * 4; c < dim; c += LT * 4) {

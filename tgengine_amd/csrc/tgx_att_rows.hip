@@ -253,7 +253,7 @@ __global__ __launch_bounds__(kRowThreads, M == 1 && C < 4 ? 3 : 2) void att_rows
       at.store(out, acc[r]);
       continue;
     }
-    const float inv = l[r] > 0.f ? 1.f / l[r] : 0.f;
+    const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
 #pragma unroll
     for (int x = 0; x < N; ++x) acc[r][x] *= inv;
     at.store(static_cast<T*>(a.o) + row * a.dim, acc[r]);
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(kRowThreads, M == 1 && C < 4 ? 3 : 2) void att_rows
       for (int x = 0; x < N; ++x) z[x] = lost<T>(acc[r][x]);
       at.store(static_cast<T*>(a.rest) + row * a.dim, z);
     }
-    if (at.gl == 0 && a.lse != nullptr) a.lse[row] = l[r] > 0.f ? (m[r] + log2f(l[r])) * kLn2 : -INFINITY;
+    if (at.gl == 0 && a.lse != nullptr) a.lse[row] = log_sum(m[r], l[r]);
   }
 }
 

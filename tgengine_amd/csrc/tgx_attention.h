@@ -431,6 +431,11 @@ constexpr int kNoLoads = 0x0f70;  // s_waitcnt: no vector load outstanding
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// A row's log sum from its maximum, in units of log 2, and its sum.  -inf stands for a row
+// without keys (a sum of 0) alone: a score of NaN or +inf makes the sum NaN, and the log sum
+// has to say so, or the gradient would take the row for one without keys.
+__device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2; }
+
 // Calls f(T{}, DP, TINY) with the head size padded to whole tiles: for f32 mostly to the
 // next 16, for bf16 to the next 32
 template <typename F>
