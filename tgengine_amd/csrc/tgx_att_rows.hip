@@ -70,14 +70,16 @@ struct Lanes {
     for (int u = 0; u < V; ++u) s = fmaf(z[u], f[N - V + u], s);
     return group_sum<LP>(s);
   }
+  // kept: ~0, or 0 to store zeros in the values' place
   template <typename U>
-  __device__ __forceinline__ void store(U* row, const float (&f)[N]) const {
+  __device__ __forceinline__ void store(U* row, const float (&f)[N], uint32_t kept = ~0u) const {
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       if (!has(j)) continue;
       Pack<U, V> p;
 #pragma unroll
       for (int u = 0; u < V; ++u) p.v[u] = from_f<U>(f[j * V + u]);
+      if constexpr (sizeof(p) == 16) p = __builtin_bit_cast(decltype(p), __builtin_bit_cast(u32x4, p) & kept);
       if constexpr (!TINY) {
         store_pack<U, V>(row + col(j), p);
       } else {
@@ -335,13 +337,12 @@ __global__ __launch_bounds__(kRowThreads, M == 1 ? (C < 4 ? 3 : 2) : (C < 4 ? 2 
             dv[x] = fmaf(p, g[r][x], dv[x]);
           }
         }
-        if (!on)  // whatever the rows hold (a gradient of NaN, say), a masked key takes none of it
-#pragma unroll
-          for (int x = 0; x < N; ++x) dk[x] = dv[x] = 0.f;
         if (t + j < w.hi) {
+          // whatever the rows hold (a gradient of NaN, say), a masked key takes none of it
+          const uint32_t bits_kept = on ? ~0u : 0u;
           const int64_t to = (key0 + (t + j) * a.kv_heads) * a.dim;
-          if (a.dk != nullptr) at.store(static_cast<T*>(a.dk) + to, dk);
-          if (a.dv != nullptr) at.store(static_cast<T*>(a.dv) + to, dv);
+          if (a.dk != nullptr) at.store(static_cast<T*>(a.dk) + to, dk, bits_kept);
+          if (a.dv != nullptr) at.store(static_cast<T*>(a.dv) + to, dv, bits_kept);
         }
       }
     }
