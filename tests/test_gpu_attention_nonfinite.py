@@ -112,3 +112,35 @@ def test_scores_of_infinity(lq, lk, d, dtype):
         assert got["dv"][1, mask[1], 0].isnan().all() and not got["dv"][1, ~mask[1]].any()
         for n in got:
             assert torch.equal(got[n][[0, 2, 3]], want[n][[0, 2, 3]]), n
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lq,lk,d", SHAPES)
+@pytest.mark.parametrize("x", [INF, -INF])
+def test_infinite_values_and_gradients(lq, lk, d, dtype, x):
+    """An infinite value at a kept key gives infinite outputs in its column, an infinite
+    gradient infinite dv in its: a probability above zero times an infinity is that infinity."""
+    q, k, v, g, mask = _inputs(lq, lk, d, dtype)
+    want = _run(q, k, v, g, mask)
+    v1, g1 = v.clone(), g.clone()
+    v1[1, lk // 3, 0, 3] = x
+    g1[1, lq - 1, 0, 2] = x
+    out, dv = _run(q, k, v1, g, mask)["out"], _run(q, k, v, g1, mask)["dv"]
+    assert bool((out[1, :, :2, 3] == x).all()) and bool((dv[1, mask[1], 0, 2] == x).all())
+    out[1, :, :2, 3] = want["out"][1, :, :2, 3]
+    dv[1, mask[1], 0, 2] = want["dv"][1, mask[1], 0, 2]
+    assert torch.equal(out, want["out"]) and torch.equal(dv, want["dv"])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lq,lk,d", SHAPES)
+def test_infinite_score_gradients(lq, lk, d, dtype):
+    """With a value of +inf and gradients above zero, out . dout is +inf and so every other
+    kept key's score gradient -inf; queries above zero take it to a dk of -inf."""
+    q, k, v, g, mask = _inputs(lq, lk, d, dtype)
+    q, g = q.abs() + 2.0 ** -4, g.abs() + 2.0 ** -4
+    v[1, lk // 3, 0, 3] = INF
+    dk = _run(q, k, v, g, mask)["dk"]
+    other = mask[1].clone()
+    other[lk // 3] = False
+    assert bool((dk[1, other, 0] == -INF).all()) and dk[1, lk // 3, 0].isnan().all() and not dk[1, ~mask[1]].any()

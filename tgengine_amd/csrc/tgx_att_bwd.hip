@@ -55,16 +55,15 @@ __global__ __launch_bounds__(256) void att_stats(const T* __restrict__ out, cons
   stats[to] = make_float2(x == -INFINITY ? INFINITY : x * kLog2e, s);
 }
 
-// sums += fragment f of x times the tile's rows from row0 on.  bf16 takes what rounding x to
-// bf16 loses through a second product with the same operand out of LDS (2^-16 of x is left
-// out): without it dq, dk and dv were 1.41 to 1.45 times as far off as one rounding of them.
-// 2 x (1,000 x 8,000 tokens), 16/4 heads of 128, 92% kept: dk and dv 494 us with it and 406
-// without, dq 314 and 257; 400 x (65 x 65), 2 heads of 100: 72 and 64, 28 and 27.
-template <typename T, int DP, typename TILE>
+// sums += fragment f of x times the tile's rows from row0 on.  bf16 takes what cutting x to
+// bf16 leaves through a second product with the same operand out of LDS: without it dq, dk and dv were 1.41 to 1.45 times as far off as one rounding of them.
+// 2 x (1,000 x 8,000 tokens), 16/4 heads of 128, 92% kept: dk and dv 488 us with it and 402
+// without, dq 308 and 252; 400 x (65 x 65), 2 heads of 100: 72 and 64, 28 and 27.
+template <typename T, int DP, typename TILE, bool SIGNED>
 __device__ __forceinline__ void mma_fine(Acc<T> (&sums)[DP / kTile<T>], const T* tile, int row0, const Acc<T>& x, int f) {
   const u32x4 xf = to_frag<T>(x, f);
   u32x4 rest;
-  if constexpr (sizeof(T) == 2) rest = lost_frag<T>(x, f);
+  if constexpr (sizeof(T) == 2) rest = rest_frag<SIGNED>(x, f);
 #pragma unroll
   for (int t = 0; t < DP / kTile<T>; ++t) {
     const u32x4 y = TILE::transposed(tile, row0, f, t);
@@ -92,8 +91,8 @@ __device__ __forceinline__ void one_by_one() {
 // KEEP (f32): ds goes to `scores`, rows of scores_row() keys, for att_scores_q.
 //
 // Bounded by the matrix units and the LDS reads that feed them, behind the steps that registers
-// keep apart, for bf16: 2 x (1,000 x 8,000 tokens), 16/4 heads of 128, 92% kept, 494 us, 488
-// TFLOP/s of four products and 732 of the six;
+// keep apart, for bf16: 2 x (1,000 x 8,000 tokens), 16/4 heads of 128, 92% kept, 488 us, 493
+// TFLOP/s of four products and 740 of the six;
 // by the matrix units for f32: 400 x (65 x 65), 2 heads of 100, 95 us, 48 TFLOP/s with the
 // padding to 80 x 80 x 112 and 29 without.
 //
@@ -226,7 +225,7 @@ void att_mma_kv(const AttArgs a, int ktiles, int splits, int64_t span, const flo
         one_by_one<T>();
 #pragma unroll
         for (int f = 0; f < kFrags<T>; ++f) {
-          mma_fine<T, DP, Tile>(dv, sg[cur], 0, s, f);
+          mma_fine<T, DP, Tile, false>(dv, sg[cur], 0, s, f);
           one_by_one<T>();
         }
 #pragma unroll
@@ -248,7 +247,7 @@ void att_mma_kv(const AttArgs a, int ktiles, int splits, int64_t span, const flo
         one_by_one<T>();
 #pragma unroll
         for (int f = 0; f < kFrags<T>; ++f) {
-          mma_fine<T, DP, Tile>(dk, sq[cur], 0, dp, f);
+          mma_fine<T, DP, Tile, true>(dk, sq[cur], 0, dp, f);
           one_by_one<T>();
         }
       }
@@ -343,8 +342,8 @@ __global__ __launch_bounds__(512, 2) void att_scores_q(const AttArgs a, int mtil
 // dq, kTile rows a wave.  S^T = K Q^T and dP^T = V dO^T have the keys down a lane's registers
 // and one row a lane; dQ^T += K^T dS^T follows.  With splits > 1 each range of `span` keys
 // leaves its sum in `part`.  W waves, or 4 to 8 for W = 0.  Bounded as att_mma_kv is: 2 x
-// (1,000 x 8,000 tokens), 16/4 heads of 128, bf16, 92% kept, 314 us, 576 TFLOP/s of three
-// products and 768 of the four.
+// (1,000 x 8,000 tokens), 16/4 heads of 128, bf16, 92% kept, 308 us, 585 TFLOP/s of three
+// products and 780 of the four.
 template <typename T, bool TINY, int DP, int W>
 __global__ __launch_bounds__(W == 0 ? 512 : 64 * W, DP > 128 ? 1 : 2) void att_mma_q(const AttArgs a, int mtiles, int splits,
                                                                      int64_t span, const float2* __restrict__ stats,
@@ -415,7 +414,7 @@ __global__ __launch_bounds__(W == 0 ? 512 : 64 * W, DP > 128 ? 1 : 2) void att_m
         if (here != ALL) dp[i] = here >> (4 * group) >> mma_row<T>(i, 0) & 1 ? dp[i] : 0.f;
       }
 #pragma unroll
-      for (int f = 0; f < kFrags<T>; ++f) mma_fine<T, DP, KTile>(dq, sk, u * TS, dp, f);
+      for (int f = 0; f < kFrags<T>; ++f) mma_fine<T, DP, KTile, true>(dq, sk, u * TS, dp, f);
     }
   }
   if (r >= rows) return;

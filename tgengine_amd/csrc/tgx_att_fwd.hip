@@ -5,16 +5,15 @@
 // running maximum and sum of the softmax are a lane's own but for an exchange between
 // the lanes of a row now and then, and P^T, still in the same registers, is the second operand of
 // O^T += V^T P^T.  Scores are in units of log 2.  bf16's matrix units take probabilities of
-// bf16: a second product adds what rounding them took (itself rounded to bf16, 2^-16 of a
-// probability), so that an output is off by its own rounding only.  Without it the two
+// bf16: a second product adds what cutting them to that left (to_frag), so that an output is off by its own rounding only.  Without it the two
 // roundings' errors together were 1.41 times the output's own, however many keys there were.
-// It uses the same reads of V: 2 x (1,000 x 8,000 tokens), 16/4 heads of 128, take 237 us
-// with it and 185 without, 200 x (200 x 200), 4 heads of 64, 61 and 55, single tokens to
+// It uses the same reads of V: 2 x (1,000 x 8,000 tokens), 16/4 heads of 128, take 224 us
+// with it and 180 without, 200 x (200 x 200), 4 heads of 64, 61 and 55, single tokens to
 // 30,001 keys 96 either way.
 //
 // What bounds it: for bf16 the softmax between the products and the LDS reads that feed
-// them (that first call, 92% kept: 510 TFLOP/s of the 1,225 that a matrix product of 8,192
-// reaches, 760 with the second product counted); for f32 the matrix units, eight times slower
+// them (that first call, 92% kept: 538 TFLOP/s of the 1,225 that a matrix product of 8,192
+// reaches, 807 with the second product counted); for f32 the matrix units, eight times slower
 // (400 x (65 x 65), 2 heads of 100: 51 us for 75 MB and 1.4 GFLOP, whose 16-row tiles pad
 // 65 to 80 and 100 to 112); for single tokens the reads of keys and values (5 x 30,001 keys
 // of 8 heads of 128, bf16, 73% kept: 97 us for 447 MB, 4.6 TB/s).
@@ -33,7 +32,6 @@ __global__ __launch_bounds__(WQ == 0 ? 512 : 64 * WQ * WK, DP > 128 ? 1 : WQ == 
                                                                              int64_t span, const AttParts part) {
   using KTile = LdsTile<T, DP, Reads::kRows>;
   using VTile = LdsTile<T, DP, Reads::kColumns>;
-  constexpr bool FINE = sizeof(T) == 2;  // the second product
   constexpr int TS = kTile<T>, KT = sizeof(T) == 2 || WK > 1 ? 64 : 32, SUB = KT / TS / WK,
                 OT = DP / TS, ST = DP / kStep;
   static_assert(WK == 1 || SUB == 1, "one tile of keys a wave");
@@ -85,7 +83,7 @@ __global__ __launch_bounds__(WQ == 0 ? 512 : 64 * WQ * WK, DP > 128 ? 1 : WQ == 
   __syncthreads();
   while (more) {  // workgroup-uniform
     st.load(vp + key * a.vs[1], a.vs[1], bits, a.dim);
-    u32x4 pf[SUB][kFrags<T>], rest[FINE ? SUB : 1][kFrags<T>];
+    u32x4 pf[SUB][kFrags<T>], rest[SUB][kFrags<T>];
     const uint64_t now = bits;
     constexpr uint32_t ALL = TS == 32 ? ~0u : 0xffffu;
     if (busy) {
@@ -129,10 +127,9 @@ __global__ __launch_bounds__(WQ == 0 ? 512 : 64 * WQ * WK, DP > 128 ? 1 : WQ == 
         }
 #pragma unroll
         for (int f = 0; f < kFrags<T>; ++f) pf[u][f] = to_frag<T>(s[u], f);
-        if constexpr (FINE) {
+        if constexpr (sizeof(T) == 2)
 #pragma unroll
-          for (int f = 0; f < kFrags<T>; ++f) rest[u][f] = lost_frag<T>(s[u], f);
-        }
+          for (int f = 0; f < kFrags<T>; ++f) rest[u][f] = rest_frag<false>(s[u], f);
       }
     }
     st.template store<VTile::ROW>(sv, a.dim);
@@ -150,7 +147,7 @@ __global__ __launch_bounds__(WQ == 0 ? 512 : 64 * WQ * WK, DP > 128 ? 1 : WQ == 
           for (int f = 0; f < kFrags<T>; ++f) {
             const u32x4 vf = VTile::transposed(sv, row0, f, t);
             o[t] = mma<T>(o[t], vf, pf[u][f]);
-            if constexpr (FINE) o[t] = mma<T>(o[t], vf, rest[u][f]);
+            if constexpr (sizeof(T) == 2) o[t] = mma<T>(o[t], vf, rest[u][f]);
           }
       }
     }

@@ -107,33 +107,45 @@ __device__ __forceinline__ constexpr int mma_row(int i, int group) {
   return sizeof(T) == 2 ? 8 * (i / 4) + 4 * group + i % 4 : 4 * group + i;
 }
 
+// What rounding to T takes from x; nothing from an infinity, nor from a value that becomes one
+template <typename T>
+__device__ __forceinline__ float lost(float x) {
+  const float y = to_f(from_f<T>(x));
+  return fabsf(y) == INFINITY ? 0.f : x - y;
+}
+
+// What cutting x to bf16 leaves, with x's sign and never 0, nor NaN for an infinity: an
+// infinite factor, or an infinite x, then gives the same infinity with both parts
+template <bool SIGNED>
+__device__ __forceinline__ float left(float x) {
+  const float cut = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+  if constexpr (!SIGNED) return fmaxf(x - cut, 0x1p-126f);  // fmaxf takes the other of NaN
+  return copysignf(fmaxf(fabsf(x) - fabsf(cut), 0x1p-126f), x);
+}
+
 // Fragment f (of kFrags) of such values as the second operand of a product that sums
-// over their rows: no lane gives a value to another.
+// over their rows: no lane gives a value to another.  bf16 comes in two parts, for a product
+// each: the values cut to bf16, and what that left (rest_frag), which is below 2^-7 of a value,
+// so that its own rounding takes at most 2^-16 of it.
 template <typename T>
 __device__ __forceinline__ u32x4 to_frag(const Acc<T>& x, int f) {
   u32x4 y;
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
-    if constexpr (sizeof(T) == 2)  // two values at a time: one conversion
-      y[u] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x[f * 8 + 2 * u], x[f * 8 + 2 * u + 1]}), bf16x2));
+    if constexpr (sizeof(T) == 2)  // the upper halves of two values
+      y[u] = __builtin_amdgcn_perm(__float_as_uint(x[f * 8 + 2 * u + 1]), __float_as_uint(x[f * 8 + 2 * u]), 0x07060302);
     else
       y[u] = __float_as_uint(x[u]);
   }
   return y;
 }
-
-// what rounding to T takes from x
-template <typename T>
-__device__ __forceinline__ float lost(float x) { return x - to_f(from_f<T>(x)); }
-
-// to_frag of what rounding to bf16 takes from the values
-template <typename T>
-__device__ __forceinline__ u32x4 lost_frag(const Acc<T>& x, int f) {
+template <bool SIGNED>  // whether values below 0 are among them
+__device__ __forceinline__ u32x4 rest_frag(const f32x16& x, int f) {
   u32x4 y;
 #pragma unroll
   for (int u = 0; u < 4; ++u)
-    y[u] = __builtin_bit_cast(uint32_t, __builtin_convertvector(
-                                            (f32x2{lost<T>(x[f * 8 + 2 * u]), lost<T>(x[f * 8 + 2 * u + 1])}), bf16x2));
+    y[u] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{left<SIGNED>(x[f * 8 + 2 * u]),
+                                                                       left<SIGNED>(x[f * 8 + 2 * u + 1])}), bf16x2));
   return y;
 }
 
