@@ -522,7 +522,8 @@ int tgx_attention_grad(const tgx_attention_args* args, void* stream);
 /* Clipping by the global norm: norm[0] = sqrt(sum of squares over all `count` tensors),
  * outs[t] = grads[t] * min(1, max_norm / (norm + 1e-6)).  The arrays are host arrays,
  * read during the call; tensor t is sizes[t] contiguous values of dtypes[t], its output
- * of out_dtypes[t] may be the tensor itself (same dtype) and must not overlap another.
+ * of out_dtypes[t] may be the tensor itself (same dtype); outputs that overlap otherwise,
+ * each other or a tensor, are refused (TGX_ERR_ARG).
  * A NaN or infinite norm scales as the formula says.  workspace:
  * tgx_clip_grad_norm_workspace_size(sizes, count) bytes. */
 size_t tgx_clip_grad_norm_workspace_size(const int64_t* sizes, int64_t count);

@@ -128,3 +128,18 @@ def test_refusals():
             C(*args, 1.0, **kw)
     with pytest.raises(RuntimeError, match="on the GPU"):
         C([g.cpu()], 1.0)
+
+
+def test_overlaps():
+    """What would be written in no order is refused; gradients that are only read may be shared."""
+    a, b = torch.randn(300, device="cuda"), torch.randn(300, device="cuda")
+    keep = [a.clone(), b.clone()]
+    tied = torch.nn.Parameter(torch.randn(40, device="cuda"))
+    tied.grad = torch.randn(40, device="cuda")
+    for grads, kw in (([a, b, a], {}), ([tied, torch.nn.Parameter(b), tied], {}), ([a, b], {"out": [b, a]}),
+                      ([a, b], {"out": [keep[0], keep[0]]}), ([a[:200], a[199:]], {}), ([a[:200]], {"out": [a[50:250]]})):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.clip_grad_norm_(grads, 1.0, **kw)
+    assert torch.equal(a, keep[0]) and torch.equal(b, keep[1])
+    _check([a, a], 1.0, out=[torch.empty_like(a), torch.empty_like(a)])
+    _check([a[:200], a[200:], b], 1.0)

@@ -110,3 +110,30 @@ def test_grids_that_one_launch_does_not_take():
         a = _att(batch=1 << 28, lq=lq, heads=2, kv_heads=2)
         assert L.tgx_attention(a, None) == 3 and "one launch" in _err()
     assert L.tgx_embed_grad(8, 8, 1, 1 << 29, 5, 4, 0, 1.0, 8, 8, 1 << 50, None) == 3 and "2^29" in _err()
+
+
+def test_clip_refuses_overlaps():
+    """Outputs that are written twice, or read for another tensor: refused before any launch."""
+    L = _lib.lib()
+
+    def call(grads, outs, sizes, types=None, out_types=None):
+        n = len(sizes)
+        P, I, S = ctypes.c_void_p * n, ctypes.c_int32 * n, ctypes.c_int64 * n
+        types = types or [0] * n
+        return L.tgx_clip_grad_norm(P(*grads), I(*types), P(*outs), I(*(out_types or types)), S(*sizes), n, 1.0, 8, None,
+                                    0, None)
+
+    a, b, c = 0x10000, 0x20000, 0x30000
+    for args in (([a, b, a], [a, b, a], [5, 7, 5]),               # a tied gradient, in place
+                 ([a, b], [c, c], [5, 7]),                        # two gradients to one output
+                 ([a, b], [b, a], [5, 5]),                        # outputs that trade places
+                 ([a, b], [c, a + 16], [5, 3]),                   # an output inside another gradient
+                 ([a], [a + 4], [5]),                             # one that is shifted against its own
+                 ([a, b, c], [a, b, c + 8], [8192, 8192, 3]),     # ... and in a list
+                 ([a, a + 8], [a, a + 8], [3, 3]),                # gradients that share a value
+                 ([a, b], [a, a + 9], [5, 2], [1, 1]),            # the last byte of bf16
+                 ([a, b], [c, c + 18], [5, 2], [0, 0], [0, 1])):
+        assert call(*args) == 1 and "overlap" in _err(), args
+    for args in (([a, b], [a, b], [5, 7]), ([a, a + 20], [a, a + 20], [5, 5]), ([a, a], [b, c], [5, 5]),
+                 ([a, a + 4], [b, c], [5, 5]), ([a, a], [a, b], [0, 5]), ([a, b], [a, a + 10], [5, 2], [1, 1])):
+        assert call(*args) == 1 and "workspace" in _err(), args  # apart: the next check speaks

@@ -12,6 +12,9 @@
 // compute units with eight workgroups each, and a part is long enough to hide its sum.
 #include "tgx_ops.h"
 
+#include <memory>
+#include <new>
+
 namespace tgx {
 namespace {
 
@@ -138,6 +141,38 @@ int64_t part_count(const int64_t* sizes, int64_t count, int64_t per) {
   return parts;
 }
 
+// Workgroups write all outputs at once, in no order: bytes that are written may not be
+// written or read for another tensor.  A tensor that is its own output counts as one.
+int check_apart(const void* const* grads, const int32_t* dtypes, void* const* outs, const int32_t* out_dtypes,
+                const int64_t* sizes, int64_t count) {
+  struct Range {
+    uint64_t lo, hi;
+    int64_t tensor;
+    bool out;
+  };
+  const std::unique_ptr<Range[]> r(new (std::nothrow) Range[static_cast<size_t>(count) * 2]);
+  if (r == nullptr) return fail(TGX_ERR_LIMIT, "tgx_clip_grad_norm: no memory to check %lld tensors", static_cast<long long>(count));
+  int64_t n = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (sizes[i] == 0) continue;
+    r[n++] = {addr(outs[i]), addr(outs[i]) + static_cast<uint64_t>(sizes[i]) * elem_bytes(out_dtypes[i]), i, true};
+    if (grads[i] != outs[i])
+      r[n++] = {addr(grads[i]), addr(grads[i]) + static_cast<uint64_t>(sizes[i]) * elem_bytes(dtypes[i]), i, false};
+  }
+  std::sort(r.get(), r.get() + n, [](const Range& x, const Range& y) { return x.lo < y.lo; });
+  const Range *any = nullptr, *out = nullptr;  // of those before, the one that reaches farthest
+  for (int64_t i = 0; i < n; ++i) {
+    const Range* before = r[i].out ? any : out;
+    if (before != nullptr && before->hi > r[i].lo)
+      return fail(TGX_ERR_ARG, "tgx_clip_grad_norm: tensors %lld and %lld overlap (an output may be its own gradient only)",
+                  static_cast<long long>(std::min(before->tensor, r[i].tensor)),
+                  static_cast<long long>(std::max(before->tensor, r[i].tensor)));
+    if (any == nullptr || r[i].hi > any->hi) any = &r[i];
+    if (r[i].out && (out == nullptr || r[i].hi > out->hi)) out = &r[i];
+  }
+  return TGX_OK;
+}
+
 }  // namespace
 }  // namespace tgx
 
@@ -168,6 +203,7 @@ extern "C" int tgx_clip_grad_norm(const void* const* grads, const int32_t* dtype
       return fail(TGX_ERR_ARG, "tgx_clip_grad_norm: tensor %lld is its own output in another dtype",
                   static_cast<long long>(i));
   }
+  if (const int rc = check_apart(grads, dtypes, outs, out_dtypes, sizes, count)) return rc;
   const int64_t per = part_values(sizes, count);
   const int64_t parts = part_count(sizes, count, per);
   if (parts >= (int64_t(1) << 24)) return fail(TGX_ERR_LIMIT, "tgx_clip_grad_norm: %lld parts", static_cast<long long>(parts));

@@ -368,10 +368,11 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm, const s
   const c10::OptionalDeviceGuard guard(grads[0].device());
   Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
   const Tensor ws = workspace(tgx_clip_grad_norm_workspace_size(size.data(), static_cast<int64_t>(n)), grads[0]);
-  check(tgx_clip_grad_norm(in.data(), dt.data(), out.data(), odt.data(), size.data(), static_cast<int64_t>(n),
-                           static_cast<float>(max_norm), norm.data_ptr<float>(), ptr(ws),
-                           ws.defined() ? ws.numel() : 0, stream_of(grads[0])),
-        "tgx_clip_grad_norm");
+  const int rc = tgx_clip_grad_norm(in.data(), dt.data(), out.data(), odt.data(), size.data(), static_cast<int64_t>(n),
+                                    static_cast<float>(max_norm), norm.data_ptr<float>(), ptr(ws),
+                                    ws.defined() ? ws.numel() : 0, stream_of(grads[0]));
+  if (rc == TGX_ERR_ARG) bad(tgx_last_error());  // tensors that overlap
+  check(rc, "tgx_clip_grad_norm");
   // written behind torch's back: what autograd saved of them is stale
   for (const Tensor& t : outs.empty() ? grads : outs)
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();

@@ -66,7 +66,9 @@ def clip_grad_norm_(grads: Union[Tensor, Iterable[Tensor]], max_norm: float,
 
     grads are contiguous tensors, or parameters whose ``.grad`` is taken (those
     without one are left out).  With ``out``, one tensor per gradient in either dtype,
-    the clipped gradients are written there and the gradients stay as they are.
+    the clipped gradients are written there and the gradients stay as they are.  What is
+    written may share no memory with another gradient or output, so that a parameter
+    that two modules share is given once.
     """
     if isinstance(grads, Tensor):
         grads = [grads]
