@@ -143,3 +143,24 @@ def test_overlaps():
     assert torch.equal(a, keep[0]) and torch.equal(b, keep[1])
     _check([a, a], 1.0, out=[torch.empty_like(a), torch.empty_like(a)])
     _check([a[:200], a[200:], b], 1.0)
+
+
+def test_leaves_are_parameters():
+    """A plain leaf that requires a gradient is clipped by its gradient, as a Parameter is; no weight is scaled."""
+    w, b, rest = (torch.randn(n, device="cuda", requires_grad=True) for n in (50, 7, 3))
+    before = [x.detach().clone() for x in (w, b, rest)]
+    ((w * 3).sum() + b.square().sum()).backward()
+    want = torch.cat([w.grad, b.grad]).double().norm()
+    norm = ops.clip_grad_norm_([w, b, rest], 1.0)
+    assert abs(float(norm) - float(want)) <= 2 ** 10 * U * float(want) and rest.grad is None
+    assert abs(float(torch.cat([w.grad, b.grad]).double().norm()) - 1.0) < 1e-5
+    assert all(torch.equal(x, y) for x, y in zip((w, b, rest), before))
+    with pytest.raises(ValueError, match="no gradients"):
+        ops.clip_grad_norm_(rest, 1.0)
+    g = torch.randn(7, device="cuda")
+    with pytest.raises(ValueError, match="must not require a gradient"):
+        ops.clip_grad_norm_([g], 1.0, out=[b])
+    assert torch.equal(b, before[1])
+    with torch.no_grad():  # as torch's own writes to a leaf
+        ops.clip_grad_norm_([g], 1e6, out=[b])
+    assert torch.equal(b, g)

@@ -359,6 +359,8 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm, const s
       if (!t->is_contiguous()) bad("clip_grad_norm_: gradients and out must be contiguous");
     }
     if (o.sizes() != g.sizes()) bad("clip_grad_norm_: out must have the gradients' shapes");
+    if (!outs.empty() && o.requires_grad() && at::GradMode::is_enabled())
+      bad("clip_grad_norm_: out must not require a gradient");
     dt[i] = dtype_of(g, "clip_grad_norm_: gradients");
     odt[i] = dtype_of(o, "clip_grad_norm_: out");
     in[i] = g.data_ptr();

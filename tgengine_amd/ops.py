@@ -64,8 +64,8 @@ def clip_grad_norm_(grads: Union[Tensor, Iterable[Tensor]], max_norm: float,
     """Scales gradients by min(1, max_norm / (norm + 1e-6)) and returns ``norm``, the
     2-norm over all of them together, as a float32 scalar on the device.
 
-    grads are contiguous tensors, or parameters whose ``.grad`` is taken (those
-    without one are left out).  With ``out``, one tensor per gradient in either dtype,
+    grads are contiguous tensors, or parameters and other leaves that require a
+    gradient, whose ``.grad`` is taken (those without one are left out).  With ``out``, one tensor per gradient in either dtype,
     the clipped gradients are written there and the gradients stay as they are.  What is
     written may share no memory with another gradient or output, so that a parameter
     that two modules share is given once.
@@ -73,7 +73,8 @@ def clip_grad_norm_(grads: Union[Tensor, Iterable[Tensor]], max_norm: float,
     if isinstance(grads, Tensor):
         grads = [grads]
     # a Parameter's isinstance check runs Python code: plain tensors skip it
-    grads = [g if type(g) is Tensor or not isinstance(g, torch.nn.Parameter) else g.grad for g in grads]
+    grads = [g.grad if g.requires_grad and g.is_leaf or type(g) is not Tensor and isinstance(g, torch.nn.Parameter) else g
+             for g in grads]
     if out is None:
         grads = [g for g in grads if g is not None]
         if not grads:
