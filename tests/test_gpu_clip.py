@@ -164,3 +164,10 @@ def test_leaves_are_parameters():
     with torch.no_grad():  # as torch's own writes to a leaf
         ops.clip_grad_norm_([g], 1e6, out=[b])
     assert torch.equal(b, g)
+
+
+@pytest.mark.parametrize("scale", [1e30, 1e19, 1e-30])
+def test_squares_beyond_32_bits(scale):
+    """Gradients whose squares pass what 32 bits hold, and whose norm does not."""
+    _check(_grads((5_000, 3, 40_001), (F, B, F), 7, scale), 1.0)
+    _check(_grads((200_003, 9), (B, F), 8, scale), scale * 10)

@@ -2,10 +2,11 @@
 //
 //   norm = sqrt(sum over all tensors of g^2),  c = min(1, max_norm / (norm + 1e-6)),  out = c g
 //
-// Two launches over all tensors together: each workgroup leaves the sum of squares of
-// its part in part[block] (32 bits a thread, a few thousand values at most), and in the
-// second launch every workgroup adds those up in the same order, in 64 bits, and scales
-// its part.  The tensors' addresses travel in the kernels' arguments, kList tensors a
+// Two launches over all tensors together: each workgroup leaves the norm of its part in
+// part[block], and in the second launch every workgroup adds up their squares in the same
+// order and scales its part.  Squares and sums are of 64 bits: in 32 those of values above
+// 2^64, as a run that diverges has them, are infinite, and clipping would make zeros of the
+// gradients.  The tensors' addresses travel in the kernels' arguments, kList tensors a
 // launch.  HBM bounds large lists: 100,000,000 bf16 values (200 MB) and 25 small tensors
 // take the squares 38 us, 5.4 TB/s, and the scaling 73 us, 5.6 TB/s; 48 layers of up to
 // 20,000 f32 values take 4.4 and 6.2 us, mostly the launches.  2,048 parts fill the 256
@@ -46,21 +47,24 @@ __device__ __forceinline__ int tensor_of(const ClipList& l, uint32_t block) {
 }
 
 template <typename T>
-__device__ __forceinline__ float squares(const T* __restrict__ p, int64_t lo, int64_t hi) {
+__device__ __forceinline__ double squares(const T* __restrict__ p, int64_t lo, int64_t hi) {
   constexpr int V = kWide<T>;
-  float s[V];
+  double s[V];
 #pragma unroll
-  for (int u = 0; u < V; ++u) s[u] = 0.f;
+  for (int u = 0; u < V; ++u) s[u] = 0.0;
   const int64_t full = lo + (hi - lo) / V * V;
 #pragma unroll 4
   for (int64_t i = lo + static_cast<int64_t>(threadIdx.x) * V; i < full; i += kClipThreads * V) {
     const Pack<T, V> x = load_pack<T, V>(p + i);
 #pragma unroll
-    for (int u = 0; u < V; ++u) s[u] += to_f(x.v[u]) * to_f(x.v[u]);
+    for (int u = 0; u < V; ++u) {
+      const double f = to_f(x.v[u]);
+      s[u] = fma(f, f, s[u]);
+    }
   }
   if (full + threadIdx.x < hi) {
-    const float x = to_f(p[full + threadIdx.x]);
-    s[0] += x * x;
+    const double x = to_f(p[full + threadIdx.x]);
+    s[0] = fma(x, x, s[0]);
   }
 #pragma unroll
   for (int w = V / 2; w > 0; w /= 2)
@@ -70,16 +74,17 @@ __device__ __forceinline__ float squares(const T* __restrict__ p, int64_t lo, in
 }
 
 __global__ __launch_bounds__(kClipThreads) void clip_squares(const ClipList l, int64_t per, float* __restrict__ part) {
-  __shared__ float lds[kClipWaves];
+  __shared__ double lds[kClipWaves];
   const int t = tensor_of(l, blockIdx.x);
   const int64_t lo = (blockIdx.x - l.first[t]) * per;
   const int64_t hi = lo + per < l.size[t] ? lo + per : l.size[t];
-  float s = l.in_bf16[t] ? squares(static_cast<const bf16*>(l.in[t]), lo, hi)
-                         : squares(static_cast<const float*>(l.in[t]), lo, hi);
-  s = group_sum<kWave>(s);
+  double s = l.in_bf16[t] ? squares(static_cast<const bf16*>(l.in[t]), lo, hi)
+                          : squares(static_cast<const float*>(l.in[t]), lo, hi);
+#pragma unroll
+  for (int off = kWave / 2; off > 0; off >>= 1) s += __shfl_xor(s, off, kWave);
   if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = s;
   __syncthreads();
-  if (threadIdx.x == 0) part[blockIdx.x] = (lds[0] + lds[1]) + (lds[2] + lds[3]);
+  if (threadIdx.x == 0) part[blockIdx.x] = static_cast<float>(sqrt((lds[0] + lds[1]) + (lds[2] + lds[3])));
 }
 
 template <typename T, typename U>
@@ -102,7 +107,7 @@ __global__ __launch_bounds__(kClipThreads) void clip_scale(const ClipList l, int
                                                            bool first) {
   __shared__ double lds[kClipWaves];
   double s = 0.0;
-  for (int i = threadIdx.x; i < parts; i += kClipThreads) s += part[i];
+  for (int i = threadIdx.x; i < parts; i += kClipThreads) s = fma(static_cast<double>(part[i]), static_cast<double>(part[i]), s);
 #pragma unroll
   for (int off = kWave / 2; off > 0; off >>= 1) s += __shfl_xor(s, off, kWave);
   if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = s;
