@@ -5,8 +5,10 @@
 //
 // Without a gradient to keep (no input asks for one, or grad mode is off) a call
 // goes straight to the launch.  The backward passes are kernels themselves and
-// leave no graph: asking for one (create_graph) raises.
+// leave no graph: asking for one (create_graph) raises.  So do the ways to follow a call
+// that see none of its launches, forward-mode derivatives and tracing.
 #include <torch/extension.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -55,6 +57,15 @@ bool keeps_grad(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
   return false;
+}
+
+// forward-mode derivatives would be taken for zeros, and a trace would record the outputs' bare
+// memory
+void reverse_mode_only(const char* what, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(0).defined())
+      throw std::runtime_error(std::string(what) + " has no forward-mode derivative");
+  if (torch::jit::tracer::isTracing()) throw std::runtime_error(std::string(what) + " cannot be traced");
 }
 
 // a backward pass that is asked for a graph of its own
@@ -132,6 +143,7 @@ class Embed : public torch::autograd::Function<Embed> {
 
 Tensor embed(const Tensor& table, const Tensor& ids, double scale) {
   check_embed(table, ids);
+  reverse_mode_only("embed", {&table});
   const Tensor flat = ids.contiguous();
   return keeps_grad({&table}) ? Embed::apply(table, flat, scale) : embed_out(table, flat, scale);
 }
@@ -218,6 +230,7 @@ class LayerNorm : public torch::autograd::Function<LayerNorm> {
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
   const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
   check_norm(x, w, b);
+  reverse_mode_only("layer_norm", {&x, &w, &b});
   if (keeps_grad({&x, &w, &b})) return LayerNorm::apply(x, weight, bias, eps);
   const c10::OptionalDeviceGuard guard(x.device());
   return norm_out(NormIn(x, w, b), x.sizes(), eps, nullptr);
@@ -333,6 +346,7 @@ Tensor cross_attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_i
                        const c10::optional<double>& scale_in) {
   Tensor mask = mask_in.value_or(Tensor());
   check_attention(q_in, k_in, v_in, mask);
+  reverse_mode_only("cross_attention", {&q_in, &k_in, &v_in});
   const Tensor q = dense_last(q_in), k = dense_last(k_in), v = dense_last(v_in);
   if (mask.defined() && mask.size(1) > 1 && mask.stride(1) != 1) mask = mask.contiguous();
   const double scale = scale_in.has_value() ? *scale_in : 1.0 / std::sqrt(static_cast<double>(q.size(3)));
@@ -353,6 +367,7 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm, const s
   for (size_t i = 0; i < n; ++i) {
     const Tensor& g = grads[i];
     const Tensor& o = outs.empty() ? g : outs[i];
+    reverse_mode_only("clip_grad_norm_", {&g, &o});
     on_gpu(g, "clip_grad_norm_: gradients");
     for (const Tensor* t : {&g, &o}) {
       same_device(*t, grads[0], "clip_grad_norm_: every tensor");

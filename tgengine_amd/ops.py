@@ -13,7 +13,8 @@ What a model does with the neighbours that ``DataPipeline.prepare`` gathers:
 Tensors are float32 or bfloat16 on the GPU; sums and statistics are held in 32
 bits.  Every call launches on the caller's current stream and does not wait for
 the device; the same inputs give the same bits.  The first three take part in
-autograd (once: their backward passes leave no graph).  There is no CPU path.
+autograd (once: their backward passes leave no graph; forward-mode derivatives and
+tracing are refused).  There is no CPU path.
 """
 from __future__ import annotations
 
