@@ -444,7 +444,7 @@ int tgx_co_occurrence(const int32_t* a_ids, const int32_t* c_ids, const uint8_t*
 
 /* out[i] = scale * table[ids[i]] for i < n, rows of dim values; an id outside
  * [0, rows) (the -1 of a padded neighbour) gives a row of zeros.  table: rows
- * `stride` values apart; ids int32 (ids_i32 != 0) or int64; out [n, dim]. */
+ * `stride` values apart (at least dim, or 0: one row for all); ids int32 (ids_i32 != 0) or int64; out [n, dim]. */
 int tgx_embed(const void* table, int64_t rows, int64_t dim, int64_t stride, int32_t dtype,
               const void* ids, int32_t ids_i32, int64_t n, float scale, void* out, void* stream);
 /* Its gradient (n < 2^29): grad [rows, dim], every row written: scale * the sum of dout[i] over

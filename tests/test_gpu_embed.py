@@ -159,3 +159,22 @@ def test_refusals():
     leaf = t.detach().requires_grad_()
     with pytest.raises(RuntimeError, match="once only"):
         torch.autograd.grad(ops.embed(leaf, i).sum(), leaf, create_graph=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [1, 7, 50])
+def test_broadcast_and_overlapping_tables(dim, dtype):
+    """One row for all ids, whose gradient is the sum of theirs; rows that share values."""
+    _, ids, dout = _case(40, dim, (30, 8), dtype, 9)
+    row = torch.randn(1, dim, device="cuda").to(dtype).requires_grad_()
+    ok = (ids >= 0) & (ids < 40)
+    out = ops.embed(row.expand(40, dim), ids, scale=1.5)
+    assert torch.equal(out, torch.where(ok[..., None], (row.float() * 1.5).to(dtype), 0.0))
+    (g,) = torch.autograd.grad(out, row, dout)
+    (full,) = torch.autograd.grad(ops.embed(row.expand(40, dim).contiguous(), ids, scale=1.5), row, dout)
+    assert torch.equal(g, full)
+    flat = torch.randn(40 + dim, device="cuda").to(dtype)
+    windows = flat.unfold(0, dim, 1)[:40]
+    assert torch.equal(ops.embed(windows, ids), ops.embed(windows.contiguous(), ids))
+    both = flat[:1].expand(40, dim)  # one value for all
+    assert torch.equal(ops.embed(both, ids), ops.embed(both.contiguous(), ids))

@@ -473,7 +473,7 @@ extern "C" int tgx_embed(const void* table, int64_t rows, int64_t dim, int64_t s
                          int32_t ids_i32, int64_t n, float scale, void* out, void* stream) {
   int rc = check_embed("tgx_embed", table, out, rows, dim, dtype, ids, n);
   if (rc) return rc;
-  if (stride < dim && rows > 1) return fail(TGX_ERR_ARG, "tgx_embed: row stride %lld below dim %lld",
+  if (stride < dim && stride != 0 && rows > 1) return fail(TGX_ERR_ARG, "tgx_embed: row stride %lld below dim %lld",
                                             static_cast<long long>(stride), static_cast<long long>(dim));
   if (n == 0) return TGX_OK;
   return by_type(dtype, [&](auto t) {

@@ -105,13 +105,16 @@ void check_embed(const Tensor& table, const Tensor& ids) {
 
 Tensor embed_out(const Tensor& table_in, const Tensor& ids, double scale) {
   const c10::OptionalDeviceGuard guard(table_in.device());
-  const Tensor table = table_in.stride(1) == 1 || table_in.size(1) == 1 ? table_in : table_in.contiguous();
+  // rows in place where they are dense and apart, or one row for all
+  const int64_t dim = table_in.size(1), step = table_in.size(0) > 1 ? table_in.stride(0) : dim;
+  const bool in_place = (dim == 1 || table_in.stride(1) == 1) && (step >= dim || step == 0);
+  const Tensor table = in_place ? table_in : table_in.contiguous();
   std::vector<int64_t> shape = ids.sizes().vec();
-  shape.push_back(table.size(1));
+  shape.push_back(dim);
   Tensor out = at::empty(shape, table.options());
-  check(tgx_embed(table.data_ptr(), table.size(0), table.size(1), table.size(0) > 1 ? table.stride(0) : table.size(1),
-                  dtype_of(table, "embed: table"), ids.data_ptr(), ids.scalar_type() == at::kInt, ids.numel(),
-                  static_cast<float>(scale), out.data_ptr(), stream_of(table)),
+  check(tgx_embed(table.data_ptr(), table.size(0), dim, in_place ? step : dim, dtype_of(table, "embed: table"),
+                  ids.data_ptr(), ids.scalar_type() == at::kInt, ids.numel(), static_cast<float>(scale),
+                  out.data_ptr(), stream_of(table)),
         "tgx_embed");
   return out;
 }
