@@ -447,7 +447,7 @@ int tgx_co_occurrence(const int32_t* a_ids, const int32_t* c_ids, const uint8_t*
  * `stride` values apart (at least dim, or 0: one row for all); ids int32 (ids_i32 != 0) or int64; out [n, dim]. */
 int tgx_embed(const void* table, int64_t rows, int64_t dim, int64_t stride, int32_t dtype,
               const void* ids, int32_t ids_i32, int64_t n, float scale, void* out, void* stream);
-/* Its gradient (n < 2^29): grad [rows, dim], every row written: scale * the sum of dout[i] over
+/* Its gradient (n <= 2^29 - 64): grad [rows, dim], every row written: scale * the sum of dout[i] over
  * the i with that id, in an order that the ids alone decide.  workspace:
  * tgx_embed_grad_workspace_size(n, dim) bytes, 16-byte aligned, no initialisation. */
 size_t tgx_embed_grad_workspace_size(int64_t n, int64_t dim);

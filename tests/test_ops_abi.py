@@ -137,3 +137,17 @@ def test_clip_refuses_overlaps():
     for args in (([a, b], [a, b], [5, 7]), ([a, a + 20], [a, a + 20], [5, 5]), ([a, a], [b, c], [5, 5]),
                  ([a, a + 4], [b, c], [5, 5]), ([a, a], [a, b], [0, 5]), ([a, b], [a, a + 10], [5, 2], [1, 1])):
         assert call(*args) == 1 and "workspace" in _err(), args  # apart: the next check speaks
+
+
+def test_launches_of_2_32_threads_are_refused():
+    """Before any launch, at the first size that reaches them."""
+    L = _lib.lib()
+
+    def norm(rows, dim, dtype):
+        return L.tgx_layer_norm(8, rows, dim, 0, dtype, None, None, dtype, 1e-5, 8, None, None, None)
+
+    for rows, dim, dtype in ((1 << 28, 257, 1), (1 << 28, 129, 0), (1 << 24, 16384, 1), (1 << 24, 4096, 0),
+                             ((1 << 31) - 100, 3, 0)):
+        assert norm(rows, dim, dtype) == 3 and "one launch" in _err(), (rows, dim)
+    for n, rc in (((1 << 29) - 1, 3), ((1 << 29) - 63, 3), ((1 << 29) - 64, 1)):  # the last: no workspace
+        assert L.tgx_embed_grad(8, 8, 1, n, 5, 4, 0, 1.0, 16, None, 0, None) == rc, n

@@ -431,14 +431,6 @@ inline int waves_for(int64_t n, int least, int most) {
   return static_cast<int>(std::max<int64_t>(ops_cdiv(n, groups), least));
 }
 
-// a grid's threads are counted in 32 bits
-inline int check_grid(const char* what, int64_t blocks, int64_t threads) {
-  if (blocks > ((int64_t(1) << 32) - 1) / threads)
-    return fail(TGX_ERR_LIMIT, "%s: %lld workgroups of %lld threads: more than one launch takes", what,
-                static_cast<long long>(blocks), static_cast<long long>(threads));
-  return TGX_OK;
-}
-
 constexpr int kNoLoads = 0x0f70;  // s_waitcnt: no vector load outstanding
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }

@@ -358,6 +358,9 @@ __global__ __launch_bounds__(kJoinThreads) void embed_join(const uint32_t* __res
 // bf16 85, 83 and 84; 1,000,000 462, 339 and 274)
 int tile_of(int64_t n) { return n <= (1 << 15) ? 16 : n <= (1 << 17) ? 32 : kMostTile; }
 
+// embed_join takes kJoinThreads threads for every tile, and a grid fewer than 2^32
+constexpr int64_t kMostGradTokens = ((int64_t(1) << 32) / kJoinThreads - 1) * kMostTile;
+
 int check_embed(const char* what, const void* a, const void* b, int64_t rows, int64_t dim, int32_t dtype,
                 const void* ids, int64_t n) {
   if (rows < 0 || dim < 1 || n < 0) return fail(TGX_ERR_ARG, "%s: rows=%lld dim=%lld n=%lld", what,
@@ -503,8 +506,8 @@ extern "C" int tgx_embed_grad(const void* dout, const void* ids, int32_t ids_i32
                               void* stream) {
   int rc = check_embed("tgx_embed_grad", grad, dout, rows, dim, dtype, ids, n);
   if (rc) return rc;
-  if (n >= int64_t(1) << 29)  // embed_join takes 512 threads for every tile of 64
-    return fail(TGX_ERR_LIMIT, "tgx_embed_grad: n=%lld (below 2^29)", static_cast<long long>(n));
+  if (n > kMostGradTokens)
+    return fail(TGX_ERR_LIMIT, "tgx_embed_grad: n=%lld (at most 2^29 - 64)", static_cast<long long>(n));
   if (rows == 0) return TGX_OK;
   if (grad == nullptr) return fail(TGX_ERR_ARG, "tgx_embed_grad: grad must not be NULL");
   hipStream_t s = static_cast<hipStream_t>(stream);

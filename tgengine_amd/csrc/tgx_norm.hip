@@ -347,8 +347,9 @@ extern "C" int tgx_layer_norm(const void* x, int64_t rows, int64_t dim, int64_t 
       using W = decltype(wt);
       return by_shape<T, false>(dim, [&](auto v, auto l, auto c) {
         constexpr int V = decltype(v)::value, L = decltype(l)::value, C = decltype(c)::value;
-        const unsigned blocks = static_cast<unsigned>(ops_cdiv(rows, kNormThreads / L * fwd_rows(C)));
-        hipLaunchKernelGGL((norm_fwd<T, W, V, L, C>), dim3(blocks), dim3(kNormThreads), 0,
+        const int64_t blocks = ops_cdiv(rows, kNormThreads / L * fwd_rows(C));
+        if (const int e = check_grid("tgx_layer_norm", blocks, kNormThreads)) return e;
+        hipLaunchKernelGGL((norm_fwd<T, W, V, L, C>), dim3(static_cast<unsigned>(blocks)), dim3(kNormThreads), 0,
                            static_cast<hipStream_t>(stream), static_cast<const T*>(x), rows, static_cast<int>(dim),
                            stride, static_cast<const W*>(weight), static_cast<const W*>(bias), eps,
                            static_cast<T*>(out), mean, rstd);

@@ -90,6 +90,14 @@ inline int fill_zero(void* p, size_t bytes, hipStream_t s) {
   return check_launch("zero_kernel");
 }
 
+// a grid's threads are counted in 32 bits
+inline int check_grid(const char* what, int64_t blocks, int64_t threads) {
+  if (blocks > ((int64_t(1) << 32) - 1) / threads)
+    return fail(TGX_ERR_LIMIT, "%s: %lld workgroups of %lld threads: more than one launch takes", what,
+                static_cast<long long>(blocks), static_cast<long long>(threads));
+  return TGX_OK;
+}
+
 // calls f(T{}) for the dtype
 template <typename F>
 int by_type(int dtype, F&& f) {
