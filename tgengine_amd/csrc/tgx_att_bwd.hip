@@ -443,6 +443,16 @@ struct QShape {
   }
 };
 
+// att_scores_q's row tiles
+struct ScoresShape {
+  int w, mtiles;
+  explicit ScoresShape(const AttArgs& a) {
+    const int64_t tiles = ops_cdiv(a.lq * a.group, kTile<float>);
+    w = waves_for(tiles, 4, 8);
+    mtiles = static_cast<int>(ops_cdiv(tiles, w));
+  }
+};
+
 // dk's and dv's key tiles, and the ranges the rows are cut in where those alone leave half
 // of the compute units without work: at most 256 workgroups, since every range writes
 // its sums of all keys (1 x (2,000 x 2,000 tokens), 2/1 heads of 128, bf16: 91 us, 436 uncut;
@@ -501,10 +511,12 @@ int att_mma_backward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
   const bool keep = scores_bytes(a, dtype) > 0;  // the same workspace holds them in the parts' place
   const KvShape kv(a, dtype);
   const QShape q(a, dtype);
-  const int64_t problems = a.batch * a.kv_heads;
+  const ScoresShape sc(a);
+  const int64_t problems = a.batch * a.kv_heads, kv_blocks = problems * kv.ktiles * kv.splits;
+  const int64_t q_blocks = problems * (keep ? sc.mtiles : q.mtiles * q.splits);
   int fits = check_grid("tgx_attention_grad", ops_cdiv(rows, 256 / kDeltaLanes), 256);
-  if (!fits) fits = check_grid("tgx_attention_grad", problems * kv.ktiles * kv.splits, 512);
-  if (!fits) fits = check_grid("tgx_attention_grad", problems * q.mtiles * q.splits, 512);
+  if (!fits && (a.dk != nullptr || a.dv != nullptr)) fits = check_grid("tgx_attention_grad", kv_blocks, 64 * kv.w);
+  if (!fits && a.dq != nullptr) fits = check_grid("tgx_attention_grad", q_blocks, 64 * (keep ? sc.w : q.w));
   if (fits) return fits;
   return by_head(dtype, a.dim, [&](auto t, auto dp, auto tiny) {
     using T = decltype(t);
@@ -516,50 +528,45 @@ int att_mma_backward(const AttArgs& a, int dtype, void* ws, hipStream_t s) {
     int rc = check_launch("att_stats");
     if (rc) return rc;
     if (a.lk > 0 && (a.dk != nullptr || a.dv != nullptr)) {
-      const KvShape f(a, dtype);
       auto go = [&](auto least) {
         constexpr int LEAST = decltype(least)::value;
-        const dim3 grid(static_cast<unsigned>(a.batch * a.kv_heads * f.ktiles * f.splits));
+        const dim3 grid(static_cast<unsigned>(kv_blocks));
         if (sizeof(T) == 4 && keep)
-          hipLaunchKernelGGL((att_mma_kv<T, TINY, DP, LEAST, sizeof(T) == 4>), grid, dim3(64 * f.w), 0, s, a, f.ktiles,
-                             f.splits, f.span, stats, part, kv_part);
+          hipLaunchKernelGGL((att_mma_kv<T, TINY, DP, LEAST, sizeof(T) == 4>), grid, dim3(64 * kv.w), 0, s, a, kv.ktiles,
+                             kv.splits, kv.span, stats, part, kv_part);
         else
-          hipLaunchKernelGGL((att_mma_kv<T, TINY, DP, LEAST, false>), grid, dim3(64 * f.w), 0, s, a, f.ktiles, f.splits,
-                             f.span, stats, part, kv_part);
+          hipLaunchKernelGGL((att_mma_kv<T, TINY, DP, LEAST, false>), grid, dim3(64 * kv.w), 0, s, a, kv.ktiles, kv.splits,
+                             kv.span, stats, part, kv_part);
         return check_launch("att_mma_kv");
       };
       if constexpr (kTwoWays<T, DP>)
-        rc = f.least == 8 ? go(std::integral_constant<int, 8>{}) : go(std::integral_constant<int, 2>{});
+        rc = kv.least == 8 ? go(std::integral_constant<int, 8>{}) : go(std::integral_constant<int, 2>{});
       else
         rc = go(std::integral_constant<int, kKvLeast<T, DP>>{});
       const int64_t keys = a.batch * a.lk * a.kv_heads;
-      if (!rc && f.splits > 1 && a.dk != nullptr)
-        rc = att_join_sums(a.dk, keys, a.dim, dtype, a.scale, f.splits, kv_part, s);
-      if (!rc && f.splits > 1 && a.dv != nullptr)
-        rc = att_join_sums(a.dv, keys, a.dim, dtype, 1.f, f.splits, kv_part + f.sums, s);
+      if (!rc && kv.splits > 1 && a.dk != nullptr)
+        rc = att_join_sums(a.dk, keys, a.dim, dtype, a.scale, kv.splits, kv_part, s);
+      if (!rc && kv.splits > 1 && a.dv != nullptr)
+        rc = att_join_sums(a.dv, keys, a.dim, dtype, 1.f, kv.splits, kv_part + kv.sums, s);
       if (rc) return rc;
     }
     if (a.dq == nullptr) return TGX_OK;
     if constexpr (sizeof(T) == 4) {
       if (keep) {
-        const int w = waves_for(ops_cdiv(a.lq * a.group, TS), 4, 8);
-        const int mtiles = static_cast<int>(ops_cdiv(a.lq * a.group, TS * w));
-        hipLaunchKernelGGL((att_scores_q<TINY, DP>), dim3(static_cast<unsigned>(a.batch * a.kv_heads * mtiles)),
-                           dim3(64 * w), 0, s, a, mtiles, part);
+        hipLaunchKernelGGL((att_scores_q<TINY, DP>), dim3(static_cast<unsigned>(q_blocks)), dim3(64 * sc.w), 0, s, a,
+                           sc.mtiles, part);
         return check_launch("att_scores_q");
       }
     }
-    const QShape f(a, dtype);
     auto go = [&](auto w) {
-      hipLaunchKernelGGL((att_mma_q<T, TINY, DP, decltype(w)::value>),
-                         dim3(static_cast<unsigned>(a.batch * a.kv_heads * f.mtiles * f.splits)), dim3(64 * f.w), 0, s,
-                         a, f.mtiles, f.splits, f.span, stats, part);
+      hipLaunchKernelGGL((att_mma_q<T, TINY, DP, decltype(w)::value>), dim3(static_cast<unsigned>(q_blocks)),
+                         dim3(64 * q.w), 0, s, a, q.mtiles, q.splits, q.span, stats, part);
       return check_launch("att_mma_q");
     };
     if constexpr (DP > 128) rc = go(std::integral_constant<int, 4>{});
     else if constexpr (sizeof(T) == 4) rc = go(std::integral_constant<int, 0>{});
-    else rc = f.w == 2 ? go(std::integral_constant<int, 2>{}) : go(std::integral_constant<int, 4>{});
-    return rc || f.splits == 1 ? rc : att_join_sums(a.dq, rows, a.dim, dtype, a.scale, f.splits, part, s);
+    else rc = q.w == 2 ? go(std::integral_constant<int, 2>{}) : go(std::integral_constant<int, 4>{});
+    return rc || q.splits == 1 ? rc : att_join_sums(a.dq, rows, a.dim, dtype, a.scale, q.splits, part, s);
   });
 }
 
