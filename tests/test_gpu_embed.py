@@ -178,3 +178,29 @@ def test_broadcast_and_overlapping_tables(dim, dtype):
     assert torch.equal(ops.embed(windows, ids), ops.embed(windows.contiguous(), ids))
     both = flat[:1].expand(40, dim)  # one value for all
     assert torch.equal(ops.embed(both, ids), ops.embed(both.contiguous(), ids))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [400, 150_000, 3_000_000])  # keys of one, two and three digits
+@pytest.mark.parametrize("n,dim", [(8_193, 6), (65_536, 5), (65_537, 5), (131_073, 12), (300_001, 20),
+                                   (2 ** 21 + 1, 3), (2 ** 21 + 1, 8)])
+def test_many_tokens(n, dim, rows, dtype):
+    """Every way to sort: one workgroup's limit, few and many ranges, tiles of 16 to 64 tokens,
+    long parts, and a hub over many tiles.  The sums in 64 bits are taken on the host: a hub's
+    hundreds of thousands of additions to one place are slow on the device."""
+    table, ids, dout = _case(rows, dim, (n,), dtype, n + rows, 1.0)
+    ids[n // 3:n // 2] = rows - 2
+    leaf = table.requires_grad_()
+    (grad,) = torch.autograd.grad(ops.embed(leaf, ids, scale=0.75), leaf, dout)
+    (again,) = torch.autograd.grad(ops.embed(leaf, ids, scale=0.75), leaf, dout)
+    assert torch.equal(grad, again)
+    flat = ids.cpu().numpy().astype(np.int64)
+    ok = (flat >= 0) & (flat < rows)
+    flat, terms = flat[ok], dout.double().cpu().numpy()[ok]
+    count = np.bincount(flat, minlength=rows)
+    r = U if dtype == torch.float32 else 2.0 ** -8
+    for c in range(dim):
+        y = np.bincount(flat, weights=terms[:, c], minlength=rows) * 0.75
+        size = np.bincount(flat, weights=np.abs(terms[:, c]), minlength=rows) * 0.75
+        off = np.abs(grad[:, c].double().cpu().numpy() - y)
+        assert (off <= (count + 3) * U * size + np.abs(y) * r).all(), c
