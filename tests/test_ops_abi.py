@@ -2,6 +2,7 @@
 layout against the ctypes mirror, and refusal of CPU tensors."""
 import ctypes
 import subprocess
+import sys
 from pathlib import Path
 
 import pytest
@@ -151,3 +152,23 @@ def test_launches_of_2_32_threads_are_refused():
         assert norm(rows, dim, dtype) == 3 and "one launch" in _err(), (rows, dim)
     for n, rc in (((1 << 29) - 1, 3), ((1 << 29) - 63, 3), ((1 << 29) - 64, 1)):  # the last: no workspace
         assert L.tgx_embed_grad(8, 8, 1, n, 5, 4, 0, 1.0, 16, None, 0, None) == rc, n
+
+
+def test_attention_rows_that_no_grid_takes():
+    """Tiles of rows that pass 32 bits: refused, where their count came to zero and divided by it.  In a process
+    of its own, which such a division would end."""
+    code = """
+import ctypes, sys
+sys.path.insert(0, sys.argv[1])
+from tgengine_amd.core import _lib
+L = _lib.lib()
+for dtype in (0, 1):
+    for lq, heads, kv in ((1 << 30, 512, 1), ((1 << 31) - 1, 512, 1), (1 << 27, 4096, 64), (1 << 30, 8, 8)):
+        a = ctypes.byref(_lib.TgxAttentionArgs(q=8, k=8, v=8, out=8, lse=8, grad_out=8, grad_q=8, grad_k=8, grad_v=8, batch=1,
+                                               lq=lq, lk=10, heads=heads, kv_heads=kv, dim=1, dtype=dtype))
+        assert L.tgx_attention_workspace_size(a) == 0 and L.tgx_attention_grad_workspace_size(a) == 0
+        for fn in (L.tgx_attention, L.tgx_attention_grad):
+            assert fn(a, None) == 3 and b"one launch" in L.tgx_last_error(), (lq, heads)
+"""
+    r = subprocess.run([sys.executable, "-c", code, str(ROOT)], capture_output=True, text=True)
+    assert r.returncode == 0, (r.returncode, r.stderr)

@@ -23,9 +23,11 @@ int check_attention(const char* what, const tgx_attention_args* a, bool grad) {
                 a->heads, a->kv_heads, a->dim);
   if (elem_bytes(a->dtype) == 0) return fail(TGX_ERR_DTYPE, "%s: dtype %d", what, a->dtype);
   if (a->dim > TGX_MAX_HEAD_DIM) return fail(TGX_ERR_LIMIT, "%s: dim=%d above %d", what, a->dim, TGX_MAX_HEAD_DIM);
+  // No kernel takes 2^31 rows or more in one grid; up to 2^32 here, so that tiles of 16 rows
+  // are counted in an int wherever the grids' own checks have not been yet
   const int64_t most = int64_t(1) << 31;
   if (a->lq >= most || a->lk >= most || a->heads > 65535 || a->batch >= most ||
-      a->batch * a->heads >= most || (a->lq > 0 && a->batch * a->heads > (int64_t(1) << 40) / a->lq) ||
+      a->batch * a->heads >= most || (a->lq > 0 && a->batch * a->heads > (int64_t(1) << 32) / a->lq) ||
       (a->lk > 0 && a->batch * a->kv_heads > (int64_t(1) << 40) / a->lk))
     return fail(TGX_ERR_LIMIT, "%s: batch=%lld lq=%lld lk=%lld heads=%d: more rows than one launch takes", what,
                 static_cast<long long>(a->batch), static_cast<long long>(a->lq), static_cast<long long>(a->lk),
