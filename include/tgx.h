@@ -436,8 +436,8 @@ int tgx_co_occurrence(const int32_t* a_ids, const int32_t* c_ids, const uint8_t*
 /* ---- Operators of a temporal attention model on prepared batches ----
  * No counterpart in the reference, whose models (tgengine/models, tgengine/nn) take
  * these steps in torch.  Values are TGX_F32 or TGX_BF16; sums, statistics and softmax
- * are held in 32 bits and each output is rounded once.  No atomics: the same inputs
- * give the same bits. */
+ * are held in 32 bits or more and each output is rounded once.  No floating-point
+ * atomics: the same inputs give the same bits. */
 #define TGX_MAX_EMBED_DIM 65536
 #define TGX_MAX_NORM_DIM 16384
 #define TGX_MAX_HEAD_DIM 256

@@ -56,9 +56,10 @@ __global__ __launch_bounds__(256) void att_stats(const T* __restrict__ out, cons
 }
 
 // sums += fragment f of x times the tile's rows from row0 on.  bf16 takes what cutting x to
-// bf16 leaves through a second product with the same operand out of LDS: without it dq, dk and dv were 1.41 to 1.45 times as far off as one rounding of them.
-// 2 x (1,000 x 8,000 tokens), 16/4 heads of 128, 92% kept: dk and dv 488 us with it and 402
-// without, dq 308 and 252; 400 x (65 x 65), 2 heads of 100: 72 and 64, 28 and 27.
+// bf16 leaves through a second product with the same operand out of LDS: without it dq, dk and
+// dv were 1.41 to 1.45 times as far off as one rounding of them.  2 x (1,000 x 8,000 tokens),
+// 16/4 heads of 128, 92% kept: dk and dv 488 us with it and 402 without, dq 308 and 252; 400 x
+// (65 x 65), 2 heads of 100: 72 and 64, 28 and 27.
 template <typename T, int DP, typename TILE, bool SIGNED>
 __device__ __forceinline__ void mma_fine(Acc<T> (&sums)[DP / kTile<T>], const T* tile, int row0, const Acc<T>& x, int f) {
   const u32x4 xf = to_frag<T>(x, f);

@@ -5,11 +5,11 @@
 // running maximum and sum of the softmax are a lane's own but for an exchange between
 // the lanes of a row now and then, and P^T, still in the same registers, is the second operand of
 // O^T += V^T P^T.  Scores are in units of log 2.  bf16's matrix units take probabilities of
-// bf16: a second product adds what cutting them to that left (to_frag), so that an output is off by its own rounding only.  Without it the two
-// roundings' errors together were 1.41 times the output's own, however many keys there were.
-// It uses the same reads of V: 2 x (1,000 x 8,000 tokens), 16/4 heads of 128, take 224 us
-// with it and 180 without, 200 x (200 x 200), 4 heads of 64, 61 and 55, single tokens to
-// 30,001 keys 96 either way.
+// bf16: a second product adds what cutting them to that left (to_frag), so that an output is
+// off by its own rounding only.  Without it the two roundings' errors together were 1.41 times
+// the output's own, however many keys there were.  It uses the same reads of V: 2 x (1,000 x
+// 8,000 tokens), 16/4 heads of 128, take 224 us with it and 180 without, 200 x (200 x 200), 4
+// heads of 64, 61 and 55, single tokens to 30,001 keys 96 either way.
 //
 // What bounds it: for bf16 the softmax between the products and the LDS reads that feed
 // them (that first call, 92% kept: 538 TFLOP/s of the 1,225 that a matrix product of 8,192

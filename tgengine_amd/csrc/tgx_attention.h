@@ -440,8 +440,11 @@ __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(
 // has to say so, or the gradient would take the row for one without keys.
 __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2; }
 
-// Calls f(T{}, DP, TINY) with the head size padded to whole tiles: for f32 mostly to the
-// next 16, for bf16 to the next 32
+// Calls f(T{}, DP, TINY) with the head size padded to one of six or seven widths, each a set of
+// kernels.  f32, bound by its matrix units, has two more between the widths of bf16: with 112
+// and 176 the forward pass, dk and dv and dq of 400 x (65 x 65), 2 heads, take 55, 109 and 31 us
+// for 100 values and 94, 199 and 52 for 172; padded to 128 and 256 they take 73, 118 and 33, and
+// 121, 254 and 67.  Heads of 177 to 192 values, which pad to 256, would win as much by one more.
 template <typename F>
 int by_head(int dtype, int dim, F&& f) {
 #define TGX_HEAD(DP) f(t, std::integral_constant<int, DP>{}, std::false_type{})

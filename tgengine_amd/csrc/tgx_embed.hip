@@ -89,6 +89,7 @@ constexpr int64_t kSmallTokens = int64_t(kSmallThreads) * kSmallItems;
 constexpr size_t small_lds(int items) {
   return static_cast<size_t>(kSmallThreads) * items * 4 + kSmallWaves * (size_t(2) << kSmallBits);
 }
+static_assert(small_lds(kSmallItems) <= 48 * 1024, "what any launch may have without asking");
 
 template <int ITEMS, typename I>
 __global__ __launch_bounds__(kSmallThreads) void embed_small_sort(const I* __restrict__ ids, int n, int64_t rows,
@@ -418,10 +419,6 @@ int sort_tokens(const I* ids, int64_t n, int64_t rows, const EmbedWs& w, const Z
     const unsigned blocks = 1 + static_cast<unsigned>(std::clamp<int64_t>(ops_cdiv(z.n16, 4 * kSmallThreads), 1, 512));
     auto go = [&](auto items) {
       constexpr int ITEMS = decltype(items)::value;
-      static const hipError_t allowed =
-          hipFuncSetAttribute(reinterpret_cast<const void*>(&embed_small_sort<ITEMS, I>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(small_lds(ITEMS)));
-      (void)allowed;  // a launch that needs it says so
       hipLaunchKernelGGL((embed_small_sort<ITEMS, I>), dim3(blocks), dim3(kSmallThreads), small_lds(ITEMS), s, ids,
                          static_cast<int>(n), rows, bits, k[0], v[0], z.p, z.head, z.n16, z.tail);
       return check_launch("embed_small_sort");

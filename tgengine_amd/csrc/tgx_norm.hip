@@ -46,10 +46,12 @@ struct Place {
 // Rows that a group of lanes takes at a time: with one pack a lane, several rows are in
 // flight, share the weights and hide each other's sums.  Lanes that take a whole row side
 // by side touch fewer cache lines than few lanes with more packs each where rows do not
-// begin on a line (786,432 x 172 bf16 rows, forward: 8 lanes of 3 packs 137 us, 32 lanes of
-// one 159, and with four rows 120; backward 206, 202, and with two rows 175).
+// begin on a line (786,432 x 172 bf16 rows, forward: 8 lanes of 3 packs 141 us, 32 lanes of
+// one 163, and with four rows 135; backward 209, 192, and with two rows 176).  Not every call
+// is faster so: with 136 and 192 values the forward pass takes 116 and 125 us, and 8 lanes of 3
+// packs 94 and 110; so do 172 values where a backward pass runs between the calls, 146 and 114.
 //
-// HBM bounds it: those 541 MB take the forward pass 128 us, 4.3 TB/s where a copy without
+// HBM bounds it: those 541 MB take the forward pass 135 us, 4.0 TB/s where a copy without
 // gaps in its lines reaches 6.2; 240 x 172 f32 rows take 4.4 us, a chain of one read, two
 // sums over the lanes and one write.
 constexpr int fwd_rows(int c) { return c == 1 ? 4 : c == 2 ? 2 : 1; }
