@@ -359,8 +359,15 @@ Tensor cross_attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_i
 }
 
 // ------------------------------------------------------------------ clipping
-Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm, const std::vector<Tensor>& outs) {
-  const size_t n = grads.size();
+Tensor clip_grad_norm(std::vector<Tensor> grads, double max_norm, const std::vector<Tensor>& outs) {
+  // a leaf that requires a gradient stands for it, as a parameter does
+  size_t n = 0;
+  for (Tensor& g : grads) {
+    Tensor t = g.requires_grad() && g.is_leaf() ? g.grad() : g;
+    if (t.defined()) grads[n++] = std::move(t);
+    else if (!outs.empty()) bad("clip_grad_norm_: out needs a gradient for each of its tensors");
+  }
+  grads.resize(n);
   if (n == 0) bad("clip_grad_norm_: no gradients");
   if (!outs.empty() && outs.size() != n) bad("clip_grad_norm_: out must have one tensor per gradient");
   std::vector<const void*> in(n);

@@ -74,8 +74,7 @@ def clip_grad_norm_(grads: Union[Tensor, Iterable[Tensor]], max_norm: float,
     if isinstance(grads, Tensor):
         grads = [grads]
     # a Parameter's isinstance check runs Python code: plain tensors skip it
-    grads = [g.grad if g.requires_grad and g.is_leaf or type(g) is not Tensor and isinstance(g, torch.nn.Parameter) else g
-             for g in grads]
+    grads = [g if type(g) is Tensor or not isinstance(g, torch.nn.Parameter) else g.grad for g in grads]
     if out is None:
         grads = [g for g in grads if g is not None]
         if not grads:
