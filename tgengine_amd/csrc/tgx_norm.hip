@@ -48,8 +48,9 @@ struct Place {
 // by side touch fewer cache lines than few lanes with more packs each where rows do not
 // begin on a line (786,432 x 172 bf16 rows, forward: 8 lanes of 3 packs 141 us, 32 lanes of
 // one 163, and with four rows 135; backward 209, 192, and with two rows 176).  Not every call
-// is faster so: with 136 and 192 values the forward pass takes 116 and 125 us, and 8 lanes of 3
-// packs 94 and 110; so do 172 values where a backward pass runs between the calls, 146 and 114.
+// is faster so: with 136 and 192 values the forward pass takes 118 and 128 us, and 94 and 111
+// with 8 lanes of 3 packs; with 172, where a backward pass runs between the calls, 131 to 154
+// and 109 to 114.
 //
 // HBM bounds it: those 541 MB take the forward pass 135 us, 4.0 TB/s where a copy without
 // gaps in its lines reaches 6.2; 240 x 172 f32 rows take 4.4 us, a chain of one read, two
