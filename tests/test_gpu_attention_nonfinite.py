@@ -144,3 +144,18 @@ def test_infinite_score_gradients(lq, lk, d, dtype):
     other = mask[1].clone()
     other[lk // 3] = False
     assert bool((dk[1, other, 0] == -INF).all()) and dk[1, lk // 3, 0].isnan().all() and not dk[1, ~mask[1]].any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lq,lk,d", SHAPES)
+def test_zeros_stay_zeros(lq, lk, d, dtype):
+    """A row whose gradient is zero has a dq of zero, and where all rows' are, so are dk and dv."""
+    q, k, v, g, mask = _inputs(lq, lk, d, dtype)
+    g[0] = 0.0
+    g[1, lq - 1, 0] = 0.0
+    g[3, :, 2:] = 0.0
+    got = _run(q, k, v, g, mask)
+    assert not got["dq"][0].any() and not got["dk"][0].any() and not got["dv"][0].any()
+    assert not got["dq"][1, lq - 1, 0].any() and not got["dk"][3, :, 1].any() and not got["dv"][3, :, 1].any()
+    zero = _run(q, k, torch.zeros_like(v), g, mask)
+    assert not zero["out"].any() and not zero["dq"].any() and not zero["dk"].any()

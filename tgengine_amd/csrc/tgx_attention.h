@@ -114,13 +114,14 @@ __device__ __forceinline__ float lost(float x) {
   return fabsf(y) == INFINITY ? 0.f : x - y;
 }
 
-// What cutting x to bf16 leaves, with x's sign and never 0, nor NaN for an infinity: an
-// infinite factor, or an infinite x, then gives the same infinity with both parts
+// What cutting x to bf16 leaves, with x's sign and never 0 unless x is, nor NaN for an infinity:
+// an infinite factor, or an infinite x, then gives the same infinity with both parts.  (The
+// median of numbers one of which is NaN is the least of the others.)
 template <bool SIGNED>
 __device__ __forceinline__ float left(float x) {
   const float cut = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
-  if constexpr (!SIGNED) return fmaxf(x - cut, 0x1p-126f);  // fmaxf takes the other of NaN
-  return copysignf(fmaxf(fabsf(x) - fabsf(cut), 0x1p-126f), x);
+  if constexpr (!SIGNED) return __builtin_amdgcn_fmed3f(x - cut, 0x1p-126f, x);
+  return copysignf(__builtin_amdgcn_fmed3f(fabsf(x) - fabsf(cut), 0x1p-126f, fabsf(x)), x);
 }
 
 // Fragment f (of kFrags) of such values as the second operand of a product that sums
