@@ -532,6 +532,48 @@ int tgx_clip_grad_norm(const void* const* grads, const int32_t* dtypes, void* co
                        float max_norm, float* norm, void* workspace, size_t workspace_bytes,
                        void* stream);
 
+/* A gated recurrence along the tokens of every batch row, over dim channels:
+ *   h_t = a_t h_{t-1} + (1 - a_t) x_t,  a_t = sigmoid(gate_t);  a masked token: h_t = h_{t-1}
+ * from h_0 = state (zeros without one).  Element (b, t, c) of x is x[b * x_stride[0] + t *
+ * x_stride[1] + c], gate alike; a stride may be 0.  mask: NULL, or bytes at mask[b *
+ * mask_stride + t], 0 = token t takes no part (its x and gate are not used, whatever they
+ * hold).  out [batch, length, dim] holds every h_t rounded, last [batch, dim] the last one. */
+typedef struct tgx_scan_args {
+  const void* x;
+  const void* gate;
+  const uint8_t* mask;
+  const float* state;      /* NULL or [batch, dim] */
+  int64_t batch;
+  int64_t length;
+  int64_t dim;
+  int64_t x_stride[2];     /* batch, token */
+  int64_t gate_stride[2];
+  int64_t mask_stride;
+  int32_t dtype;
+  int32_t reserved;
+  void* out;
+  float* last;
+  float* starts;           /* NULL, or [batch, tgx_scan_starts(length), dim]: states within the rows,
+                              which the gradient reads */
+  /* tgx_scan_grad: starts as tgx_scan wrote them (out and last are not read); grad_out
+   * [batch, length, dim] and grad_last [batch, dim], each NULL for zeros; grad_x and
+   * grad_gate [batch, length, dim] and grad_state [batch, dim], each may be NULL */
+  const void* grad_out;
+  const float* grad_last;
+  void* grad_x;
+  void* grad_gate;
+  float* grad_state;
+  void* workspace;         /* 16-byte aligned, no initialisation; NULL when 0 bytes are needed */
+  size_t workspace_bytes;
+} tgx_scan_args;
+
+int64_t tgx_scan_starts(int64_t length);
+/* bytes of workspace that tgx_scan or tgx_scan_grad of these arguments needs (0 for
+ * arguments that they refuse) */
+size_t tgx_scan_workspace_size(const tgx_scan_args* args);
+int tgx_scan(const tgx_scan_args* args, void* stream);
+int tgx_scan_grad(const tgx_scan_args* args, void* stream);
+
 const char* tgx_last_error(void);
 int tgx_abi_version(void);
 

@@ -1,0 +1,327 @@
+"""gated_scan against the recurrence in 64 bits, one token after the other.
+
+u = 2^-24.  The gates: the exponent's argument is off by 2 u |g|, its power and the
+reciprocal by a unit in the last place each, so a and 1 - a are off by s = (2 |g| + 6) u
+relatively.  A state is a sum of products of gates; with M the same sum of absolute values,
+one token adds (s + 3 u) M to the error (a gate, a product, a sum, and a joint of two
+pieces), and what was there shrinks by a.  dh alike.  dx and dgate are products of those;
+outputs are rounded once (r = u in f32, 2^-8 in bf16).  1.01 stands for products of
+errors, 1e-37 for values that the power's instruction flushes."""
+import pytest
+import torch
+
+from tgengine_amd import ops
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+F, B = torch.float32, torch.bfloat16
+
+
+def _case(shape, dtype, mask="none", state=True, seed=0, wide=2.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    b, n, d = shape
+
+    def r(*s):
+        return torch.randn(*s, generator=g, device="cuda")
+
+    c = {"x": r(b, n, d).to(dtype), "gate": (r(b, n, d) * wide).to(dtype), "state": r(b, d) if state else None,
+         "mask": None, "grads": (r(b, n, d).to(dtype), r(b, d))}
+    at = torch.arange(n, device="cuda")
+    held = torch.randint(0, n + 1, (b, 1), generator=g, device="cuda")
+    if mask == "recent":
+        c["mask"] = at >= n - held
+    elif mask == "prefix":
+        c["mask"] = at < held
+    elif mask == "holes":
+        c["mask"] = torch.rand(b, n, generator=g, device="cuda") < 0.6
+    elif mask == "empty":
+        c["mask"] = torch.zeros(b, n, device="cuda", dtype=torch.bool)
+    return c
+
+
+def _exact(c):
+    """{name: (value, bound)}"""
+    x, gate, (gout, glast) = c["x"].double(), c["gate"].double(), c["grads"]
+    b, n, d = x.shape
+    r = U if c["x"].dtype == F else 2.0 ** -8
+    keep = torch.ones(b, n, device="cuda", dtype=torch.bool) if c["mask"] is None else c["mask"].bool()
+    x = torch.where(keep[..., None], x, 0.0)
+    gate = torch.where(keep[..., None], gate, 0.0)
+    a, rest = torch.sigmoid(gate), torch.sigmoid(-gate)
+    a, rest = torch.where(keep[..., None], a, 1.0), torch.where(keep[..., None], rest, 0.0)
+    s = torch.where(keep[..., None], (2 * gate.abs() + 6) * U, 0.0)
+    h = torch.zeros(b, d, device="cuda", dtype=torch.float64) if c["state"] is None else c["state"].double()
+    m, e = h.abs(), torch.zeros_like(h)
+    hs, es, before = [], [], []
+    for t in range(n):
+        before.append((h, e))
+        h = a[:, t] * h + rest[:, t] * x[:, t]
+        m = a[:, t] * m + rest[:, t] * x[:, t].abs()
+        e = a[:, t] * e + (s[:, t] + 3 * U) * m
+        hs.append(h)
+        es.append(e)
+    out = {"last": (h, e)}
+    dh, dm, de = glast.double(), glast.double().abs(), torch.zeros_like(h)
+    dx, dg = [], []
+    for t in range(n - 1, -1, -1):
+        g = gout[:, t].double()
+        dh, dm, de = dh + g, dm + g.abs(), de
+        de = de + 2 * U * dm
+        old, eold = before[t]
+        off = old - x[:, t]
+        f, q = a[:, t], rest[:, t]
+        v = dh * q
+        dx.append((v, de * q + v.abs() * (s[:, t] + 2 * U)))
+        w = v * f * off
+        dg.append((w, de * q * f * off.abs() + dh.abs() * q * f * (eold + U * off.abs()) + w.abs() * (2 * s[:, t] + 4 * U)))
+        dh, dm, de = f * dh, f * dm, f * (de + (s[:, t] + 3 * U) * dm)
+    out["state"] = (dh, de)
+    if n:
+        out["out"] = torch.stack(hs, 1), torch.stack(es, 1)
+        for name, v in (("x", dx), ("gate", dg)):
+            out[name] = tuple(torch.stack([p[i] for p in v[::-1]], 1) for i in (0, 1))
+        for name in ("out", "x", "gate"):
+            out[name] = out[name][0], out[name][1] + r * out[name][0].abs()
+    for name in ("last", "state"):
+        out[name] = out[name][0], out[name][1] + U * out[name][0].abs()
+    return out
+
+
+def _run(c, names=("x", "gate", "state"), grads=None):
+    leaves = {n: c[n].detach().requires_grad_() for n in names if c[n] is not None}
+    y = ops.gated_scan(*(leaves.get(n, c[n]) for n in ("x", "gate")), mask=c["mask"], state=leaves.get("state", c["state"]))
+    got = {"out": y[0].detach(), "last": y[1].detach()}
+    pairs = [(o, g) for o, g in zip(y, grads or c["grads"]) if g is not None]
+    d = torch.autograd.grad([p[0] for p in pairs], list(leaves.values()), [p[1] for p in pairs])
+    return {**got, **dict(zip(leaves, d))}
+
+
+def _holds(got, want):
+    for name, t in got.items():
+        if t.numel() == 0:
+            continue
+        y, e = want[name]
+        assert t.shape == y.shape
+        off, e = (t.double() - y).abs(), 1.01 * e + 1e-37
+        assert bool((off <= e).all()), f"{name}: {float((off / e).max()):.3g} of the bound"
+
+
+def _check(c):
+    got, want = _run(c), _exact(c)
+    _holds(got, want)
+    assert got["out"].dtype == got["x"].dtype == c["x"].dtype and got["last"].dtype == F
+    with torch.no_grad():
+        out, last = ops.gated_scan(c["x"], c["gate"], c["mask"], c["state"])
+    assert torch.equal(out, got["out"]) and torch.equal(last, got["last"])
+    again = _run(c)
+    assert all(torch.equal(again[n], got[n]) for n in got)
+    return got
+
+
+SHAPES = [(1, 1, 1), (3, 1, 172), (2, 2, 1), (4, 3, 2), (5, 15, 3), (5, 16, 100), (5, 17, 101), (7, 33, 172), (12, 64, 50),
+          (4, 65, 7), (3, 127, 12), (2, 128, 33), (2, 500, 5), (1, 3001, 2), (2, 2050, 64), (300, 20, 172), (1, 40, 4099),
+          (2000, 5, 19), (33, 257, 256)]
+
+
+@pytest.mark.parametrize("dtype", [F, B])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_against_64_bits(shape, dtype):
+    _check(_case(shape, dtype))
+
+
+@pytest.mark.parametrize("dtype", [F, B])
+@pytest.mark.parametrize("mask", ["recent", "prefix", "holes", "empty"])
+@pytest.mark.parametrize("shape", [(9, 1, 3), (17, 20, 172), (40, 32, 25), (3, 130, 6), (2, 1500, 40)])
+def test_masks(shape, mask, dtype):
+    """Rows of any number of tokens; NaN, infinities and the type's ends where tokens take no part."""
+    for state in (True, False):
+        c = _case(shape, dtype, mask, state, seed=3)
+        got = _check(c)
+        for bad in (float("nan"), float("inf"), torch.finfo(dtype).min):
+            d = {**c, **{n: torch.where(c["mask"][..., None], c[n], bad) for n in ("x", "gate")}}
+            new = _run(d)
+            assert all(torch.equal(new[n], got[n]) for n in got)
+        as_bytes = {**c, "mask": c["mask"].to(torch.uint8) * 7}
+        assert all(torch.equal(v, got[n]) for n, v in _run(as_bytes).items())
+        left = ~c["mask"]
+        assert not got["x"][left].any() and not got["gate"][left].any()
+        none = ~c["mask"].any(1)
+        if bool(none.any()):
+            assert torch.equal(got["last"][none], c["state"][none] if state else torch.zeros_like(got["last"][none]))
+
+
+@pytest.mark.parametrize("dtype", [F, B])
+def test_far_gates(dtype):
+    """Gates that forget all, keep all, and everything between."""
+    _check(_case((6, 200, 40), dtype, wide=30.0))
+    c = _case((4, 40, 16), dtype)
+    c["gate"][:, 10:20] = float("inf")
+    got = _run(c)
+    assert torch.equal(got["out"][:, 19], got["out"][:, 9]) and not got["x"][:, 10:20].any()
+    c["gate"][:, 10:20] = float("-inf")
+    got = _run(c)
+    assert torch.equal(got["out"][:, 10:20], c["x"][:, 10:20]) and torch.equal(got["gate"][:, 10:20], torch.zeros_like(got["gate"][:, 10:20]))
+
+
+@pytest.mark.parametrize("dtype", [F, B])
+@pytest.mark.parametrize("shape", [(5, 33, 50), (2, 700, 12)])
+def test_layouts(shape, dtype):
+    """Strides, shifted starts, side by side and broadcast inputs give the bits of contiguous ones."""
+    c = _case(shape, dtype, "holes")
+    b, n, d = shape
+    want = _run(c)
+
+    def same(**more):
+        got = _run({**c, **more})
+        assert all(torch.equal(got[k], want[k]) for k in want)
+
+    both = torch.stack([c["x"], c["gate"]], 2)
+    same(x=both[:, :, 0], gate=both[:, :, 1])
+    same(x=c["x"].transpose(0, 1).contiguous().transpose(0, 1))
+    same(gate=c["gate"].transpose(1, 2).contiguous().transpose(1, 2))
+    odd = torch.empty(b * n * d + 1, device="cuda", dtype=dtype)[1:].view(shape)
+    same(x=odd.copy_(c["x"]))
+    wide = torch.zeros(b, n + 3, device="cuda", dtype=torch.bool)
+    wide[:, 2:2 + n] = c["mask"]
+    same(mask=wide[:, 2:2 + n])
+    same(mask=c["mask"].t().contiguous().t())
+    same(state=torch.stack([c["state"]] * 2, -1)[..., 0])
+    same(grads=tuple(torch.stack([g] * 2, -1)[..., 0] for g in c["grads"]))
+    c["mask"] = c["mask"][:1].expand(b, n)
+    c["gate"] = c["gate"][:1, :1].expand(shape)  # a decay for each channel
+    want = _run({**c, "gate": c["gate"].contiguous(), "mask": c["mask"].contiguous()})
+    same()
+    decay = c["gate"][:1, :1].detach().contiguous().requires_grad_()
+    y = ops.gated_scan(c["x"], decay.expand(shape), c["mask"], c["state"])
+    got, = torch.autograd.grad(y, decay, c["grads"])
+    total = want["gate"].double().sum((0, 1), keepdim=True)
+    # torch sums the rows' rounded gradients and rounds to the type
+    assert bool(((got.double() - total).abs() <= want["gate"].double().abs().sum((0, 1), keepdim=True)
+                 * (U * 64 if dtype == F else 2.0 ** -7)).all())
+
+
+@pytest.mark.parametrize("dtype", [F, B])
+def test_from_call_to_call(dtype):
+    """Parts of a history, and single tokens, carried by their states: the whole's states, within its bounds."""
+    c = _case((6, 70, 172), dtype, "holes")
+    want = _exact(c)
+    for cuts in ([0, 1, 34, 70], list(range(71))):
+        state, outs = c["state"], []
+        for i, j in zip(cuts, cuts[1:]):
+            out, state = ops.gated_scan(c["x"][:, i:j], c["gate"][:, i:j], c["mask"][:, i:j], state)
+            outs.append(out)
+        _holds({"out": torch.cat(outs, 1), "last": state}, want)
+
+
+@pytest.mark.parametrize("dtype", [F, B])
+@pytest.mark.parametrize("shape", [(5, 40, 172), (1, 1000, 8)])
+def test_partial_gradients(shape, dtype):
+    c = _case(shape, dtype, "recent")
+    want = _run(c)
+    for names in (("x",), ("gate",), ("state",), ("gate", "state")):
+        got = _run(c, names)
+        assert all(torch.equal(got[n], want[n]) for n in got)
+    zero = [torch.zeros_like(g) for g in c["grads"]]
+    for i in (0, 1):
+        only, full = list(c["grads"]), list(c["grads"])
+        only[i], full[i] = None, zero[i]
+        a, b = _run(c, grads=only), _run(c, grads=full)
+        assert all(torch.equal(a[n], b[n]) for n in a)
+    none = {**c, "state": None}
+    a, b = _run(none), _run({**c, "state": torch.zeros_like(c["state"])})
+    assert all(torch.equal(a[n], b[n]) for n in a)
+
+
+def test_not_finite_stays_in_its_channel():
+    c = _case((4, 50, 30), F)
+    want = _run(c)
+    c["x"][1, 7, 3], c["gate"][2, 9, 4] = float("inf"), float("nan")
+    got = _run(c)
+    touched = torch.zeros(4, 30, device="cuda", dtype=torch.bool)
+    touched[1, 3] = touched[2, 4] = True
+    for n in ("out", "x", "gate"):
+        assert torch.equal(got[n].transpose(1, 2)[~touched], want[n].transpose(1, 2)[~touched])
+    assert got["out"][1, 7:, 3].isinf().all() and got["out"][2, 9:, 4].isnan().all()
+    assert torch.equal(got["out"][1, :7, 3], want["out"][1, :7, 3])
+
+
+def test_gradient_against_differences():
+    """Central differences of the forward kernel, h = 2^-7: h^2 of curvature and u / h of rounding,
+    together below 2^-9 of the sum of |out * g|."""
+    c = _case((3, 90, 20), F, "holes")
+    got = _run(c)
+    size = sum((got[n].double() * g.double()).abs().sum() for n, g in zip(("out", "last"), c["grads"]))
+    h = 2.0 ** -7
+    for name in ("x", "gate", "state"):
+        step = torch.randn_like(c[name])
+        step = step / step.norm()
+        f = []
+        for s in (h, -h):
+            d = {**c, name: c[name] + s * step}
+            y = ops.gated_scan(d["x"], d["gate"], d["mask"], d["state"])
+            f.append(sum((a.double() * g.double()).sum() for a, g in zip(y, c["grads"])))
+        assert abs((f[0] - f[1]) / (2 * h) - (got[name].double() * step.double()).sum()) <= size * 2.0 ** -9, name
+
+
+@pytest.mark.parametrize("shape", [(20, 30, 172), (1, 900, 8)])
+def test_streams_and_graph_replays(shape):
+    """On a side stream, and forward and backward captured: replays see new inputs, between eager calls."""
+    c = _case(shape, B, "holes")
+    want = _run(c)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _run(c)
+    side.synchronize()
+    assert all(torch.equal(got[n], want[n]) for n in want)
+    static = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            _run(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = _run(static)
+    for seed in range(4):
+        new = _case(shape, B, "holes", seed=10 + seed)
+        new["grads"] = c["grads"]
+        for n in ("x", "gate", "state", "mask"):
+            static[n].copy_(new[n])
+        graph.replay()
+        torch.cuda.synchronize()
+        want = _run(new)
+        assert all(torch.equal(held[n], want[n]) for n in want)
+
+
+def test_empty():
+    for shape in ((0, 5, 8), (3, 0, 8), (0, 0, 8)):
+        c = _case(shape, F)
+        got = _run(c)
+        assert got["out"].shape == shape and got["x"].shape == shape
+        assert torch.equal(got["last"], c["state"]) and torch.equal(got["state"], c["grads"][1])
+        out, last = ops.gated_scan(c["x"], c["gate"])
+        assert not last.any() and last.shape == (shape[0], 8)
+
+
+def test_refusals():
+    x = torch.randn(2, 5, 8, device="cuda")
+    S = ops.gated_scan
+    m = torch.ones(2, 5, device="cuda", dtype=torch.bool)
+    for args, text in (((x[0], x[0]), r"\(batch, tokens, dim\)"), ((x, x[:, :4]), "shape of x"), ((x, x.bfloat16()), "same dtype"),
+                       ((x.half(), x.half()), "float32 or bfloat16"), ((x, x.cpu()), "device"), ((x, x, m[:, :4]), "mask must be"),
+                       ((x, x, m.float()), "must be bool"), ((x, x, m.cpu()), "device"), ((x[..., :0], x[..., :0]), "dim"),
+                       ((x, x, m, torch.zeros(2, 7, device="cuda")), "state must be"),
+                       ((x, x, m, torch.zeros(2, 8, device="cuda", dtype=B)), "state must be float32"),
+                       ((x, x, m, torch.zeros(2, 8)), "device")):
+        with pytest.raises(ValueError, match=text):
+            S(*args)
+    with pytest.raises(RuntimeError, match="on the GPU"):
+        S(x.cpu(), x.cpu())
+    y = x.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="once only"):
+        torch.autograd.grad(S(y, y)[0].sum(), y, create_graph=True)
+    out, _ = S(y, x)
+    x.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        out.sum().backward()

@@ -20,7 +20,7 @@ OUT_DIR = PKG / "_lib"
 LIB = OUT_DIR / "libtgx.so"
 SOURCES = ["tgx_common.hip", "tgx_ring.hip", "tgx_recent.hip", "tgx_csr.hip", "tgx_negpool.hip",
            "tgx_embed.hip", "tgx_norm.hip", "tgx_attention.hip", "tgx_att_fwd.hip", "tgx_att_bwd.hip", "tgx_att_rows.hip",
-           "tgx_clip.hip"]
+           "tgx_clip.hip", "tgx_scan.hip"]
 
 ARCH = "gfx950"
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
@@ -55,7 +55,8 @@ def build_host(verbose: bool = False) -> Path:
            *[f"-I{p}" for p in ce.include_paths()], f"-I{sysconfig.get_paths()['include']}",
            # torch's HIP stream API (the caller's current stream); host code only
            "-D__HIP_PLATFORM_AMD__", f"-I{ROCM}/include",
-           f"-I{INCLUDE}", str(CSRC / "tgx_host.cpp"), str(CSRC / "tgx_ops.cpp"), "-o", str(tmp),
+           f"-I{INCLUDE}", str(CSRC / "tgx_host.cpp"), str(CSRC / "tgx_ops.cpp"),
+           str(CSRC / "tgx_ops_block.cpp"), "-o", str(tmp),
            *[f"-L{p}" for p in ce.library_paths()], "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu",
            "-ltorch_python", f"-L{OUT_DIR}", "-ltgx", "-Wl,-rpath,$ORIGIN/_lib"]
     if verbose:

@@ -101,6 +101,14 @@ class TgxAttentionArgs(ctypes.Structure):
                 ("workspace", c_vp), ("workspace_bytes", ctypes.c_size_t)]
 
 
+class TgxScanArgs(ctypes.Structure):
+    _fields_ = [("x", c_vp), ("gate", c_vp), ("mask", c_vp), ("state", c_vp), ("batch", c_i64), ("length", c_i64),
+                ("dim", c_i64), ("x_stride", c_i64 * 2), ("gate_stride", c_i64 * 2), ("mask_stride", c_i64),
+                ("dtype", c_i32), ("reserved", c_i32), ("out", c_vp), ("last", c_vp), ("starts", c_vp),
+                ("grad_out", c_vp), ("grad_last", c_vp), ("grad_x", c_vp), ("grad_gate", c_vp), ("grad_state", c_vp),
+                ("workspace", c_vp), ("workspace_bytes", ctypes.c_size_t)]
+
+
 SIGNATURES = {
     "tgx_ring_append": (c_i32, [ctypes.POINTER(TgxRing), c_vp, c_vp, c_vp, c_vp, c_i64, c_i64,
                                 c_vp, ctypes.c_size_t, c_vp, c_vp]),
@@ -156,6 +164,10 @@ SIGNATURES.update({
     "tgx_clip_grad_norm_workspace_size": (ctypes.c_size_t, [c_vp, c_i64]),
     "tgx_clip_grad_norm": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, ctypes.c_float, c_vp, c_vp,
                                    ctypes.c_size_t, c_vp]),
+    "tgx_scan_starts": (c_i64, [c_i64]),
+    "tgx_scan_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(TgxScanArgs)]),
+    "tgx_scan": (c_i32, [ctypes.POINTER(TgxScanArgs), c_vp]),
+    "tgx_scan_grad": (c_i32, [ctypes.POINTER(TgxScanArgs), c_vp]),
 })
 
 _lock = threading.Lock()

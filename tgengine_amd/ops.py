@@ -18,7 +18,7 @@ tracing are refused).  There is no CPU path.
 """
 from __future__ import annotations
 
-from typing import Iterable, Optional, Sequence, Union
+from typing import Iterable, Optional, Sequence, Tuple, Union
 
 import torch
 from torch import Tensor
@@ -58,6 +58,20 @@ def cross_attention(q: Tensor, k: Tensor, v: Tensor, mask: Optional[Tensor] = No
     D ** -0.5.
     """
     return _host().cross_attention(q, k, v, mask, scale)
+
+
+def gated_scan(x: Tensor, gate: Tensor, mask: Optional[Tensor] = None,
+               state: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+    """A gated recurrence along the tokens: h = a h + (1 - a) x with a = sigmoid(gate).
+
+    x and gate are (B, L, D) of one dtype, in any strides with a dense last dimension.
+    Returns every state, (B, L, D) in x's dtype, and the last one, (B, D) in float32.
+    state, (B, D) in float32, is the one before the first token (zeros without it): the
+    last state of a call is the next call's, down to one token at a time.  mask is
+    (B, L), True where a token takes part: the others leave the state as it is, and
+    their x and gate are not used, whatever they hold.
+    """
+    return _host().gated_scan(x, gate, mask, state)
 
 
 def clip_grad_norm_(grads: Union[Tensor, Iterable[Tensor]], max_norm: float,
