@@ -574,6 +574,54 @@ size_t tgx_scan_workspace_size(const tgx_scan_args* args);
 int tgx_scan(const tgx_scan_args* args, void* stream);
 int tgx_scan_grad(const tgx_scan_args* args, void* stream);
 
+/* The residual sum after a block and the norm before the next one, over `rows` rows of dim
+ * values:
+ *   sum = residual + scale sigmoid(gate) n,  n = x or norm(x) post_weight
+ *   out = norm(sum) weight + bias,  norm(v) = (v - mean v) / sqrt(var v + eps)
+ * scale, weight, bias and post_weight [dim] of wdtype; gate, scale, post_weight (then n = x),
+ * weight and bias may be NULL.  center = 0: norm(v) = v / sqrt(mean v^2 + eps).  Rows of x,
+ * residual and gate are their strides apart; out and sum [rows, dim]. */
+typedef struct tgx_residual_norm_args {
+  const void* x;
+  const void* residual;
+  const void* gate;
+  const void* weight;
+  const void* bias;
+  const void* scale;
+  const void* post_weight;
+  int64_t rows;
+  int64_t dim;             /* 1 .. TGX_MAX_NORM_DIM */
+  int64_t x_stride;
+  int64_t residual_stride;
+  int64_t gate_stride;
+  int32_t dtype;
+  int32_t wdtype;
+  int32_t center;
+  float eps;
+  void* out;
+  void* sum;
+  float* stats;            /* NULL, or kept for the gradient: [2, rows], with post_weight [4, rows] */
+  /* tgx_residual_norm_grad: stats as tgx_residual_norm wrote them (out and sum are not read);
+   * grad_out and grad_sum [rows, dim], each NULL for zeros; every other may be NULL.  Without
+   * gate, scale and post_weight the gradient of x is grad_residual (grad_x has to be NULL), and
+   * x may hold the sum instead, with residual NULL. */
+  const void* grad_out;
+  const void* grad_sum;
+  void* grad_x;
+  void* grad_residual;
+  void* grad_gate;
+  void* grad_weight;
+  void* grad_bias;
+  void* grad_scale;
+  void* grad_post_weight;
+  void* workspace;         /* 16-byte aligned, no initialisation; needed with a gradient of wdtype */
+  size_t workspace_bytes;
+} tgx_residual_norm_args;
+
+int tgx_residual_norm(const tgx_residual_norm_args* args, void* stream);
+size_t tgx_residual_norm_grad_workspace_size(const tgx_residual_norm_args* args);
+int tgx_residual_norm_grad(const tgx_residual_norm_args* args, void* stream);
+
 const char* tgx_last_error(void);
 int tgx_abi_version(void);
 

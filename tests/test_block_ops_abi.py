@@ -12,7 +12,7 @@ from tgengine_amd.core import _lib
 
 ROOT = Path(__file__).resolve().parent.parent
 
-STRUCTS = {"tgx_scan_args": _lib.TgxScanArgs}
+STRUCTS = {"tgx_scan_args": _lib.TgxScanArgs, "tgx_residual_norm_args": _lib.TgxResidualNormArgs}
 
 
 def _err():
@@ -64,8 +64,40 @@ def test_scan_checks():
     assert [L.tgx_scan_starts(n) for n in (0, 1, 16, 17, 32, 33)] == [0, 0, 0, 1, 1, 2]
 
 
+def _res(**more):
+    a = _lib.TgxResidualNormArgs(x=8, residual=8, out=8, sum=8, rows=3, dim=4, x_stride=4, residual_stride=4, eps=1e-5)
+    for n, v in more.items():
+        setattr(a, n, v)
+    return ctypes.byref(a)
+
+
+def test_residual_norm_checks():
+    L = _lib.lib()
+    for fn in (L.tgx_residual_norm, L.tgx_residual_norm_grad):
+        assert fn(None, None) == 1 and "args is NULL" in _err()
+        assert fn(_res(rows=-1), None) == 1 and fn(_res(dim=0), None) == 1
+        assert fn(_res(gate_stride=-4), None) == 1 and "strides" in _err()
+        assert fn(_res(dtype=2), None) == 2 and fn(_res(wdtype=-1), None) == 2
+        assert fn(_res(dim=16385), None) == 3 and fn(_res(rows=1 << 31), None) == 3
+        assert fn(_res(x=None), None) == 1 and "x must" in _err()
+        assert fn(_res(residual=None, scale=8), None) == 1 and "residual" in _err()
+        assert fn(_res(rows=0, x=None, residual=None), None) == 0
+    assert L.tgx_residual_norm(_res(residual=None), None) == 1
+    assert L.tgx_residual_norm(_res(sum=None), None) == 1 and "out and sum" in _err()
+    for rows, dim in ((1 << 28, 200), (1 << 24, 16384), (1 << 30, 40)):
+        assert L.tgx_residual_norm(_res(rows=rows, dim=dim), None) == 3 and "one launch" in _err()
+    G = L.tgx_residual_norm_grad
+    assert G(_res(grad_residual=8), None) == 1 and "stats" in _err()
+    assert G(_res(grad_x=8, stats=8), None) == 1 and "grad_x" in _err()
+    need = L.tgx_residual_norm_grad_workspace_size(_res(scale=8))
+    assert need == 4 * L.tgx_residual_norm_grad_workspace_size(_res()) // 2 > 0
+    for more in (dict(), dict(workspace=16, workspace_bytes=need - 1), dict(workspace=8, workspace_bytes=need)):
+        assert G(_res(scale=8, grad_scale=8, stats=8, **more), None) == 1 and "workspace" in _err()
+    assert L.tgx_residual_norm_grad_workspace_size(None) == 0 == L.tgx_residual_norm_grad_workspace_size(_res(dim=0))
+
+
 def test_no_cpu_path():
     x = torch.randn(2, 3, 8)
-    for call in (lambda: ops.gated_scan(x, x),):
+    for call in (lambda: ops.gated_scan(x, x), lambda: ops.residual_norm(x, x)):
         with pytest.raises(RuntimeError, match="on the GPU"):
             call()

@@ -109,6 +109,16 @@ class TgxScanArgs(ctypes.Structure):
                 ("workspace", c_vp), ("workspace_bytes", ctypes.c_size_t)]
 
 
+class TgxResidualNormArgs(ctypes.Structure):
+    _fields_ = [("x", c_vp), ("residual", c_vp), ("gate", c_vp), ("weight", c_vp), ("bias", c_vp), ("scale", c_vp),
+                ("post_weight", c_vp), ("rows", c_i64), ("dim", c_i64), ("x_stride", c_i64), ("residual_stride", c_i64),
+                ("gate_stride", c_i64), ("dtype", c_i32), ("wdtype", c_i32), ("center", c_i32), ("eps", ctypes.c_float),
+                ("out", c_vp), ("sum", c_vp), ("stats", c_vp), ("grad_out", c_vp), ("grad_sum", c_vp), ("grad_x", c_vp),
+                ("grad_residual", c_vp), ("grad_gate", c_vp), ("grad_weight", c_vp), ("grad_bias", c_vp),
+                ("grad_scale", c_vp), ("grad_post_weight", c_vp), ("workspace", c_vp),
+                ("workspace_bytes", ctypes.c_size_t)]
+
+
 SIGNATURES = {
     "tgx_ring_append": (c_i32, [ctypes.POINTER(TgxRing), c_vp, c_vp, c_vp, c_vp, c_i64, c_i64,
                                 c_vp, ctypes.c_size_t, c_vp, c_vp]),
@@ -168,6 +178,9 @@ SIGNATURES.update({
     "tgx_scan_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(TgxScanArgs)]),
     "tgx_scan": (c_i32, [ctypes.POINTER(TgxScanArgs), c_vp]),
     "tgx_scan_grad": (c_i32, [ctypes.POINTER(TgxScanArgs), c_vp]),
+    "tgx_residual_norm": (c_i32, [ctypes.POINTER(TgxResidualNormArgs), c_vp]),
+    "tgx_residual_norm_grad_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(TgxResidualNormArgs)]),
+    "tgx_residual_norm_grad": (c_i32, [ctypes.POINTER(TgxResidualNormArgs), c_vp]),
 })
 
 _lock = threading.Lock()

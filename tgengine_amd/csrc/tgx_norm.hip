@@ -8,40 +8,10 @@
 // once and its variance is the mean of squares about the mean, not a difference of
 // sums.  Statistics and sums are held in 32 bits; y and dx are rounded once, dw and
 // db once after the last sum.
-#include "tgx_ops.h"
+#include "tgx_norm_rows.h"
 
 namespace tgx {
 namespace {
-
-constexpr int kNormThreads = 256;
-
-// the sum over the L lanes of a row; L = 256: the whole workgroup, through `lds` [4]
-template <int L>
-__device__ __forceinline__ float row_sum(float x, float* lds) {
-  if constexpr (L <= kWave) {
-    return group_sum<L>(x);
-  } else {
-    x = group_sum<kWave>(x);
-    __syncthreads();
-    if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = x;
-    __syncthreads();
-    return (lds[0] + lds[1]) + (lds[2] + lds[3]);
-  }
-}
-
-// the lane's C packs of a row of `dim` values: pack j starts at at(j); its values below
-// skip(j) belong to the pack before (the last pack of a row overlaps it), and a pack
-// past the row has none
-template <int V, int L>
-struct Place {
-  int lane, dim, packs;
-  __device__ Place(int dim_) : lane(threadIdx.x & (L - 1)), dim(dim_), packs((dim_ + V - 1) / V) {}
-  __device__ int at(int j) const { return min((j * L + lane) * V, dim - V); }
-  __device__ int skip(int j) const {
-    const int p = j * L + lane;
-    return p < packs ? max(p * V - (dim - V), 0) : V;
-  }
-};
 
 // Rows that a group of lanes takes at a time: with one pack a lane, several rows are in
 // flight, share the weights and hide each other's sums.  Lanes that take a whole row side

@@ -1,5 +1,6 @@
 // Element types and wide accesses shared by the model-side operators
-// (tgx_embed.hip, tgx_norm.hip, tgx_attention.hip, tgx_clip.hip).
+// (tgx_embed.hip, tgx_norm.hip, tgx_attention.hip, tgx_clip.hip, tgx_scan.hip,
+// tgx_resnorm.hip, tgx_adamw.hip).
 #pragma once
 
 #include "tgx_internal.h"
@@ -46,6 +47,15 @@ inline size_t ops_align(size_t x) { return (x + 255) & ~static_cast<size_t>(255)
 
 inline uint64_t addr(const void* p) { return reinterpret_cast<uint64_t>(p); }
 inline int elem_bytes(int dtype) { return feat_elem_bytes(dtype); }
+
+// a = sigmoid(g) and 1 - a, each to a few units in its last place: neither is a difference
+__device__ __forceinline__ void sigmoids(float g, float& a, float& rest) {
+  const float e = __builtin_amdgcn_exp2f(-1.44269504f * __builtin_fabsf(g));
+  const float r = __builtin_amdgcn_rcpf(1.f + e);
+  const float small = e * r;
+  a = g < 0.f ? small : r;  // NaN: r, which is NaN
+  rest = g < 0.f ? r : small;
+}
 
 template <int L>
 __device__ __forceinline__ float group_sum(float x) {  // over groups of L <= 64 neighbouring lanes

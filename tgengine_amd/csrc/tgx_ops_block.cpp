@@ -119,9 +119,161 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& x_in, const Tensor& gate_in,
   return {out[0], out[1]};
 }
 
+// ------------------------------------------------------------------ residual norm
+// the operator's tensors; those left out are undefined
+struct Res {
+  Tensor x, residual, gate, weight, bias, scale, post;
+  bool parts() const { return gate.defined() || scale.defined() || post.defined(); }
+};
+
+void check_residual_norm(const Res& t) {
+  on_gpu(t.x, "residual_norm: x");
+  if (t.x.dim() < 1 || t.x.size(-1) < 1) bad("residual_norm: x must have a last dimension of 1 or more");
+  dtype_of(t.x, "residual_norm: x");
+  for (const Tensor* r : {&t.residual, &t.gate}) {
+    if (!r->defined()) continue;
+    if (r->sizes() != t.x.sizes()) bad("residual_norm: residual and gate must have the shape of x");
+    if (r->scalar_type() != t.x.scalar_type()) bad("residual_norm: x, residual and gate must have the same dtype");
+    same_device(*r, t.x, "residual_norm: residual and gate");
+  }
+  const Tensor* first = nullptr;
+  for (const Tensor* w : {&t.weight, &t.bias, &t.scale, &t.post}) {
+    if (!w->defined()) continue;
+    if (w->dim() != 1 || w->size(0) != t.x.size(-1))
+      bad("residual_norm: weight, bias, scale and post_weight must be (dim,)");
+    dtype_of(*w, "residual_norm: weight, bias, scale and post_weight");
+    same_device(*w, t.x, "residual_norm: weight, bias, scale and post_weight");
+    if (first != nullptr && first->scalar_type() != w->scalar_type())
+      bad("residual_norm: weight, bias, scale and post_weight must have the same dtype");
+    first = w;
+  }
+}
+
+// the arguments, and the contiguous copies that they point to
+struct ResCall {
+  Res t;
+  tgx_residual_norm_args a{};
+  ResCall(const Res& in, bool center, double eps) {
+    int64_t rows = 0;
+    a.dim = in.x.size(-1);
+    t.x = as_rows(in.x, a.rows, a.x_stride);
+    if (in.residual.defined()) t.residual = as_rows(in.residual, rows, a.residual_stride);
+    if (in.gate.defined()) t.gate = as_rows(in.gate, rows, a.gate_stride);
+    a.dtype = a.wdtype = dtype_of(in.x, "residual_norm: x");
+    const Tensor* from[] = {&in.weight, &in.bias, &in.scale, &in.post};
+    Tensor* to[] = {&t.weight, &t.bias, &t.scale, &t.post};
+    for (int i = 0; i < 4; ++i) {
+      if (!from[i]->defined()) continue;
+      *to[i] = from[i]->contiguous();
+      a.wdtype = dtype_of(*to[i], "residual_norm: weight");
+    }
+    a.x = t.x.data_ptr();
+    a.residual = ptr(t.residual);
+    a.gate = ptr(t.gate);
+    a.weight = ptr(t.weight);
+    a.bias = ptr(t.bias);
+    a.scale = ptr(t.scale);
+    a.post_weight = ptr(t.post);
+    a.center = center;
+    a.eps = static_cast<float>(eps);
+  }
+};
+
+// {y, sum}; stats: what a gradient needs
+variable_list residual_norm_out(const Res& t, bool center, double eps, Tensor* stats) {
+  ResCall c(t, center, eps);
+  Tensor out = at::empty(t.x.sizes(), t.x.options()), sum = at::empty(t.x.sizes(), t.x.options());
+  if (stats != nullptr) *stats = at::empty({t.post.defined() ? 4 : 2, c.a.rows}, t.x.options().dtype(at::kFloat));
+  c.a.out = out.data_ptr();
+  c.a.sum = sum.data_ptr();
+  c.a.stats = stats != nullptr ? stats->data_ptr<float>() : nullptr;
+  check(tgx_residual_norm(&c.a, stream_of(t.x)), "tgx_residual_norm");
+  return {out, sum};
+}
+
+class ResidualNorm : public torch::autograd::Function<ResidualNorm> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual, const OptTensor& weight,
+                               const OptTensor& bias, const OptTensor& gate, const OptTensor& scale,
+                               const OptTensor& post, bool center, double eps) {
+    const c10::OptionalDeviceGuard guard(x.device());
+    const Res t{x, residual, gate.value_or(Tensor()), weight.value_or(Tensor()), bias.value_or(Tensor()),
+                scale.value_or(Tensor()), post.value_or(Tensor())};
+    Tensor stats;
+    variable_list out = residual_norm_out(t, center, eps, &stats);
+    // an f32 sum is not rounded: alone it gives all that x and residual would
+    const bool whole = !t.parts() && x.scalar_type() == at::kFloat;
+    ctx->save_for_backward({whole ? out[1] : x, whole ? Tensor() : residual, t.weight, t.bias, t.gate, t.scale, t.post, stats});
+    ctx->saved_data["center"] = center;
+    ctx->saved_data["eps"] = eps;
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    only_once("residual_norm");
+    variable_list d(9);
+    if (!grads[0].defined() && !grads[1].defined()) return d;
+    const variable_list saved = ctx->get_saved_variables();
+    const Res t{saved[0], saved[1], saved[4], saved[2], saved[3], saved[5], saved[6]};
+    const c10::OptionalDeviceGuard guard(t.x.device());
+    ResCall c(t, ctx->saved_data["center"].toBool(), ctx->saved_data["eps"].toDouble());
+    const Tensor g = grads[0].defined() ? grads[0].contiguous() : Tensor();
+    const Tensor gs = grads[1].defined() ? grads[1].contiguous() : Tensor();
+    c.a.grad_out = ptr(g);
+    c.a.grad_sum = ptr(gs);
+    c.a.stats = saved[7].data_ptr<float>();
+    // inputs are counted without those left out
+    const Tensor* in[] = {&t.weight, &t.bias, &t.gate, &t.scale, &t.post};
+    void** to[] = {&c.a.grad_weight, &c.a.grad_bias, &c.a.grad_gate, &c.a.grad_scale, &c.a.grad_post_weight};
+    const bool wx = ctx->needs_input_grad(0), wr = ctx->needs_input_grad(1);
+    bool sums = false;
+    for (size_t i = 0, at = 2; i < 5; ++i) {
+      if (!in[i]->defined()) continue;
+      if (ctx->needs_input_grad(at++)) {
+        d[2 + i] = at::empty(in[i]->sizes(), in[i]->options());
+        *to[i] = d[2 + i].data_ptr();
+        sums |= i != 2;
+      }
+    }
+    if (wr || (wx && !t.parts())) d[1] = at::empty(t.x.sizes(), t.x.options());
+    if (wx && t.parts()) d[0] = at::empty(t.x.sizes(), t.x.options());
+    c.a.grad_residual = ptr(d[1]);
+    c.a.grad_x = ptr(d[0]);
+    Tensor ws;
+    if (sums) ws = workspace(tgx_residual_norm_grad_workspace_size(&c.a), t.x);
+    c.a.workspace = ptr(ws);
+    c.a.workspace_bytes = ws.defined() ? ws.numel() : 0;
+    check(tgx_residual_norm_grad(&c.a, stream_of(t.x)), "tgx_residual_norm_grad");
+    if (wx && !t.parts()) d[0] = d[1];
+    if (!wr) d[1] = Tensor();
+    return d;
+  }
+};
+
+std::tuple<Tensor, Tensor> residual_norm(const Tensor& x, const Tensor& residual, const OptTensor& weight,
+                                         const OptTensor& bias, const OptTensor& gate, const OptTensor& scale,
+                                         const OptTensor& post, bool center, double eps) {
+  const Res t{x, residual, gate.value_or(Tensor()), weight.value_or(Tensor()), bias.value_or(Tensor()),
+              scale.value_or(Tensor()), post.value_or(Tensor())};
+  check_residual_norm(t);
+  const std::initializer_list<const Tensor*> all = {&t.x, &t.residual, &t.weight, &t.bias, &t.gate, &t.scale, &t.post};
+  reverse_mode_only("residual_norm", all);
+  variable_list out;
+  if (keeps_grad(all)) {
+    out = ResidualNorm::apply(x, residual, weight, bias, gate, scale, post, center, eps);
+  } else {
+    const c10::OptionalDeviceGuard guard(x.device());
+    out = residual_norm_out(t, center, eps, nullptr);
+  }
+  return {out[0], out[1]};
+}
+
 }  // namespace
 
 void bind_block_ops(py::module_& m) {
   m.def("gated_scan", &gated_scan, py::arg("x"), py::arg("gate"), py::arg("mask") = py::none(),
         py::arg("state") = py::none());
+  m.def("residual_norm", &residual_norm, py::arg("x"), py::arg("residual"), py::arg("weight") = py::none(),
+        py::arg("bias") = py::none(), py::arg("gate") = py::none(), py::arg("scale") = py::none(),
+        py::arg("post_weight") = py::none(), py::arg("center") = true, py::arg("eps") = 1e-5);
 }

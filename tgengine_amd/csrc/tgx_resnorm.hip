@@ -1,0 +1,127 @@
+// The residual sum after a block and the norm before the next one, forward.
+//
+//   n = x, or with post the block's own norm: (x - mx) rx post
+//   s = residual + scale sigmoid(gate) n          (a factor that is left out is 1)
+//   y = (s - m) r weight + bias
+//
+// m is the mean of a row and r = 1 / sqrt(mean (s - m)^2 + eps); rows that are not centred
+// take m = 0.  L lanes share a row and hold it in registers as C packs each, so that x,
+// residual and gate are read once and the norm works on the sum before it is rounded: s and
+// y are rounded once each.  Statistics and sums are of 32 bits.
+#include "tgx_resnorm.h"
+
+namespace tgx {
+namespace {
+
+template <typename T, typename W, int V, int L, int C, bool PARTS>
+__global__ __launch_bounds__(res_threads(L)) void resnorm_fwd(const ResArgs a) {
+  constexpr int N = res_threads(L), G = N / L;
+  __shared__ float lds[N / kWave];
+  const Place<V, L> at(a.dim);
+  const int64_t mine = static_cast<int64_t>(blockIdx.x) * G + threadIdx.x / L;
+  const int64_t row = min(mine, a.rows - 1);
+  Pack<T, V> px[C], pr[C], pg[C];
+#pragma unroll
+  for (int j = 0; j < C; ++j) {
+    px[j] = load_pack<T, V>(static_cast<const T*>(a.x) + row * a.x_stride + at.at(j));
+    pr[j] = load_pack<T, V>(static_cast<const T*>(a.residual) + row * a.residual_stride + at.at(j));
+    if constexpr (PARTS)
+      if (a.gate != nullptr) pg[j] = load_pack<T, V>(static_cast<const T*>(a.gate) + row * a.gate_stride + at.at(j));
+  }
+  float s[C][V];
+#pragma unroll
+  for (int j = 0; j < C; ++j)
+#pragma unroll
+    for (int u = 0; u < V; ++u) s[j][u] = to_f(px[j].v[u]);
+  float mx = 0.f, rx = 0.f;
+  if constexpr (PARTS) {
+    if (a.post != nullptr) {
+      row_stats<V, L, C>(s, at, a, lds, mx, rx);
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        const Pack<W, V> w = load_pack<W, V>(static_cast<const W*>(a.post) + at.at(j));
+#pragma unroll
+        for (int u = 0; u < V; ++u) s[j][u] = (s[j][u] - mx) * rx * to_f(w.v[u]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      Pack<W, V> w;
+      if (a.scale != nullptr) w = load_pack<W, V>(static_cast<const W*>(a.scale) + at.at(j));
+#pragma unroll
+      for (int u = 0; u < V; ++u) {
+        float by = a.scale != nullptr ? to_f(w.v[u]) : 1.f;
+        if (a.gate != nullptr) {
+          float f, rest;
+          sigmoids(to_f(pg[j].v[u]), f, rest);
+          by *= f;
+        }
+        s[j][u] = fmaf(by, s[j][u], to_f(pr[j].v[u]));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < C; ++j)
+#pragma unroll
+      for (int u = 0; u < V; ++u) s[j][u] += to_f(pr[j].v[u]);
+  }
+  float m, r;
+  row_stats<V, L, C>(s, at, a, lds, m, r);
+  if (mine >= a.rows) return;
+#pragma unroll
+  for (int j = 0; j < C; ++j) {
+    if (at.skip(j) == V) continue;
+    const int c = at.at(j);
+    Pack<W, V> w, b;
+    if (a.weight != nullptr) w = load_pack<W, V>(static_cast<const W*>(a.weight) + c);
+    if (a.bias != nullptr) b = load_pack<W, V>(static_cast<const W*>(a.bias) + c);
+    Pack<T, V> o, t;
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+      float y = (s[j][u] - m) * r;
+      if (a.weight != nullptr) y *= to_f(w.v[u]);
+      if (a.bias != nullptr) y += to_f(b.v[u]);
+      o.v[u] = from_f<T>(y);
+      t.v[u] = from_f<T>(s[j][u]);
+    }
+    store_pack<T, V>(static_cast<T*>(a.out) + row * a.dim + c, o);
+    store_pack<T, V>(static_cast<T*>(a.sum) + row * a.dim + c, t);
+  }
+  if (at.lane == 0 && a.stats != nullptr) {
+    a.stats[row] = m;
+    a.stats[a.rows + row] = r;
+    if (PARTS && a.post != nullptr) {
+      a.stats[2 * a.rows + row] = mx;
+      a.stats[3 * a.rows + row] = rx;
+    }
+  }
+}
+
+}  // namespace
+}  // namespace tgx
+
+using namespace tgx;
+
+extern "C" int tgx_residual_norm(const tgx_residual_norm_args* args, void* stream) {
+  if (const int rc = check_resnorm("tgx_residual_norm", args, false)) return rc;
+  if (args->rows == 0) return TGX_OK;
+  if (args->out == nullptr || args->sum == nullptr)
+    return fail(TGX_ERR_ARG, "tgx_residual_norm: out and sum must not be NULL");
+  return by_type(args->dtype, [&](auto t) {
+    using T = decltype(t);
+    return by_type(args->wdtype, [&](auto wt) {
+      using W = decltype(wt);
+      return res_shape<T>(args->dim, [&](auto v, auto l, auto c) {
+        constexpr int V = decltype(v)::value, L = decltype(l)::value, C = decltype(c)::value, N = res_threads(L);
+        const int64_t blocks = ops_cdiv(args->rows, N / L);
+        if (const int e = check_grid("tgx_residual_norm", blocks, N)) return e;
+        const dim3 grid(static_cast<unsigned>(blocks)), block(N);
+        if (has_parts(args))
+          hipLaunchKernelGGL((resnorm_fwd<T, W, V, L, C, true>), grid, block, 0, static_cast<hipStream_t>(stream), res_args(args));
+        else
+          hipLaunchKernelGGL((resnorm_fwd<T, W, V, L, C, false>), grid, block, 0, static_cast<hipStream_t>(stream), res_args(args));
+        return check_launch("resnorm_fwd");
+      });
+    });
+  });
+}

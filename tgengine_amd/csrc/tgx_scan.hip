@@ -46,15 +46,6 @@ struct ScanArgs {
   int32_t dim, per;  // per: tokens a piece, whole spans
 };
 
-// a = sigmoid(g) and 1 - a, each to a few units in its last place: neither is a difference
-__device__ __forceinline__ void sigmoids(float g, float& a, float& rest) {
-  const float e = __builtin_amdgcn_exp2f(-1.44269504f * __builtin_fabsf(g));
-  const float r = __builtin_amdgcn_rcpf(1.f + e);
-  const float small = e * r;
-  a = g < 0.f ? small : r;  // NaN: r, which is NaN
-  rest = g < 0.f ? r : small;
-}
-
 // which thread does what
 template <int V>
 struct Part {

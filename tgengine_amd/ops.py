@@ -74,6 +74,23 @@ def gated_scan(x: Tensor, gate: Tensor, mask: Optional[Tensor] = None,
     return _host().gated_scan(x, gate, mask, state)
 
 
+def residual_norm(x: Tensor, residual: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, *,
+                  gate: Optional[Tensor] = None, scale: Optional[Tensor] = None, post_weight: Optional[Tensor] = None,
+                  center: bool = True, eps: float = 1e-5) -> Tuple[Tensor, Tensor]:
+    """The residual sum after a block and the norm before the next one, in one pass.
+
+    x is the block's output and residual what ran past it, of one shape and dtype.
+    Returns (y, sum) with sum = residual + scale * sigmoid(gate) * n and
+    y = norm(sum) * weight + bias.  n is x, or norm(x) * post_weight where the block
+    ends with a norm of its own; gate has x's shape and scale, like weight, bias and
+    post_weight, is (dim,); what is left out is not there.  norm is over the last
+    dimension (1 to 16,384 values): with ``center`` as in ``layer_norm``, without it by
+    the root of the mean square alone.  The four vectors are of one dtype, which may be
+    float32 beside bfloat16 tokens.
+    """
+    return _host().residual_norm(x, residual, weight, bias, gate, scale, post_weight, center, eps)
+
+
 def clip_grad_norm_(grads: Union[Tensor, Iterable[Tensor]], max_norm: float,
                     out: Optional[Sequence[Tensor]] = None) -> Tensor:
     """Scales gradients by min(1, max_norm / (norm + 1e-6)) and returns ``norm``, the
