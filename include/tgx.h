@@ -622,6 +622,50 @@ int tgx_residual_norm(const tgx_residual_norm_args* args, void* stream);
 size_t tgx_residual_norm_grad_workspace_size(const tgx_residual_norm_args* args);
 int tgx_residual_norm_grad(const tgx_residual_norm_args* args, void* stream);
 
+/* One AdamW step over `count` tensors: t = *step + 1 is written back,
+ *   g = grad * min(1, max_norm / (*grad_norm + 1e-6))      (grad_norm NULL: grad)
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *   param = param (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
+ * The table is a host array, read during the call; step, lr_device (in place of lr) and
+ * grad_norm are on the device, so that a captured step counts, and takes a new rate and norm,
+ * at every replay.  bits = 32: exp_avg and exp_avg_sq hold m and v in f32.  bits = 8: m and
+ * sqrt(v) as e4m3 (OCP, with NaN, without infinities) times scales [2][blocks], a power of two
+ * for each TGX_ADAMW_BLOCK values, the last block with what is left; all zeros before the first step.  They are
+ * rounded down or up by a dither of the value's place and t, and a second average above zero stays
+ * so.  Memory that is written may overlap nothing else (TGX_ERR_ARG). */
+#define TGX_ADAMW_BLOCK 256
+typedef struct tgx_adamw_tensor {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* scales;           /* NULL with 32 bits */
+  int64_t* step;           /* one value */
+  int64_t size;            /* values, one after the other */
+  int32_t dtype;
+  int32_t grad_dtype;
+  int32_t bits;
+  int32_t reserved;
+} tgx_adamw_tensor;
+
+typedef struct tgx_adamw_args {
+  const tgx_adamw_tensor* tensors;
+  int64_t count;           /* at most 65535 */
+  double lr;
+  double beta1;
+  double beta2;
+  double eps;
+  double weight_decay;
+  double max_norm;
+  const float* lr_device;  /* NULL: lr */
+  const float* grad_norm;  /* NULL: gradients as they are */
+  void* workspace;         /* tgx_adamw_workspace_size(count) bytes, 16-byte aligned, no initialisation */
+  size_t workspace_bytes;
+} tgx_adamw_args;
+
+size_t tgx_adamw_workspace_size(int64_t count);
+int tgx_adamw(const tgx_adamw_args* args, void* stream);
+
 const char* tgx_last_error(void);
 int tgx_abi_version(void);
 

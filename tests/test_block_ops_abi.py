@@ -12,7 +12,8 @@ from tgengine_amd.core import _lib
 
 ROOT = Path(__file__).resolve().parent.parent
 
-STRUCTS = {"tgx_scan_args": _lib.TgxScanArgs, "tgx_residual_norm_args": _lib.TgxResidualNormArgs}
+STRUCTS = {"tgx_scan_args": _lib.TgxScanArgs, "tgx_residual_norm_args": _lib.TgxResidualNormArgs,
+           "tgx_adamw_tensor": _lib.TgxAdamwTensor, "tgx_adamw_args": _lib.TgxAdamwArgs}
 
 
 def _err():
@@ -96,8 +97,61 @@ def test_residual_norm_checks():
     assert L.tgx_residual_norm_grad_workspace_size(None) == 0 == L.tgx_residual_norm_grad_workspace_size(_res(dim=0))
 
 
+def _tensor(at=0x10000, **more):
+    """A tensor of 300 f32 values whose memory begins at `at`, 4 KB a piece."""
+    t = dict(param=at, grad=at + 0x1000, exp_avg=at + 0x2000, exp_avg_sq=at + 0x3000, scales=at + 0x4000, step=at + 0x5000,
+             size=300, dtype=0, grad_dtype=0, bits=32)
+    return _lib.TgxAdamwTensor(**{**t, **more})
+
+
+def _adamw(*tensors, **more):
+    t = (_lib.TgxAdamwTensor * max(1, len(tensors)))(*tensors)
+    a = _lib.TgxAdamwArgs(tensors=t, count=len(tensors), lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=1e-2)
+    for n, v in more.items():
+        setattr(a, n, v)
+    return _lib.lib().tgx_adamw(ctypes.byref(a), None)
+
+
+def test_adamw_checks():
+    L = _lib.lib()
+    assert L.tgx_adamw(None, None) == 1 and "args is NULL" in _err()
+    assert L.tgx_adamw_workspace_size(0) == 0 and L.tgx_adamw_workspace_size(3) >= 96
+    assert _adamw() == 0 and _adamw(_tensor(), count=-1) == 1
+    assert _adamw(_tensor()) == 1 and "workspace" in _err()
+    for more in (dict(lr=-1.0), dict(lr=float("nan")), dict(beta1=1.0), dict(beta2=-0.1), dict(beta2=float("nan")), dict(eps=-1.0),
+                 dict(weight_decay=float("nan"))):
+        assert _adamw(_tensor(), **more) == 1 and "lr=" in _err()
+    assert _adamw(_tensor(), lr=float("nan"), lr_device=0x90000) == 1 and "workspace" in _err()
+    assert _adamw(_tensor(), grad_norm=0x90000, max_norm=-1.0) == 1 and "max_norm" in _err()
+    for more in (dict(size=-1), dict(param=None), dict(grad=None), dict(exp_avg=None), dict(exp_avg_sq=None), dict(step=None)):
+        assert _adamw(_tensor(), _tensor(0x20000, **more)) == 1 and "tensor 1" in _err()
+    assert _adamw(_tensor(dtype=2)) == 2 and _adamw(_tensor(grad_dtype=-1)) == 2
+    assert _adamw(_tensor(bits=16)) == 1 and "16 bits" in _err()
+    assert _adamw(_tensor(bits=8, scales=None)) == 1 and "scales" in _err()
+    assert _adamw(_tensor(bits=8)) == 1 and "workspace" in _err()
+    assert _adamw(_tensor(size=0, param=None, grad=None, exp_avg=None, exp_avg_sq=None)) == 1 and "workspace" in _err()
+    assert _adamw(_tensor(size=1 << 40)) == 3
+
+
+def test_adamw_refuses_overlaps():
+    """Memory that is written and used for anything else: refused before any launch."""
+    a, b = 0x10000, 0x20000
+    for tensors in ((_tensor(a), _tensor(b, param=a)), (_tensor(a), _tensor(b, step=a + 0x5000)),
+                    (_tensor(a, grad=a),), (_tensor(a, exp_avg_sq=a + 0x2000),), (_tensor(a), _tensor(b, grad=a + 1196)),
+                    (_tensor(a, step=a + 0x1000),), (_tensor(a, bits=8, scales=a + 0x2000 + 296),),
+                    (_tensor(a, bits=8, exp_avg_sq=a + 0x2000 + 299),), (_tensor(a, dtype=1, grad=a + 599),)):
+        assert _adamw(*tensors) == 1 and "overlap" in _err()
+    assert _adamw(_tensor(a), grad_norm=a, max_norm=1.0) == 1 and "overlap" in _err()
+    assert _adamw(_tensor(a), lr_device=a + 0x2000 + 4) == 1 and "overlap" in _err()
+    for tensors in ((_tensor(a), _tensor(b, grad=a + 0x1000)),  # two that share a gradient
+                    (_tensor(a, bits=8, exp_avg_sq=a + 0x2000 + 300),), (_tensor(a, dtype=1, grad=a + 600),),
+                    (_tensor(a), _tensor(b, grad=a + 1200))):
+        assert _adamw(*tensors) == 1 and "workspace" in _err()
+
+
 def test_no_cpu_path():
     x = torch.randn(2, 3, 8)
-    for call in (lambda: ops.gated_scan(x, x), lambda: ops.residual_norm(x, x)):
+    for call in (lambda: ops.gated_scan(x, x), lambda: ops.residual_norm(x, x),
+                 lambda: ops.adamw_([x], [x], [x], [x], [torch.zeros((), dtype=torch.int64)])):
         with pytest.raises(RuntimeError, match="on the GPU"):
             call()

@@ -119,6 +119,22 @@ class TgxResidualNormArgs(ctypes.Structure):
                 ("workspace_bytes", ctypes.c_size_t)]
 
 
+TGX_ADAMW_BLOCK = 256
+
+
+class TgxAdamwTensor(ctypes.Structure):
+    _fields_ = [("param", c_vp), ("grad", c_vp), ("exp_avg", c_vp), ("exp_avg_sq", c_vp), ("scales", c_vp),
+                ("step", c_vp), ("size", c_i64), ("dtype", c_i32), ("grad_dtype", c_i32), ("bits", c_i32),
+                ("reserved", c_i32)]
+
+
+class TgxAdamwArgs(ctypes.Structure):
+    _fields_ = [("tensors", ctypes.POINTER(TgxAdamwTensor)), ("count", c_i64), ("lr", ctypes.c_double),
+                ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
+                ("weight_decay", ctypes.c_double), ("max_norm", ctypes.c_double), ("lr_device", c_vp),
+                ("grad_norm", c_vp), ("workspace", c_vp), ("workspace_bytes", ctypes.c_size_t)]
+
+
 SIGNATURES = {
     "tgx_ring_append": (c_i32, [ctypes.POINTER(TgxRing), c_vp, c_vp, c_vp, c_vp, c_i64, c_i64,
                                 c_vp, ctypes.c_size_t, c_vp, c_vp]),
@@ -181,6 +197,8 @@ SIGNATURES.update({
     "tgx_residual_norm": (c_i32, [ctypes.POINTER(TgxResidualNormArgs), c_vp]),
     "tgx_residual_norm_grad_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(TgxResidualNormArgs)]),
     "tgx_residual_norm_grad": (c_i32, [ctypes.POINTER(TgxResidualNormArgs), c_vp]),
+    "tgx_adamw_workspace_size": (ctypes.c_size_t, [c_i64]),
+    "tgx_adamw": (c_i32, [ctypes.POINTER(TgxAdamwArgs), c_vp]),
 })
 
 _lock = threading.Lock()

@@ -12,6 +12,7 @@
 // 20,000 f32 values take 4.4 and 6.2 us, mostly the launches.  2,048 parts fill the 256
 // compute units with eight workgroups each, and a part is long enough to hide its sum.
 #include "tgx_ops.h"
+#include "tgx_ranges.h"
 
 #include <memory>
 #include <new>
@@ -150,11 +151,6 @@ int64_t part_count(const int64_t* sizes, int64_t count, int64_t per) {
 // written or read for another tensor.  A tensor that is its own output counts as one.
 int check_apart(const void* const* grads, const int32_t* dtypes, void* const* outs, const int32_t* out_dtypes,
                 const int64_t* sizes, int64_t count) {
-  struct Range {
-    uint64_t lo, hi;
-    int64_t tensor;
-    bool out;
-  };
   const std::unique_ptr<Range[]> r(new (std::nothrow) Range[static_cast<size_t>(count) * 2]);
   if (r == nullptr) return fail(TGX_ERR_LIMIT, "tgx_clip_grad_norm: no memory to check %lld tensors", static_cast<long long>(count));
   int64_t n = 0;
@@ -164,17 +160,10 @@ int check_apart(const void* const* grads, const int32_t* dtypes, void* const* ou
     if (grads[i] != outs[i])
       r[n++] = {addr(grads[i]), addr(grads[i]) + static_cast<uint64_t>(sizes[i]) * elem_bytes(dtypes[i]), i, false};
   }
-  std::sort(r.get(), r.get() + n, [](const Range& x, const Range& y) { return x.lo < y.lo; });
-  const Range *any = nullptr, *out = nullptr;  // of those before, the one that reaches farthest
-  for (int64_t i = 0; i < n; ++i) {
-    const Range* before = r[i].out ? any : out;
-    if (before != nullptr && before->hi > r[i].lo)
-      return fail(TGX_ERR_ARG, "tgx_clip_grad_norm: tensors %lld and %lld overlap (an output may be its own gradient only)",
-                  static_cast<long long>(std::min(before->tensor, r[i].tensor)),
-                  static_cast<long long>(std::max(before->tensor, r[i].tensor)));
-    if (any == nullptr || r[i].hi > any->hi) any = &r[i];
-    if (r[i].out && (out == nullptr || r[i].hi > out->hi)) out = &r[i];
-  }
+  int64_t one, other;
+  if (overlap(r.get(), n, one, other))
+    return fail(TGX_ERR_ARG, "tgx_clip_grad_norm: tensors %lld and %lld overlap (an output may be its own gradient only)",
+                static_cast<long long>(one), static_cast<long long>(other));
   return TGX_OK;
 }
 

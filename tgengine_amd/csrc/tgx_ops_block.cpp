@@ -268,9 +268,90 @@ std::tuple<Tensor, Tensor> residual_norm(const Tensor& x, const Tensor& residual
   return {out[0], out[1]};
 }
 
+// ------------------------------------------------------------------ AdamW
+void adamw(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& exp_avg,
+           const std::vector<Tensor>& exp_avg_sq, const std::vector<Tensor>& steps, const std::vector<OptTensor>& scales,
+           double lr, const OptTensor& lr_in, double beta1, double beta2, double eps, double weight_decay,
+           const OptTensor& norm_in, double max_norm) {
+  const size_t n = params.size();
+  if (n == 0) bad("adamw_: no parameters");
+  if (grads.size() != n || exp_avg.size() != n || exp_avg_sq.size() != n || steps.size() != n || (!scales.empty() && scales.size() != n))
+    bad("adamw_: every list must have one tensor per parameter");
+  std::vector<tgx_adamw_tensor> table(n);
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor &p = params[i], &g = grads[i], &m = exp_avg[i], &v = exp_avg_sq[i], &t = steps[i];
+    reverse_mode_only("adamw_", {&p, &g});
+    on_gpu(p, "adamw_: parameters");
+    if (p.requires_grad() && !p.is_leaf() && at::GradMode::is_enabled())
+      bad("adamw_: parameters must be leaves, or gradients switched off");
+    for (const Tensor* x : {&p, &g, &m, &v, &t}) {
+      same_device(*x, params[0], "adamw_: every tensor");
+      if (!x->is_contiguous()) bad("adamw_: every tensor must be contiguous");
+    }
+    for (const Tensor* x : {&g, &m, &v})
+      if (x->sizes() != p.sizes()) bad("adamw_: gradients and averages must have their parameters' shapes");
+    if (t.scalar_type() != at::kLong || t.numel() != 1) bad("adamw_: steps must be int64 of one value");
+    if (m.scalar_type() != v.scalar_type() || (m.scalar_type() != at::kFloat && m.scalar_type() != at::kFloat8_e4m3fn))
+      bad("adamw_: the averages must be both float32 or both float8_e4m3fn");
+    const bool held = m.scalar_type() != at::kFloat;
+    tgx_adamw_tensor& a = table[i];
+    if (held) {
+      const Tensor s = scales.empty() ? Tensor() : scales[i].value_or(Tensor());
+      const int64_t blocks = (p.numel() + TGX_ADAMW_BLOCK - 1) / TGX_ADAMW_BLOCK;
+      if (!s.defined() || s.scalar_type() != at::kFloat || s.dim() != 2 || s.size(0) != 2 || s.size(1) != blocks ||
+          !s.is_contiguous())
+        bad("adamw_: 8-bit averages need scales, float32 (2, " + std::to_string(blocks) + ")");
+      same_device(s, params[0], "adamw_: every tensor");
+      a.scales = s.data_ptr<float>();
+    }
+    a.param = p.data_ptr();
+    a.grad = g.data_ptr();
+    a.exp_avg = m.data_ptr();
+    a.exp_avg_sq = v.data_ptr();
+    a.step = t.data_ptr<int64_t>();
+    a.size = p.numel();
+    a.dtype = dtype_of(p, "adamw_: parameters");
+    a.grad_dtype = dtype_of(g, "adamw_: gradients");
+    a.bits = held ? 8 : 32;
+  }
+  tgx_adamw_args a{};
+  a.tensors = table.data();
+  a.count = static_cast<int64_t>(n);
+  a.lr = lr;
+  a.beta1 = beta1;
+  a.beta2 = beta2;
+  a.eps = eps;
+  a.weight_decay = weight_decay;
+  a.max_norm = max_norm;
+  const Tensor rate = lr_in.value_or(Tensor()), norm = norm_in.value_or(Tensor());
+  for (const Tensor* x : {&rate, &norm}) {
+    if (!x->defined()) continue;
+    if (x->scalar_type() != at::kFloat || x->numel() != 1) bad("adamw_: lr and grad_norm must be float32 of one value");
+    same_device(*x, params[0], "adamw_: every tensor");
+  }
+  a.lr_device = static_cast<const float*>(ptr(rate));
+  a.grad_norm = static_cast<const float*>(ptr(norm));
+  const c10::OptionalDeviceGuard guard(params[0].device());
+  const Tensor ws = workspace(tgx_adamw_workspace_size(a.count), params[0]);
+  a.workspace = ptr(ws);
+  a.workspace_bytes = ws.numel();
+  const int rc = tgx_adamw(&a, stream_of(params[0]));
+  if (rc == TGX_ERR_ARG) bad(tgx_last_error());  // constants out of range, tensors that overlap
+  check(rc, "tgx_adamw");
+  // written behind torch's back: what autograd saved of them is stale
+  auto written = [](const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  };
+  for (size_t i = 0; i < n; ++i) {
+    for (const std::vector<Tensor>* l : {&params, &exp_avg, &exp_avg_sq, &steps}) written((*l)[i]);
+    if (table[i].bits == 8) written(*scales[i]);
+  }
+}
+
 }  // namespace
 
 void bind_block_ops(py::module_& m) {
+  m.def("adamw", &adamw);
   m.def("gated_scan", &gated_scan, py::arg("x"), py::arg("gate"), py::arg("mask") = py::none(),
         py::arg("state") = py::none());
   m.def("residual_norm", &residual_norm, py::arg("x"), py::arg("residual"), py::arg("weight") = py::none(),

@@ -8,11 +8,16 @@ What a model does with the neighbours that ``DataPipeline.prepare`` gathers:
   weight and bias.
 * ``cross_attention``: query tokens to the states of another sequence under
   ``NeighborData.mask``, from one query per node to long sequences on both sides.
+* ``gated_scan``: a gated recurrence along the same tokens under the same mask, from a
+  node's state and to it, from one new token to long histories.
+* ``residual_norm``: the residual sum after a block, with the block's own norm, gate and
+  scale, and the norm before the next one.
 * ``clip_grad_norm_``: the global norm of all gradients, and clipping by it.
+* ``adamw_`` and ``AdamW``: a step over all parameters, averages in 32 bits or 8.
 
 Tensors are float32 or bfloat16 on the GPU; sums and statistics are held in 32
 bits.  Every call launches on the caller's current stream and does not wait for
-the device; the same inputs give the same bits.  The first three take part in
+the device; the same inputs give the same bits.  The first five take part in
 autograd (once: their backward passes leave no graph; forward-mode derivatives and
 tracing are refused).  There is no CPU path.
 """
@@ -113,3 +118,88 @@ def clip_grad_norm_(grads: Union[Tensor, Iterable[Tensor]], max_norm: float,
     elif any(g is None for g in grads):
         raise ValueError("clip_grad_norm_: out needs a gradient for each of its tensors")
     return _host().clip_grad_norm(grads, max_norm, [] if out is None else list(out))
+
+
+def adamw_(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Sequence[Tensor], exp_avg_sq: Sequence[Tensor],
+           steps: Sequence[Tensor], *, lr: Union[float, Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
+           eps: float = 1e-8, weight_decay: float = 1e-2, scales: Optional[Sequence[Optional[Tensor]]] = None,
+           grad_norm: Optional[Tensor] = None, max_norm: Optional[float] = None) -> None:
+    """One AdamW step over all tensors together, in place.
+
+    Every list has one contiguous tensor per parameter; ``AdamW`` keeps them.  exp_avg and
+    exp_avg_sq are both float32 and hold the averages of the gradients and of their
+    squares, or both float8_e4m3fn and hold the first and the square root of the second
+    in units of ``scales``: float32 (2, blocks), a power of two for every 256 values.
+    All of them are zeros before the first step.  steps are int64 of one value and
+    counted on the device, so that a step captured in a graph counts at every replay; lr
+    may be a float32 tensor on the device for the same reason.
+
+    With ``grad_norm``, the float32 scalar that ``clip_grad_norm_`` returns, the gradients
+    are scaled by min(1, max_norm / (grad_norm + 1e-6)) as they are read:
+    ``clip_grad_norm_(grads, float("inf"))`` takes the norm and writes nothing else.
+    """
+    if (grad_norm is None) != (max_norm is None):
+        raise ValueError("adamw_: grad_norm and max_norm come together")
+    rate = lr if isinstance(lr, Tensor) and lr.is_cuda else None
+    _host().adamw(list(params), list(grads), list(exp_avg), list(exp_avg_sq), list(steps),
+                  [] if scales is None else list(scales), 0.0 if rate is not None else float(lr), rate, betas[0], betas[1],
+                  eps, weight_decay, grad_norm, 0.0 if max_norm is None else max_norm)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW over all parameters of a group in one step of kernels (``adamw_``).
+
+    ``bits=8`` keeps both averages in 8 bits a value (and a scale for every 256), for
+    tensors of 4,096 values or more; smaller ones stay in 32 bits, which cost nothing.
+    ``step`` takes the norm of ``clip_grad_norm_`` and a max_norm, to clip without writing
+    the gradients.  A step can be captured in a graph once every parameter has taken one
+    outside.  Parameters without a gradient are left out of a step.
+    """
+
+    def __init__(self, params, lr: Union[float, Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
+                 eps: float = 1e-8, weight_decay: float = 1e-2, bits: int = 32):
+        if not (float(lr) >= 0.0 and eps >= 0.0 and weight_decay >= 0.0 and all(0.0 <= b < 1.0 for b in betas)):
+            raise ValueError(f"AdamW: lr={float(lr)} betas={betas} eps={eps} weight_decay={weight_decay}")
+        if bits not in (8, 32):
+            raise ValueError("AdamW: bits must be 8 or 32")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, bits=bits))
+
+    def _new(self, p: Tensor, bits: int) -> dict:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: a parameter's first step cannot be captured: its averages would start again at every replay")
+        held = bits == 8 and p.numel() >= 4096
+        kind = dict(dtype=torch.float8_e4m3fn if held else torch.float32, device=p.device)
+        out = {"step": torch.zeros((), dtype=torch.int64, device=p.device),
+               "exp_avg": torch.zeros(p.shape, **kind), "exp_avg_sq": torch.zeros(p.shape, **kind)}
+        if held:
+            out["scales"] = torch.zeros(2, -(-p.numel() // 256), device=p.device)
+        return out
+
+    @torch.no_grad()
+    def step(self, closure=None, *, grad_norm: Optional[Tensor] = None, max_norm: Optional[float] = None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            params = [p for p in group["params"] if p.grad is not None]
+            if not params:
+                continue
+            for p in params:
+                if not self.state[p]:
+                    self.state[p].update(self._new(p, group["bits"]))
+            states = [self.state[p] for p in params]
+            adamw_(params, [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p in params],
+                   [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states], [s["step"] for s in states],
+                   lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
+                   scales=[s.get("scales") for s in states], grad_norm=grad_norm, max_norm=max_norm)
+        return loss
+
+    def load_state_dict(self, state_dict) -> None:
+        super().load_state_dict(state_dict)
+        # the averages keep their own types, whatever their parameters' are
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(ids, params):
+            if i in state_dict["state"]:
+                self.state[p] = {k: v.to(p.device, copy=True) for k, v in state_dict["state"][i].items()}
