@@ -33,7 +33,11 @@ constexpr int kAdamThreads = 256;
 constexpr int kBlock = TGX_ADAMW_BLOCK;
 constexpr int kVals = 4;            // a lane's share of a block
 constexpr int kList = 56;           // tensors per launch: their table stays below the 4 KB of kernel arguments
-constexpr int64_t kMostParts = 2048;  // parts of all tensors together, about
+// Parts of all tensors together, about.  Short parts keep the bytes that are in flight beside
+// each other: a table of 100,000,000 bf16 values with 32-bit averages takes 403 us in 131,072
+// parts, 424 in 16,384 and 597 in 2,048; one of 172,000,000 f32 values with 8-bit ones 536 in
+// 65,536, 555 in 16,384 and 580 in 262,144, where no wavefront has a next block to load.
+constexpr int64_t kMostParts[2] = {131072, 65536};  // 32 bits, 8
 static_assert(kBlock == kWave * kVals, "a wavefront takes a block");
 
 struct AdamList {
@@ -100,21 +104,34 @@ __device__ __forceinline__ int adam_tensor(const AdamList& l, uint32_t block) {
   return lo;
 }
 
-// n <= kVals values from p on, the others 0
+// the first n of kVals values from p on, the others 0
 template <typename T>
-__device__ __forceinline__ Pack<T, kVals> load_some(const T* p, int n) {
-  if (n == kVals) return load_pack<T, kVals>(p);
-  Pack<T, kVals> x;
+__device__ __forceinline__ Pack<std::remove_const_t<T>, kVals> load_some(T* p, int n) {
+  Pack<std::remove_const_t<T>, kVals> x;
 #pragma unroll
-  for (int u = 0; u < kVals; ++u) x.v[u] = u < n ? p[u] : static_cast<T>(0.f);
+  for (int u = 0; u < kVals; ++u) x.v[u] = u < n ? p[u] : static_cast<std::remove_const_t<T>>(0.f);
   return x;
 }
 template <typename T>
 __device__ __forceinline__ void store_some(T* p, const Pack<T, kVals>& x, int n) {
-  if (n == kVals) return store_pack<T, kVals>(p, x);
 #pragma unroll
   for (int u = 0; u < kVals; ++u)
     if (u < n) p[u] = x.v[u];
+}
+
+// kVals values that nothing reads again before the caches have forgotten them.  Loads and
+// stores that both say so take the step of a table with 32-bit averages from 409 us to 373
+// (stores alone 410, loads alone 420), with 8-bit ones from 539 to 537.
+template <typename T>
+using Words = uint32_t __attribute__((ext_vector_type(sizeof(T) * kVals / 4), aligned(sizeof(T))));
+template <typename T>
+__device__ __forceinline__ Pack<std::remove_const_t<T>, kVals> load_once(T* p) {
+  const Words<T> w = __builtin_nontemporal_load(reinterpret_cast<const Words<T>*>(p));
+  return __builtin_bit_cast(Pack<std::remove_const_t<T>, kVals>, w);
+}
+template <typename T>
+__device__ __forceinline__ void store_once(T* p, const Pack<T, kVals>& x) {
+  __builtin_nontemporal_store(__builtin_bit_cast(Words<T>, x), reinterpret_cast<Words<T>*>(p));
 }
 
 __device__ __forceinline__ float stepped(float p, float m, float root, const Factors& f, float eps) {
@@ -127,90 +144,165 @@ __device__ __forceinline__ void adam_wide(P* __restrict__ p, const G* __restrict
                                           const Constants& c) {
   const float b1 = static_cast<float>(c.b1), b2 = static_cast<float>(c.b2);
   const float c1 = static_cast<float>(c.c1), c2 = static_cast<float>(c.c2);
-  for (int64_t i = lo + static_cast<int64_t>(threadIdx.x) * kVals; i < hi; i += kAdamThreads * kVals) {
-    const int n = static_cast<int>(min(hi - i, static_cast<int64_t>(kVals)));
-    Pack<P, kVals> pp = load_some(p + i, n);
-    const Pack<G, kVals> pg = load_some(g + i, n);
-    Pack<float, kVals> pm = load_some(m + i, n), pv = load_some(v + i, n);
+  auto one = [&](P& p, G g, float& m, float& v) {
+    const float d = to_f(g) * f.clip_f;
+    m = b1 * m + c1 * d;
+    v = b2 * v + c2 * d * d;
+    p = from_f<P>(stepped(to_f(p), m, sqrtf(v), f, c.eps));
+  };
+  const int64_t full = lo + (hi - lo) / kVals * kVals;
+  for (int64_t i = lo + static_cast<int64_t>(threadIdx.x) * kVals; i < full; i += kAdamThreads * kVals) {
+    Pack<P, kVals> pp = load_once(p + i);
+    const Pack<G, kVals> pg = load_once(g + i);
+    Pack<float, kVals> pm = load_once(m + i), pv = load_once(v + i);
 #pragma unroll
-    for (int u = 0; u < kVals; ++u) {
-      const float d = to_f(pg.v[u]) * f.clip_f;
-      pm.v[u] = b1 * pm.v[u] + c1 * d;
-      pv.v[u] = b2 * pv.v[u] + c2 * d * d;
-      pp.v[u] = from_f<P>(stepped(to_f(pp.v[u]), pm.v[u], sqrtf(pv.v[u]), f, c.eps));
-    }
-    store_some(p + i, pp, n);
-    store_some(m + i, pm, n);
-    store_some(v + i, pv, n);
+    for (int u = 0; u < kVals; ++u) one(pp.v[u], pg.v[u], pm.v[u], pv.v[u]);
+    store_once(p + i, pp);
+    store_once(m + i, pm);
+    store_once(v + i, pv);
   }
+  const int64_t i = full + threadIdx.x;
+  if (i < hi) one(p[i], g[i], m[i], v[i]);
 }
 
-__device__ __forceinline__ int exponent(double x) {  // of a value that is not 0: floor(log2 |x|)
-  return static_cast<int>((__double_as_longlong(x) >> 52) & 0x7ff) - 1023;
-}
 __device__ __forceinline__ double power(int k) { return __longlong_as_double(static_cast<int64_t>(k + 1023) << 52); }
-constexpr int kNotFinite = 1024;  // the exponent of infinities and NaN
+__device__ __forceinline__ uint32_t high(double x) { return static_cast<uint32_t>(__double_as_longlong(x) >> 32) & 0x7fffffffu; }
+constexpr uint32_t kNotFinite = 0x7ff00000u;  // the high word of infinity
 
-// the exponent of a block's power of two; e: of the lane's largest finite value
-__device__ __forceinline__ int block_power(int e) {
-#pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) e = max(e, __shfl_xor(e, off, kWave));
-  return max(e - 7, -126);
+// the largest x of the wavefront, the same in every lane
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+#define TGX_MAX(ctrl, rows) \
+  x = max(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), ctrl, rows, 0xf, false)))
+  TGX_MAX(0x111, 0xf);  // lanes 1, 2, 4 and 8 before, in rows of 16
+  TGX_MAX(0x112, 0xf);
+  TGX_MAX(0x114, 0xf);
+  TGX_MAX(0x118, 0xf);
+  TGX_MAX(0x142, 0xa);  // the last lane of a row to the next one
+  TGX_MAX(0x143, 0xc);  // and of the first half to the second
+#undef TGX_MAX
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), kWave - 1));
 }
 
-// the e4m3 code of |x| / 2^k, below 256, by the dither w / 2^32
-__device__ __forceinline__ uint32_t code(double x, int k, uint32_t w, bool above) {
-  const int e = exponent(x);
-  if (e == kNotFinite) return 0x7f;
-  const int top = max(e - k, -6);  // the binade; its spacing is 2^(top - 3)
-  const double y = fabs(x) * power(3 - top - k) + static_cast<double>(w) * 0x1p-32;
-  uint32_t n = static_cast<uint32_t>(y);
-  if (above) n = max(n, 1u);
-  return x == 0.0 ? 0u : static_cast<uint32_t>((top + 6) << 3) + n;
+// the exponent of a block's power of two, from the high word of its largest finite value
+// (0: a block of zeros)
+__device__ __forceinline__ int block_power(uint32_t top) {
+  return max(static_cast<int>(top >> 20) - 1023 - 7, -126);
+}
+
+// the e4m3 code of |x| / 2^k, below 256, by the dither w / 2^32: a value's place between
+// its two neighbours is what stands behind the three leading bits of its mantissa, where w is
+// added, and a carry makes it the upper one.  Below 2^(k - 6) the spacing stays that of the
+// binade above: the values are lifted into it.
+__device__ __forceinline__ uint32_t code(double x, int k, uint32_t w) {
+  const bool low = high(x) < static_cast<uint32_t>(k - 6 + 1023) << 20;
+  const double z = fabs(x) + (low ? power(k - 6) : 0.0);
+  const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(z)) + (static_cast<uint64_t>(w) << 17);
+  const uint32_t c = static_cast<uint32_t>(bits >> 49) - (static_cast<uint32_t>(k - 7 + 1023) << 3) - (low ? 8u : 0u);
+  return x == 0.0 ? 0u : high(x) >= kNotFinite ? 0x7fu : c;
 }
 
 constexpr uint32_t kPlace = 0xC13FA9A9u, kTurn = 0x91E10DA5u;  // 2^32 / p, 2^32 / p^2
+
+// sqrt(v) to 2^-46 of itself: an estimate of 2^-24 and one step of Newton's.  The next border
+// between two 8-bit values is closer than that for one in 10^12 of them.
+__device__ __forceinline__ double root_of(double v) {
+  const double y = __builtin_amdgcn_rsq(v), r = v * y;
+  return v == 0.0 ? 0.0 : fma(0.5 * y, fma(-r, r, v), r);
+}
+
+// kVals values of a block, n of them real: the averages' new ones in 64 bits, the parameters
+// stepped, and the high words of the largest finite averages
+template <typename P, typename G>
+struct Held {
+  Pack<P, kVals> p;
+  Pack<G, kVals> g;
+  Pack<uint8_t, kVals> m, v;
+  float sm, sv;
+  double first[kVals], root[kVals];
+
+  __device__ __forceinline__ void step(const Factors& f, const Constants& c, uint32_t& em, uint32_t& ev) {
+    const double bm = c.b1 * sm, bv = c.b2 * (static_cast<double>(sv) * sv);
+    float least = 1e30f, most = 0.f, den[kVals];
+#pragma unroll
+    for (int u = 0; u < kVals; ++u) {
+      const double d = static_cast<double>(to_f(g.v[u])) * f.clip;
+      // powers of two and squares of 4-bit mantissas: b sm, b sv sv and r r are exact
+      const float r = __builtin_amdgcn_cvt_f32_fp8(v.v[u], 0);
+      first[u] = bm * static_cast<double>(__builtin_amdgcn_cvt_f32_fp8(m.v[u], 0)) + c.c1 * d;
+      root[u] = root_of(bv * static_cast<double>(r * r) + c.c2 * (d * d));
+      const uint32_t e1 = high(first[u]), e2 = high(root[u]);
+      em = max(em, e1 < kNotFinite ? e1 : 0u);
+      ev = max(ev, e2 < kNotFinite ? e2 : 0u);
+      den[u] = static_cast<float>(root[u]) * f.even + c.eps;
+      least = fminf(least, den[u]);
+      most = fmaxf(most, den[u]);
+    }
+    // the reciprocal's instruction ends where its result or its argument is no normal number
+    const bool usual = least > 1e-30f && most < 1e30f;
+#pragma unroll
+    for (int u = 0; u < kVals; ++u) {
+      const float up = f.by * static_cast<float>(first[u]);
+      const float q = usual ? up * __builtin_amdgcn_rcpf(den[u]) : up / den[u];
+      p.v[u] = from_f<P>(to_f(p.v[u]) * f.keep - q);
+    }
+  }
+
+  __device__ __forceinline__ void hold(uint32_t i, uint32_t turn, int km, int kv) {
+#pragma unroll
+    for (int u = 0; u < kVals; ++u) {
+      const uint32_t w = (i + u) * kPlace + turn;
+      m.v[u] = static_cast<uint8_t>(code(first[u], km, w) | (first[u] < 0.0 ? 0x80u : 0u));
+      const uint32_t r = code(root[u], kv, w + 0x80000000u);
+      v.v[u] = static_cast<uint8_t>(r == 0 && root[u] > 0.0 ? 1u : r);
+    }
+  }
+};
 
 template <typename P, typename G>
 __device__ __forceinline__ void adam_held(P* __restrict__ p, const G* __restrict__ g, uint8_t* __restrict__ m,
                                           uint8_t* __restrict__ v, float* __restrict__ scales, int64_t blocks, int64_t lo,
                                           int64_t hi, const Factors& f, const Constants& c) {
   const int lane = threadIdx.x & (kWave - 1);
-  for (int64_t b = lo / kBlock + threadIdx.x / kWave; b * kBlock < hi; b += kAdamThreads / kWave) {  // wave-uniform
+  const uint32_t turn = f.t * kTurn;
+  auto read = [&](Held<P, G>& x, int64_t b, auto load) {
     const int64_t i = b * kBlock + lane * kVals;
-    const int n = static_cast<int>(max(static_cast<int64_t>(0), min(hi - i, static_cast<int64_t>(kVals))));
-    Pack<P, kVals> pp = load_some(p + i, n);
-    const Pack<G, kVals> pg = load_some(g + i, n);
-    const Pack<uint8_t, kVals> pm = load_some(m + i, n), pv = load_some(v + i, n);
-    const double sm = scales[b], sv = scales[blocks + b];
-    double first[kVals], root[kVals];
-    int em = -2000, ev = -2000;
-#pragma unroll
-    for (int u = 0; u < kVals; ++u) {
-      const double d = static_cast<double>(to_f(pg.v[u])) * f.clip;
-      const double r = static_cast<double>(__builtin_amdgcn_cvt_f32_fp8(pv.v[u], 0)) * sv;
-      first[u] = c.b1 * (static_cast<double>(__builtin_amdgcn_cvt_f32_fp8(pm.v[u], 0)) * sm) + c.c1 * d;
-      root[u] = sqrt(c.b2 * (r * r) + c.c2 * (d * d));
-      const int e1 = exponent(first[u]), e2 = exponent(root[u]);
-      if (e1 != kNotFinite && first[u] != 0.0) em = max(em, e1);
-      if (e2 != kNotFinite && root[u] != 0.0) ev = max(ev, e2);
-      pp.v[u] = from_f<P>(stepped(to_f(pp.v[u]), static_cast<float>(first[u]), static_cast<float>(root[u]), f, c.eps));
-    }
-    const int km = block_power(em), kv = block_power(ev);
-    Pack<uint8_t, kVals> om, ov;
-#pragma unroll
-    for (int u = 0; u < kVals; ++u) {
-      const uint32_t w = (static_cast<uint32_t>(i) + u) * kPlace + f.t * kTurn;
-      om.v[u] = static_cast<uint8_t>(code(first[u], km, w, false) | (first[u] < 0.0 ? 0x80u : 0u));
-      ov.v[u] = static_cast<uint8_t>(code(root[u], kv, w + 0x80000000u, true));
-    }
-    store_some(p + i, pp, n);
-    store_some(m + i, om, n);
-    store_some(v + i, ov, n);
+    x.p = load(p + i);
+    x.g = load(g + i);
+    x.m = load(m + i);
+    x.v = load(v + i);
+    x.sm = scales[b];
+    x.sv = scales[blocks + b];
+  };
+  auto write = [&](Held<P, G>& x, int64_t b, auto store) {
+    const int64_t i = b * kBlock + lane * kVals;
+    uint32_t em = 0, ev = 0;
+    x.step(f, c, em, ev);
+    const int km = block_power(wave_max(em)), kv = block_power(wave_max(ev));
+    x.hold(static_cast<uint32_t>(i), turn, km, kv);
+    store(p + i, x.p);
+    store(m + i, x.m);
+    store(v + i, x.v);
     if (lane == 0) {
       scales[b] = static_cast<float>(power(km));
       scales[blocks + b] = static_cast<float>(power(kv));
     }
+  };
+  auto all = [](auto* q) { return load_once(q); };
+  // wave-uniform: a wavefront takes whole blocks, the next one's values on their way while it
+  // steps one, and one wavefront the rest
+  constexpr int kWaves = kAdamThreads / kWave;
+  const int64_t whole = hi / kBlock, first = lo / kBlock + threadIdx.x / kWave;
+  Held<P, G> x, next;
+  if (first < whole) read(next, first, all);
+  for (int64_t b = first; b < whole; b += kWaves) {
+    x = next;
+    read(next, min(b + kWaves, whole - 1), all);
+    write(x, b, [](auto* q, const auto& y) { store_once(q, y); });
+  }
+  if (whole * kBlock < hi && (whole - first) % kWaves == 0) {
+    const int n = static_cast<int>(hi - whole * kBlock) - lane * kVals;  // of this lane's, none where it is negative
+    read(x, whole, [n](auto* q) { return load_some(q, n); });
+    write(x, whole, [n](auto* q, const auto& y) { store_some(q, y, n); });
   }
 }
 
@@ -239,11 +331,11 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_step(const AdamList l, int
 
 // values per part: one round of a workgroup or more, and as many as keep the parts near
 // kMostParts; whole blocks
-int64_t adam_part(const tgx_adamw_tensor* t, int64_t count) {
+int64_t adam_part(const tgx_adamw_tensor* t, int64_t count, int bits) {
   int64_t all = 0;
-  for (int64_t i = 0; i < count; ++i) all += t[i].size;
+  for (int64_t i = 0; i < count; ++i) all += t[i].bits == bits ? t[i].size : 0;
   constexpr int64_t round = kAdamThreads * kVals;
-  return std::max<int64_t>(1, ops_cdiv(ops_cdiv(all, kMostParts), round)) * round;
+  return std::max<int64_t>(1, ops_cdiv(ops_cdiv(all, kMostParts[bits == 8]), round)) * round;
 }
 
 int check_adamw(const tgx_adamw_args* a) {
@@ -311,7 +403,6 @@ extern "C" int tgx_adamw(const tgx_adamw_args* args, void* stream) {
   const size_t need = tgx_adamw_workspace_size(a.count);
   if (a.workspace == nullptr || a.workspace_bytes < need || !aligned16(a.workspace))
     return fail(TGX_ERR_ARG, "tgx_adamw: workspace of %zu bytes, 16-byte aligned, needed", need);
-  const int64_t per = adam_part(a.tensors, a.count);
   hipStream_t s = static_cast<hipStream_t>(stream);
   Factors* factors = static_cast<Factors*>(a.workspace);
   const Constants c{a.beta1, a.beta2, 1.0 - a.beta1, 1.0 - a.beta2, static_cast<float>(a.eps)};
@@ -324,6 +415,7 @@ extern "C" int tgx_adamw(const tgx_adamw_args* args, void* stream) {
     if (const int rc = check_launch("adamw_begin")) return rc;
   }
   for (const int bits : {32, 8}) {
+    const int64_t per = adam_part(a.tensors, a.count, bits);
     for (int64_t i = 0; i < a.count;) {
       AdamList l{};
       uint32_t n = 0;
