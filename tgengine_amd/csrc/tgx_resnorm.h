@@ -26,7 +26,7 @@ struct ResArgs {
   void* dx;
   void* dres;
   void* dgate;
-  float* part;  // [blocks][kSums][dim]
+  float* part;  // [blocks][sums_of][dim]
 };
 
 // column sums of the backward pass: weight, bias, scale, post
@@ -34,8 +34,8 @@ constexpr int kSums = 4;
 constexpr int sums_of(bool parts) { return parts ? kSums : 2; }
 
 // Calls f(V, L, C): a row of `dim` values on L lanes, C packs of V values each.  One pack a
-// lane up to a wavefront; more lanes before more packs, because the backward pass keeps up
-// to four sums for each value of its packs.
+// lane up to a whole workgroup, because the backward pass keeps up to four sums for each
+// value of its packs.
 template <typename T, typename F>
 int res_shape(int64_t dim, F&& f) {
 #define TGX_SHAPE(V, L, C) \
@@ -47,9 +47,9 @@ int res_shape(int64_t dim, F&& f) {
   if (packs <= 16) return TGX_SHAPE(V, 16, 1);
   if (packs <= 32) return TGX_SHAPE(V, 32, 1);
   if (packs <= 64) return TGX_SHAPE(V, 64, 1);
-  if (packs <= 128) return TGX_SHAPE(V, 64, 2);
+  if (packs <= 128) return TGX_SHAPE(V, 128, 1);
   if (packs <= 256) return TGX_SHAPE(V, 256, 1);
-  if (packs <= 512) return TGX_SHAPE(V, 256, 2);
+  if (packs <= 512) return TGX_SHAPE(V, 512, 1);
   if (packs <= 1024) return TGX_SHAPE(V, 1024, 1);
   if constexpr (V == 8) {
     return TGX_SHAPE(V, 1024, 2);
@@ -61,7 +61,8 @@ int res_shape(int64_t dim, F&& f) {
 }
 static_assert(TGX_MAX_NORM_DIM <= 1024 * 2 * 8 && TGX_MAX_NORM_DIM <= 1024 * 4 * 4, "a row fits its workgroup");
 
-constexpr int res_threads(int lanes) { return lanes > kNormThreads ? lanes : kNormThreads; }
+// a workgroup: several rows of up to a wavefront each, or one
+constexpr int res_threads(int lanes) { return lanes > kWave ? lanes : kNormThreads; }
 
 // the mean of a row's values (0 where rows are not centred) and 1 / sqrt(their mean square
 // about it + eps)

@@ -15,10 +15,54 @@
 namespace tgx {
 namespace {
 
-template <typename T, typename W, int V, int L, int C, bool PARTS>
+// Bits of a kernel's kind: what the call's sums have.  Without kScaled, x joins the sum as it is.
+constexpr int kScaled = 1, kGate = 2, kPost = 4;
+
+template <size_t N>
+struct __attribute__((packed, aligned(2))) Regs {
+  uint32_t v[N];
+};
+
+// What a second pass over a row needs of a value it forms again from what was read, rather
+// than have six values more a value leave the device half empty.  `again` makes the compiler
+// do so.
+template <typename T, int V>
+__device__ __forceinline__ void again(Pack<T, V>& p) {
+  if constexpr (sizeof(p) % 4 == 0) {
+    auto w = __builtin_bit_cast(Regs<sizeof(p) / 4>, p);
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(p) / 4); ++i) asm volatile("" : "+v"(w.v[i]));
+    p = __builtin_bit_cast(Pack<T, V>, w);
+  }
+}
+
+// both sums over the L lanes of a row; `lds` [2][2][L / 64], whose halves take turns, so that
+// one barrier a call is enough
+template <int L>
+__device__ __forceinline__ void row_sums(float& x, float& y, float* lds, int turn) {
+  if constexpr (L <= kWave) {
+    x = group_sum<L>(x);
+    y = group_sum<L>(y);
+  } else {
+    constexpr int N = L / kWave;
+    x = group_sum<kWave>(x);
+    y = group_sum<kWave>(y);
+    float* at = lds + (turn & 1) * 2 * N;
+    if ((threadIdx.x & (kWave - 1)) == 0) {
+      at[threadIdx.x / kWave] = x;
+      at[N + threadIdx.x / kWave] = y;
+    }
+    __syncthreads();
+    x = group_sum<N>(at[threadIdx.x & (N - 1)]);
+    y = group_sum<N>(at[N + (threadIdx.x & (N - 1))]);
+  }
+}
+
+template <typename T, typename W, int V, int L, int C, int KIND>
 __global__ __launch_bounds__(res_threads(L)) void resnorm_bwd(const ResArgs a) {
-  constexpr int N = res_threads(L), R = N / L, S = sums_of(PARTS);
-  __shared__ float lds[N / kWave];
+  constexpr bool SCALED = KIND & kScaled, GATE = KIND & kGate, POST = KIND & kPost;
+  constexpr int N = res_threads(L), R = N / L, S = sums_of(SCALED);
+  __shared__ float lds[L > kWave ? 4 * L / kWave : 1];
   __shared__ float join[R > 1 ? N * V : 1];
   const Place<V, L> at(a.dim);
   const float inv = 1.f / static_cast<float>(a.dim);
@@ -29,116 +73,155 @@ __global__ __launch_bounds__(res_threads(L)) void resnorm_bwd(const ResArgs a) {
     for (int j = 0; j < C; ++j)
 #pragma unroll
       for (int u = 0; u < V; ++u) acc[k][j][u] = 0.f;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * R;
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * R; base < a.rows; base += step) {  // workgroup-uniform
-    const int64_t mine = base + threadIdx.x / L, row = min(mine, a.rows - 1);
-    const bool live = mine < a.rows;
-    Pack<T, V> px[C], pr[C], pg[C], py[C], ps[C];
+  Pack<W, V> w[C], wp[C], wc[C];
+#pragma unroll
+  for (int j = 0; j < C; ++j) {
+#pragma unroll
+    for (int u = 0; u < V; ++u) w[j].v[u] = wc[j].v[u] = from_f<W>(1.f);
+    if (a.weight != nullptr) w[j] = load_pack<W, V>(static_cast<const W*>(a.weight) + at.at(j));
+    if (POST) wp[j] = load_pack<W, V>(static_cast<const W*>(a.post) + at.at(j));
+    if (SCALED && a.scale != nullptr) wc[j] = load_pack<W, V>(static_cast<const W*>(a.scale) + at.at(j));
+  }
+  struct Row {
+    Pack<T, V> x[C], r[C], g[C], y[C], s[C];
+    float m, rstd, mx, rx;
+  };
+  // gradients that are not given are zeros, and so are those of rows past the last: they add
+  // nothing to a sum
+  auto read = [&](Row& o, int64_t mine) {
+    const int64_t row = min(mine, a.rows - 1);
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       const int c = at.at(j);
-      px[j] = load_pack<T, V>(static_cast<const T*>(a.x) + row * a.x_stride + c);
-      if (a.residual != nullptr) pr[j] = load_pack<T, V>(static_cast<const T*>(a.residual) + row * a.residual_stride + c);
-      if (PARTS && a.gate != nullptr) pg[j] = load_pack<T, V>(static_cast<const T*>(a.gate) + row * a.gate_stride + c);
-      if (a.dout != nullptr) py[j] = load_pack<T, V>(static_cast<const T*>(a.dout) + row * a.dim + c);
-      if (a.dsum != nullptr) ps[j] = load_pack<T, V>(static_cast<const T*>(a.dsum) + row * a.dim + c);
+      o.x[j] = load_pack<T, V>(static_cast<const T*>(a.x) + row * a.x_stride + c);
+      if (SCALED || a.residual != nullptr) o.r[j] = load_pack<T, V>(static_cast<const T*>(a.residual) + row * a.residual_stride + c);
+      if (GATE) o.g[j] = load_pack<T, V>(static_cast<const T*>(a.gate) + row * a.gate_stride + c);
+      if (a.dout != nullptr) o.y[j] = load_pack<T, V>(static_cast<const T*>(a.dout) + row * a.dim + c);
+      if (a.dsum != nullptr) o.s[j] = load_pack<T, V>(static_cast<const T*>(a.dsum) + row * a.dim + c);
     }
-    const float m = a.stats[row], r = a.stats[a.rows + row];
-    float mx = 0.f, rx = 1.f;
-    if (PARTS && a.post != nullptr) mx = a.stats[2 * a.rows + row], rx = a.stats[3 * a.rows + row];
-    // h; n, hx, and the two factors of n
-    float h[C][V], n[C][V], hx[C][V], sig[C][V], rest[C][V], by[C][V];
+    o.m = a.stats[row];
+    o.rstd = a.stats[a.rows + row];
+    if (POST) o.mx = a.stats[2 * a.rows + row], o.rx = a.stats[3 * a.rows + row];
+  };
+  auto clear = [](Pack<T, V>& p, int n) {
+#pragma unroll
+    for (int u = 0; u < V; ++u) p.v[u] = u < n ? from_f<T>(0.f) : p.v[u];
+  };
+  const int64_t step = static_cast<int64_t>(gridDim.x) * R;
+  Row now, next;
+  read(next, static_cast<int64_t>(blockIdx.x) * R + threadIdx.x / L);
+  int turn = 0;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * R; base < a.rows; base += step) {  // workgroup-uniform
+    const int64_t mine = base + threadIdx.x / L;
+    now = next;
+    read(next, mine + step);  // on its way while this row is worked on
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      again(w[j]);
+      if constexpr (POST) again(wp[j]);
+      if constexpr (SCALED) again(wc[j]);
+      if (a.dout == nullptr || mine >= a.rows) clear(now.y[j], V);
+      if (a.dsum == nullptr || mine >= a.rows) clear(now.s[j], V);
+    }
+    const float m = now.m, r = now.rstd, mx = POST ? now.mx : 0.f, rx = POST ? now.rx : 1.f;
+    // the smaller of sigmoid(gate) and 1 - sigmoid(gate): the other is 1 less it
+    float small[C][V];
+    struct Value {
+      float h, hx, n, sig, rest, by;
+    };
+    auto value = [&](int j, int u) {
+      Value v{0.f, 0.f, to_f(now.x[j].v[u]), 1.f, 1.f, 1.f};
+      if constexpr (SCALED) {
+        if constexpr (POST) {
+          v.hx = (v.n - mx) * rx;
+          v.n = v.hx * to_f(wp[j].v[u]);
+        }
+        v.by = to_f(wc[j].v[u]);
+        if constexpr (GATE) {
+          const bool neg = to_f(now.g[j].v[u]) < 0.f;
+          const float big = 1.f - small[j][u];
+          v.sig = neg ? small[j][u] : big;
+          v.rest = neg ? big : small[j][u];
+          v.by *= v.sig;
+        }
+        v.h = (fmaf(v.by, v.n, to_f(now.r[j].v[u])) - m) * r;
+      } else {
+        v.h = ((a.residual != nullptr ? v.n + to_f(now.r[j].v[u]) : v.n) - m) * r;
+      }
+      return v;
+    };
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int j = 0; j < C; ++j) {
-      Pack<W, V> w, wp, wc;
-      if (a.weight != nullptr) w = load_pack<W, V>(static_cast<const W*>(a.weight) + at.at(j));
-      if (PARTS && a.post != nullptr) wp = load_pack<W, V>(static_cast<const W*>(a.post) + at.at(j));
-      if (PARTS && a.scale != nullptr) wc = load_pack<W, V>(static_cast<const W*>(a.scale) + at.at(j));
-      const int skip = live ? at.skip(j) : V;
+      Pack<T, V> y = now.y[j];
+      if (at.skip(j) > 0) clear(y, at.skip(j));  // values of the pack before
 #pragma unroll
       for (int u = 0; u < V; ++u) {
-        float s = to_f(px[j].v[u]);
-        if constexpr (PARTS) {
-          hx[j][u] = (s - mx) * rx;
-          if (a.post != nullptr) s = hx[j][u] * to_f(wp.v[u]);
-          n[j][u] = s;
-          by[j][u] = a.scale != nullptr ? to_f(wc.v[u]) : 1.f;
-          sig[j][u] = rest[j][u] = 1.f;
-          if (a.gate != nullptr) {
-            sigmoids(to_f(pg[j].v[u]), sig[j][u], rest[j][u]);
-            by[j][u] *= sig[j][u];
-          }
-          s = fmaf(by[j][u], s, to_f(pr[j].v[u]));
-        } else if (a.residual != nullptr) {
-          s += to_f(pr[j].v[u]);
+        if constexpr (GATE) {
+          const float e = __builtin_amdgcn_exp2f(-1.44269504f * __builtin_fabsf(to_f(now.g[j].v[u])));
+          small[j][u] = e * __builtin_amdgcn_rcpf(1.f + e);
         }
-        h[j][u] = (s - m) * r;
-        const float d = a.dout != nullptr ? to_f(py[j].v[u]) : 0.f;
-        const float g = a.weight != nullptr ? d * to_f(w.v[u]) : d;
-        if (u >= skip) {
-          s1 += g;
-          s2 = fmaf(g, h[j][u], s2);
-          acc[0][j][u] = fmaf(d, h[j][u], acc[0][j][u]);
-          acc[1][j][u] += d;
-        }
+        const float h = value(j, u).h, dy = to_f(y.v[u]), g = dy * to_f(w[j].v[u]);
+        s1 += g;
+        s2 = fmaf(g, h, s2);
+        acc[0][j][u] = fmaf(dy, h, acc[0][j][u]);
+        acc[1][j][u] += dy;
       }
+      again(now.x[j]);
     }
-    if (a.dout != nullptr) {
-      s1 = a.center ? row_sum<L>(s1, lds) * inv : 0.f;
-      s2 = row_sum<L>(s2, lds) * inv;
-    }
-    float t1 = 0.f, t2 = 0.f;
+    row_sums<L>(s1, s2, lds, turn++);
+    s1 = a.center ? s1 * inv : 0.f;
+    s2 *= inv;
+    float t1 = 0.f, t2 = 0.f, q[C][V];
 #pragma unroll
     for (int j = 0; j < C; ++j) {
-      Pack<W, V> w, wp;
-      if (a.weight != nullptr) w = load_pack<W, V>(static_cast<const W*>(a.weight) + at.at(j));
-      if (PARTS && a.post != nullptr) wp = load_pack<W, V>(static_cast<const W*>(a.post) + at.at(j));
-      const int skip = live ? at.skip(j) : V;
+      const int skip = mine < a.rows ? at.skip(j) : V;
       Pack<T, V> od, og, ox;
 #pragma unroll
       for (int u = 0; u < V; ++u) {
-        float d = 0.f;
-        if (a.dout != nullptr) {
-          const float e = to_f(py[j].v[u]);
-          const float g = a.weight != nullptr ? e * to_f(w.v[u]) : e;
-          d = r * (g - s1 - h[j][u] * s2);
-        }
-        if (a.dsum != nullptr) d += to_f(ps[j].v[u]);
+        const Value v = value(j, u);
+        const float g = to_f(now.y[j].v[u]) * to_f(w[j].v[u]);
+        const float d = fmaf(r, fmaf(-v.h, s2, g - s1), to_f(now.s[j].v[u]));
         od.v[u] = from_f<T>(d);
-        if constexpr (PARTS) {
-          const float dn = d * by[j][u];
-          og.v[u] = from_f<T>(dn * n[j][u] * rest[j][u]);
-          const float q = a.post != nullptr ? dn * to_f(wp.v[u]) : dn;
-          if (u >= skip) {
-            acc[2][j][u] = fmaf(d * sig[j][u], n[j][u], acc[2][j][u]);
-            acc[3][j][u] = fmaf(dn, hx[j][u], acc[3][j][u]);
-            t1 += q;
-            t2 = fmaf(q, hx[j][u], t2);
+        if constexpr (SCALED) {
+          const float dn = d * v.by;
+          acc[2][j][u] = fmaf(d * v.sig, v.n, acc[2][j][u]);
+          if constexpr (GATE) og.v[u] = from_f<T>(dn * v.n * v.rest);
+          if constexpr (POST) {
+            acc[3][j][u] = fmaf(dn, v.hx, acc[3][j][u]);
+            q[j][u] = dn * to_f(wp[j].v[u]);
+            const float own = u >= skip ? q[j][u] : 0.f;
+            t1 += own;
+            t2 = fmaf(own, v.hx, t2);
+          } else {
+            ox.v[u] = from_f<T>(dn);
           }
-          ox.v[u] = from_f<T>(q);
-          n[j][u] = q;
         }
       }
+      again(now.x[j]);
       if (skip == V) continue;
-      const int64_t to = row * a.dim + at.at(j);
+      const int64_t to = mine * a.dim + at.at(j);
       if (a.dres != nullptr) store_pack<T, V>(static_cast<T*>(a.dres) + to, od);
-      if constexpr (PARTS) {
+      if constexpr (GATE)
         if (a.dgate != nullptr) store_pack<T, V>(static_cast<T*>(a.dgate) + to, og);
-        if (a.dx != nullptr && a.post == nullptr) store_pack<T, V>(static_cast<T*>(a.dx) + to, ox);
-      }
+      if constexpr (SCALED && !POST)
+        if (a.dx != nullptr) store_pack<T, V>(static_cast<T*>(a.dx) + to, ox);
     }
-    if constexpr (PARTS) {
-      if (a.post == nullptr || a.dx == nullptr) continue;
-      t1 = a.center ? row_sum<L>(t1, lds) * inv : 0.f;
-      t2 = row_sum<L>(t2, lds) * inv;
+    if constexpr (POST) {
+      if (a.dx == nullptr) continue;
+      row_sums<L>(t1, t2, lds, turn++);
+      t1 = a.center ? t1 * inv : 0.f;
+      t2 *= inv;
 #pragma unroll
       for (int j = 0; j < C; ++j) {
-        if (!live || at.skip(j) == V) continue;
+        if (mine >= a.rows || at.skip(j) == V) continue;
         Pack<T, V> ox;
 #pragma unroll
-        for (int u = 0; u < V; ++u) ox.v[u] = from_f<T>(rx * (n[j][u] - t1 - hx[j][u] * t2));
-        store_pack<T, V>(static_cast<T*>(a.dx) + row * a.dim + at.at(j), ox);
+        for (int u = 0; u < V; ++u) {
+          const float hx = (to_f(now.x[j].v[u]) - mx) * rx;
+          ox.v[u] = from_f<T>(rx * fmaf(-hx, t2, q[j][u] - t1));
+        }
+        store_pack<T, V>(static_cast<T*>(a.dx) + mine * a.dim + at.at(j), ox);
       }
     }
   }
@@ -173,7 +256,10 @@ __global__ __launch_bounds__(res_threads(L)) void resnorm_bwd(const ResArgs a) {
 }
 
 // the sums over the workgroups' parts [blocks][sums][dim], kCols columns per workgroup
-constexpr int kCols = 16;
+#ifndef KC
+#define KC 32
+#endif
+constexpr int kCols = KC;
 constexpr int kJoinThreads = 1024;
 
 struct SumOuts {
@@ -203,11 +289,16 @@ __global__ __launch_bounds__(kJoinThreads) void resnorm_join(const float* __rest
   }
 }
 
-// workgroups: enough to fill the device, and rows enough for each that its sums stay small
+#ifndef RB
+#define RB 1024
+#endif
+// workgroups: about what the device holds, and rows enough for each that its sums stay small
 // beside the rows it reads
-int64_t res_blocks(int64_t rows, int64_t dim) {
+int64_t res_blocks(int64_t rows, int64_t dim, int dtype) {
   const int64_t per = std::max<int64_t>(1, 2048 / std::max<int64_t>(dim, 1)) * 4;
-  return std::clamp<int64_t>(ops_cdiv(rows, per), 1, 2048);
+  const int64_t lanes = ops_cdiv(dim * elem_bytes(dtype), 16);
+  const int64_t most = lanes <= 256 ? RB : lanes <= 512 ? RB / 2 : RB / 4;
+  return std::clamp<int64_t>(ops_cdiv(rows, per), 1, most);
 }
 
 }  // namespace
@@ -217,7 +308,7 @@ using namespace tgx;
 
 extern "C" size_t tgx_residual_norm_grad_workspace_size(const tgx_residual_norm_args* args) {
   if (check_resnorm("tgx_residual_norm_grad", args, true) || args->rows == 0) return 0;
-  return static_cast<size_t>(res_blocks(args->rows, args->dim)) * sums_of(has_parts(args)) * args->dim * 4;
+  return static_cast<size_t>(res_blocks(args->rows, args->dim, args->dtype)) * sums_of(has_parts(args)) * args->dim * 4;
 }
 
 extern "C" int tgx_residual_norm_grad(const tgx_residual_norm_args* args, void* stream) {
@@ -236,7 +327,7 @@ extern "C" int tgx_residual_norm_grad(const tgx_residual_norm_args* args, void* 
   hipStream_t s = static_cast<hipStream_t>(stream);
   ResArgs a = res_args(args);
   a.part = sums ? static_cast<float*>(args->workspace) : nullptr;
-  const int64_t blocks = args->rows > 0 ? res_blocks(args->rows, args->dim) : 0;
+  const int64_t blocks = args->rows > 0 ? res_blocks(args->rows, args->dim, args->dtype) : 0;
   if (blocks > 0 && (sums || a.dx != nullptr || a.dres != nullptr || a.dgate != nullptr)) {
     const int rc = by_type(args->dtype, [&](auto t) {
       using T = decltype(t);
@@ -245,9 +336,16 @@ extern "C" int tgx_residual_norm_grad(const tgx_residual_norm_args* args, void* 
         return res_shape<T>(args->dim, [&](auto v, auto l, auto c) {
           constexpr int V = decltype(v)::value, L = decltype(l)::value, C = decltype(c)::value;
           const dim3 grid(static_cast<unsigned>(blocks)), block(res_threads(L));
-          if (parts) hipLaunchKernelGGL((resnorm_bwd<T, W, V, L, C, true>), grid, block, 0, s, a);
-          else hipLaunchKernelGGL((resnorm_bwd<T, W, V, L, C, false>), grid, block, 0, s, a);
-          return check_launch("resnorm_bwd");
+          auto launch = [&](auto kind) {
+            hipLaunchKernelGGL((resnorm_bwd<T, W, V, L, C, decltype(kind)::value>), grid, block, 0, s, a);
+            return check_launch("resnorm_bwd");
+          };
+          if (!parts) return launch(std::integral_constant<int, 0>{});
+          if (a.post == nullptr)
+            return a.gate == nullptr ? launch(std::integral_constant<int, kScaled>{})
+                                     : launch(std::integral_constant<int, kScaled | kGate>{});
+          return a.gate == nullptr ? launch(std::integral_constant<int, kScaled | kPost>{})
+                                   : launch(std::integral_constant<int, kScaled | kGate | kPost>{});
         });
       });
     });
