@@ -557,7 +557,7 @@ typedef struct tgx_scan_args {
                               which the gradient reads */
   /* tgx_scan_grad: starts as tgx_scan wrote them (out and last are not read); grad_out
    * [batch, length, dim] and grad_last [batch, dim], each NULL for zeros; grad_x and
-   * grad_gate [batch, length, dim] and grad_state [batch, dim], each may be NULL */
+   * grad_gate [batch, length, dim]; grad_state NULL or [batch, dim] */
   const void* grad_out;
   const float* grad_last;
   void* grad_x;

@@ -53,8 +53,9 @@ def test_scan_checks():
     assert L.tgx_scan(_scan(batch=1 << 30, length=1), None) == 3 and "one launch" in _err()
     assert L.tgx_scan(_scan(last=None), None) == 1 and "out and last" in _err()
     assert L.tgx_scan(_scan(out=None), None) == 1
-    assert L.tgx_scan_grad(_scan(), None) == 0  # no gradient asked for
-    assert L.tgx_scan_grad(_scan(length=40, grad_x=8), None) == 1 and "starts" in _err()
+    for more in (dict(), dict(grad_x=8), dict(grad_gate=8)):
+        assert L.tgx_scan_grad(_scan(**more), None) == 1 and "grad_x and grad_gate" in _err()
+    assert L.tgx_scan_grad(_scan(length=40, grad_x=8, grad_gate=8), None) == 1 and "starts" in _err()
     # long rows of few channels are cut, and their pieces need room
     need = L.tgx_scan_workspace_size(_scan(length=5000))
     assert need > 0 and L.tgx_scan(_scan(length=5000), None) == 1 and "workspace" in _err()
@@ -62,7 +63,7 @@ def test_scan_checks():
     assert L.tgx_scan(_scan(length=5000, workspace=16, workspace_bytes=need - 1), None) == 1
     assert L.tgx_scan_workspace_size(None) == 0 and L.tgx_scan_workspace_size(_scan()) == 0
     assert L.tgx_scan_workspace_size(_scan(dtype=7, length=5000)) == 0
-    assert [L.tgx_scan_starts(n) for n in (0, 1, 16, 17, 32, 33)] == [0, 0, 0, 1, 1, 2]
+    assert [L.tgx_scan_starts(n) for n in (0, 1, 8, 9, 16, 17, 33)] == [0, 0, 0, 1, 1, 2, 4]
 
 
 def _res(**more):

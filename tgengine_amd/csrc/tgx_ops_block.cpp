@@ -85,9 +85,8 @@ class Scan : public torch::autograd::Function<Scan> {
     a.starts = saved[4].data_ptr<float>();
     a.grad_out = ptr(g);
     a.grad_last = static_cast<const float*>(ptr(gl));
-    Tensor d[3];
-    for (int i = 0; i < 2; ++i)
-      if (ctx->needs_input_grad(i)) d[i] = at::empty(x.sizes(), x.options());
+    Tensor d[3];  // the first two come together
+    for (int i = 0; i < 2; ++i) d[i] = at::empty(x.sizes(), x.options());
     if (state.defined() && ctx->needs_input_grad(2)) d[2] = at::empty(state.sizes(), state.options());
     a.grad_x = ptr(d[0]);
     a.grad_gate = ptr(d[1]);
@@ -96,6 +95,8 @@ class Scan : public torch::autograd::Function<Scan> {
     a.workspace = ptr(ws);
     a.workspace_bytes = ws.defined() ? ws.numel() : 0;
     check(tgx_scan_grad(&a, stream_of(x)), "tgx_scan_grad");
+    for (int i = 0; i < 2; ++i)
+      if (!ctx->needs_input_grad(i)) d[i] = Tensor();
     return {d[0], d[1], d[2], Tensor()};
   }
 };
