@@ -86,10 +86,12 @@ __global__ __launch_bounds__(res_threads(L)) void resnorm_bwd(const ResArgs a) {
     Pack<T, V> x[C], r[C], g[C], y[C], s[C];
     float m, rstd, mx, rx;
   };
+  // from the last row: what the forward pass read last is still in the caches
+  auto row_of = [&](int64_t mine) { return a.rows - 1 - mine; };
   // gradients that are not given are zeros, and so are those of rows past the last: they add
   // nothing to a sum
   auto read = [&](Row& o, int64_t mine) {
-    const int64_t row = min(mine, a.rows - 1);
+    const int64_t row = row_of(min(mine, a.rows - 1));
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       const int c = at.at(j);
@@ -200,7 +202,7 @@ __global__ __launch_bounds__(res_threads(L)) void resnorm_bwd(const ResArgs a) {
       }
       again(now.x[j]);
       if (skip == V) continue;
-      const int64_t to = mine * a.dim + at.at(j);
+      const int64_t to = row_of(mine) * a.dim + at.at(j);
       if (a.dres != nullptr) store_pack<T, V>(static_cast<T*>(a.dres) + to, od);
       if constexpr (GATE)
         if (a.dgate != nullptr) store_pack<T, V>(static_cast<T*>(a.dgate) + to, og);
@@ -221,7 +223,7 @@ __global__ __launch_bounds__(res_threads(L)) void resnorm_bwd(const ResArgs a) {
           const float hx = (to_f(now.x[j].v[u]) - mx) * rx;
           ox.v[u] = from_f<T>(rx * fmaf(-hx, t2, q[j][u] - t1));
         }
-        store_pack<T, V>(static_cast<T*>(a.dx) + mine * a.dim + at.at(j), ox);
+        store_pack<T, V>(static_cast<T*>(a.dx) + row_of(mine) * a.dim + at.at(j), ox);
       }
     }
   }

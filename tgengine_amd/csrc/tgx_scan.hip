@@ -349,7 +349,8 @@ __device__ __forceinline__ Pack<T, V> kept_pack(const Pack<T, V>& p, bool keep) 
 
 template <typename T, int V, typename O, bool MASK, bool DOUT>
 __global__ __launch_bounds__(kScanThreads) void scan_bwd(const ScanArgs a) {
-  const uint32_t id = blockIdx.x * kScanThreads + threadIdx.x;
+  // from the last rows: what the forward pass read last is still in the caches
+  const uint32_t id = (gridDim.x - 1 - blockIdx.x) * kScanThreads + threadIdx.x;
   if (id >= a.items) return;
   const Part<T, V, O> at(a, id);
   float c[V];
