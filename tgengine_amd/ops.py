@@ -165,7 +165,7 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, bits=bits))
 
     def _new(self, p: Tensor, bits: int) -> dict:
-        if torch.cuda.is_current_stream_capturing():
+        if p.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: a parameter's first step cannot be captured: its averages would start again at every replay")
         held = bits == 8 and p.numel() >= 4096
         kind = dict(dtype=torch.float8_e4m3fn if held else torch.float32, device=p.device)
@@ -186,6 +186,8 @@ class AdamW(torch.optim.Optimizer):
             if not params:
                 continue
             for p in params:
+                if p.grad.layout is not torch.strided:
+                    raise RuntimeError("AdamW: sparse gradients are not supported")
                 if not self.state[p]:
                     self.state[p].update(self._new(p, group["bits"]))
             states = [self.state[p] for p in params]
