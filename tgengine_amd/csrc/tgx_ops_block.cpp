@@ -2,6 +2,8 @@
 // the residual sum with its norms, and the AdamW step.  Same rules as tgx_ops.cpp.
 #include "tgx_ops_host.h"
 
+#include <torch/csrc/autograd/python_variable.h>
+
 namespace {
 
 // ------------------------------------------------------------------ gated scan
@@ -270,14 +272,33 @@ std::tuple<Tensor, Tensor> residual_norm(const Tensor& x, const Tensor& residual
 }
 
 // ------------------------------------------------------------------ AdamW
-void adamw(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& exp_avg,
-           const std::vector<Tensor>& exp_avg_sq, const std::vector<Tensor>& steps, const std::vector<OptTensor>& scales,
-           double lr, const OptTensor& lr_in, double beta1, double beta2, double eps, double weight_decay,
-           const OptTensor& norm_in, double max_norm) {
-  const size_t n = params.size();
+// the tensors of a list, not counted again: the caller holds the list
+class Tensors {
+ public:
+  Tensors(const py::list& l, size_t n, const char* what) : list_(l.ptr()) {
+    if (l.size() != n) bad("adamw_: every list must have one tensor per parameter");
+    for (size_t i = 0; i < n; ++i)
+      if (!THPVariable_Check(PyList_GET_ITEM(list_, i))) throw py::type_error(std::string("adamw_: ") + what + " must be tensors");
+  }
+  const Tensor& operator[](size_t i) const { return THPVariable_Unpack(PyList_GET_ITEM(list_, i)); }
+
+ private:
+  PyObject* list_;
+};
+
+void adamw(const py::list& params_in, const py::list& grads_in, const py::list& exp_avg_in, const py::list& exp_avg_sq_in,
+           const py::list& steps_in, const py::list& scales, double lr, const OptTensor& lr_in, double beta1, double beta2,
+           double eps, double weight_decay, const OptTensor& norm_in, double max_norm) {
+  const size_t n = params_in.size();
   if (n == 0) bad("adamw_: no parameters");
-  if (grads.size() != n || exp_avg.size() != n || exp_avg_sq.size() != n || steps.size() != n || (!scales.empty() && scales.size() != n))
-    bad("adamw_: every list must have one tensor per parameter");
+  const Tensors params(params_in, n, "parameters"), grads(grads_in, n, "gradients"), exp_avg(exp_avg_in, n, "averages"),
+      exp_avg_sq(exp_avg_sq_in, n, "averages"), steps(steps_in, n, "steps");
+  if (scales.size() != 0 && scales.size() != n) bad("adamw_: every list must have one tensor per parameter");
+  auto scale_of = [&](size_t i) {
+    PyObject* o = scales.size() == 0 ? Py_None : PyList_GET_ITEM(scales.ptr(), i);
+    if (o != Py_None && !THPVariable_Check(o)) throw py::type_error("adamw_: scales must be tensors or None");
+    return o == Py_None ? Tensor() : THPVariable_Unpack(o);
+  };
   std::vector<tgx_adamw_tensor> table(n);
   for (size_t i = 0; i < n; ++i) {
     const Tensor &p = params[i], &g = grads[i], &m = exp_avg[i], &v = exp_avg_sq[i], &t = steps[i];
@@ -297,7 +318,7 @@ void adamw(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, 
     const bool held = m.scalar_type() != at::kFloat;
     tgx_adamw_tensor& a = table[i];
     if (held) {
-      const Tensor s = scales.empty() ? Tensor() : scales[i].value_or(Tensor());
+      const Tensor s = scale_of(i);
       const int64_t blocks = (p.numel() + TGX_ADAMW_BLOCK - 1) / TGX_ADAMW_BLOCK;
       if (!s.defined() || s.scalar_type() != at::kFloat || s.dim() != 2 || s.size(0) != 2 || s.size(1) != blocks ||
           !s.is_contiguous())
@@ -344,8 +365,8 @@ void adamw(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, 
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
   };
   for (size_t i = 0; i < n; ++i) {
-    for (const std::vector<Tensor>* l : {&params, &exp_avg, &exp_avg_sq, &steps}) written((*l)[i]);
-    if (table[i].bits == 8) written(*scales[i]);
+    for (const Tensors* l : {&params, &exp_avg, &exp_avg_sq, &steps}) written((*l)[i]);
+    if (table[i].bits == 8) written(scale_of(i));
   }
 }
 
