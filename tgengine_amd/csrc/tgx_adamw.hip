@@ -48,10 +48,12 @@ struct AdamList {
   float* scales[kList];
   int64_t size[kList];
   uint32_t first[kList + 1];  // first part of each tensor among this launch's
-  uint16_t at[kList];         // its factors
-  uint8_t p_bf16[kList], g_bf16[kList];
+  // In words, as everything here: scalar loads drop the two lowest bits of a base and of an offset
+  // apart, and the compiler may add the 7 t between a byte's and an address's place to either.
+  uint32_t kind[kList];       // 4 * the number of its factors + kParamBf16 + kGradBf16
   int32_t count;
 };
+constexpr uint32_t kParamBf16 = 1, kGradBf16 = 2;
 static_assert(sizeof(AdamList) <= 3800, "kernel arguments");
 
 struct Factors {
@@ -94,14 +96,12 @@ __global__ __launch_bounds__(kSteps) void adamw_begin(const StepList l, double l
   to[l.first + threadIdx.x] = f;
 }
 
+// the tensor that this workgroup's part belongs to: lane i knows whether it lies behind the
+// first part of tensor i
+static_assert(kList <= kWave, "a lane for each tensor");
 __device__ __forceinline__ int adam_tensor(const AdamList& l, uint32_t block) {
-  int lo = 0, hi = l.count;  // first[lo] <= block < first[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (l.first[mid] <= block) lo = mid;
-    else hi = mid;
-  }
-  return lo;
+  const int lane = threadIdx.x & (kWave - 1);
+  return __popcll(__ballot(lane < l.count && l.first[min(lane, kList)] <= block)) - 1;
 }
 
 // the first n of kVals values from p on, the others 0
@@ -312,7 +312,8 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_step(const AdamList l, int
   const int t = adam_tensor(l, blockIdx.x);
   const int64_t lo = (blockIdx.x - l.first[t]) * per, size = l.size[t];
   const int64_t hi = lo + per < size ? lo + per : size;
-  const Factors f = factors[l.at[t]];
+  const uint32_t kind = l.kind[t];
+  const Factors f = factors[kind / 4];
   auto with = [&](auto* p, auto* g) {
     if constexpr (HELD)
       adam_held(p, g, static_cast<uint8_t*>(l.m[t]), static_cast<uint8_t*>(l.v[t]), l.scales[t], (size + kBlock - 1) / kBlock,
@@ -320,11 +321,11 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_step(const AdamList l, int
     else
       adam_wide(p, g, static_cast<float*>(l.m[t]), static_cast<float*>(l.v[t]), lo, hi, f, c);
   };
-  if (l.p_bf16[t]) {
-    if (l.g_bf16[t]) with(static_cast<bf16*>(l.p[t]), static_cast<const bf16*>(l.g[t]));
+  if (kind & kParamBf16) {
+    if (kind & kGradBf16) with(static_cast<bf16*>(l.p[t]), static_cast<const bf16*>(l.g[t]));
     else with(static_cast<bf16*>(l.p[t]), static_cast<const float*>(l.g[t]));
   } else {
-    if (l.g_bf16[t]) with(static_cast<float*>(l.p[t]), static_cast<const bf16*>(l.g[t]));
+    if (kind & kGradBf16) with(static_cast<float*>(l.p[t]), static_cast<const bf16*>(l.g[t]));
     else with(static_cast<float*>(l.p[t]), static_cast<const float*>(l.g[t]));
   }
 }
@@ -428,9 +429,8 @@ extern "C" int tgx_adamw(const tgx_adamw_args* args, void* stream) {
         l.v[l.count] = t.exp_avg_sq;
         l.scales[l.count] = t.scales;
         l.size[l.count] = t.size;
-        l.at[l.count] = static_cast<uint16_t>(i);
-        l.p_bf16[l.count] = t.dtype == TGX_BF16;
-        l.g_bf16[l.count] = t.grad_dtype == TGX_BF16;
+        l.kind[l.count] = static_cast<uint32_t>(i) * 4 + (t.dtype == TGX_BF16 ? kParamBf16 : 0u) +
+                          (t.grad_dtype == TGX_BF16 ? kGradBf16 : 0u);
         l.first[l.count++] = n;
         n += static_cast<uint32_t>(ops_cdiv(t.size, per));
       }
