@@ -192,22 +192,23 @@ __device__ __forceinline__ int block_power(uint32_t top) {
 // the e4m3 code of |x| / 2^k, below 256, by the dither w / 2^32: a value's place between
 // its two neighbours is what stands behind the three leading bits of its mantissa, where w is
 // added, and a carry makes it the upper one.  Below 2^(k - 6) the spacing stays that of the
-// binade above: the values are lifted into it.
+// binade above: the values, zero among them, are lifted into it.
 __device__ __forceinline__ uint32_t code(double x, int k, uint32_t w) {
   const bool low = high(x) < static_cast<uint32_t>(k - 6 + 1023) << 20;
   const double z = fabs(x) + (low ? power(k - 6) : 0.0);
   const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(z)) + (static_cast<uint64_t>(w) << 17);
-  const uint32_t c = static_cast<uint32_t>(bits >> 49) - (static_cast<uint32_t>(k - 7 + 1023) << 3) - (low ? 8u : 0u);
-  return x == 0.0 ? 0u : high(x) >= kNotFinite ? 0x7fu : c;
+  const uint32_t base = static_cast<uint32_t>(k - 7 + 1023) << 3;
+  return static_cast<uint32_t>(bits >> 49) - (low ? base + 8 : base);
 }
+constexpr uint32_t kNan = 0x7f;
 
 constexpr uint32_t kPlace = 0xC13FA9A9u, kTurn = 0x91E10DA5u;  // 2^32 / p, 2^32 / p^2
 
 // sqrt(v) to 2^-46 of itself: an estimate of 2^-24 and one step of Newton's.  The next border
 // between two 8-bit values is closer than that for one in 10^12 of them.
 __device__ __forceinline__ double root_of(double v) {
-  const double y = __builtin_amdgcn_rsq(v), r = v * y;
-  return v == 0.0 ? 0.0 : fma(0.5 * y, fma(-r, r, v), r);
+  const double y = fmin(__builtin_amdgcn_rsq(v), 1e150), r = v * y;  // finite, for v = 0
+  return fma(0.5 * y, fma(-r, r, v), r);
 }
 
 // kVals values of a block, n of them real: the averages' new ones in 64 bits, the parameters
@@ -230,9 +231,8 @@ struct Held {
       const float r = __builtin_amdgcn_cvt_f32_fp8(v.v[u], 0);
       first[u] = bm * static_cast<double>(__builtin_amdgcn_cvt_f32_fp8(m.v[u], 0)) + c.c1 * d;
       root[u] = root_of(bv * static_cast<double>(r * r) + c.c2 * (d * d));
-      const uint32_t e1 = high(first[u]), e2 = high(root[u]);
-      em = max(em, e1 < kNotFinite ? e1 : 0u);
-      ev = max(ev, e2 < kNotFinite ? e2 : 0u);
+      em = max(em, high(first[u]));
+      ev = max(ev, high(root[u]));
       den[u] = static_cast<float>(root[u]) * f.even + c.eps;
       least = fminf(least, den[u]);
       most = fmaxf(most, den[u]);
@@ -251,9 +251,27 @@ struct Held {
 #pragma unroll
     for (int u = 0; u < kVals; ++u) {
       const uint32_t w = (i + u) * kPlace + turn;
-      m.v[u] = static_cast<uint8_t>(code(first[u], km, w) | (first[u] < 0.0 ? 0x80u : 0u));
+      const uint32_t sign = static_cast<uint32_t>(__double_as_longlong(first[u]) >> 56) & 0x80u;
+      m.v[u] = static_cast<uint8_t>(code(first[u], km, w) | sign);
       const uint32_t r = code(root[u], kv, w + 0x80000000u);
-      v.v[u] = static_cast<uint8_t>(r == 0 && root[u] > 0.0 ? 1u : r);
+      v.v[u] = static_cast<uint8_t>(root[u] > 0.0 ? max(r, 1u) : 0u);
+    }
+  }
+
+  // the largest finite averages of a block that holds others
+  __device__ __forceinline__ void finite(uint32_t& em, uint32_t& ev) const {
+    em = ev = 0;
+#pragma unroll
+    for (int u = 0; u < kVals; ++u) {
+      em = max(em, high(first[u]) < kNotFinite ? high(first[u]) : 0u);
+      ev = max(ev, high(root[u]) < kNotFinite ? high(root[u]) : 0u);
+    }
+  }
+  __device__ __forceinline__ void not_finite() {
+#pragma unroll
+    for (int u = 0; u < kVals; ++u) {
+      if (high(first[u]) >= kNotFinite) m.v[u] = kNan;
+      if (high(root[u]) >= kNotFinite) v.v[u] = kNan;
     }
   }
 };
@@ -277,8 +295,17 @@ __device__ __forceinline__ void adam_held(P* __restrict__ p, const G* __restrict
     const int64_t i = b * kBlock + lane * kVals;
     uint32_t em = 0, ev = 0;
     x.step(f, c, em, ev);
-    const int km = block_power(wave_max(em)), kv = block_power(wave_max(ev));
+    em = wave_max(em);
+    ev = wave_max(ev);
+    const bool others = max(em, ev) >= kNotFinite;  // wave-uniform, as em and ev
+    if (others) {
+      x.finite(em, ev);
+      em = wave_max(em);
+      ev = wave_max(ev);
+    }
+    const int km = block_power(em), kv = block_power(ev);
     x.hold(static_cast<uint32_t>(i), turn, km, kv);
+    if (others) x.not_finite();
     store(p + i, x.p);
     store(m + i, x.m);
     store(v + i, x.v);

@@ -48,7 +48,8 @@ inline size_t ops_align(size_t x) { return (x + 255) & ~static_cast<size_t>(255)
 inline uint64_t addr(const void* p) { return reinterpret_cast<uint64_t>(p); }
 inline int elem_bytes(int dtype) { return feat_elem_bytes(dtype); }
 
-// a = sigmoid(g) and 1 - a, each to a few units in its last place: neither is a difference
+// a = sigmoid(g) and 1 - a, each to |g| + 3 units in its last place (the rounding of the
+// exponent's argument, a power, a sum, a reciprocal): neither is a difference
 __device__ __forceinline__ void sigmoids(float g, float& a, float& rest) {
   const float e = __builtin_amdgcn_exp2f(-1.44269504f * __builtin_fabsf(g));
   const float r = __builtin_amdgcn_rcpf(1.f + e);
