@@ -176,6 +176,17 @@ def test_values_far_apart():
     assert bool((root[g != 0] > 0).all()) and not root[g == 0].any()
 
 
+def test_averages_on_borders():
+    """Averages that are powers of two and numbers of the format themselves: gradients equal to the first
+    average, whose squares' roots are those numbers."""
+    c = _make((2048,), (F,), 8, fresh=True, steps=[0])
+    values = torch.tensor(TABLE[:-1] * 20, device="cuda")[:2048].float()
+    c["grads"][0].copy_(torch.where(torch.arange(2048, device="cuda") % 2 == 0, values, -values))
+    for betas in ((0.0, 0.0), (0.5, 0.0), (0.9, 0.0), (0.9, 0.75), (0.5, 0.5), (0.9, 0.999)):
+        for _ in range(3):
+            _check(c, betas=betas, eps=1e-3)
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 def test_not_finite_stays_in_its_place(bits, bad):
