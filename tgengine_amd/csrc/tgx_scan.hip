@@ -19,6 +19,13 @@
 //
 // A masked token's x and gate are not used: its loads go to the span's first token, whose
 // line is read anyway.
+//
+// Memory bounds it: 24,576 rows of 32 tokens and 172 bf16 channels take 175 us forward (0.75
+// GB) and 270 backward (1.29 GB), 4.3 and 4.8 TB/s; with the gates' arithmetic taken out they
+// took the same.  4 bytes a lane and rows that end inside a line are what keeps it below a
+// copy's 5 to 6.  2 rows of 30,001 tokens and 256 channels: 18 + 7 + 21 us forward and 22 + 7 + 31
+// backward for the ends, what is between the pieces, and the pieces, which read x, gate and
+// dout a second time.  A single token of 12 rows: 3 us.
 #include "tgx_ops.h"
 
 namespace tgx {
