@@ -136,7 +136,8 @@ def adamw_(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Sequence[
 
     With ``grad_norm``, the float32 scalar that ``clip_grad_norm_`` returns, the gradients
     are scaled by min(1, max_norm / (grad_norm + 1e-6)) as they are read:
-    ``clip_grad_norm_(grads, float("inf"))`` takes the norm and writes nothing else.
+    ``clip_grad_norm_(grads, float("inf"))`` takes the norm and writes nothing else if it
+    is finite (otherwise the gradients become NaN, as inf / inf is).
     """
     if (grad_norm is None) != (max_norm is None):
         raise ValueError("adamw_: grad_norm and max_norm come together")
