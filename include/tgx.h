@@ -535,9 +535,10 @@ int tgx_clip_grad_norm(const void* const* grads, const int32_t* dtypes, void* co
 /* A gated recurrence along the tokens of every batch row, over dim channels:
  *   h_t = a_t h_{t-1} + (1 - a_t) x_t,  a_t = sigmoid(gate_t);  a masked token: h_t = h_{t-1}
  * from h_0 = state (zeros without one).  Element (b, t, c) of x is x[b * x_stride[0] + t *
- * x_stride[1] + c], gate alike; a stride may be 0.  mask: NULL, or bytes at mask[b *
+ * x_stride[1] + c], gate alike; a stride may be 0, but not below.  mask: NULL, or bytes at mask[b *
  * mask_stride + t], 0 = token t takes no part (its x and gate are not used, whatever they
- * hold).  out [batch, length, dim] holds every h_t rounded, last [batch, dim] the last one. */
+ * hold).  out [batch, length, dim] holds every h_t rounded, last [batch, dim] the last one.  What is
+ * written may share no memory with what is read. */
 typedef struct tgx_scan_args {
   const void* x;
   const void* gate;
@@ -580,7 +581,8 @@ int tgx_scan_grad(const tgx_scan_args* args, void* stream);
  *   out = norm(sum) weight + bias,  norm(v) = (v - mean v) / sqrt(var v + eps)
  * scale, weight, bias and post_weight [dim] of wdtype; gate, scale, post_weight (then n = x),
  * weight and bias may be NULL.  center = 0: norm(v) = v / sqrt(mean v^2 + eps).  Rows of x,
- * residual and gate are their strides apart; out and sum [rows, dim]. */
+ * residual and gate are their strides apart; out and sum [rows, dim].  What is written may share
+ * no memory with what is read. */
 typedef struct tgx_residual_norm_args {
   const void* x;
   const void* residual;

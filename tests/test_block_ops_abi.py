@@ -45,6 +45,9 @@ def test_scan_checks():
         assert fn(None, None) == 1 and "args is NULL" in _err()
         assert fn(_scan(batch=-1), None) == 1 and "batch=-1" in _err()
         assert fn(_scan(dim=0), None) == 1 and fn(_scan(length=-1), None) == 1
+        for more in (dict(x_stride=(-12, 4)), dict(x_stride=(12, -4)), dict(gate_stride=(0, -1)), dict(mask_stride=-3)):
+            more = {n: (ctypes.c_int64 * 2)(*v) if isinstance(v, tuple) else v for n, v in more.items()}
+            assert fn(_scan(**more), None) == 1 and "stride of -" in _err()
         assert fn(_scan(dtype=2), None) == 2
         assert fn(_scan(length=(1 << 30) + 1), None) == 3 and fn(_scan(batch=1 << 20, dim=1 << 20), None) == 3
         assert fn(_scan(batch=1 << 30, dim=5), None) == 3

@@ -456,6 +456,8 @@ int check_scan(const char* what, const tgx_scan_args* a) {
   if (a->batch < 0 || a->length < 0 || a->dim < 1)
     return fail(TGX_ERR_ARG, "%s: batch=%lld length=%lld dim=%lld", what, static_cast<long long>(a->batch),
                 static_cast<long long>(a->length), static_cast<long long>(a->dim));
+  for (int64_t s : {a->x_stride[0], a->x_stride[1], a->gate_stride[0], a->gate_stride[1], a->mask_stride})
+    if (s < 0) return fail(TGX_ERR_ARG, "%s: a stride of %lld", what, static_cast<long long>(s));
   if (elem_bytes(a->dtype) == 0) return fail(TGX_ERR_DTYPE, "%s: dtype %d", what, a->dtype);
   const int64_t most = int64_t(1) << 30;
   if (a->length > most || a->dim > most || a->batch > most || a->batch > (int64_t(1) << 32) / a->dim)
