@@ -159,3 +159,16 @@ def test_no_cpu_path():
                  lambda: ops.adamw_([x], [x], [x], [x], [torch.zeros((), dtype=torch.int64)])):
         with pytest.raises(RuntimeError, match="on the GPU"):
             call()
+
+
+def test_adamw_groups_are_checked():
+    one, other = (torch.nn.Parameter(torch.zeros(3)) for _ in range(2))
+    adam = ops.AdamW([one], bits=8)
+    with pytest.raises(ValueError, match="bits"):
+        adam.add_param_group({"params": [other], "bits": 16})
+    with pytest.raises(ValueError, match="bits"):
+        ops.AdamW([{"params": [one], "bits": 4}])
+    with pytest.raises(ValueError, match="bits"):
+        ops.AdamW([one], bits=4)
+    adam.add_param_group({"params": [other], "bits": 32, "lr": 1e-2})
+    assert [g["bits"] for g in adam.param_groups] == [8, 32]

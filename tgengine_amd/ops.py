@@ -161,9 +161,12 @@ class AdamW(torch.optim.Optimizer):
                  eps: float = 1e-8, weight_decay: float = 1e-2, bits: int = 32):
         if not (float(lr) >= 0.0 and eps >= 0.0 and weight_decay >= 0.0 and all(0.0 <= b < 1.0 for b in betas)):
             raise ValueError(f"AdamW: lr={float(lr)} betas={betas} eps={eps} weight_decay={weight_decay}")
-        if bits not in (8, 32):
-            raise ValueError("AdamW: bits must be 8 or 32")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, bits=bits))
+
+    def add_param_group(self, param_group: dict) -> None:
+        if param_group.get("bits", self.defaults["bits"]) not in (8, 32):
+            raise ValueError("AdamW: bits must be 8 or 32")
+        super().add_param_group(param_group)
 
     def _new(self, p: Tensor, bits: int) -> dict:
         if p.is_cuda and torch.cuda.is_current_stream_capturing():
