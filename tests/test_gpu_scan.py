@@ -120,7 +120,7 @@ def _check(c):
 
 SHAPES = [(1, 1, 1), (3, 1, 172), (2, 2, 1), (4, 3, 2), (5, 15, 3), (5, 16, 100), (5, 17, 101), (7, 33, 172), (12, 64, 50),
           (4, 65, 7), (3, 127, 12), (2, 128, 33), (2, 500, 5), (1, 3001, 2), (2, 2050, 64), (300, 20, 172), (1, 40, 4099),
-          (2000, 5, 19), (33, 257, 256)]
+          (2000, 5, 19), (33, 257, 256), (1, 17001, 2)]
 
 
 @pytest.mark.parametrize("dtype", [F, B])

@@ -23,7 +23,7 @@
 // Memory bounds it: 24,576 rows of 32 tokens and 172 bf16 channels take 175 us forward (0.75
 // GB) and 270 backward (1.29 GB), 4.3 and 4.8 TB/s; with the gates' arithmetic taken out they
 // took the same.  4 bytes a lane and rows that end inside a line are what keeps it below a
-// copy's 5 to 6.  2 rows of 30,001 tokens and 256 channels: 18 + 7 + 21 us forward and 22 + 7 + 31
+// copy's 5 to 6.  2 rows of 30,001 tokens and 256 channels: 19 + 4.5 + 20 us forward and 22 + 5 + 30
 // backward for the ends, what is between the pieces, and the pieces, which read x, gate and
 // dout a second time.  A single token of 12 rows: 3 us.
 #include "tgx_ops.h"
@@ -305,9 +305,12 @@ __global__ __launch_bounds__(kScanThreads) void scan_ends(const ScanArgs a) {
 
 // Turns the (A, E) between the pieces into what enters each, in E's place.  kSegments threads
 // share a channel's pieces: each composes its own, then takes what the segments before it
-// make of the outer state through them.
-constexpr int kSegments = 16;
+// make of the outer state through them.  Its pieces stay in registers on the way if they are
+// no more than kOwn: 251 pieces of 2 rows of 256 channels take 4.5 us with 32 segments, 6.5
+// with 16, which read their pieces twice, and 5.8 with 64, of 16-byte loads.
+constexpr int kSegments = 32;
 constexpr int kCarryChannels = kScanThreads / kSegments;
+constexpr int kOwn = 8;
 
 template <bool BACK>
 __global__ __launch_bounds__(kScanThreads) void scan_carry(const ScanArgs a) {
@@ -321,10 +324,27 @@ __global__ __launch_bounds__(kScanThreads) void scan_carry(const ScanArgs a) {
   const int64_t plane = a.batch * a.pieces * a.dim;
   float* ends = a.ends + row * a.pieces * a.dim + c;
   auto piece = [&](int p) { return ends + static_cast<int64_t>(BACK ? pieces - 1 - p : p) * a.dim; };
-  float all = 1.f, end = 0.f;
-  if (live) {
+  const float* outer = BACK ? a.dlast : a.state;
+  float h = live && outer != nullptr ? outer[row * a.dim + c] : 0.f;
+  float all = 1.f, end = 0.f, f[kOwn], g[kOwn];
+  const bool own = per <= kOwn;
+  if (live && own) {
+    // the last piece leads nowhere, and its place holds nothing
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      const bool there = lo + i < min(hi, pieces - 1);
+      const float* e = piece(min(lo + i, pieces - 1));
+      f[i] = there ? e[0] : 1.f;
+      g[i] = there ? e[plane] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      all *= f[i];
+      end = fmaf(f[i], end, g[i]);
+    }
+  } else if (live) {
 #pragma unroll 8
-    for (int p = lo; p < min(hi, pieces - 1); ++p) {  // the last one leads nowhere
+    for (int p = lo; p < min(hi, pieces - 1); ++p) {
       const float* e = piece(p);
       all *= e[0];
       end = fmaf(e[0], end, e[plane]);
@@ -334,9 +354,15 @@ __global__ __launch_bounds__(kScanThreads) void scan_carry(const ScanArgs a) {
   lds[1][seg][lane] = end;
   __syncthreads();
   if (!live) return;
-  const float* outer = BACK ? a.dlast : a.state;
-  float h = outer != nullptr ? outer[row * a.dim + c] : 0.f;
   for (int s = 0; s < seg; ++s) h = fmaf(lds[0][s][lane], h, lds[1][s][lane]);
+  if (own) {
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      if (lo + i < hi) piece(lo + i)[plane] = h;
+      h = fmaf(f[i], h, g[i]);
+    }
+    return;
+  }
 #pragma unroll 8
   for (int p = lo; p < hi; ++p) {
     float* e = piece(p);
@@ -426,7 +452,8 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd(const ScanArgs a) {
   if (at.piece == 0 && a.dstate != nullptr) store_floats(a.dstate, at.states, c);
 }
 
-// channels a thread takes: 4 bytes of them (8 in the forward pass make 4% of a difference)
+// channels a thread takes: 4 bytes of them (8 are 2% faster in the forward pass and 40% slower
+// backward, whose registers they fill)
 template <typename T>
 constexpr int kChannels = 4 / sizeof(T);
 
