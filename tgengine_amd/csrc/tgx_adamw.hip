@@ -23,7 +23,7 @@
 //
 // HBM bounds the 32-bit step of a large table: 100,000,000 bf16 values (2.2 GB) 372 us, 5.9
 // TB/s, as a large copy.  The 8-bit one has as much to compute as to move: 172,000,000 f32
-// values (2.77 GB) 496 us, 5.6 TB/s, 83 vector instructions a value keep the units busy
+// values (2.77 GB) 496 us, 5.6 TB/s, 85 vector instructions a value keep the units busy
 // nearly all of it.  16 tensors of up to 20,001 values take 2.8 and 3.9 us, mostly the
 // launches, behind a host call of 9 to 12.
 #include "tgx_ops.h"
