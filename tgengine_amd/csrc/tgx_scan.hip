@@ -31,6 +31,9 @@
 namespace tgx {
 namespace {
 
+// 24,576 rows of 32 tokens and 172 bf16 channels take 175 us forward and 279 backward, with 128
+// threads 188 and 292, with 512 184 and 318; 600 rows of 512 tokens and 100 f32 channels 89 and
+// 141, 102 and 158, 136 and 223.
 constexpr int kScanThreads = 256;
 constexpr int kSpan = 8;
 
