@@ -23,6 +23,7 @@ tracing are refused).  There is no CPU path.
 """
 from __future__ import annotations
 
+import copy
 from typing import Iterable, Optional, Sequence, Tuple, Union
 
 import torch
@@ -147,6 +148,17 @@ def adamw_(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Sequence[
                   eps, weight_decay, grad_norm, 0.0 if max_norm is None else max_norm)
 
 
+def _kept(state, device: torch.device):
+    """A copy of an optimizer's state for one parameter, its tensors on ``device`` in their own types."""
+    if isinstance(state, Tensor):
+        return state.to(device, copy=True)
+    if isinstance(state, dict):
+        return {k: _kept(v, device) for k, v in state.items()}
+    if type(state) in (list, tuple):
+        return type(state)(_kept(v, device) for v in state)
+    return copy.deepcopy(state)
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW over all parameters of a group in one step of kernels (``adamw_``).
 
@@ -202,10 +214,21 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict) -> None:
-        super().load_state_dict(state_dict)
-        # the averages keep their own types, whatever their parameters' are
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
-        for i, p in zip(ids, params):
-            if i in state_dict["state"]:
-                self.state[p] = {k: v.to(p.device, copy=True) for k, v in state_dict["state"][i].items()}
+        given = {}
+
+        def own_types(_) -> None:
+            # the base class casts state to its parameter's type; the averages, scales and steps keep theirs
+            ids = [i for g in given["param_groups"] for i in g["params"]]
+            params = [p for g in self.param_groups for p in g["params"]]
+            for i, p in zip(ids, params):
+                if i in given["state"]:
+                    self.state[p] = _kept(given["state"][i], p.device)
+
+        # behind the caller's hooks that change what is loaded, before those that see it loaded
+        hooks = [self.register_load_state_dict_pre_hook(lambda _, state: given.update(state)),
+                 self.register_load_state_dict_post_hook(own_types, prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
