@@ -286,6 +286,9 @@ __global__ __launch_bounds__(kScanThreads) void scan_ends(const ScanArgs a) {
         load_span<T, V, O>(s.g, a.gate, at.gate + t * at.gate_step, at.gate_step, s.bits);
       },
       [&](const Tokens<T, V>& s, int, int n) {
+        float held[V];  // masked tokens' gradients, as in scan_bwd
+#pragma unroll
+        for (int u = 0; u < V; ++u) held[u] = 0.f;
 #pragma unroll
         for (int j = 0; j < kSpan; ++j) {
           const int i = BACK ? kSpan - 1 - j : j;
@@ -296,11 +299,19 @@ __global__ __launch_bounds__(kScanThreads) void scan_ends(const ScanArgs a) {
             float f, rest;
             sigmoids(to_f(s.g[i].v[u]), f, rest);
             f = keep ? f : 1.f;
-            if constexpr (BACK) end[u] = f * (end[u] + (given ? to_f(s.x[i].v[u]) : 0.f));
-            else end[u] = keep ? fmaf(f, end[u], rest * to_f(s.x[i].v[u])) : end[u];
+            if constexpr (BACK) {
+              const float d = held[u] + (given ? to_f(s.x[i].v[u]) : 0.f);
+              end[u] = keep ? f * (end[u] + d) : end[u];
+              held[u] = keep ? 0.f : d;
+            } else {
+              end[u] = keep ? fmaf(f, end[u], rest * to_f(s.x[i].v[u])) : end[u];
+            }
             all[u] *= f;
           }
         }
+        if (BACK && MASK)
+#pragma unroll
+          for (int u = 0; u < V; ++u) end[u] += held[u];
       });
   store_floats(a.ends, at.ends, all);
   store_floats(a.ends + a.batch * a.pieces * a.dim, at.ends, end);
@@ -418,9 +429,13 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd(const ScanArgs a) {
         // dx = rest dh, dgate = grow dh, and f dh goes on to the token before.  Of f and rest the
         // smaller one is kept, and the gate's sign says which that is: 16 registers less, and a
         // third wavefront a SIMD.
-        float h[V], small[kSpan][V], grow[kSpan][V];
+        // Gradients of masked tokens that follow each other are added up for themselves, and a
+        // span's sum to what came from the right: one by one, 500 of them would lose 500 roundings.
+        // 600 rows of 512 tokens and 100 f32 channels, masked: the state's gradient is off by 1.3e-7
+        // instead of 3.3e-7 (root mean squares), 210 us trained both ways; in bf16 214 instead of 211.
+        float h[V], held[V], small[kSpan][V], grow[kSpan][V];
 #pragma unroll
-        for (int u = 0; u < V; ++u) h[u] = s.h[u];
+        for (int u = 0; u < V; ++u) h[u] = s.h[u], held[u] = 0.f;
 #pragma unroll
         for (int i = 0; i < kSpan; ++i)
 #pragma unroll
@@ -442,15 +457,21 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd(const ScanArgs a) {
           Pack<T, V> px, pg;
 #pragma unroll
           for (int u = 0; u < V; ++u) {
-            const float dh = (DOUT ? to_f(s.d[i].v[u]) : 0.f) + c[u], big = 1.f - small[i][u];
+            float d = DOUT ? to_f(s.d[i].v[u]) : 0.f;
+            if constexpr (MASK) d += held[u];
+            const float dh = d + c[u], big = 1.f - small[i][u];
             const bool neg = to_f(s.g[i].v[u]) < 0.f;
             px.v[u] = from_f<T>(dh * (neg ? big : small[i][u]));
             pg.v[u] = from_f<T>(dh * grow[i][u]);
-            c[u] = keep ? dh * (neg ? small[i][u] : big) : dh;
+            c[u] = keep ? dh * (neg ? small[i][u] : big) : c[u];
+            held[u] = keep ? 0.f : d;
           }
           store_at<T, V>(a.dx, to, kept_pack(px, keep));
           store_at<T, V>(a.dgate, to, kept_pack(pg, keep));
         }
+        if constexpr (MASK)
+#pragma unroll
+          for (int u = 0; u < V; ++u) c[u] += held[u];
       });
   if (at.piece == 0 && a.dstate != nullptr) store_floats(a.dstate, at.states, c);
 }
