@@ -48,12 +48,22 @@ inline size_t ops_align(size_t x) { return (x + 255) & ~static_cast<size_t>(255)
 inline uint64_t addr(const void* p) { return reinterpret_cast<uint64_t>(p); }
 inline int elem_bytes(int dtype) { return feat_elem_bytes(dtype); }
 
-// a = sigmoid(g) and 1 - a, each to |g| + 3 units in its last place (the rounding of the
-// exponent's argument, a power, a sum, a reciprocal): neither is a difference
-__device__ __forceinline__ void sigmoids(float g, float& a, float& rest) {
+// The smaller of sigmoid(g) and 1 - sigmoid(g), sigmoid(g) itself where g < 0, and the larger one
+// as a reciprocal.  u = 2^-24.  The power's argument is off by 1.3 u |g| (its constant and a
+// product), the power and the reciprocal by 2 u each, their sum and product by u: small is off by
+// (1.3 |g| + 6) u relatively, the larger by 5 u, and 1 - small by 7 u.  Where |g| is above 87.3 the
+// power's instruction, and small with it, is 0.  A step of Newton's at the reciprocal takes the root
+// mean square of small's errors from 0.98 u to 0.94 u, for |g| about 2, and the scan of 600 rows of
+// 512 tokens and 100 bf16 channels from 67 us to 72.
+__device__ __forceinline__ float sigmoid_small(float g, float& larger) {
   const float e = __builtin_amdgcn_exp2f(-1.44269504f * __builtin_fabsf(g));
-  const float r = __builtin_amdgcn_rcpf(1.f + e);
-  const float small = e * r;
+  larger = __builtin_amdgcn_rcpf(1.f + e);
+  return e * larger;
+}
+// a = sigmoid(g) and 1 - a: neither is a difference
+__device__ __forceinline__ void sigmoids(float g, float& a, float& rest) {
+  float r;
+  const float small = sigmoid_small(g, r);
   a = g < 0.f ? small : r;  // NaN: r, which is NaN
   rest = g < 0.f ? r : small;
 }

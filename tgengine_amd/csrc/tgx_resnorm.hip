@@ -66,9 +66,11 @@ __global__ __launch_bounds__(res_threads(L)) void resnorm_fwd(const ResArgs a) {
         for (int u = 0; u < V; ++u) {
           float by = a.scale != nullptr ? to_f(w.v[u]) : 1.f;
           if (a.gate != nullptr) {
-            float f, rest;
-            sigmoids(to_f(pg[j].v[u]), f, rest);
-            by *= f;
+            // 1 less the smaller one, as the backward pass, which keeps only that, forms it again
+            const float g = to_f(pg[j].v[u]);
+            float larger;
+            const float small = sigmoid_small(g, larger);
+            by *= g < 0.f ? small : 1.f - small;
           }
           s[i][j][u] = fmaf(by, s[i][j][u], to_f(pr[i][j].v[u]));
         }

@@ -164,8 +164,8 @@ __global__ __launch_bounds__(res_threads(L)) void resnorm_bwd(const ResArgs a) {
 #pragma unroll
       for (int u = 0; u < V; ++u) {
         if constexpr (GATE) {
-          const float e = __builtin_amdgcn_exp2f(-1.44269504f * __builtin_fabsf(to_f(now.g[j].v[u])));
-          small[j][u] = e * __builtin_amdgcn_rcpf(1.f + e);
+          float larger;
+          small[j][u] = sigmoid_small(to_f(now.g[j].v[u]), larger);
         }
         const float h = value(j, u).h, dy = to_f(y.v[u]), g = dy * to_f(w[j].v[u]);
         s1 += g;
