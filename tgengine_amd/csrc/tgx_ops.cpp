@@ -20,8 +20,9 @@ void check_embed(const Tensor& table, const Tensor& ids) {
   same_device(ids, table, "embed: ids");
 }
 
-Tensor embed_out(const Tensor& table_in, const Tensor& ids, double scale) {
-  const c10::OptionalDeviceGuard guard(table_in.device());
+Tensor embed_out(const Tensor& given, const Tensor& ids, double scale) {
+  const c10::OptionalDeviceGuard guard(given.device());
+  const Tensor table_in = stored(given);
   // rows in place where they are dense and apart, or one row for all
   const int64_t dim = table_in.size(1), step = table_in.size(0) > 1 ? table_in.stride(0) : dim;
   const bool in_place = (dim == 1 || table_in.stride(1) == 1) && (step >= dim || step == 0);
@@ -48,7 +49,7 @@ class Embed : public torch::autograd::Function<Embed> {
     only_once("embed");
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
     const Tensor ids = ctx->get_saved_variables()[0];
-    const Tensor g = grads[0].contiguous();
+    const Tensor g = dense(grads[0]);
     const c10::OptionalDeviceGuard guard(g.device());
     const int64_t rows = ctx->saved_data["rows"].toInt(), dim = g.size(-1), n = ids.numel();
     Tensor out = at::empty({rows, dim}, g.options());
@@ -77,8 +78,8 @@ struct NormIn {
     dim = x_in.size(-1);
     x = as_rows(x_in, rows, stride);
     dt = dtype_of(x, "layer_norm: x");
-    w = weight.defined() ? weight.contiguous() : weight;
-    b = bias.defined() ? bias.contiguous() : bias;
+    w = weight.defined() ? dense(weight) : weight;
+    b = bias.defined() ? dense(bias) : bias;
     const Tensor& any = w.defined() ? w : b;
     wdt = any.defined() ? dtype_of(any, "layer_norm: weight") : dt;
   }
@@ -129,7 +130,7 @@ class LayerNorm : public torch::autograd::Function<LayerNorm> {
     const variable_list saved = ctx->get_saved_variables();
     const c10::OptionalDeviceGuard guard(saved[0].device());
     const NormIn in(saved[0], saved[1], saved[2]);
-    const Tensor g = grads[0].contiguous();
+    const Tensor g = dense(grads[0]);
     Tensor dx, dw, db;
     if (ctx->needs_input_grad(0)) dx = at::empty(saved[0].sizes(), in.x.options());
     // inputs are counted without those left out
@@ -239,7 +240,7 @@ class Attention : public torch::autograd::Function<Attention> {
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &q = saved[0], &k = saved[1], &v = saved[2];
     const c10::OptionalDeviceGuard guard(q.device());
-    const Tensor g = grads[0].contiguous();
+    const Tensor g = dense(grads[0]);
     tgx_attention_args a = attention_args(q, k, v, saved[3], ctx->saved_data["scale"].toDouble());
     a.out = saved[4].data_ptr();
     a.lse = saved[5].data_ptr<float>();
@@ -289,9 +290,12 @@ Tensor clip_grad_norm(std::vector<Tensor> grads, double max_norm, const std::vec
   std::vector<int32_t> dt(n), odt(n);
   std::vector<int64_t> size(n);
   for (size_t i = 0; i < n; ++i) {
+    reverse_mode_only("clip_grad_norm_", {&grads[i]});
+    if (!outs.empty()) grads[i] = stored(grads[i]);  // scaled in place, signs that are turned stay so
     const Tensor& g = grads[i];
     const Tensor& o = outs.empty() ? g : outs[i];
-    reverse_mode_only("clip_grad_norm_", {&g, &o});
+    reverse_mode_only("clip_grad_norm_", {&o});
+    if (!outs.empty() && o.is_neg()) bad("clip_grad_norm_: out must not be a view of turned signs");
     on_gpu(g, "clip_grad_norm_: gradients");
     for (const Tensor* t : {&g, &o}) {
       same_device(*t, grads[0], "clip_grad_norm_: every tensor");

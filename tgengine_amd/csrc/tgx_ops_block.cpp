@@ -82,8 +82,8 @@ class Scan : public torch::autograd::Function<Scan> {
     const Tensor &x = saved[0], &gate = saved[1], &state = saved[2];
     const c10::OptionalDeviceGuard guard(x.device());
     tgx_scan_args a = scan_args(x, gate, saved[3], state);
-    const Tensor g = grads[0].defined() ? grads[0].contiguous() : Tensor();
-    const Tensor gl = grads[1].defined() ? grads[1].contiguous() : Tensor();
+    const Tensor g = grads[0].defined() ? dense(grads[0]) : Tensor();
+    const Tensor gl = grads[1].defined() ? dense(grads[1]) : Tensor();
     a.starts = saved[4].data_ptr<float>();
     a.grad_out = ptr(g);
     a.grad_last = static_cast<const float*>(ptr(gl));
@@ -110,7 +110,7 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& x_in, const Tensor& gate_in,
   reverse_mode_only("gated_scan", {&x_in, &gate_in, &state});
   const Tensor x = dense_last(x_in), gate = dense_last(gate_in);
   if (mask.defined() && mask.size(1) > 1 && mask.stride(1) != 1) mask = mask.contiguous();
-  if (state.defined()) state = state.contiguous();
+  if (state.defined()) state = dense(state);
   variable_list out;
   if (keeps_grad({&x, &gate, &state})) {
     out = Scan::apply(x, gate, state.defined() ? OptTensor(state) : c10::nullopt,
@@ -167,7 +167,7 @@ struct ResCall {
     Tensor* to[] = {&t.weight, &t.bias, &t.scale, &t.post};
     for (int i = 0; i < 4; ++i) {
       if (!from[i]->defined()) continue;
-      *to[i] = from[i]->contiguous();
+      *to[i] = dense(*from[i]);
       a.wdtype = dtype_of(*to[i], "residual_norm: weight");
     }
     a.x = t.x.data_ptr();
@@ -220,8 +220,8 @@ class ResidualNorm : public torch::autograd::Function<ResidualNorm> {
     const Res t{saved[0], saved[1], saved[4], saved[2], saved[3], saved[5], saved[6]};
     const c10::OptionalDeviceGuard guard(t.x.device());
     ResCall c(t, ctx->saved_data["center"].toBool(), ctx->saved_data["eps"].toDouble());
-    const Tensor g = grads[0].defined() ? grads[0].contiguous() : Tensor();
-    const Tensor gs = grads[1].defined() ? grads[1].contiguous() : Tensor();
+    const Tensor g = grads[0].defined() ? dense(grads[0]) : Tensor();
+    const Tensor gs = grads[1].defined() ? dense(grads[1]) : Tensor();
     c.a.grad_out = ptr(g);
     c.a.grad_sum = ptr(gs);
     c.a.stats = saved[7].data_ptr<float>();
@@ -300,6 +300,7 @@ void adamw(const py::list& params_in, const py::list& grads_in, const py::list& 
     return o == Py_None ? Tensor() : THPVariable_Unpack(o);
   };
   std::vector<tgx_adamw_tensor> table(n);
+  std::vector<Tensor> copies;
   for (size_t i = 0; i < n; ++i) {
     const Tensor &p = params[i], &g = grads[i], &m = exp_avg[i], &v = exp_avg_sq[i], &t = steps[i];
     reverse_mode_only("adamw_", {&p, &g});
@@ -326,8 +327,11 @@ void adamw(const py::list& params_in, const py::list& grads_in, const py::list& 
       same_device(s, params[0], "adamw_: every tensor");
       a.scales = s.data_ptr<float>();
     }
+    for (const Tensor* x : {&p, &m, &v})
+      if (x->is_neg()) bad("adamw_: parameters and averages must not be views of turned signs");
+    if (g.is_neg()) copies.push_back(stored(g));
     a.param = p.data_ptr();
-    a.grad = g.data_ptr();
+    a.grad = (g.is_neg() ? copies.back() : g).data_ptr();
     a.exp_avg = m.data_ptr();
     a.exp_avg_sq = v.data_ptr();
     a.step = t.data_ptr<int64_t>();
@@ -345,9 +349,10 @@ void adamw(const py::list& params_in, const py::list& grads_in, const py::list& 
   a.eps = eps;
   a.weight_decay = weight_decay;
   a.max_norm = max_norm;
-  const Tensor rate = lr_in.value_or(Tensor()), norm = norm_in.value_or(Tensor());
-  for (const Tensor* x : {&rate, &norm}) {
+  Tensor rate = lr_in.value_or(Tensor()), norm = norm_in.value_or(Tensor());
+  for (Tensor* x : {&rate, &norm}) {
     if (!x->defined()) continue;
+    *x = stored(*x);
     if (x->scalar_type() != at::kFloat || x->numel() != 1) bad("adamw_: lr and grad_norm must be float32 of one value");
     same_device(*x, params[0], "adamw_: every tensor");
   }

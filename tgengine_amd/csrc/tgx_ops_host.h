@@ -75,9 +75,17 @@ inline Tensor workspace(size_t bytes, const Tensor& like) {
 
 inline void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// the values in memory: torch may hold them with their signs turned (the imaginary part of a
+// conjugate)
+inline Tensor stored(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
+// and one after the other
+inline Tensor dense(const Tensor& t) { return stored(t.contiguous()); }
+
 // rows of the last dimension as (rows, row stride), or a contiguous copy where the
 // tensor's rows are not one even step apart
-inline Tensor as_rows(const Tensor& t, int64_t& rows, int64_t& stride) {
+inline Tensor as_rows(const Tensor& in, int64_t& rows, int64_t& stride) {
+  const Tensor t = stored(in);
   const int64_t dim = t.size(-1);
   rows = dim > 0 ? t.numel() / dim : 0;
   stride = dim;
@@ -90,6 +98,6 @@ inline Tensor as_rows(const Tensor& t, int64_t& rows, int64_t& stride) {
 }
 
 // the tensor itself where its last dimension is one value after the other
-inline Tensor dense_last(const Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+inline Tensor dense_last(const Tensor& t) { return stored(t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous()); }
 
 }  // namespace
