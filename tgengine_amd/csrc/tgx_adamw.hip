@@ -13,19 +13,21 @@
 // that shrinks by 0.05% a step would stay where it is for ever.  u is the fraction of
 // i / p + t / p^2 (+ 1/2 for the root), i the value's place and p^3 = p + 1, a sequence
 // that is even over neighbouring values and steps alike, and needs no state.  In a
-// simulation of 8,192 roots whose gradients fall to a tenth after 3,000 steps, they stand at
-// 0.93 of the exact ones after 3,000 more (deviation 0.13); with independent dithers at 1.02
-// (deviation 0.35), rounded to the nearest at 4.1.  A root
+// simulation of 8,192 roots that begin at their exact values and whose gradients fall to a tenth
+// after 3,000 steps, they stand at 0.94 of the exact ones after 3,000 more (deviation 0.13); with
+// independent dithers at 1.02 (deviation 0.35), rounded to the nearest at 4.1.  Roots that begin at
+// zero end alike but for the nearest: 0.4 before the gradients fall, 1.6 at the end.  A root
 // above zero is stored above zero, since the next step divides by it.  The 8-bit averages
 // are updated in 64 bits, so that what is stored is what the formulas say and not
 // what an intermediate rounding makes of a value next to a border; this step's update uses
 // the averages before they are rounded.
 //
-// HBM bounds the 32-bit step of a large table: 100,000,000 bf16 values (2.2 GB) 372 us, 5.9
-// TB/s, as a large copy.  The 8-bit one has as much to compute as to move: 172,000,000 f32
-// values (2.77 GB) 496 us, 5.6 TB/s, 85 vector instructions a value keep the units busy
-// nearly all of it.  16 tensors of up to 20,001 values take 2.8 and 3.9 us, mostly the
-// launches, behind a host call of 9 to 12.
+// HBM bounds the 32-bit step of a large table: 100,000,000 bf16 values (2.2 GB) 369 to 382 us
+// (medians of three runs), 5.9 TB/s, as a large copy.  The 8-bit one has as much to compute as to
+// move: 172,000,000 f32 values (2.77 GB) 496 us a call, 5.6 TB/s, 85 vector instructions a value
+// keep the units busy nearly all of it.  Their clock decides: 478 us for the launches after a
+// pause, up to 734 after some in a row, and 530 to 590 from then on.  16 tensors of up to 20,001 values
+// take 3.0 and 4.0 us, mostly the launches, behind a host call of 12.
 #include "tgx_ops.h"
 #include "tgx_ranges.h"
 

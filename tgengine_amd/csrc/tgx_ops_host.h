@@ -82,8 +82,9 @@ inline Tensor stored(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t;
 // and one after the other
 inline Tensor dense(const Tensor& t) { return stored(t.contiguous()); }
 
-// rows of the last dimension as (rows, row stride), or a contiguous copy where the
-// tensor's rows are not one even step apart
+// rows of the last dimension as (rows, row stride): in place where the tensor is contiguous or
+// of two dimensions with dense rows, and otherwise a contiguous copy, also where more dimensions
+// have rows one even step apart (a half of a projection of (batch, tokens, 2 dim))
 inline Tensor as_rows(const Tensor& in, int64_t& rows, int64_t& stride) {
   const Tensor t = stored(in);
   const int64_t dim = t.size(-1);

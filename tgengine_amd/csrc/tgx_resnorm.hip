@@ -9,9 +9,12 @@
 // residual and gate are read once and the norm works on the sum before it is rounded: s and
 // y are rounded once each.  Statistics and sums are of 32 bits.
 //
-// HBM bounds it: 786,432 x 172 bf16 rows (1.08 GB, rows that begin inside a line) 182 us, 5.9
-// TB/s alone and 193 between backward passes; 8,001 x 4,096 gated bf16 rows (0.33 GB) 61 us, 5.4
-// TB/s; 240 x 172 f32 rows 3.5 us, a chain of one read, two sums and one write.
+// HBM bounds it, and vector instructions are close: 786,432 x 172 bf16 rows (1.08 GB, rows that
+// begin inside a line) take 179 us at best, 6.0 TB/s, and 198 in the median between backward
+// passes; their 106M instructions keep the vector units busy all the time, so that the time goes
+// with the clock, which falls in long runs.  8,001 x 4,096 gated bf16 rows (0.33 GB) 63 us (61 at
+// best), 5.2 TB/s, units busy 77%; 240 x 172 f32 rows 3.6 us, a chain of one read, two sums and one
+// write.
 #include "tgx_resnorm.h"
 
 namespace tgx {

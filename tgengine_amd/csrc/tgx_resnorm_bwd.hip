@@ -11,9 +11,12 @@
 // lanes own fixed columns, whose sums over rows stay in registers until the end, are joined
 // over the workgroup's rows in LDS in a fixed order and left in part[block][.][dim].
 //
-// HBM bounds the sum alone: 786,432 x 172 bf16 rows (five tensors, 1.35 GB) 293 us, 4.6 TB/s.
-// With a gate and a scale there is as much to compute: 8,001 x 4,096 bf16 rows (seven tensors,
-// 0.46 GB) 116 us and 8.5 for the join, 4.0 TB/s.
+// The sum alone is bound by vector instructions beside HBM: 786,432 x 172 bf16 rows (five
+// tensors, 1.35 GB) take 288 us at best, 4.7 TB/s, and 306 in the median, with the vector units
+// busy 86% (128M instructions; 22 of the 32 lanes of a row hold values).  With a gate and a scale
+// 176 registers allow two wavefronts a SIMD, one workgroup of 8,001 x 4,096 bf16 rows (seven tensors,
+// 0.46 GB) on a compute unit: 121 us (118 at best) and 9 for the join, 3.8 TB/s, units busy 52%,
+// so that neither is full: each row's barrier is waited for with nothing beside it.
 #include "tgx_resnorm.h"
 
 namespace tgx {

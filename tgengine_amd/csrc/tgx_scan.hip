@@ -21,9 +21,9 @@
 // line is read anyway.
 //
 // Memory bounds it: 24,576 rows of 32 tokens and 172 bf16 channels take 175 us forward (0.75
-// GB) and 270 backward (1.29 GB), 4.3 and 4.8 TB/s; with the gates' arithmetic taken out they
+// GB) and 282 backward (1.29 GB; medians), 4.3 and 4.6 TB/s; with the gates' arithmetic taken out they
 // took the same.  4 bytes a lane and rows that end inside a line are what keeps it below a
-// copy's 5 to 6.  2 rows of 30,001 tokens and 256 channels: 19 + 4.5 + 20 us forward and 22 + 5 + 30
+// copy's 5 to 6.  2 rows of 30,001 tokens and 256 channels: 19 + 5 + 21 us forward and 24 + 5 + 31
 // backward for the ends, what is between the pieces, and the pieces, which read x, gate and
 // dout a second time.  A single token of 12 rows: 3 us.
 #include "tgx_ops.h"
@@ -31,7 +31,7 @@
 namespace tgx {
 namespace {
 
-// 24,576 rows of 32 tokens and 172 bf16 channels take 175 us forward and 279 backward, with 128
+// In one sweep 24,576 rows of 32 tokens and 172 bf16 channels take 175 us forward and 279 backward, with 128
 // threads 188 and 292, with 512 184 and 318; 600 rows of 512 tokens and 100 f32 channels 89 and
 // 141, 102 and 158, 136 and 223.
 constexpr int kScanThreads = 256;
@@ -490,7 +490,11 @@ struct Pieces {
 // of 512 tokens and 100 f32 channels (60,000 threads) take 95 us forward and 149 backward in
 // one piece, in two 84 and 141, and 47 and 53 for what is between them; 2 rows of 30,001 tokens
 // and 256 bf16 channels 47 and 61 with 65,536 threads, 47 and 59 with 131,072, 72 and 93 with
-// 32,768.
+// 32,768.  What this rule costs where it makes few pieces, whole calls forward and trained: two
+// lose (300 rows of 512 tokens and 100 f32 channels 53 and 170 us, in one piece 33 and 153; 600
+// such rows in bf16 67 and 207, 50 and 173), three are even (200 x 1,024 x 100 f32 66 and 229,
+// 59 and 284; 600 x 512 x 64 bf16 48 and 122, 49 and 131), and five or more win on long rows
+// (120 x 1,024 x 100 f32 43 and 132, 58 and 211).
 constexpr int64_t kFill = 65536;
 Pieces cut(const tgx_scan_args* a) {
   const int64_t v = a->dtype == TGX_BF16 && a->dim >= kChannels<bf16> ? kChannels<bf16> : 1;
