@@ -290,11 +290,10 @@ Tensor clip_grad_norm(std::vector<Tensor> grads, double max_norm, const std::vec
   std::vector<int32_t> dt(n), odt(n);
   std::vector<int64_t> size(n);
   for (size_t i = 0; i < n; ++i) {
-    reverse_mode_only("clip_grad_norm_", {&grads[i]});
     if (!outs.empty()) grads[i] = stored(grads[i]);  // scaled in place, signs that are turned stay so
     const Tensor& g = grads[i];
     const Tensor& o = outs.empty() ? g : outs[i];
-    reverse_mode_only("clip_grad_norm_", {&o});
+    reverse_mode_only("clip_grad_norm_", {&g, &o});
     if (!outs.empty() && o.is_neg()) bad("clip_grad_norm_: out must not be a view of turned signs");
     on_gpu(g, "clip_grad_norm_: gradients");
     for (const Tensor* t : {&g, &o}) {
